@@ -162,6 +162,24 @@ int warp34_kv_cache_write_strided_bf16(const warp34_exec* ex, const warp34_kv_la
                                        int row_stride_elems);                /* warp34_cuda.h:364-365 */
 
 /* ------------------------------------------------------------------------------------
+ * The cache read back: row i of k_out / v_out ([num_rows, row_stride], 16-bit, head h at h * head_dim)
+ * is the decoded K / V row of slot_mapping[i] (page * block_size + offset; negative: the output row is
+ * left untouched), rotated rows rotated back, computed in 32 bits and rounded once.  No counterpart in
+ * the reference.  Any layout the append writes, K and V each in its own format; FP16 rows can be read
+ * as bf16 and BF16 rows as fp16.  k_out or v_out may be NULL (that slab is not touched).  slot_mapping
+ * is a DEVICE pointer; slots must lie inside the slabs and may come more than once.
+ * Row strides are in elements and at least local_kv_heads * head_dim (hipErrorInvalidValue); head_dim
+ * and strides are multiples of 8, outputs 16-byte aligned, 16-bit rows 16-byte, 8-bit rows 4-byte, TQ4
+ * rows 2-byte aligned (hipErrorNotSupported otherwise).
+ * ------------------------------------------------------------------------------------ */
+int warp34_kv_cache_read_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
+                             const int32_t* slot_mapping, int num_rows, void* k_out, void* v_out,
+                             int k_row_stride, int v_row_stride);
+int warp34_kv_cache_read_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
+                              const int32_t* slot_mapping, int num_rows, void* k_out, void* v_out,
+                              int k_row_stride, int v_row_stride);
+
+/* ------------------------------------------------------------------------------------
  * Paged GQA attention (replaces op_paged_attn.cu:1266-1448 and op_kv_cache.cu:1192-1241).
  *
  * q_in / attn_out: [total_tokens, num_q_heads, head_dim] contiguous, fp16 for _f16 and
@@ -283,6 +301,24 @@ int warp34_apply_attn_output_gate_f16(const warp34_exec* ex, const void* attn_ou
 int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
                                      const warp34_attention_batch* batch, const void* q_in,
                                      const void* gate, void* attn_out, int num_q_heads);
+
+/* Attention results over disjoint key sets joined by the natural logarithms of their sums (a shared
+ * prefix and a private rest, keys spread over ranks): lse = ln sum_p exp(lse_p), out = sum_p
+ * exp(lse_p - lse) out_p, in 32 bits, rounded once.  No counterpart in the reference.
+ * parts: [num_parts][num_rows, head_dim], parts part_stride elements apart; lse_parts: fp32
+ * [num_parts][num_rows], lse_part_stride elements apart; a row is one (token, query head).  A part
+ * whose lse is minus infinity saw no key and its row is not looked at; where all of them are, the row
+ * is zeros and its lse minus infinity.  lse_out may be NULL.  out may be the memory of one of the
+ * parts; lse_out must not overlap lse_parts.  num_rows <= 0 returns 0 without a launch.  With more than
+ * one part the strides are at least num_rows * head_dim and num_rows (hipErrorInvalidValue); head_dim
+ * (at most 2048) and part_stride are multiples of 8, parts and out 16-byte aligned
+ * (hipErrorNotSupported otherwise). */
+int warp34_attention_merge_f16(const warp34_exec* ex, const void* parts, const float* lse_parts, int num_parts,
+                               int64_t part_stride, int64_t lse_part_stride, void* out, float* lse_out,
+                               int64_t num_rows, int head_dim);
+int warp34_attention_merge_bf16(const warp34_exec* ex, const void* parts, const float* lse_parts, int num_parts,
+                                int64_t part_stride, int64_t lse_part_stride, void* out, float* lse_out,
+                                int64_t num_rows, int head_dim);
 
 /* QSA sparse paged attention: query token t attends over its own list of selected 4-token groups
  * (replaces ops/op_qsa.cu:716-1158,1446-1571,1711-1751).  Group j of token t is rows

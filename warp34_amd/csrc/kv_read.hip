@@ -1,0 +1,290 @@
+// Reading a paged cache back: the K and V rows of given slots, decoded to 16-bit rows, the other half of the append (kv_write.hip).
+//
+//   plain rows    x[e] = code(e) * d(block of e)                      (16-bit rows: the element itself)
+//   rotated rows  x[e] = sign(e) / 16 * sum_f (-1)^popcount(e & f) code(f) d(block of f)
+//
+// computed in 32 bits and rounded once.  Bound: HBM, a row's bytes read once and 2 x head_dim bytes written once.
+#include "attn_lanes.h"
+#include "kv_encode.h"
+
+namespace w34 {
+
+// One slab (K or V) and where its rows go; base 0: not wanted.
+struct ReadSide {
+    uint64_t base, page_stride, head_stride, token_stride;
+    uint16_t* out;
+    int64_t row_stride;  // elements
+    int format;
+};
+struct ReadParams {
+    ReadSide side[2];
+    const int32_t* slots;
+    int rows, head_dim, block_size;
+    uint32_t block_magic;
+};
+
+__device__ __forceinline__ int slot_page(int slot, const ReadParams& P) {
+    int page = (int)__umulhi((uint32_t)slot, P.block_magic);  // the quotient or one less
+    return page + ((slot - page * P.block_size >= P.block_size) ? 1 : 0);
+}
+__device__ __forceinline__ const uint8_t* row_address(const ReadSide& S, const ReadParams& P, int slot, int head) {
+    const int page = slot_page(slot, P);
+    return reinterpret_cast<const uint8_t*>((uintptr_t)S.base) + (uint64_t)(uint32_t)page * S.page_stride + (uint64_t)(uint32_t)head * S.head_stride +
+           (uint64_t)(uint32_t)(slot - page * P.block_size) * S.token_stride;
+}
+// Lane l of a wave holds centroid l % 16; a code's low four bits pick one from the wave, all of whose lanes take part.
+__device__ __forceinline__ float lane_centroid() {
+    const int n = lane_id() & 15;
+    float c = kCentroids[0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) c = n == i ? kCentroids[i] : c;
+    return c;
+}
+__device__ __forceinline__ float centroid_of(float mine, uint32_t code) {
+    return __int_as_float(__builtin_amdgcn_ds_bpermute((int)(code & 15u) << 2, __float_as_int(mine)));
+}
+template <typename TOut>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+    return (uint32_t)TOut::from_f32(a) | (uint32_t)TOut::from_f32(b) << 16;
+}
+
+// Rows stored as they are: a thread takes eight elements of one row, head_dim / 8 threads a row.  blockIdx.y: the kv head,
+// blockIdx.z: K or V.  (No thread leaves before the end: the table of the centroids is spread over the lanes of a wave.)
+template <typename TOut>
+__global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, int first_side, int rows_per_block) {
+    const ReadSide& S = P.side[first_side + (int)blockIdx.z];
+    const int head = (int)blockIdx.y;
+    const int pieces = P.head_dim >> 3;
+    const int r = small_div((int)threadIdx.x, pieces), e = ((int)threadIdx.x - r * pieces) * 8;
+    const int64_t row = (int64_t)blockIdx.x * rows_per_block + r;
+    const int slot = r < rows_per_block && row < P.rows ? P.slots[row] : -1;
+    const bool live = slot >= 0;  // else: row untouched
+    const uint8_t* src = row_address(S, P, live ? slot : 0, head);
+    uint4 w = {0u, 0u, 0u, 0u};
+    if (S.format == WARP34_KV_FORMAT_FP16 || S.format == WARP34_KV_FORMAT_BF16) {
+        if (live) w = *reinterpret_cast<const uint4*>(src + 2 * e);
+        if (S.format != TOut::kStorageFormat) {
+            uint32_t* x = &w.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint16_t lo = (uint16_t)x[k], hi = (uint16_t)(x[k] >> 16);
+                x[k] = S.format == WARP34_KV_FORMAT_FP16 ? pack_out<TOut>(F16::to_f32(lo), F16::to_f32(hi))
+                                                         : pack_out<TOut>(BF16::to_f32(lo), BF16::to_f32(hi));
+            }
+        }
+    } else {
+        float v[8], d = 0.f;
+        if (S.format == WARP34_KV_FORMAT_TQ4) {  // blocks of 66 bytes: fp16 scale, 128 codes of four bits
+            uint32_t word = 0u;
+            if (live) {
+                const uint8_t* block = src + 66 * (e >> 7);
+                const uint16_t* codes = reinterpret_cast<const uint16_t*>(block + 2 + ((e & 127) >> 1));
+                word = (uint32_t)codes[0] | (uint32_t)codes[1] << 16;
+                d = F16::to_f32(*reinterpret_cast<const uint16_t*>(block));
+            }
+            const float mine = lane_centroid();
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = centroid_of(mine, word >> (4 * k));
+        } else {
+            uint32_t codes[2] = {0u, 0u};
+            const bool fp8 = S.format == WARP34_KV_FORMAT_FP8_E4M3;
+            if (live) {  // Q8_0: blocks of 68 bytes
+                const uint8_t* block = fp8 ? src : src + 68 * (e >> 6);
+                const uint32_t* at = reinterpret_cast<const uint32_t*>(fp8 ? src + e : block + 4 + (e & 63));
+                codes[0] = at[0], codes[1] = at[1];
+                d = *reinterpret_cast<const float*>(fp8 ? src + 256 + 4 * (e >> 7) : block);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t c = codes[k];
+                if (fp8) {
+                    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+                    v[4 * k] = a[0], v[4 * k + 1] = a[1], v[4 * k + 2] = b[0], v[4 * k + 3] = b[1];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[4 * k + i] = (float)(int8_t)(c >> (8 * i));
+                }
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] *= d;
+        w = uint4{pack_out<TOut>(v[0], v[1]), pack_out<TOut>(v[2], v[3]), pack_out<TOut>(v[4], v[5]), pack_out<TOut>(v[6], v[7])};
+    }
+    if (live) *reinterpret_cast<uint4*>(S.out + row * S.row_stride + (int64_t)head * P.head_dim + e) = w;
+}
+
+// Rotated rows of 256 elements, a wave a row, kReadRows rows at a time so that their loads travel together.  The transform is a
+// product of two 16 x 16 ones: with X[r][c] = x[16 r + c] and H[r][c] = (-1)^popcount(r & c), Y = H X H.  Two MFMAs do it:
+//   Z = X H      A = X (lane (n, b) holds X[n][4 b .. 4 b + 3], the elements it loads), B = H; lane (n, b) gets Z[4 b + i][n]
+//   Y^T = Z^T H  those registers are the A operand Z^T as they stand; lane (n, b) gets Y[n][4 b + i], the elements it stores
+// Operands have two fp16 parts in the halves of a 16x16x32 product (22 bits), so the result is as good as the 60 additions a row in
+// 32 bits that the MFMAs stand for.  X goes in relative to the row's largest block scale: whatever the scales, the parts stay
+// inside fp16's range.
+constexpr int kReadRows = 4;
+
+__device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
+    u4 r;
+    uint32_t hi, lo;
+    split_weights(x[0], x[1], hi, lo);
+    r[0] = hi, r[2] = lo;
+    split_weights(x[2], x[3], hi, lo);
+    r[1] = hi, r[3] = lo;
+    return __builtin_bit_cast(h8, r);
+}
+
+template <typename TOut, int FORMAT>
+__global__ __launch_bounds__(256) void kv_read_rotated_kernel(const ReadParams P, int first_side) {
+    const ReadSide& S = P.side[first_side + (int)blockIdx.z];
+    const int head = (int)blockIdx.y;
+    const int lane = lane_id();
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int n = lane & 15, b = lane >> 4, e = 16 * n + 4 * b;
+    const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * kReadRows;
+
+    uint32_t code[kReadRows];
+    uint32_t scale[kReadRows];
+    bool live[kReadRows];
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+        const int slot = row0 + k < P.rows ? P.slots[row0 + k] : -1;
+        live[k] = slot >= 0;
+        code[k] = scale[k] = 0u;
+        if (live[k]) {
+            const uint8_t* src = row_address(S, P, slot, head);
+            if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
+                const uint8_t* block = src + 66 * (e >> 7);
+                scale[k] = *reinterpret_cast<const uint16_t*>(block);
+                code[k] = *reinterpret_cast<const uint16_t*>(block + 2 + ((e & 127) >> 1));
+            } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
+                code[k] = *reinterpret_cast<const uint32_t*>(src + e);
+                scale[k] = *reinterpret_cast<const uint32_t*>(src + 256 + 4 * (e >> 7));
+            } else {
+                const uint8_t* block = src + 68 * (e >> 6);
+                code[k] = *reinterpret_cast<const uint32_t*>(block + 4 + (e & 63));
+                scale[k] = *reinterpret_cast<const uint32_t*>(block);
+            }
+        }
+    }
+    h8 had;
+    float sign[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        had[i] = had[4 + i] = (__builtin_popcount((unsigned)((4 * b + i) & n)) & 1) ? (_Float16)-1.0f : (_Float16)1.0f;
+        sign[i] = apply_sign(0.0625f, e + i);
+    }
+    const float mine = FORMAT == WARP34_KV_FORMAT_TQ4 ? lane_centroid() : 0.f;
+#pragma unroll
+    for (int k = 0; k < kReadRows; ++k) {
+        if (!live[k]) continue;  // the whole wave
+        float x[4], d;
+        if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
+            d = F16::to_f32((uint16_t)scale[k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = centroid_of(mine, code[k] >> (4 * i));
+        } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
+            d = __uint_as_float(scale[k]);
+            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[k], true);
+            x[0] = lo[0], x[1] = lo[1], x[2] = hi[0], x[3] = hi[1];
+        } else {
+            d = __uint_as_float(scale[k]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(code[k] >> (8 * i));
+        }
+        // the largest scale of the row: the blocks' lanes differ in bit 3 of n, for Q8_0 in bit 2 as well
+        float top = fabsf(d);
+        top = fmaxf(top, lane_xor<8>(top, lane));
+        if constexpr (FORMAT == WARP34_KV_FORMAT_Q8_0) top = fmaxf(top, lane_xor<4>(top, lane));
+        const float share = top > 0.f ? d * (1.0f / top) : 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[i] *= share;
+            asm("" : "+v"(x[i]));  // both parts are taken from the product rounded to 32 bits
+        }
+        const f4 none = {0.f, 0.f, 0.f, 0.f};
+        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(x), had, none, 0, 0, 0);
+        const float zs[4] = {z[0], z[1], z[2], z[3]};
+        const f4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(zs), had, none, 0, 0, 0);
+        uint2 w;
+        w.x = pack_out<TOut>(y[0] * top * sign[0], y[1] * top * sign[1]);
+        w.y = pack_out<TOut>(y[2] * top * sign[2], y[3] * top * sign[3]);
+        *reinterpret_cast<uint2*>(S.out + (row0 + k) * S.row_stride + (int64_t)head * 256 + e) = w;
+    }
+}
+
+static bool rotated_rows(int format, int transform, int head_dim) {
+    return transform == WARP34_KV_TRANSFORM_RADEMACHER_WHT256 && head_dim == 256 && (format == WARP34_KV_FORMAT_TQ4 || is_8bit_format(format));
+}
+
+// 16-bit rows are loaded 16 bytes at a time, the parts of the others by what their elements are aligned to
+static bool rows_aligned_for_read(int format, uint64_t strides_and_base) {
+    const unsigned mask = format == WARP34_KV_FORMAT_TQ4 ? 1u : is_8bit_format(format) ? 3u : 15u;
+    return (strides_and_base & mask) == 0;
+}
+
+template <typename TOut>
+static int kv_read_entry(const warp34_exec* ex, const warp34_kv_layer_layout* l, const int32_t* slots, int num_rows, void* k_out, void* v_out,
+                         int k_row_stride, int v_row_stride) {
+    if (!ex || !l || (!k_out && !v_out)) return (int)hipErrorInvalidValue;
+    if (num_rows <= 0 || l->local_kv_heads <= 0) return 0;
+    if (!slots || l->block_size <= 0 || l->head_dim <= 0 || l->head_dim > 256 || l->local_kv_heads > 65535) return (int)hipErrorInvalidValue;
+    const int64_t min_stride = (int64_t)l->local_kv_heads * l->head_dim;
+    ReadParams P{};
+    P.slots = slots;
+    P.rows = num_rows;
+    P.head_dim = l->head_dim;
+    P.block_size = l->block_size;
+    P.block_magic = block_magic_for(l->block_size);
+    P.side[0] = ReadSide{l->k_base, l->k_page_stride_bytes, l->k_head_stride_bytes, l->k_token_stride_bytes, (uint16_t*)k_out, k_row_stride, l->k_format};
+    P.side[1] = ReadSide{l->v_base, l->v_page_stride_bytes, l->v_head_stride_bytes, l->v_token_stride_bytes, (uint16_t*)v_out, v_row_stride, l->v_format};
+    const int transforms[2] = {l->k_transform, l->v_transform};
+    for (const ReadSide& S : P.side) {
+        if (!S.out) continue;
+        if (!S.base || S.row_stride < min_stride) return (int)hipErrorInvalidValue;
+        if (!format_supported_for_write(S.format, transforms[&S - P.side], l->head_dim) || (l->head_dim & 7) != 0 ||
+            !rows_aligned_for_read(S.format, S.base | S.page_stride | S.head_stride | S.token_stride) || (((uintptr_t)S.out) & 15u) != 0 ||
+            (S.row_stride & 7) != 0) {
+            return (int)hipErrorNotSupported;
+        }
+    }
+    const bool rotated[2] = {rotated_rows(l->k_format, l->k_transform, l->head_dim), rotated_rows(l->v_format, l->v_transform, l->head_dim)};
+    const int rows_per_block = 256 / (l->head_dim >> 3);
+    const auto blocks = [&](int per_block) { return (unsigned)(((int64_t)num_rows + per_block - 1) / per_block); };
+    const unsigned heads = (unsigned)l->local_kv_heads;
+    const auto launch = [&](int first, int sides) {
+        hipStream_t stream = (hipStream_t)ex->stream;
+        if (!rotated[first]) {
+            hipLaunchKernelGGL((kv_read_plain_kernel<TOut>), dim3(blocks(rows_per_block), heads, (unsigned)sides), dim3(256), 0, stream, P, first,
+                               rows_per_block);
+            return;
+        }
+        const dim3 grid(blocks(4 * kReadRows), heads, (unsigned)sides);
+        if (P.side[first].format == WARP34_KV_FORMAT_TQ4) {
+            hipLaunchKernelGGL((kv_read_rotated_kernel<TOut, WARP34_KV_FORMAT_TQ4>), grid, dim3(256), 0, stream, P, first);
+        } else if (P.side[first].format == WARP34_KV_FORMAT_FP8_E4M3) {
+            hipLaunchKernelGGL((kv_read_rotated_kernel<TOut, WARP34_KV_FORMAT_FP8_E4M3>), grid, dim3(256), 0, stream, P, first);
+        } else {
+            hipLaunchKernelGGL((kv_read_rotated_kernel<TOut, WARP34_KV_FORMAT_Q8_0>), grid, dim3(256), 0, stream, P, first);
+        }
+    };
+    const bool together = k_out && v_out && rotated[0] == rotated[1] && (!rotated[0] || l->k_format == l->v_format);
+    if (together) {
+        launch(0, 2);
+    } else {
+        if (k_out) launch(0, 1);
+        if (v_out) launch(1, 1);
+    }
+    return (int)hipGetLastError();
+}
+
+}  // namespace w34
+
+using namespace w34;
+
+extern "C" int warp34_kv_cache_read_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const int32_t* slot_mapping, int num_rows,
+                                        void* k_out, void* v_out, int k_row_stride, int v_row_stride) {
+    return kv_read_entry<F16>(ex, layout, slot_mapping, num_rows, k_out, v_out, k_row_stride, v_row_stride);
+}
+extern "C" int warp34_kv_cache_read_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout, const int32_t* slot_mapping, int num_rows,
+                                         void* k_out, void* v_out, int k_row_stride, int v_row_stride) {
+    return kv_read_entry<BF16>(ex, layout, slot_mapping, num_rows, k_out, v_out, k_row_stride, v_row_stride);
+}

@@ -104,6 +104,16 @@ SIGNATURES = {
     "warp34_kv_cache_write_strided": (C.c_int, [_EX, _LAY, _BAT, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "warp34_kv_cache_write_bf16": (C.c_int, [_EX, _LAY, _BAT, C.c_void_p, C.c_void_p]),
     "warp34_kv_cache_write_strided_bf16": (C.c_int, [_EX, _LAY, _BAT, C.c_void_p, C.c_void_p, C.c_int]),
+    # (exec, layout, slot_mapping, num_rows, k_out, v_out, k_row_stride, v_row_stride)
+    "warp34_kv_cache_read_f16":
+        (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    "warp34_kv_cache_read_bf16":
+        (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    # (exec, parts, lse_parts, num_parts, part_stride, lse_part_stride, out, lse_out, num_rows, head_dim)
+    "warp34_attention_merge_f16":
+        (C.c_int, [_EX, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int]),
+    "warp34_attention_merge_bf16":
+        (C.c_int, [_EX, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int]),
     "warp34_paged_attention_f16": (C.c_int, [_EX, _LAY, _BAT, C.c_void_p, C.c_void_p, C.c_int]),
     "warp34_paged_attention_bf16": (C.c_int, [_EX, _LAY, _BAT, C.c_void_p, C.c_void_p, C.c_int]),
     "warp34_paged_attention_f16_force_kernel_for_test":
