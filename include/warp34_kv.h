@@ -117,11 +117,24 @@ typedef struct {
     int32_t        reserved;
 } warp34_attention_batch;
 
+/* What warp34_paged_attention_scored_* adds to an attention batch (no counterpart in the reference) -- 40 bytes.
+ * The pointers are DEVICE pointers and may be NULL. */
+typedef struct {
+    const float*   distance_slopes; /* [num_q_heads]: the score falls by slope * |position of the token - of the key| */
+    const int32_t* document_starts; /* [total_tokens]: keys before this position are hidden from the token */
+    const int32_t* prefix_ends;     /* [total_tokens]: keys before this position are seen though they come after the token */
+    float*         lse_out;         /* [total_tokens, num_q_heads]: natural logarithm of the row's sum of exponentials */
+    float          softcap;         /* cap > 0: scores become cap * tanh(score / cap); 0: none */
+    int32_t        reserved;
+} warp34_attention_scores;
+
 #if defined(__cplusplus)
+static_assert(sizeof(warp34_attention_scores) == 40, "warp34_attention_scores ABI size");
 static_assert(sizeof(warp34_exec) == 32, "warp34_exec ABI size");
 static_assert(sizeof(warp34_kv_layer_layout) == 104, "warp34_kv_layer_layout ABI size");
 static_assert(sizeof(warp34_attention_batch) == 96, "warp34_attention_batch ABI size");
 #else
+_Static_assert(sizeof(warp34_attention_scores) == 40, "warp34_attention_scores ABI size");
 _Static_assert(sizeof(warp34_exec) == 32, "warp34_exec ABI size");
 _Static_assert(sizeof(warp34_kv_layer_layout) == 104, "warp34_kv_layer_layout ABI size");
 _Static_assert(sizeof(warp34_attention_batch) == 96, "warp34_attention_batch ABI size");
@@ -301,6 +314,29 @@ int warp34_apply_attn_output_gate_f16(const warp34_exec* ex, const void* attn_ou
 int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
                                      const warp34_attention_batch* batch, const void* q_in,
                                      const void* gate, void* attn_out, int num_q_heads);
+
+/* Paged attention with score terms and masks for each token (no counterpart in the reference):
+ *   x(t, k) = sm_scale * q_t . k_k;  softcap > 0: x = softcap * tanh(x / softcap);  x -= slope[head] * |pos_t - k|
+ *   keys of token t: [max(min_kv, document_starts[t]), max(max_kv, prefix_ends[t] - 1)], the latter clamped to
+ *   seq_after - 1, with min_kv and max_kv of warp34_paged_attention_*
+ *   out = softmax(x) V,  lse = ln sum_k exp(x); a token without keys gives zeros and minus infinity
+ * Packed documents are document_starts, prompts that open with a part that is seen both ways are prefix_ends,
+ * score caps are softcap, heads that look near first are distance_slopes; lse_out is what
+ * warp34_attention_merge_* joins such results by.  Layouts, batches, q_in / attn_out, masked tokens and requests
+ * (their lse_out stays untouched as well) and alignments are those of warp34_paged_attention_*.  Key and value
+ * rows that a token sees must be finite, and what their decoded values are must fit fp16 for the quantised formats;
+ * rows that no token of the request sees may hold anything.  softcap must be finite and not negative
+ * (hipErrorInvalidValue).  Scratch as for the other attention calls, of the size
+ * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass, in another order of
+ * summation. */
+int warp34_paged_attention_scored_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
+                                      const warp34_attention_batch* batch, const warp34_attention_scores* scores,
+                                      const void* q_in, void* attn_out, int num_q_heads);
+int warp34_paged_attention_scored_bf16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
+                                       const warp34_attention_batch* batch, const warp34_attention_scores* scores,
+                                       const void* q_in, void* attn_out, int num_q_heads);
+size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_layer_layout* layout, int num_reqs, int total_tokens,
+                                                   int max_q_len, int num_q_heads);
 
 /* Attention results over disjoint key sets joined by the natural logarithms of their sums (a shared
  * prefix and a private rest, keys spread over ranks): lse = ln sum_p exp(lse_p), out = sum_p

@@ -56,3 +56,67 @@ def slab_rows(slab, pool, slots):
     base = page * pool.page + at * pool.tok
     where = base[:, None, None] + np.arange(pool.kv_heads)[None, :, None] * pool.head + np.arange(pool.tok)[None, None, :]
     return slab[where]
+
+
+def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, window=0, noncausal=False, documents=None, prefixes=None,
+                     scale=None, dt=DT_BF16):
+    """Scored attention of q (float64 [tokens, heads, head_dim]) over a HostPool's pages, in float64.
+
+    Returns (out, lse, out_bound, lse_bound).  The bounds are what 16-bit operands and 32-bit sums may do, worst case:
+      score    the products are summed in 32 bits (2^-20 of sum |q_i k_i|), the terms are rounded a few times (2^-20 of their sizes);
+               TQ4 keys come from a table of fp16 numbers within 9.4e-5 of the centroids: that much of sum |q_i k_i| in the stored domain
+      weight   two 16-bit parts: 2^-21 (fp16), 2^-16 (bf16); with an error d_k of a score, a weight p_k moves by p_k (d_k + sum p d)
+      value    TQ4: 9.4e-5 of each stored element, which the rotation back adds up with 1 / 16
+      output   half a step."""
+    fmt, hd, kvh, bs = pool.fmt, pool.head_dim, pool.kv_heads, pool.block_size
+    heads = q.shape[1]
+    scale = hd ** -0.5 if scale is None else scale
+    rot_k = pool.transform == XF_WHT256 and fmt not in (FMT_FP16, FMT_BF16)
+    out, lse = np.zeros(q.shape), np.full(q.shape[:2], -np.inf)
+    out_bound, lse_bound = np.zeros(q.shape), np.zeros(q.shape[:2])
+    table = 9.4e-5 if fmt == FMT_TQ4 else 0.0
+    weight = 2.0 ** -16 if fmt == FMT_BF16 else 2.0 ** -21
+    for r, s in enumerate(seqs):
+        slots = oracle.slot_mapping(bt[r], 0, s, bs) if s else np.zeros(0, dtype=np.int64)
+        kb, vb = slab_rows(pool.k, pool, slots), slab_rows(pool.v, pool, slots)
+        ks = stored_rows(kb, fmt, hd)
+        k, v = decoded_rows(kb, fmt, pool.transform, hd), decoded_rows(vb, fmt, pool.v_transform, hd)
+        v_sum = np.abs(stored_rows(vb, fmt, hd)).sum(-1) / 16.0
+        pos = np.arange(qsl[r + 1] - qsl[r]) + ctx[r]
+        key = np.arange(s)
+        for t in range(qsl[r], qsl[r + 1]):
+            p_t = pos[t - qsl[r]]
+            hi = s - 1 if noncausal else p_t
+            if prefixes is not None:
+                hi = max(hi, prefixes[t] - 1)
+            hi = min(hi, s - 1)
+            lo = max(0, p_t - window + 1) if window else 0
+            if documents is not None:
+                lo = max(lo, documents[t])
+            if lo > hi:
+                continue
+            seen = slice(lo, hi + 1)
+            for h in range(heads):
+                g = h // (heads // kvh)
+                qs = q[t, h]
+                if rot_k:
+                    qs = (qs * oracle.signs()) @ _hadamard()
+                raw = (k[seen, g] @ q[t, h]) * scale
+                size = (np.abs(ks[seen, g]) @ np.abs(qs)) * abs(scale)
+                x = cap * np.tanh(raw / cap) if cap else raw
+                far = slopes[h] * np.abs(p_t - key[seen]) if slopes is not None else np.zeros_like(x)
+                d = size * (2.0 ** -20 + table) + 2.0 ** -20 * (np.abs(x) + np.abs(far) + cap)
+                x = x - far
+                top = x.max()
+                p = np.exp(x - top)
+                total = p.sum()
+                p = p / total
+                lse[t, h] = top + np.log(total)
+                out[t, h] = p @ v[seen, g]
+                mean = p @ d
+                moved = p * (d + mean + weight)
+                lse_bound[t, h] = mean + 2.0 ** -20 * (np.abs(lse[t, h]) + np.abs(top) + 1)
+                out_bound[t, h] = moved @ np.abs(v[seen, g]) + HALF_STEP[dt] * np.abs(out[t, h]) + HALF_TINY[dt]
+                if fmt == FMT_TQ4:
+                    out_bound[t, h] += table * (p @ v_sum[seen, g])
+    return out, lse, out_bound, lse_bound

@@ -30,6 +30,7 @@ SOURCES = [
     (os.path.join(CSRC, "attn_output_gate.hip"), ["-ffp-contract=off"]),
     (os.path.join(CSRC, "fused_qk_norm.hip"), ["-ffp-contract=off"] + PRELOAD),
     (os.path.join(CSRC, "paged_attn.hip"), PRELOAD),
+    (os.path.join(CSRC, "scored_attn.hip"), PRELOAD),
     (os.path.join(CSRC, "kv_read.hip"), []),
     (os.path.join(CSRC, "attention_merge.hip"), []),
     (os.path.join(CSRC, "runtime.hip"), []),

@@ -43,6 +43,7 @@
 #include <type_traits>
 
 #include "attn_lanes.h"
+#include "attn_launch.h"
 
 namespace w34 {
 
@@ -204,7 +205,6 @@ __device__ __forceinline__ int div_block(int pos, const AttnParams& P) {
 __device__ __forceinline__ int div_q_group(int col, const AttnParams& P) {
     return (int)(((uint32_t)col * P.q_group_magic) >> 16);
 }
-__host__ inline uint32_t q_group_magic_for(int q_group) { return (65536u + (uint32_t)q_group - 1u) / (uint32_t)q_group; }
 
 struct ChunkGeom {
     int u_first, n_units, upc, n_chunks;
@@ -2340,48 +2340,6 @@ static int choose_max_chunks(const warp34_exec* ex, int total_tokens, int num_q_
         want = std::max(want, (int)std::min<long long>(fit, one_round(tiles, kv_subs)));
     }
     return want < 2 ? 1 : want;
-}
-
-// One attribute call per kernel instantiation and device.  The record is process-wide and
-// lock-free: slot i belongs to the first kernel that claims it, bit d of its mask says that
-// device d is configured.  Kernels that address their dequantisation table absolutely
-// (lds_base_zero) also have their static LDS size checked here: it must be zero, so that the
-// dynamic block starts at LDS address 0.
-constexpr int kLdsRecordSlots = 128;
-static std::atomic<const void*> g_lds_fn[kLdsRecordSlots];
-static std::atomic<unsigned long long> g_lds_devs[kLdsRecordSlots];
-
-template <typename KernelT>
-static int ensure_dynamic_lds(KernelT kernel, int bytes, bool lds_base_zero = false) {
-    int dev = 0;
-    hipError_t rc = hipGetDevice(&dev);
-    if (rc != hipSuccess) return (int)rc;
-    const void* fn = (const void*)kernel;
-    int slot = -1;
-    for (int i = 0; i < kLdsRecordSlots; ++i) {
-        const void* cur = g_lds_fn[i].load(std::memory_order_acquire);
-        if (cur == nullptr) {
-            const void* expect = nullptr;
-            if (g_lds_fn[i].compare_exchange_strong(expect, fn, std::memory_order_acq_rel)) cur = fn;
-            else cur = expect;
-        }
-        if (cur == fn) {
-            slot = i;
-            break;
-        }
-    }
-    const bool tracked = slot >= 0 && dev >= 0 && dev < 64;
-    if (tracked && ((g_lds_devs[slot].load(std::memory_order_acquire) >> dev) & 1ull)) return 0;
-    if (lds_base_zero) {
-        hipFuncAttributes attr;
-        rc = hipFuncGetAttributes(&attr, fn);
-        if (rc != hipSuccess) return (int)rc;
-        if (attr.sharedSizeBytes != 0) return (int)hipErrorInvalidConfiguration;
-    }
-    rc = hipFuncSetAttribute(fn, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (rc != hipSuccess) return (int)rc;
-    if (tracked) g_lds_devs[slot].fetch_or(1ull << dev, std::memory_order_release);
-    return 0;
 }
 
 // Decode batches of several requests take the balanced path: no request has more than one

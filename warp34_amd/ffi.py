@@ -85,6 +85,20 @@ class Warp34AttentionBatch(C.Structure):
     ]
 
 
+class Warp34AttentionScores(C.Structure):
+    """What warp34_paged_attention_scored_* adds to a batch: device pointers (None: not used) and the cap."""
+
+    _fields_ = [
+        ("distance_slopes", C.c_void_p),
+        ("document_starts", C.c_void_p),
+        ("prefix_ends", C.c_void_p),
+        ("lse_out", C.c_void_p),
+        ("softcap", C.c_float),
+        ("reserved", C.c_int32),
+    ]
+
+
+assert C.sizeof(Warp34AttentionScores) == 40
 assert C.sizeof(Warp34Exec) == 32
 assert C.sizeof(Warp34KvLayerLayout) == 104
 assert C.sizeof(Warp34AttentionBatch) == 96
@@ -92,6 +106,7 @@ assert C.sizeof(Warp34AttentionBatch) == 96
 _EX = C.POINTER(Warp34Exec)
 _LAY = C.POINTER(Warp34KvLayerLayout)
 _BAT = C.POINTER(Warp34AttentionBatch)
+_SCO = C.POINTER(Warp34AttentionScores)
 
 # name -> (restype, argtypes); every symbol the headers under include/ declare
 SIGNATURES = {
@@ -109,6 +124,10 @@ SIGNATURES = {
         (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "warp34_kv_cache_read_bf16":
         (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    "warp34_paged_attention_scored_f16": (C.c_int, [_EX, _LAY, _BAT, _SCO, C.c_void_p, C.c_void_p, C.c_int]),
+    "warp34_paged_attention_scored_bf16": (C.c_int, [_EX, _LAY, _BAT, _SCO, C.c_void_p, C.c_void_p, C.c_int]),
+    # (layout, num_reqs, total_tokens, max_q_len, num_q_heads)
+    "warp34_paged_attention_scored_scratch_bytes": (C.c_size_t, [_LAY, C.c_int, C.c_int, C.c_int, C.c_int]),
     # (exec, parts, lse_parts, num_parts, part_stride, lse_part_stride, out, lse_out, num_rows, head_dim)
     "warp34_attention_merge_f16":
         (C.c_int, [_EX, C.c_void_p, C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int]),
