@@ -64,7 +64,7 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
 
     Returns (out, lse, out_bound, lse_bound).  The bounds are what 16-bit operands and 32-bit sums may do, worst case:
       score    the products are summed in 32 bits (2^-20 of sum |q_i k_i|), the terms are rounded a few times (2^-20 of their sizes);
-               TQ4 keys come from a table of fp16 numbers within 9.4e-5 of the centroids: that much of sum |q_i k_i| in the stored domain
+               rotated queries and TQ4 keys have two fp16 parts, 2^-21 of them missing: of sum |q_i k_i| in the stored domain
       weight   two 16-bit parts: 2^-21 (fp16), 2^-16 (bf16); with an error d_k of a score, a weight p_k moves by p_k (d_k + sum p d)
       value    TQ4: 9.4e-5 of each stored element, which the rotation back adds up with 1 / 16
       output   half a step."""
@@ -105,7 +105,7 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                 size = (np.abs(ks[seen, g]) @ np.abs(qs)) * abs(scale)
                 x = cap * np.tanh(raw / cap) if cap else raw
                 far = slopes[h] * np.abs(p_t - key[seen]) if slopes is not None else np.zeros_like(x)
-                d = size * (2.0 ** -20 + table) + 2.0 ** -20 * (np.abs(x) + np.abs(far) + cap)
+                d = size * (2.0 ** -20 + 2.0 ** -20) + 2.0 ** -20 * (np.abs(x) + np.abs(far) + cap)
                 x = x - far
                 top = x.max()
                 p = np.exp(x - top)

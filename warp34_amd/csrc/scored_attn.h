@@ -128,7 +128,7 @@ __device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
 // The cut of a batch: chunks of `per` half units, the shortest length with which all tiles together need no more than P.target chunks;
 // a live tile has at least one.  halves: [entries] in LDS, -1 for tiles without tokens.
 constexpr int kMinHalvesPerChunk = 8;   // one for each wave of a decode workgroup
-constexpr int kMaxSplitEntries = 8192;  // entries of a batch that is split
+constexpr int kMaxSplitEntries = 512;   // entries of a batch that is split
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
 __device__ __forceinline__ int chunk_length(const ScoredParams& P, const int* halves, int lane) {
     int total = 0, live = 0, longest = 0;

@@ -23,6 +23,35 @@ typedef u2v u2_at4 __attribute__((aligned(4)));
 
 constexpr int kScoredWaves = 8;
 
+// TQ4 keys: the look-ups' fp16 numbers are up to 9.4e-5 from the centroids, which would be 1e-4 of a score and 2e-5 of a row's lse where a
+// few keys carry it.  So the keys have a table of their own behind the other, entries of eight bytes: the pair of the first table and the
+// pair of what is missing, 32 copies (a read of eight bytes goes by 32 lanes at a time).
+constexpr int kKeyTable = 65536;
+__host__ __device__ constexpr uint32_t centroid_rest_of(int code) {
+    return __builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[code] - (float)(_Float16)(kLutGain * kCentroids[code])));
+}
+__device__ __forceinline__ uint32_t centroid_rest(uint32_t code) {
+    uint32_t r = centroid_rest_of(0);
+#pragma unroll
+    for (int c = 1; c < 16; ++c) r = code == (uint32_t)c ? centroid_rest_of(c) : r;
+    return r;
+}
+__device__ __forceinline__ void build_key_table(uint8_t* smem, int tid, int wave) {  // by 512 threads, as build_pair_table
+    const uint32_t code = (uint32_t)tid >> 4 & 15u, lo = centroid_bits(code), lo_rest = centroid_rest(code);
+    const bool odd = (wave >> 2) != 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t v = lo | (odd ? centroid_bits_of(2 * i + 1) << 16 : centroid_bits_of(2 * i) << 16);
+        const uint32_t w = lo_rest | (odd ? centroid_rest_of(2 * i + 1) << 16 : centroid_rest_of(2 * i) << 16);
+        *reinterpret_cast<u4*>(smem + kKeyTable + (tid + 512 * i) * 16) = u4{v, w, v, w};
+    }
+}
+typedef __attribute__((address_space(3))) const u2v lds_cu2;
+// lane_bits: (lane % 32) * 8 | 0x100, whose second byte is the table's place
+__device__ __forceinline__ u2v key_read(uint32_t code_word, uint32_t lane_bits, int byte) {
+    return *reinterpret_cast<lds_cu2*>((uintptr_t)__builtin_amdgcn_perm(code_word, lane_bits, 0x0c010400u + ((uint32_t)byte << 8)));
+}
+
 template <typename T>
 __device__ __forceinline__ T load_as(const uint8_t* p) { return *reinterpret_cast<const T*>(p); }
 
@@ -59,13 +88,14 @@ struct ScoredRows {
     }
 };
 
-// LDS: [TQ4 table][tile counts | query columns | waves' regions and joined columns][(m, l) of the waves][scales of the waves]
+// LDS: [TQ4 tables][query columns][tile counts], over which the waves' regions and the joined columns lie at the end; [(m, l) of the
+// waves][scales of the waves]
 template <int KVF, int HD>
 struct ScoredLds {
     using R = ScoredRows<KVF, HD>;
     static constexpr int kColStride = HD + 8;                     // floats of a column in a region
     static constexpr int kRegion = 16 * kColStride * 4;
-    static constexpr int kTable = R::kTq4 ? 65536 : 0;
+    static constexpr int kTable = R::kTq4 ? 2 * kKeyTable : 0;
     static constexpr int kQStride = HD + 8;                       // 16-bit elements
     static constexpr int kQ = kTable, kQLow = kQ + 16 * kQStride * 2, kQScale = kQLow + 16 * kQStride * 2;
     static constexpr int kCounts = kQScale + 64;                  // entries x 4 bytes
@@ -144,7 +174,10 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     const bool sloped = P.slopes != nullptr;
 
     // ---- TQ4 table, query operands ----
-    if constexpr (R::kTq4) build_pair_table(smem, tid, wave);
+    if constexpr (R::kTq4) {
+        build_pair_table(smem, tid, wave);
+        build_key_table(smem, tid, wave);
+    }
     u4 q_high[R::kOps], q_low[R::kOps];
     float cs = P.scale2, cc = P.cap_arg;
     if constexpr (R::k16) {
@@ -281,7 +314,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         __builtin_amdgcn_wave_barrier();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
     };
-    const uint32_t lut_lane = (uint32_t)lane << 2;
+    const uint32_t lut_lane = (uint32_t)lane << 2, key_lane = ((uint32_t)lane & 31u) << 3 | 0x100u;
 
     f4 o[R::kGroups * R::kJ];
 #pragma unroll
@@ -313,11 +346,15 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 #pragma unroll
                 for (int mm = 0; mm < kPerBlock; ++mm) {
                     const int m = blk * kPerBlock + mm;
-                    u4 a;
+                    u4 a, rest;
                     if constexpr (R::kTq4) {
                         const uint32_t word = kr[m >> 2][m & 3];
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) a[k] = lut_read(word, lut_lane, 0x0c0c0400u + ((uint32_t)k << 8));
+                        for (int k = 0; k < 4; ++k) {
+                            const u2v pair = key_read(word, key_lane, k);
+                            a[k] = pair[0];
+                            rest[k] = pair[1];
+                        }
                     } else {
 #pragma unroll
                         for (int w = 0; w < 2; ++w) {
@@ -337,6 +374,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
                         }
                     }
                     part = mfma_rows<false>(a, q_high[m], part);
+                    if constexpr (R::kTq4) part = mfma_rows<false>(rest, q_high[m], part);
                     if (two_parts) part = mfma_rows<false>(a, q_low[m], part);
                 }
                 const f4 d = *reinterpret_cast<const f4*>(scale_area + 16 * blk + 4 * b);
