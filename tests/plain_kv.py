@@ -59,7 +59,7 @@ def slab_rows(slab, pool, slots):
 
 
 def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, window=0, noncausal=False, documents=None, prefixes=None,
-                     scale=None, dt=DT_BF16):
+                     scale=None, dt=DT_BF16, chunk=False):
     """Scored attention of q (float64 [tokens, heads, head_dim]) over a HostPool's pages, in float64.
 
     Returns (out, lse, out_bound, lse_bound).  The bounds are what 16-bit operands and 32-bit sums may do, worst case:
@@ -67,7 +67,13 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                rotated queries and TQ4 keys have two fp16 parts, 2^-21 of them missing: of sum |q_i k_i| in the stored domain
       weight   two 16-bit parts: 2^-21 (fp16), 2^-16 (bf16); with an error d_k of a score, a weight p_k moves by p_k (d_k + sum p d)
       value    TQ4: 9.4e-5 of each stored element, which the rotation back adds up with 1 / 16
-      output   half a step."""
+      small    fp16 weights have an absolute error of 2^-25 as well (half the distance of fp16's smallest numbers), relative to the
+               row's largest, which is 1, and so its sum at least 1: 2^-25 of each |v_k| over that sum.  Where block scales ride on
+               the weights it is 2^-25 of the largest code (in the units of the weights: TQ4 0.17, E4M3 448 / 256, Q8_0 127 / 128),
+               which the rotation back adds up to 16 times that.  Values of their own below 2^-14: 2^-25 once more
+      output   half a step.
+    chunk: the call's chunk kernel, whose rotated queries and TQ4 keys are one fp16 part (2^-11 and 9.4e-5 of sum |q_i k_i|) and whose
+    weights are one 16-bit part over 16-bit rows (half a step) and over 8-bit rows as they are (and so are those values)."""
     fmt, hd, kvh, bs = pool.fmt, pool.head_dim, pool.kv_heads, pool.block_size
     heads = q.shape[1]
     scale = hd ** -0.5 if scale is None else scale
@@ -76,6 +82,16 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
     out_bound, lse_bound = np.zeros(q.shape), np.zeros(q.shape[:2])
     table = 9.4e-5 if fmt == FMT_TQ4 else 0.0
     weight = 2.0 ** -16 if fmt == FMT_BF16 else 2.0 ** -21
+    operand = 2.0 ** -20
+    if chunk:
+        operand = (2.0 ** -11 if rot_k else 0.0) + table
+        if fmt in (FMT_FP16, FMT_BF16):
+            weight = HALF_STEP[dt]
+        elif fmt != FMT_TQ4 and pool.v_transform != XF_WHT256:
+            weight = 2.0 ** -10
+    ride = {FMT_TQ4: 0.17, FMT_FP8: 1.75, FMT_Q8_0: 1.0}.get(fmt, 0.0) * (16.0 if pool.v_transform == XF_WHT256 else 1.0)
+    if chunk and fmt in (FMT_FP8, FMT_Q8_0) and pool.v_transform != XF_WHT256:
+        ride = 0.0
     for r, s in enumerate(seqs):
         slots = oracle.slot_mapping(bt[r], 0, s, bs) if s else np.zeros(0, dtype=np.int64)
         kb, vb = slab_rows(pool.k, pool, slots), slab_rows(pool.v, pool, slots)
@@ -105,11 +121,12 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                 size = (np.abs(ks[seen, g]) @ np.abs(qs)) * abs(scale)
                 x = cap * np.tanh(raw / cap) if cap else raw
                 far = slopes[h] * np.abs(p_t - key[seen]) if slopes is not None else np.zeros_like(x)
-                d = size * (2.0 ** -20 + 2.0 ** -20) + 2.0 ** -20 * (np.abs(x) + np.abs(far) + cap)
+                d = size * (2.0 ** -20 + operand) + 2.0 ** -20 * (np.abs(x) + np.abs(far) + cap)
                 x = x - far
                 top = x.max()
                 p = np.exp(x - top)
                 total = p.sum()
+                small = 2.0 ** -25 * (ride * p.size if ride else np.abs(v[seen, g]).sum(0)) / total + 2.0 ** -25
                 p = p / total
                 lse[t, h] = top + np.log(total)
                 out[t, h] = p @ v[seen, g]
@@ -117,6 +134,8 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                 moved = p * (d + mean + weight)
                 lse_bound[t, h] = mean + 2.0 ** -20 * (np.abs(lse[t, h]) + np.abs(top) + 1)
                 out_bound[t, h] = moved @ np.abs(v[seen, g]) + HALF_STEP[dt] * np.abs(out[t, h]) + HALF_TINY[dt]
+                if fmt != FMT_BF16:
+                    out_bound[t, h] += small
                 if fmt == FMT_TQ4:
                     out_bound[t, h] += table * (p @ v_sum[seen, g])
     return out, lse, out_bound, lse_bound

@@ -8,6 +8,7 @@ from oracle import DT_BF16
 from plain_kv import scored_attention
 
 SENTINEL = 0x5500
+CHUNK_FROM = 128  # query columns of a request from which the call takes its chunk kernel
 
 
 def scores_struct(G, cap=0.0, slopes=None, documents=None, prefixes=None, lse=None):
@@ -56,8 +57,11 @@ def check_scored(pool, bt, seqs, q, dt, aq, ctx, heads, *, hb=None, scratch=8 <<
         hb = oracle.HostBatch(aq, seqs, bt, context_lens_before=ctx)
     hb.sliding_window, hb.mask_mode = kinds["window"], 1 if kinds["noncausal"] else 0
     bits, lse = run_scored(pool, hb, q, dt, heads, scratch=scratch, with_lse=with_lse, max_q_len=max_q_len, max_seq_len=max_seq_len, **terms)
+    longest = int(np.diff(hb.qsl).max()) if max_q_len is None else max_q_len
+    group = next(d for d in range(min(16, heads // pool.kv_heads), 0, -1) if heads // pool.kv_heads % d == 0)
+    chunk = (longest if longest > 0 else hb.total_tokens) * group >= CHUNK_FROM
     want, want_lse, bound, lse_bound = scored_attention(pool, bt, seqs, oracle.bits_to_f32(q, dt).astype(np.float64), aq, ctx,
-                                                        scale=hb.sm_scale, dt=dt, **kinds, **terms)
+                                                        scale=hb.sm_scale, dt=dt, chunk=chunk, **kinds, **terms)
     rows = np.ones(hb.total_tokens, dtype=bool) if rows is None else np.asarray(rows, dtype=bool)
     got = oracle.bits_to_f32(bits, dt).astype(np.float64)
     assert (bits[~rows] == SENTINEL).all()

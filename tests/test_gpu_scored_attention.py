@@ -9,7 +9,7 @@ import oracle
 from cases import make_case
 from oracle import DT_BF16, DT_F16, FMT_BF16, FMT_FP16, FMT_FP8, FMT_Q8_0, FMT_TQ4, XF_IDENTITY, XF_WHT256
 from plain_kv import scored_attention
-from scored_harness import SENTINEL, check_scored, run_scored, scores_struct
+from scored_harness import CHUNK_FROM, SENTINEL, check_scored, run_scored, scores_struct
 
 gpu = pytest.mark.gpu
 FORMS = [(FMT_TQ4, XF_WHT256, XF_WHT256, DT_F16, 256), (FMT_TQ4, XF_WHT256, XF_WHT256, DT_BF16, 256),
@@ -156,7 +156,7 @@ def test_what_unseen_rows_hold_does_not_matter(fmt, dt, qs):
         for h in range(pool.kv_heads):
             s[:, h][w] = 0
     want, want_lse, bound, lse_bound = scored_attention(pool, bt, [seq], oracle.bits_to_f32(q, dt).astype(np.float64), aq, ctx, cap=30.0,
-                                                        window=40, scale=hb.sm_scale, dt=dt)
+                                                        window=40, scale=hb.sm_scale, dt=dt, chunk=qs[0] * 4 >= CHUNK_FROM)
     got = oracle.bits_to_f32(bits, dt).astype(np.float64)
     assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
 
@@ -278,7 +278,8 @@ def test_captured_call_follows_lengths_tables_and_terms(qs):
         new_q = np.roll(q, turn, axis=0)
         qd.copy_(G.to_dev(new_q))
         want, want_lse, bound, lse_bound = scored_attention(pool, bt, lens, oracle.bits_to_f32(new_q, DT_BF16).astype(np.float64), aq, now_ctx,
-                                                            cap=30.0, documents=new_doc, scale=hb.sm_scale, dt=DT_BF16)
+                                                            cap=30.0, documents=new_doc, scale=hb.sm_scale, dt=DT_BF16,
+                                                            chunk=max(qs) * 4 >= CHUNK_FROM)
         for which in (0, 1, 0):
             outs[which].zero_()
             graphs[which].replay()
@@ -399,3 +400,113 @@ def test_scratch_query():
         assert size(C.byref(layout), *args) == 0
     assert size(None, 1, 1, 1, 16) == 0
     assert SENTINEL
+
+
+@gpu
+@pytest.mark.parametrize("fmt,xf,v_xf,dt,hd", FORMS)
+@pytest.mark.parametrize("seqs,qs,terms", [([70], [70], {"cap": 30.0}), ([333, 1100], [100, 65], {"sloped": True}),
+                                           ([200, 90], [150, 90], {"cap": 5.0, "window": 50})])
+def test_chunks(fmt, xf, v_xf, dt, hd, seqs, qs, terms):
+    """Many query columns: several tiles, ranges that end inside a unit, keys split and joined."""
+    pool, bt, k, v, q, aq, ctx = case(fmt, 16, seqs, qs, 1000 + hd, dt, xf=xf, v_xf=v_xf, head_dim=hd)
+    terms = dict(terms)
+    if terms.pop("sloped", False):
+        terms["slopes"] = slopes_of(8)
+    for scratch in (0, 64 << 20):
+        check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, scratch=scratch, **terms)
+
+
+@gpu
+@pytest.mark.parametrize("kv_heads,heads", [(1, 1), (2, 16), (1, 24), (1, 17), (3, 9), (1, 64)])
+def test_chunk_head_layouts(kv_heads, heads):
+    seqs, qs = [300], [150]
+    pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1020 + heads, DT_F16, kv_heads=kv_heads, q_heads=heads, head_dim=128)
+    check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, heads, cap=20.0, slopes=slopes_of(heads))
+
+
+@gpu
+@pytest.mark.parametrize("block", [16, 48, 128])
+@pytest.mark.parametrize("fmt,dt", [(FMT_TQ4, DT_BF16), (FMT_BF16, DT_BF16)])
+def test_chunk_page_sizes_and_odd_starts(fmt, dt, block):
+    """Windows that open at odd half units, so that a unit of keys lies in two pages."""
+    seqs, qs = [500, 97], [64, 33]
+    pool, bt, k, v, q, aq, ctx = case(fmt, block, seqs, qs, 1040 + block, dt)
+    for window in (0, 130, 150):
+        check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, scratch=64 << 20, cap=30.0, window=window)
+
+
+@gpu
+@pytest.mark.parametrize("fmt,xf,dt", [(FMT_TQ4, XF_WHT256, DT_F16), (FMT_BF16, XF_IDENTITY, DT_BF16), (FMT_Q8_0, XF_IDENTITY, DT_F16),
+                                       (FMT_FP8, XF_WHT256, DT_F16)])
+@pytest.mark.parametrize("scratch", [0, 64 << 20])
+def test_chunk_documents_prefixes_windows_and_empty_rows(fmt, xf, dt, scratch):
+    seqs, qs = [400, 161, 250], [170, 161, 3]
+    pool, bt, k, v, q, aq, ctx = case(fmt, 16, seqs, qs, 1060, dt, xf=xf)
+    rng = np.random.default_rng(6)
+    pos = np.concatenate([np.arange(n) + c for n, c in zip(qs, ctx)])
+    doc = (pos // 37 * 37).astype(np.int32)
+    doc[::9] = 100000
+    doc[40:80] = 1 << 30                 # tiles of which whole waves see nothing
+    doc[5] = -4
+    pre = rng.integers(-3, 600, pos.size).astype(np.int32)
+    check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, scratch=scratch, documents=doc)
+    check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, scratch=scratch, documents=doc, prefixes=pre, cap=30.0, slopes=slopes_of(8))
+    check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, scratch=scratch, noncausal=True, window=100, slopes=slopes_of(8))
+
+
+@gpu
+def test_chunk_whose_tokens_all_see_nothing():
+    pool, bt, k, v, q, aq, ctx = case(FMT_TQ4, 16, [200], [100], 1070, DT_BF16)
+    check_scored(pool, bt, [200], q, DT_BF16, aq, ctx, 8, documents=np.full(100, 5000, dtype=np.int32))
+
+
+@gpu
+@pytest.mark.parametrize("scratch", [0, 64 << 20])
+def test_chunk_masked_tokens_and_requests_stay_untouched(scratch):
+    seqs, qs = [300, 500, 90], [140, 60, 90]
+    pool, bt, k, v, q, aq, ctx = case(FMT_TQ4, 16, seqs, qs, 1080, DT_F16)
+    tmask = np.ones(aq[-1], dtype=np.uint8)
+    tmask[::5] = 0
+    tmask[40:100] = 0
+    rmask = np.array([1, 0, 1], dtype=np.uint8)
+    hb = oracle.HostBatch(aq, seqs, bt, context_lens_before=ctx, valid_token_mask=tmask, valid_req_mask=rmask)
+    rows = tmask.astype(bool)
+    rows[aq[1]:aq[2]] = False
+    check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 8, hb=hb, rows=rows, cap=30.0, scratch=scratch)
+
+
+@gpu
+@pytest.mark.parametrize("fmt,xf,dt", [(FMT_TQ4, XF_WHT256, DT_BF16), (FMT_FP8, XF_IDENTITY, DT_F16), (FMT_FP8, XF_WHT256, DT_F16),
+                                       (FMT_Q8_0, XF_IDENTITY, DT_F16), (FMT_FP16, XF_IDENTITY, DT_F16), (FMT_BF16, XF_IDENTITY, DT_BF16)])
+def test_chunk_what_unseen_rows_hold_does_not_matter(fmt, xf, dt):
+    """Bytes of 0xFF behind the sequence and before the window, in the pages of a chunk."""
+    seq, n = 213, 137
+    pool, bt, k, v, q, aq, ctx = case(fmt, 16, [seq], [n], 1090, dt, xf=xf)
+    window = 40
+    seen_from = seq - n - window + 1
+    wild = np.ones(pool.k.size // pool.page * 16, dtype=bool)
+    wild[oracle.slot_mapping(bt[0], seen_from, seq - seen_from, 16)] = False
+    views = [s.reshape(-1, pool.kv_heads, 16, pool.tok) for s in (pool.k, pool.v)]
+    keep = [s.copy() for s in views]
+    for s in views:
+        for h in range(pool.kv_heads):
+            s[:, h][wild.reshape(-1, 16)] = 0xFF
+    hb = oracle.HostBatch(aq, [seq], bt, context_lens_before=ctx)
+    hb.sliding_window = window
+    bits, lse = run_scored(pool, hb, q, dt, 8, cap=30.0)
+    for s, old in zip(views, keep):
+        s[:] = old
+    want, want_lse, bound, lse_bound = scored_attention(pool, bt, [seq], oracle.bits_to_f32(q, dt).astype(np.float64), aq, ctx, cap=30.0,
+                                                        window=window, scale=hb.sm_scale, dt=dt, chunk=True)
+    got = oracle.bits_to_f32(bits, dt).astype(np.float64)
+    assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dt", [(FMT_FP16, DT_F16), (FMT_TQ4, DT_BF16)])
+@pytest.mark.parametrize("tokens", [1, 15, 16, 17, 31, 32, 33, 64, 65])
+def test_requests_of_any_number_of_tokens(fmt, dt, tokens):
+    """From one kernel's range into the other's: 8 query heads of a kv head, so 128 columns at 16 tokens, 256 at 32."""
+    seqs, qs = [tokens + 200, tokens], [tokens, tokens]
+    pool, bt, k, v, q, aq, ctx = case(fmt, 16, seqs, qs, 1100 + tokens, dt, kv_heads=1)
+    check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, cap=30.0)

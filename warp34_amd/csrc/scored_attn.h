@@ -30,6 +30,7 @@ struct ScoredParams {
     int tiles;        // tiles of a request (a bound)
     int entries;      // requests x tiles: tiles of the batch, some of them empty
     int target;       // slots for chunks, for each kv head; 0: no split, a workgroup for each entry
+    int min_halves;   // shortest chunk
     float* part_acc;  // [slot][kv_sub][column][head_dim]
     float* part_ml;   // [slot][kv_sub][column]{m, l}
     int32_t* table;   // [entry]{first slot, chunks}
@@ -41,20 +42,24 @@ struct ScoredParams {
 // arguments go through the series.
 constexpr float kWideCap = 512.0f;
 
-// One score in the log2 domain; dot: q . k times what the column's scale is in, cs / cc: the column's scale times scale2 / cap_arg.
-template <bool CAP>
-__device__ __forceinline__ float score_term(float dot, float cs, float cc, const ScoredParams& P) {
+// N scores in the log2 domain; s: q . k times what the column's scale is in, cs / cc: the column's scale times scale2 / cap_arg.
+// (The choice stands outside the loop: one uniform branch.)
+template <bool CAP, int N, typename V>
+__device__ __forceinline__ void score_terms(V& s, float cs, float cc, const ScoredParams& P) {
     if constexpr (!CAP) {
-        return dot * cs;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] *= cs;
+    } else if (!P.wide_cap) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(-2.0f * P.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * cc) + 1.0f), P.cap2);
     } else {
-        const float a = dot * cc;
-        float x = __builtin_fmaf(-2.0f * P.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a) + 1.0f), P.cap2);
-        if (P.wide_cap) {  // uniform
-            const float u = a * (0.5f / kLog2e), uu = u * u;
-            const float series = dot * cs * __builtin_fmaf(uu, __builtin_fmaf(uu, __builtin_fmaf(uu, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-            x = fabsf(u) < 0.1f ? series : x;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float a = s[i] * cc, u = a * (0.5f / kLog2e), uu = u * u;
+            const float x = __builtin_fmaf(-2.0f * P.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a) + 1.0f), P.cap2);
+            const float series = __builtin_fmaf(uu, __builtin_fmaf(uu, __builtin_fmaf(uu, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+            s[i] = fabsf(u) < 0.1f ? s[i] * cs * series : x;
         }
-        return x;
     }
 }
 
@@ -127,7 +132,6 @@ __device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
 
 // The cut of a batch: chunks of `per` half units, the shortest length with which all tiles together need no more than P.target chunks;
 // a live tile has at least one.  halves: [entries] in LDS, -1 for tiles without tokens.
-constexpr int kMinHalvesPerChunk = 8;   // one for each wave of a decode workgroup
 constexpr int kMaxSplitEntries = 512;   // entries of a batch that is split
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
 __device__ __forceinline__ int chunk_length(const ScoredParams& P, const int* halves, int lane) {
@@ -140,7 +144,7 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, const int* ha
     total = __builtin_amdgcn_readfirstlane(wave_sum(total));
     live = __builtin_amdgcn_readfirstlane(wave_sum(live));
     // too short / long enough: sum of ceil(h / per) <= total / per + live
-    int low = max(kMinHalvesPerChunk, (total + P.target - 1) / P.target) - 1;
+    int low = max(P.min_halves, (total + P.target - 1) / P.target) - 1;
     int high = max(low + 1, (total + P.target - live - 1) / max(P.target - live, 1));
     while (high - low > 1 && P.entries <= 64) {
         const int mid = (low + high) >> 1;
@@ -219,12 +223,15 @@ __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, 
         if (c < chunks) ml = *reinterpret_cast<const f2*>(P.part_ml + 2 * record(c));
         const float w = __builtin_amdgcn_exp2f(ml[0] - m);
         l += ml[1] * w;
+        // a wave's eight records at most, their loads together
         const int end = min(64, chunks - base);
-#pragma unroll 8
-        for (int k = wave; k < end; k += 8) {
-            const float wk = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), k));
-            acc += *reinterpret_cast<const f4*>(P.part_acc + record(base + k) * HD + at) * wk;
-        }
+        f4 part[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (wave + 8 * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + wave + 8 * k) * HD + at);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (wave + 8 * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), wave + 8 * k));
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);

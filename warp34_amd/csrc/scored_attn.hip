@@ -2,21 +2,47 @@
 #include <algorithm>
 
 #include "attn_launch.h"
+#include "scored_chunk.h"
 #include "scored_decode.h"
 
 namespace w34 {
 
 constexpr int kScoredSlots = 128;       // chunks for each kv head of a batch of up to 64 tiles: with two kv heads one for every CU
 constexpr int kScoredSplitTiles = 512;  // from here on a kv head's tiles fill the chip by themselves
+constexpr int kDecodeCols = 16;         // query columns of a workgroup of the decode kernel
+constexpr int kDecodeMinHalves = 8;     // shortest chunk: a half unit for each wave
+constexpr int kChunkMinHalves = 16;     // eight units
 
-// Bytes of the partial records of `slots` chunks and of the tiles' table.
-static size_t scored_slot_bytes(int kv_subs, int head_dim) { return (size_t)kv_subs * 16 * (size_t)(head_dim + 2) * 4; }
-static size_t scored_table_bytes(long long entries) { return ((size_t)entries * 8 + 15) / 16 * 16; }
-static int scored_slots(long long entries) {
-    if (entries >= kScoredSplitTiles) return 0;
-    return kScoredSlots * (int)((std::max<long long>(2 * entries, kScoredSlots) + kScoredSlots - 1) / kScoredSlots);
+// Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
+constexpr int kChunkFrom = 128;
+
+// The tiles of a batch: the kernel, a tile's tokens, tiles of a request, chunk slots for each kv head (0: no split).
+struct ScoredShape {
+    bool chunk;
+    int cols, tok_tile;
+    long long tiles, entries;
+    int slots;
+};
+static ScoredShape scored_shape(int num_reqs, int total_tokens, int max_q_len, int q_group) {
+    ScoredShape s;
+    const int q_len = max_q_len > 0 ? std::min(max_q_len, total_tokens) : total_tokens;
+    s.chunk = (long long)q_len * q_group >= kChunkFrom;
+    s.cols = s.chunk ? kChunkCols : kDecodeCols;
+    s.tok_tile = s.cols / q_group;
+    s.tiles = ((long long)q_len + s.tok_tile - 1) / s.tok_tile;
+    s.entries = s.tiles * num_reqs;
+    s.slots = 0;
+    if (s.chunk) {
+        if (s.entries < kScoredSlots) s.slots = kScoredSlots;
+    } else if (s.entries < kScoredSplitTiles) {
+        s.slots = kScoredSlots * (int)((std::max<long long>(2 * s.entries, kScoredSlots) + kScoredSlots - 1) / kScoredSlots);
+    }
+    return s;
 }
 static_assert(kScoredSplitTiles <= kMaxSplitEntries, "tile counts in LDS");
+// Bytes of the partial records of a slot, and of the tiles' table.
+static size_t scored_slot_bytes(const ScoredShape& s, int kv_subs, int head_dim) { return (size_t)kv_subs * s.cols * (size_t)(head_dim + 2) * 4; }
+static size_t scored_table_bytes(long long entries) { return ((size_t)entries * 8 + 15) / 16 * 16; }
 
 // Largest divisor of the q heads of a kv head that fits a column tile
 static int scored_q_group(int gqa) {
@@ -54,42 +80,61 @@ template <typename TQ, int KVF, int HD>
 static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const warp34_attention_batch& B = P.B;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
-    if (kv_subs > 65535) return (int)hipErrorInvalidValue;
-    P.tok_tile = std::max(1, 16 / P.q_group);
-    const long long tiles = ((long long)(B.max_q_len > 0 ? std::min(B.max_q_len, B.total_tokens) : B.total_tokens) + P.tok_tile - 1) / P.tok_tile;
-    const long long entries = tiles * B.num_reqs;
-    if (entries > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
-    P.tiles = (int)tiles;
-    P.entries = (int)entries;
+    const ScoredShape s = scored_shape(B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
+    if (kv_subs > 65535 || s.entries > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
+    P.tok_tile = s.tok_tile;
+    P.tiles = (int)s.tiles;
+    P.entries = (int)s.entries;
+    P.min_halves = s.chunk ? kChunkMinHalves : kDecodeMinHalves;
     // chunks: as many as the scratch holds, none where a tile has too few keys for two
-    long long slots = scored_slots(entries);
-    const size_t table = scored_table_bytes(entries), per_slot = scored_slot_bytes(kv_subs, HD);
+    long long slots = s.slots;
+    const size_t table = scored_table_bytes(s.entries);
     if (ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0 || ex->scratch_size <= table) slots = 0;
-    else slots = std::min<long long>(slots, (long long)((ex->scratch_size - table) / per_slot));
+    else slots = std::min<long long>(slots, (long long)((ex->scratch_size - table) / scored_slot_bytes(s, kv_subs, HD)));
     if (B.max_seq_len > 0) {
-        const long long most = (((long long)B.max_seq_len + 30) / 16 + kMinHalvesPerChunk - 1) / kMinHalvesPerChunk;  // chunks of a tile
-        slots = B.max_seq_len <= 16 * kMinHalvesPerChunk ? 0 : std::min(slots, entries * (most + 1));
+        const long long most = (((long long)B.max_seq_len + 30) / 16 + P.min_halves - 1) / P.min_halves;  // chunks of a tile
+        slots = B.max_seq_len <= 16 * P.min_halves ? 0 : std::min(slots, s.entries * (most + 1));
     }
-    if (slots < entries + std::max<long long>(2, entries / 2)) slots = 0;
+    if (slots < s.entries + std::max<long long>(2, s.entries / 2)) slots = 0;
     P.target = (int)slots;
     if (slots > 0) {
         uint8_t* at = reinterpret_cast<uint8_t*>((uintptr_t)ex->scratch_ptr);
         P.table = reinterpret_cast<int32_t*>(at);
         P.part_acc = reinterpret_cast<float*>(at + table);
-        P.part_ml = P.part_acc + (size_t)slots * kv_subs * 16 * HD;
+        P.part_ml = P.part_acc + (size_t)slots * kv_subs * s.cols * HD;
     }
     hipStream_t stream = (hipStream_t)ex->stream;
-    using M = ScoredLds<KVF, HD>;
-    const dim3 grid((unsigned)(slots > 0 ? slots : entries), (unsigned)kv_subs);
-    const auto launch = [&](auto kernel) {
-        const int rc = ensure_dynamic_lds(kernel, M::kBytes, true);
+    const dim3 grid((unsigned)(slots > 0 ? slots : s.entries), (unsigned)kv_subs);
+    const auto launch = [&](auto kernel, int threads, int lds) {
+        const int rc = ensure_dynamic_lds(kernel, lds, true);
         if (rc) return rc;
-        hipLaunchKernelGGL(kernel, grid, dim3(kScoredWaves * 64), M::kBytes, stream, P);
+        hipLaunchKernelGGL(kernel, grid, dim3((unsigned)threads), (unsigned)lds, stream, P);
         return (int)hipGetLastError();
     };
-    const int rc = P.cap2 > 0.f ? launch(scored_decode_kernel<TQ, KVF, HD, true>) : launch(scored_decode_kernel<TQ, KVF, HD, false>);
+    const bool cap = P.cap2 > 0.f;
+    int rc;
+    if (!s.chunk) {
+        rc = cap ? launch(scored_decode_kernel<TQ, KVF, HD, true>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes)
+                 : launch(scored_decode_kernel<TQ, KVF, HD, false>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes);
+    } else {
+        using R = ScoredRows<KVF, HD>;
+        constexpr int lds = ChunkLds<KVF, HD>::kBytes;
+        const bool ride = R::kTq4 || (!R::k16 && P.rot_out != 0);
+        const auto pick = [&](auto c) {
+            constexpr bool CAP = decltype(c)::value;
+            if constexpr (R::kTq4) {
+                return launch(scored_chunk_kernel<TQ, KVF, HD, CAP, true>, kChunkWaves * 64, lds);
+            } else if constexpr (R::k16) {
+                return launch(scored_chunk_kernel<TQ, KVF, HD, CAP, false>, kChunkWaves * 64, lds);
+            } else {
+                return ride ? launch(scored_chunk_kernel<TQ, KVF, HD, CAP, true>, kChunkWaves * 64, lds)
+                            : launch(scored_chunk_kernel<TQ, KVF, HD, CAP, false>, kChunkWaves * 64, lds);
+            }
+        };
+        rc = cap ? pick(std::true_type{}) : pick(std::false_type{});
+    }
     if (rc || slots == 0) return rc;
-    hipLaunchKernelGGL((scored_join_kernel<TQ, HD>), dim3((unsigned)entries, (unsigned)kv_subs, 16u), dim3(512), 0, stream, P, 16,
+    hipLaunchKernelGGL((scored_join_kernel<TQ, HD>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P, s.cols,
                        ScoredRows<KVF, HD>::kOutScale);
     return (int)hipGetLastError();
 }
@@ -152,9 +197,7 @@ extern "C" size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_la
                                                               int num_q_heads) {
     if (!layout || layout->local_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % layout->local_kv_heads != 0 || num_reqs <= 0 || total_tokens <= 0)
         return 0;
-    const int gqa = num_q_heads / layout->local_kv_heads, group = scored_q_group(gqa), tok_tile = std::max(1, 16 / group);
-    const long long tiles = ((long long)(max_q_len > 0 ? std::min(max_q_len, total_tokens) : total_tokens) + tok_tile - 1) / tok_tile;
-    const long long entries = tiles * num_reqs;
-    const int slots = scored_slots(entries);
-    return slots == 0 ? 0 : scored_table_bytes(entries) + (size_t)slots * scored_slot_bytes(layout->local_kv_heads * (gqa / group), layout->head_dim);
+    const int gqa = num_q_heads / layout->local_kv_heads, group = scored_q_group(gqa);
+    const ScoredShape s = scored_shape(num_reqs, total_tokens, max_q_len, group);
+    return s.slots == 0 ? 0 : scored_table_bytes(s.entries) + (size_t)s.slots * scored_slot_bytes(s, layout->local_kv_heads * (gqa / group), layout->head_dim);
 }

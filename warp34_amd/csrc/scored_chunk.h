@@ -1,0 +1,549 @@
+// Scored paged attention of many query columns for each kv head: chunks of prompts.
+//
+// Workgroup = 256 query columns (tokens x the q heads of a kv head) x a range of keys, eight waves of 32 columns each.  The workgroup
+// walks the keys in units of 32, one barrier a unit; between two barriers
+//   the rows of a later unit travel from the pages to LDS (LDS-direct loads: no register holds them),
+//   quantised rows of the next unit are widened into the 16-bit tiles that the products read, and
+//   every wave multiplies the present unit:  S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs.
+// A lane (n, b) has the scores of column n for the keys (i & 3) + 8 (i >> 2) + 4 b, i = 0 .. 15: eight of them are, where they stand, a
+// B operand of the value product over 16 keys, whose A operand comes out of row-major LDS by the transposing reads
+// (ds_read_b64_tr_b16: lane l of 16 gets column l of four rows of 16 values).  So both tiles are row-major and nothing is shuffled.
+//   key tile    row r, 16-byte piece p at p ^ (r & 15): the operand reads of 16 rows touch all banks
+//   value tile  row r, piece p at p ^ 4 (r & 3): the four rows of a transposing read touch all banks
+#pragma once
+
+#include "scored_decode.h"
+
+namespace w34 {
+
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s4v lds_s4;
+typedef __attribute__((address_space(3))) const f4 lds_f4c;
+
+constexpr int kChunkWaves = 8;
+constexpr int kChunkCols = 32 * kChunkWaves;
+constexpr int kChunkUnit = 32;
+
+template <bool IS_BF16>
+__device__ __forceinline__ f16v mfma_tile(u4 a, u4 b, f16v c) {
+    if constexpr (IS_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf8, a), __builtin_bit_cast(bf8, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+    }
+}
+// 16 bytes a lane to LDS: lane l's from base + voffset + IMM to lds + IMM + 16 l
+template <int IMM>
+__device__ __forceinline__ void load_to_lds(uint32_t voffset, const uint8_t* base, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" : : "v"(voffset), "s"(base), "s"(lds), "n"(IMM) : "memory");
+}
+__device__ __forceinline__ const uint8_t* uniform_pointer(const uint8_t* p) {
+    const uint64_t a = (uint64_t)(uintptr_t)p;
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32));
+    return reinterpret_cast<const uint8_t*>((uintptr_t)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ void chunk_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
+__device__ __forceinline__ u4 lds_u4(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const u4*>((uintptr_t)at); }
+__device__ __forceinline__ uint32_t lds_u1(uint32_t at) { return *reinterpret_cast<lds_cu32*>((uintptr_t)at); }
+__device__ __forceinline__ f4 lds_f4(uint32_t at) { return *reinterpret_cast<lds_f4c*>((uintptr_t)at); }
+__device__ __forceinline__ void lds_put(uint32_t at, u4 v) { *reinterpret_cast<__attribute__((address_space(3))) u4*>((uintptr_t)at) = v; }
+
+template <int KVF, int HD>
+struct ChunkLds {
+    using R = ScoredRows<KVF, HD>;
+    static constexpr int kRow = 2 * HD;                       // of a tile
+    static constexpr int kTile = kChunkUnit * kRow;           // keys or values
+    static constexpr int kTable = R::kTq4 ? 65536 : 0;
+    static constexpr int kTiles = kTable;                     // two units of {keys, values}
+    static constexpr int kRun = 16 * R::kRowBytes;            // of a page
+    static constexpr int kRawUnit = R::k16 ? 0 : (4 * kRun + 16);
+    static constexpr int kRaw = kTiles + 4 * kTile;           // two units of {keys 0-15, 16-31, values 0-15, 16-31} as stored
+    static constexpr int kScale = kRaw + 2 * kRawUnit;        // two units of {key scales [4][32], value scales [4][32]}
+    static constexpr int kLoop = kScale + (R::k16 ? 0 : 2 * 2 * 4 * 32 * 4);
+    // before the loop: tile counts of the batch; eight query columns of each wave at a time.  After it: eight columns of sums.
+    static constexpr int kColStride = HD + 8;
+    static constexpr int kCounts = kTiles + kChunkWaves * 8 * kColStride * 4;
+    static constexpr int kQScale = kCounts + kMaxSplitEntries * 4;
+    static constexpr int kEnds = kQScale + kChunkCols * 4;
+    static constexpr int kBytes = kLoop > kEnds ? kLoop : kEnds;
+    static_assert(kBytes <= 160 * 1024 && kRun % 16 == 0, "chunk LDS budget");
+};
+
+// VF: the values' block scales ride on the weights, which then have two fp16 parts (TQ4; rotated 8-bit rows: values rounded as
+// fp16(d * code) have errors in common where a block holds few codes, which the rotation back gathers in one channel).  Otherwise 8-bit
+// values are fp16(d * code) and weights one operand.
+template <typename TQ, int KVF, int HD, bool CAP, bool VF>
+__global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const ScoredParams P) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    using R = ScoredRows<KVF, HD>;
+    using M = ChunkLds<KVF, HD>;
+    constexpr bool IS_BF16 = R::k16 && TQ::kStorageFormat == WARP34_KV_FORMAT_BF16;
+    constexpr int kSteps = HD / 16, kDims = HD / 32;
+    const int tid = (int)threadIdx.x, lane = tid & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int n = lane & 31, b = lane >> 5;
+    const warp34_kv_layer_layout& L = P.L;
+    const warp34_attention_batch& B = P.B;
+    const int kv_sub = (int)blockIdx.y;
+    const int kv_head = P.q_subgroups == 1 ? kv_sub : fast_div(kv_sub, P.q_subgroups);
+    const int head0 = kv_head * P.gqa + (kv_sub - kv_head * P.q_subgroups) * P.q_group;
+
+    // ---- what this workgroup works on ----
+    ScoredWork work = {(int)blockIdx.x, 0, 1, 0};
+    int per = 0x7ffffffe;
+    if (P.target > 0) {
+        int* halves = reinterpret_cast<int*>(smem + M::kCounts);
+        for (int e = tid; e < P.entries; e += kChunkWaves * 64) {
+            const ScoredTile t = scored_tile(P, e);
+            int first = 0, last = -1;
+            if (t.tokens > 0) tile_keys(P, t, first, last);
+            halves[e] = t.tokens > 0 ? tile_halves(first, last) : -1;
+        }
+        __syncthreads();
+        per = (chunk_length(P, halves, lane) + 1) & ~1;
+        work = find_work(P, halves, per, (int)blockIdx.x, lane);
+        if (work.entry < 0) return;
+        if (work.chunk == 0 && kv_sub == 0 && tid == 0) {
+            P.table[2 * work.entry] = work.first_slot;
+            P.table[2 * work.entry + 1] = work.chunks;
+        }
+    } else {
+        work.entry = (int)(gridDim.x - 1 - blockIdx.x);  // the tiles with most keys first
+    }
+    const ScoredTile t = scored_tile(P, work.entry);
+    if (t.tokens <= 0) return;
+    int key_first, key_last;
+    tile_keys(P, t, key_first, key_last);
+    key_first = __builtin_amdgcn_readfirstlane(key_first);
+    key_last = __builtin_amdgcn_readfirstlane(key_last);
+    const int all_halves = tile_halves(key_first, key_last);
+    const int begin = ((key_first >> 4) + work.chunk * min(per, all_halves)) * 16;  // keys
+    const int end = key_first > key_last ? begin : min(begin + min(per, all_halves) * 16, key_last + 1);
+    const int units = (end - begin + kChunkUnit - 1) / kChunkUnit;
+
+    // ---- this lane's column ----
+    const int col = 32 * wave + n;
+    const int my_t = column_token(col, P);
+    const int my_tok = min(t.tok0 + my_t, B.total_tokens - 1);
+    const bool col_ok = my_t < t.tokens && (B.valid_token_mask == nullptr || B.valid_token_mask[my_tok] != 0);
+    const int my_head = min(head0 + (col - my_t * P.q_group), P.num_q_heads - 1);
+    const int my_pos = t.pos0 + my_t;
+    int lo = 0, hi = -1;
+    if (col_ok) token_keys(P, my_tok, my_pos, t.seq_after, lo, hi);
+    // keys that every live column of the wave sees, and that any sees
+    int all_from = col_ok ? lo : 0, all_to = col_ok ? hi : 0x7fffffff;
+    int any_from = lo <= hi ? lo : 0x7fffffff, any_to = lo <= hi ? hi : -1;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        all_from = max(all_from, __shfl_xor(all_from, d, 64));
+        all_to = min(all_to, __shfl_xor(all_to, d, 64));
+        any_from = min(any_from, __shfl_xor(any_from, d, 64));
+        any_to = max(any_to, __shfl_xor(any_to, d, 64));
+    }
+    all_from = __builtin_amdgcn_readfirstlane(all_from);
+    all_to = __builtin_amdgcn_readfirstlane(all_to);
+    any_from = __builtin_amdgcn_readfirstlane(any_from);
+    any_to = __builtin_amdgcn_readfirstlane(any_to);
+    const uint32_t live = (uint32_t)__ballot(col_ok);
+    const bool sloped = P.slopes != nullptr;
+    const float slope2 = sloped && col_ok ? P.slopes[my_head] * kLog2e : 0.f;
+
+    // ---- table and query operands: lane (n, b) holds Q[column n][16 m + 8 b .. + 7] ----
+    if constexpr (R::kTq4) build_pair_table(smem, tid, wave);
+    u4 q[kSteps];
+    float cs = P.scale2, cc = P.cap_arg;
+    if constexpr (R::k16) {
+        const uint16_t* src = P.q + ((size_t)my_tok * P.num_q_heads + (size_t)my_head) * HD + 8 * b;
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+            q[m] = *reinterpret_cast<const u4*>(src + 16 * m);
+            if (!col_ok) q[m] = u4{0u, 0u, 0u, 0u};
+        }
+    } else {
+        // eight columns of the wave at a time: rotated where the keys are, relative to a power of two above their largest element
+        uint16_t* area = reinterpret_cast<uint16_t*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
+        float* scales = reinterpret_cast<float*>(smem + M::kQScale) + 32 * wave;
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+#pragma unroll 1
+            for (int c8 = 0; c8 < 8; ++c8) {
+                const int c = 8 * g + c8, ct = column_token(32 * wave + c, P);
+                float v[4] = {0.f, 0.f, 0.f, 0.f};
+                if ((live >> c) & 1u) {
+                    const uint16_t* src = P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + 4 * lane;
+                    const uint2 raw = *reinterpret_cast<const uint2*>(src);
+                    v[0] = TQ::to_f32((uint16_t)raw.x), v[1] = TQ::to_f32((uint16_t)(raw.x >> 16));
+                    v[2] = TQ::to_f32((uint16_t)raw.y), v[3] = TQ::to_f32((uint16_t)(raw.y >> 16));
+                }
+                if (P.rot_q) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[k] = apply_sign(v[k], 4 * lane + k);
+                    wht256_wave(v, lane);
+                }
+                float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+                const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
+                *reinterpret_cast<uint2*>(area + c8 * M::kColStride + 4 * lane) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
+                if (lane == 0) scales[c] = __builtin_amdgcn_ldexpf(1.0f, e);
+            }
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_wave_barrier();
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            if ((n >> 3) == g) {
+#pragma unroll
+                for (int m = 0; m < kSteps; ++m) q[m] = *reinterpret_cast<const u4*>(area + (n & 7) * M::kColStride + 16 * m + 8 * b);
+            }
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_wave_barrier();
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        }
+        const float mine = scales[n] * R::kOutScale;
+        cs *= mine;
+        cc *= mine;
+    }
+    __syncthreads();  // the areas become tiles
+
+    // ---- loader: waves 2 i and 2 i + 1 bring half each of run i (keys 0-15, 16-31, values 0-15, 16-31) ----
+    const int run = wave >> 1, part = wave & 1;
+    const bool loads_v = run >= 2;
+    const uint8_t* slab = reinterpret_cast<const uint8_t*>((uintptr_t)(loads_v ? L.v_base : L.k_base)) +
+                          (uint64_t)(uint32_t)kv_head * (loads_v ? L.v_head_stride_bytes : L.k_head_stride_bytes);
+    const uint64_t page_stride = loads_v ? L.v_page_stride_bytes : L.k_page_stride_bytes;
+    const int32_t* blocks = B.block_tables + (size_t)t.req * B.max_blocks_per_req;
+    int slot_base = page_slot(begin, P);
+    int pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
+    constexpr int kShare = M::kRun / 2;
+    const auto issue = [&](int u) {
+        const int pos = begin + u * kChunkUnit + 16 * (run & 1);
+        uint64_t off = 0;
+        if (pos <= key_last) {  // (a run behind the keys: rows of page 0, which nobody sees)
+            const int slot = page_slot(pos, P);
+            if (slot - slot_base >= 64) {
+                slot_base = slot;
+                pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
+            }
+            const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, slot - slot_base), 0);
+            off = (uint64_t)page * page_stride + (uint32_t)(pos - slot * L.block_size) * (uint32_t)R::kRowBytes;
+        }
+        const uint8_t* src = uniform_pointer(slab + off + part * kShare);
+        if constexpr (R::k16) {
+            // rows 8 part + ..: the piece that belongs to a lane's place
+            constexpr int kPieces = M::kRow / 16, kRows = 64 / kPieces;  // of a row, of an instruction
+            const uint32_t dst = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile + (loads_v ? M::kTile : 0) + (run & 1) * M::kRun + part * kShare);
+            const int r = lane / kPieces, p = lane % kPieces;
+            const auto one = [&](auto imm) {
+                constexpr int i = decltype(imm)::value;
+                const int row = 8 * part + i * kRows + r;
+                const uint32_t v = (uint32_t)(r * M::kRow + 16 * (p ^ (loads_v ? 4 * (row & 3) : (row & 15))));
+                load_to_lds<1024 * i>(v, src, dst);
+            };
+            one(std::integral_constant<int, 0>{});
+            one(std::integral_constant<int, 1>{});
+            if constexpr (kShare > 2048) {
+                one(std::integral_constant<int, 2>{});
+                one(std::integral_constant<int, 3>{});
+            }
+        } else {
+            const uint32_t dst = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit + run * M::kRun + part * kShare), v = 16u * (uint32_t)lane;
+            load_to_lds<0>(v, src, dst);
+            if constexpr (kShare >= 2048) load_to_lds<1024>(v, src, dst);
+            constexpr int kRest = kShare % 1024;
+            if (v < (uint32_t)kRest) load_to_lds<kShare - kRest>(v, src, dst);
+        }
+    };
+    // ---- raw rows of unit u -> its tiles and scales; a thread takes 16 elements of a key row and of a value row ----
+    const auto widen = [&](int u) {
+        if constexpr (!R::k16) {
+            const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit), tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
+            const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 1024);
+            const int r = tid >> 4, c = tid & 15;
+            const int row_pos = begin + u * kChunkUnit + r;
+            const bool seen = row_pos >= key_first && row_pos <= key_last;
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const uint32_t src = raw + (uint32_t)(side * 2 * M::kRun + r * R::kRowBytes);
+                u4 w[2];
+                if constexpr (R::kTq4) {
+                    // (reads of four bytes must be aligned, the codes of the first half start at byte 2)
+                    const uint32_t at = src + (c >= 8 ? 68u : 0u) + 8u * (c & 7);
+                    const uint32_t shift = c >= 8 ? 0u : 16u, d0 = lds_u1(at), d1 = lds_u1(at + 4), d2 = lds_u1(at + 8);
+                    uint32_t codes[2] = {__builtin_amdgcn_alignbit(d1, d0, shift), __builtin_amdgcn_alignbit(d2, d1, shift)};
+                    const uint32_t lut_lane = (uint32_t)lane << 2;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[h][k] = lut_read(codes[h], lut_lane, 0x0c0c0400u + ((uint32_t)k << 8));
+                } else {
+                    const uint32_t at = R::kFp8 ? src + 16u * c : src + 68u * (c >> 2) + 4u + 16u * (c & 3);
+                    const float d = side == 1 && !VF ? __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * (c >> 3) : src + 68u * (c >> 2))) : 1.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t code = lds_u1(at + 4 * k);
+                        if (side == 1) code = seen ? code : 0u;
+                        uint32_t x, y;
+                        if (side == 1 && !VF) {
+                            float f[4];
+                            if constexpr (R::kFp8) {
+                                const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), s = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
+                                f[0] = p[0], f[1] = p[1], f[2] = s[0], f[3] = s[1];
+                            } else {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(code >> (8 * i));
+                            }
+                            const float dd = seen ? d : 0.f;
+                            x = pack_h2(f[0] * dd, f[1] * dd);
+                            y = pack_h2(f[2] * dd, f[3] * dd);
+                        } else if constexpr (R::kFp8) {
+                            if (side == 0) {
+                                x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, false));
+                                y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, true));
+                            } else {
+                                x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 0.00390625f, false));
+                                y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 0.00390625f, true));
+                            }
+                        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16, 0x4800 | (q + 128) is 9 + q / 128
+                            const uint32_t u8 = code ^ 0x80808080u, one = side == 0 ? 0x64646464u : 0x48484848u;
+                            const _Float16 zero = side == 0 ? (_Float16)1152.0f : (_Float16)9.0f;
+                            const h2 bias = {zero, zero};
+                            x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, u8, 0x04010400u)) - bias);
+                            y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, u8, 0x04030402u)) - bias);
+                        }
+                        w[k >> 1][2 * (k & 1)] = x;
+                        w[k >> 1][2 * (k & 1) + 1] = y;
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int p = 2 * c + h;
+                    lds_put(tiles + (uint32_t)(side * M::kTile + r * M::kRow + 16 * (p ^ (side ? 4 * (r & 3) : (r & 15)))), w[h]);
+                }
+            }
+            // scales: [block][row] of the keys, then of the values
+            constexpr int kKinds = VF ? 2 : 1;
+            if (tid < kKinds * R::kScales * 32) {
+                const int side = tid / (R::kScales * 32), blk = tid / 32 % R::kScales, row = tid & 31;
+                const uint32_t src = raw + (uint32_t)(side * 2 * M::kRun + row * R::kRowBytes);
+                float d;
+                if constexpr (R::kTq4) {
+                    d = F16::to_f32(*reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)(src + 66u * blk)));
+                } else {
+                    d = __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * blk : src + 68u * blk));
+                }
+                if (side == 1) {
+                    const int p = begin + u * kChunkUnit + row;
+                    d = p >= key_first && p <= key_last ? d * R::kValueGain : 0.f;
+                }
+                *reinterpret_cast<__attribute__((address_space(3))) float*>((uintptr_t)(scale + (uint32_t)(side * 512 + blk * 128 + 4 * row))) = d;
+            }
+        }
+    };
+
+    f16v o[kDims];
+#pragma unroll
+    for (int k = 0; k < kDims; ++k)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[k][i] = 0.f;
+    float m_run = kNegBig, l_run = 0.f;
+
+    const auto multiply = [&](int u) {
+        const int u0 = begin + u * kChunkUnit;
+        if (u0 > any_to || u0 + kChunkUnit - 1 < any_from) return;  // uniform
+        const uint32_t tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
+        const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 1024);
+        // ---- scores ----
+        f16v s;
+        {
+            const uint32_t row = tiles + (uint32_t)(n * M::kRow), swap = 16u * (uint32_t)(b ^ (n & 15));
+            constexpr int kBlocks = R::k16 ? 1 : R::kScales, kPer = kSteps / kBlocks;
+#pragma unroll
+            for (int blk = 0; blk < kBlocks; ++blk) {
+                f16v part_s;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) part_s[i] = 0.f;
+#pragma unroll
+                for (int mm = 0; mm < kPer; ++mm) {
+                    const int m = blk * kPer + mm;
+                    part_s = mfma_tile<IS_BF16>(lds_u4(row + (swap ^ (uint32_t)(32 * (m & 7))) + 256u * (m >> 3)), q[m], part_s);
+                }
+                if constexpr (R::k16) {
+                    s = part_s;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const f4 d = lds_f4(scale + (uint32_t)(128 * blk + 32 * k + 16 * b));
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[4 * k + i] = blk == 0 ? d[i] * part_s[4 * k + i] : __builtin_fmaf(d[i], part_s[4 * k + i], s[4 * k + i]);
+                    }
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- terms, masks, softmax ----
+        const bool masked = !(u0 >= all_from && u0 + kChunkUnit - 1 <= all_to);  // uniform
+        score_terms<CAP, 16>(s, cs, cc, P);
+        if (sloped) {
+            const float at = (float)(my_pos - u0 - 4 * b);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope2, fabsf(at - (float)((i & 3) + 8 * (i >> 2))), s[i]);
+        }
+        if (masked) {
+            const int from = lo - u0 - 4 * b, to = hi - u0 - 4 * b;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int k = (i & 3) + 8 * (i >> 2);
+                s[i] = k >= from && k <= to ? s[i] : -INFINITY;
+            }
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        {
+            const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+            top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        }
+        if (__ballot(top > m_run) != 0ull) {
+            const float m_new = fmaxf(m_run, top);
+            const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
+            m_run = m_new;
+            l_run *= alpha;
+#pragma unroll
+            for (int k = 0; k < kDims; ++k) o[k] *= alpha;
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s[i] = __builtin_amdgcn_exp2f(s[i] - m_run);
+            sum += s[i];
+        }
+        l_run += sum;
+        __builtin_amdgcn_sched_barrier(0);
+        // ---- values ----
+        // lane l reads row (l & 15) >> 2 of four, 8 bytes at 8 (l & 3) of the 32 of its 16 channels
+        const int j = lane & 15;
+        const uint32_t v_at = tiles + (uint32_t)(M::kTile + (4 * b + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
+        const auto v_operand = [&](int dt, int step) -> u4 {
+            const uint32_t at = (v_at ^ (64u * (uint32_t)(dt & 3))) + 256u * (uint32_t)(dt >> 2) + (uint32_t)(step * 16 * M::kRow);
+            const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
+            const s4v c = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(at + 8u * M::kRow)));
+            const u2v x = __builtin_bit_cast(u2v, a), y = __builtin_bit_cast(u2v, c);
+            return u4{x[0], x[1], y[0], y[1]};
+        };
+        if constexpr (VF) {
+            constexpr int kPerGroup = kDims / R::kGroups;
+#pragma unroll
+            for (int g = 0; g < R::kGroups; ++g) {
+                u4 high[2], low[2];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f4 d = lds_f4(scale + (uint32_t)(512 + 128 * g + 32 * k + 16 * b));
+                    float w[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = mul_legacy(s[4 * k + i], d[i]);
+                    uint32_t h0, h1, l0, l1;
+                    split_weights(w[0], w[1], h0, l0);
+                    split_weights(w[2], w[3], h1, l1);
+                    high[k >> 1][2 * (k & 1)] = h0, high[k >> 1][2 * (k & 1) + 1] = h1;
+                    low[k >> 1][2 * (k & 1)] = l0, low[k >> 1][2 * (k & 1) + 1] = l1;
+                }
+#pragma unroll
+                for (int dt = g * kPerGroup; dt < (g + 1) * kPerGroup; ++dt)
+#pragma unroll
+                    for (int step = 0; step < 2; ++step) {
+                        const u4 a = v_operand(dt, step);
+                        o[dt] = mfma_tile<false>(a, high[step], o[dt]);
+                        o[dt] = mfma_tile<false>(a, low[step], o[dt]);
+                    }
+            }
+        } else {
+            u4 w[2];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) w[k >> 2][k & 3] = IS_BF16 ? pack_bf2(s[2 * k], s[2 * k + 1]) : pack_h2(s[2 * k], s[2 * k + 1]);
+#pragma unroll
+            for (int dt = 0; dt < kDims; ++dt)
+#pragma unroll
+                for (int step = 0; step < 2; ++step) o[dt] = mfma_tile<IS_BF16>(v_operand(dt, step), w[step], o[dt]);
+        }
+    };
+    // 16-bit value rows that no token of the tile sees count as zeros: a page's rest may hold anything
+    const auto clear_unseen = [&](int u) {
+        if constexpr (R::k16) {
+            const int u0 = begin + u * kChunkUnit;
+            if (u0 >= key_first && u0 + kChunkUnit - 1 <= key_last) return;  // uniform
+            constexpr int kPieces = M::kTile / 16;
+            for (int p = tid; p < kPieces; p += kChunkWaves * 64) {
+                const int pos = u0 + p / (M::kRow / 16);
+                if (pos < key_first || pos > key_last)
+                    lds_put((uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile + M::kTile + 16 * p), u4{0u, 0u, 0u, 0u});
+            }
+            chunk_barrier();
+        }
+    };
+
+    if (units > 0) issue(0);
+    if constexpr (!R::k16) {
+        if (units > 1) issue(1);
+        chunk_barrier();
+        if (units > 0) widen(0);
+    }
+    for (int u = 0; u < units; ++u) {
+        chunk_barrier();  // unit u's tiles are whole, the next one's rows have landed; nobody reads what is overwritten below
+        if constexpr (R::k16) {
+            if (u + 1 < units) issue(u + 1);
+            clear_unseen(u);
+        } else {
+            if (u + 2 < units) issue(u + 2);
+            if (u + 1 < units) widen(u + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(u);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
+        l_run = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    chunk_barrier();
+
+    // ---- rows out, eight columns of a wave at a time through LDS ----
+    float* area = reinterpret_cast<float*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
+    const int kv_subs = (int)gridDim.y;
+#pragma unroll 1
+    for (int g = 0; g < 4; ++g) {
+        if ((n >> 3) == g) {
+#pragma unroll
+            for (int dt = 0; dt < kDims; ++dt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<f4*>(area + (n & 7) * M::kColStride + 32 * dt + 8 * k + 4 * b) = f4{o[dt][4 * k], o[dt][4 * k + 1], o[dt][4 * k + 2], o[dt][4 * k + 3]};
+        }
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_wave_barrier();
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+#pragma unroll 1
+        for (int c8 = 0; c8 < 8; ++c8) {
+            const int c = 8 * g + c8;
+            if (!((live >> c) & 1u)) continue;
+            const f4 acc = *reinterpret_cast<const f4*>(area + c8 * M::kColStride + ((4 * lane) & (HD - 1)));
+            const float m_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), c));
+            const float l_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_run), c));
+            if (work.chunks > 1) {
+                const size_t record = ((size_t)blockIdx.x * kv_subs + kv_sub) * kChunkCols + 32 * wave + c;
+                if (4 * lane < HD) *reinterpret_cast<f4*>(P.part_acc + record * HD + 4 * lane) = acc;
+                if (lane == 0) *reinterpret_cast<f2*>(P.part_ml + 2 * record) = f2{m_c, l_c};
+            } else {
+                float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+                const int ct = column_token(32 * wave + c, P);
+                finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, VF ? R::kOutScale : 1.0f);
+            }
+        }
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_wave_barrier();
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    }
+}
+
+}  // namespace w34

@@ -389,9 +389,8 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 
         // ---- terms, masks, softmax ----
         const bool masked = !(half * 16 >= all_from && half * 16 + 15 <= all_to);  // uniform
-        float x[4], p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x[i] = score_term<CAP>(s[i], cs, cc, P);
+        score_terms<CAP, 4>(s, cs, cc, P);
+        float x[4] = {s[0], s[1], s[2], s[3]}, p[4];
         if (sloped) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-slope2, fabsf((float)(my_pos - (pos + i))), x[i]);
