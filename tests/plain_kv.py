@@ -72,8 +72,9 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                the weights it is 2^-25 of the largest code (in the units of the weights: TQ4 0.17, E4M3 448 / 256, Q8_0 127 / 128),
                which the rotation back adds up to 16 times that.  Values of their own below 2^-14: 2^-25 once more
       output   half a step.
-    chunk: the call's chunk kernel, whose rotated queries and TQ4 keys are one fp16 part (2^-11 and 9.4e-5 of sum |q_i k_i|) and whose
-    weights are one 16-bit part over 16-bit rows (half a step) and over 8-bit rows as they are (and so are those values)."""
+    chunk: the call's chunk kernel, whose rotated queries and TQ4 keys are one fp16 part (2^-11 and 9.4e-5 of sum |q_i k_i|), whose
+    weights are one 16-bit part (half a step) and whose quantised values are fp16(scale * code): 2^-11 of each stored element, or 2^-25
+    below 2^-14, which the rotation back adds up with 1 / 16."""
     fmt, hd, kvh, bs = pool.fmt, pool.head_dim, pool.kv_heads, pool.block_size
     heads = q.shape[1]
     scale = hd ** -0.5 if scale is None else scale
@@ -83,14 +84,14 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
     table = 9.4e-5 if fmt == FMT_TQ4 else 0.0
     weight = 2.0 ** -16 if fmt == FMT_BF16 else 2.0 ** -21
     operand = 2.0 ** -20
+    rounded = 0.0  # of a stored value
     if chunk:
         operand = (2.0 ** -11 if rot_k else 0.0) + table
-        if fmt in (FMT_FP16, FMT_BF16):
-            weight = HALF_STEP[dt]
-        elif fmt != FMT_TQ4 and pool.v_transform != XF_WHT256:
-            weight = 2.0 ** -10
+        weight = HALF_STEP[dt] if fmt in (FMT_FP16, FMT_BF16) else 2.0 ** -11
+        rounded = 0.0 if fmt in (FMT_FP16, FMT_BF16) else 2.0 ** -11
+    rotated_back = pool.v_transform == XF_WHT256 and fmt not in (FMT_FP16, FMT_BF16)
     ride = {FMT_TQ4: 0.17, FMT_FP8: 1.75, FMT_Q8_0: 1.0}.get(fmt, 0.0) * (16.0 if pool.v_transform == XF_WHT256 else 1.0)
-    if chunk and fmt in (FMT_FP8, FMT_Q8_0) and pool.v_transform != XF_WHT256:
+    if chunk:
         ride = 0.0
     for r, s in enumerate(seqs):
         slots = oracle.slot_mapping(bt[r], 0, s, bs) if s else np.zeros(0, dtype=np.int64)
@@ -126,7 +127,7 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                 top = x.max()
                 p = np.exp(x - top)
                 total = p.sum()
-                small = 2.0 ** -25 * (ride * p.size if ride else np.abs(v[seen, g]).sum(0)) / total + 2.0 ** -25
+                small = 2.0 ** -25 * (ride * p.size if ride else np.abs(v[seen, g]).sum(0)) / total + 2.0 ** -25 * (16.0 if rotated_back else 1.0)
                 p = p / total
                 lse[t, h] = top + np.log(total)
                 out[t, h] = p @ v[seen, g]
@@ -136,6 +137,8 @@ def scored_attention(pool, bt, seqs, q, qsl, ctx, *, cap=0.0, slopes=None, windo
                 out_bound[t, h] = moved @ np.abs(v[seen, g]) + HALF_STEP[dt] * np.abs(out[t, h]) + HALF_TINY[dt]
                 if fmt != FMT_BF16:
                     out_bound[t, h] += small
-                if fmt == FMT_TQ4:
-                    out_bound[t, h] += table * (p @ v_sum[seen, g])
+                if rotated_back:
+                    out_bound[t, h] += (table + rounded) * (p @ v_sum[seen, g])
+                else:
+                    out_bound[t, h] += (table + rounded) * (p @ np.abs(v[seen, g]))
     return out, lse, out_bound, lse_bound

@@ -21,9 +21,10 @@ struct ScoredParams {
     const int32_t* document_starts;
     const int32_t* prefix_ends;
     float* lse;
-    float scale2;     // sm_scale log2e
+    float scale2;     // |sm_scale| log2e, not 0 (hidden keys have scores of minus infinity)
+    uint32_t q_flip;  // sm_scale < 0: the sign bits of a pair of query elements
     float cap2;       // cap log2e; 0: no cap
-    float cap_arg;    // 2 sm_scale log2e / cap: exp2 of it times q.k is exp(2 x / cap)
+    float cap_arg;    // 2 |sm_scale| log2e / cap: exp2 of it times q.k is exp(2 x / cap)
     int wide_cap;     // the cap is so large that tanh of a small argument needs its series (kWideCap)
     int num_q_heads, gqa, q_group, q_subgroups;
     int tok_tile;     // query tokens of a tile
@@ -42,24 +43,29 @@ struct ScoredParams {
 // arguments go through the series.
 constexpr float kWideCap = 512.0f;
 
-// N scores in the log2 domain; s: q . k times what the column's scale is in, cs / cc: the column's scale times scale2 / cap_arg.
-// (The choice stands outside the loop: one uniform branch.)
+// Scores s (q . k times what the column's scale is in) become y with x = y ca + cb in the log2 domain, ca >= 0, so that the largest y is
+// the largest x and exp2's argument x - m is one fma.  No cap: y = s, x = y cs.  Cap: y = -1 / (exp(2 x / cap) + 1), x = cap2 + 2 cap2 y.
+// cs >= 0 and cc: the column's scale times scale2 / cap_arg.  (The choice stands outside the loop: one uniform branch.)
+struct ScoreMap {
+    float ca, cb;
+};
 template <bool CAP, int N, typename V>
-__device__ __forceinline__ void score_terms(V& s, float cs, float cc, const ScoredParams& P) {
+__device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const ScoredParams& P) {
     if constexpr (!CAP) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i] *= cs;
+        return ScoreMap{cs, 0.f};
     } else if (!P.wide_cap) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = __builtin_fmaf(-2.0f * P.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[i] * cc) + 1.0f), P.cap2);
+        for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * cc));
+        return ScoreMap{2.0f * P.cap2, P.cap2};
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float a = s[i] * cc, u = a * (0.5f / kLog2e), uu = u * u;
-            const float x = __builtin_fmaf(-2.0f * P.cap2, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a) + 1.0f), P.cap2);
+            const float x = __builtin_fmaf(2.0f * P.cap2, __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(a)), P.cap2);
             const float series = __builtin_fmaf(uu, __builtin_fmaf(uu, __builtin_fmaf(uu, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
             s[i] = fabsf(u) < 0.1f ? s[i] * cs * series : x;
         }
+        return ScoreMap{1.0f, 0.f};
     }
 }
 

@@ -1,5 +1,6 @@
 // Scored paged attention: checks, dispatch and entry points.
 #include <algorithm>
+#include <cmath>
 
 #include "attn_launch.h"
 #include "scored_chunk.h"
@@ -117,21 +118,9 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
         rc = cap ? launch(scored_decode_kernel<TQ, KVF, HD, true>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes)
                  : launch(scored_decode_kernel<TQ, KVF, HD, false>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes);
     } else {
-        using R = ScoredRows<KVF, HD>;
         constexpr int lds = ChunkLds<KVF, HD>::kBytes;
-        const bool ride = R::kTq4 || (!R::k16 && P.rot_out != 0);
-        const auto pick = [&](auto c) {
-            constexpr bool CAP = decltype(c)::value;
-            if constexpr (R::kTq4) {
-                return launch(scored_chunk_kernel<TQ, KVF, HD, CAP, true>, kChunkWaves * 64, lds);
-            } else if constexpr (R::k16) {
-                return launch(scored_chunk_kernel<TQ, KVF, HD, CAP, false>, kChunkWaves * 64, lds);
-            } else {
-                return ride ? launch(scored_chunk_kernel<TQ, KVF, HD, CAP, true>, kChunkWaves * 64, lds)
-                            : launch(scored_chunk_kernel<TQ, KVF, HD, CAP, false>, kChunkWaves * 64, lds);
-            }
-        };
-        rc = cap ? pick(std::true_type{}) : pick(std::false_type{});
+        rc = cap ? launch(scored_chunk_kernel<TQ, KVF, HD, true>, kChunkWaves * 64, lds)
+                 : launch(scored_chunk_kernel<TQ, KVF, HD, false>, kChunkWaves * 64, lds);
     }
     if (rc || slots == 0) return rc;
     hipLaunchKernelGGL((scored_join_kernel<TQ, HD>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P, s.cols,
@@ -161,9 +150,10 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.document_starts = scores->document_starts;
     P.prefix_ends = scores->prefix_ends;
     P.lse = scores->lse_out;
-    P.scale2 = batch->sm_scale * kLog2e;
+    P.scale2 = std::max(std::fabs(batch->sm_scale), 1.0e-30f) * kLog2e;
+    P.q_flip = batch->sm_scale < 0.f ? 0x80008000u : 0u;
     P.cap2 = scores->softcap * kLog2e;
-    P.cap_arg = scores->softcap > 0.f ? 2.0f * batch->sm_scale * kLog2e / scores->softcap : 0.f;
+    P.cap_arg = scores->softcap > 0.f ? 2.0f * std::fabs(batch->sm_scale) * kLog2e / scores->softcap : 0.f;
     P.wide_cap = scores->softcap > kWideCap ? 1 : 0;
     P.num_q_heads = num_q_heads;
     P.gqa = num_q_heads / layout->local_kv_heads;

@@ -24,6 +24,9 @@ typedef __attribute__((address_space(3))) const f4 lds_f4c;
 constexpr int kChunkWaves = 8;
 constexpr int kChunkCols = 32 * kChunkWaves;
 constexpr int kChunkUnit = 32;
+// A column's maximum is raised only by scores that exceed it by more than this (log2 domain): a weight may be up to 2^8, which costs
+// none of its bits, and the multiplication of 128 sums a lane is spared in nearly all units.
+constexpr float kChunkSlack = 8.0f;
 
 template <bool IS_BF16>
 __device__ __forceinline__ f16v mfma_tile(u4 a, u4 b, f16v c) {
@@ -38,6 +41,11 @@ template <int IMM>
 __device__ __forceinline__ void load_to_lds(uint32_t voffset, const uint8_t* base, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 offset:%3" : : "v"(voffset), "s"(base), "s"(lds), "n"(IMM) : "memory");
 }
+// The value again where it is asked for: what follows from it is worked out anew in every unit and not kept in registers.
+__device__ __forceinline__ int here(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
 __device__ __forceinline__ const uint8_t* uniform_pointer(const uint8_t* p) {
     const uint64_t a = (uint64_t)(uintptr_t)p;
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)a), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32));
@@ -46,6 +54,7 @@ __device__ __forceinline__ const uint8_t* uniform_pointer(const uint8_t* p) {
 __device__ __forceinline__ void chunk_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 __device__ __forceinline__ u4 lds_u4(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const u4*>((uintptr_t)at); }
 __device__ __forceinline__ uint32_t lds_u1(uint32_t at) { return *reinterpret_cast<lds_cu32*>((uintptr_t)at); }
+__device__ __forceinline__ uint32_t lds_u16(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)at); }
 __device__ __forceinline__ f4 lds_f4(uint32_t at) { return *reinterpret_cast<lds_f4c*>((uintptr_t)at); }
 __device__ __forceinline__ void lds_put(uint32_t at, u4 v) { *reinterpret_cast<__attribute__((address_space(3))) u4*>((uintptr_t)at) = v; }
 
@@ -59,8 +68,8 @@ struct ChunkLds {
     static constexpr int kRun = 16 * R::kRowBytes;            // of a page
     static constexpr int kRawUnit = R::k16 ? 0 : (4 * kRun + 16);
     static constexpr int kRaw = kTiles + 4 * kTile;           // two units of {keys 0-15, 16-31, values 0-15, 16-31} as stored
-    static constexpr int kScale = kRaw + 2 * kRawUnit;        // two units of {key scales [4][32], value scales [4][32]}
-    static constexpr int kLoop = kScale + (R::k16 ? 0 : 2 * 2 * 4 * 32 * 4);
+    static constexpr int kScale = kRaw + 2 * kRawUnit;        // two units of key scales [4][32]
+    static constexpr int kLoop = kScale + (R::k16 ? 0 : 2 * 4 * 32 * 4);
     // before the loop: tile counts of the batch; eight query columns of each wave at a time.  After it: eight columns of sums.
     static constexpr int kColStride = HD + 8;
     static constexpr int kCounts = kTiles + kChunkWaves * 8 * kColStride * 4;
@@ -70,10 +79,11 @@ struct ChunkLds {
     static_assert(kBytes <= 160 * 1024 && kRun % 16 == 0, "chunk LDS budget");
 };
 
-// VF: the values' block scales ride on the weights, which then have two fp16 parts (TQ4; rotated 8-bit rows: values rounded as
-// fp16(d * code) have errors in common where a block holds few codes, which the rotation back gathers in one channel).  Otherwise 8-bit
-// values are fp16(d * code) and weights one operand.
-template <typename TQ, int KVF, int HD, bool CAP, bool VF>
+// Roundings, beside those of the inputs' types: rotated queries and TQ4 keys are one fp16 part (the keys' block scales multiply the
+// scores in 32 bits); quantised values are fp16(scale * code), TQ4 ones from the fp16 table; weights are one operand of the values'
+// type.  (Weights that carry the block scales would spare the values' rounding and need two parts, half as many products again: a
+// block-wide error of a weight is gathered in one channel by the rotation back.)
+template <typename TQ, int KVF, int HD, bool CAP>
 __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const ScoredParams P) {
     extern __shared__ __align__(16) uint8_t smem[];
     using R = ScoredRows<KVF, HD>;
@@ -157,7 +167,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         const uint16_t* src = P.q + ((size_t)my_tok * P.num_q_heads + (size_t)my_head) * HD + 8 * b;
 #pragma unroll
         for (int m = 0; m < kSteps; ++m) {
-            q[m] = *reinterpret_cast<const u4*>(src + 16 * m);
+            q[m] = *reinterpret_cast<const u4*>(src + 16 * m) ^ P.q_flip;
             if (!col_ok) q[m] = u4{0u, 0u, 0u, 0u};
         }
     } else {
@@ -172,7 +182,8 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                 float v[4] = {0.f, 0.f, 0.f, 0.f};
                 if ((live >> c) & 1u) {
                     const uint16_t* src = P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + 4 * lane;
-                    const uint2 raw = *reinterpret_cast<const uint2*>(src);
+                    uint2 raw = *reinterpret_cast<const uint2*>(src);
+                    raw.x ^= P.q_flip, raw.y ^= P.q_flip;
                     v[0] = TQ::to_f32((uint16_t)raw.x), v[1] = TQ::to_f32((uint16_t)(raw.x >> 16));
                     v[2] = TQ::to_f32((uint16_t)raw.y), v[3] = TQ::to_f32((uint16_t)(raw.y >> 16));
                 }
@@ -184,7 +195,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                 float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
                 for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-                const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+                const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
                 *reinterpret_cast<uint2*>(area + c8 * M::kColStride + 4 * lane) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
@@ -234,7 +245,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             // rows 8 part + ..: the piece that belongs to a lane's place
             constexpr int kPieces = M::kRow / 16, kRows = 64 / kPieces;  // of a row, of an instruction
             const uint32_t dst = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile + (loads_v ? M::kTile : 0) + (run & 1) * M::kRun + part * kShare);
-            const int r = lane / kPieces, p = lane % kPieces;
+            const int at_lane = here(lane), r = at_lane / kPieces, p = at_lane % kPieces;
             const auto one = [&](auto imm) {
                 constexpr int i = decltype(imm)::value;
                 const int row = 8 * part + i * kRows + r;
@@ -248,7 +259,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                 one(std::integral_constant<int, 3>{});
             }
         } else {
-            const uint32_t dst = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit + run * M::kRun + part * kShare), v = 16u * (uint32_t)lane;
+            const uint32_t dst = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit + run * M::kRun + part * kShare), v = 16u * (uint32_t)here(lane);
             load_to_lds<0>(v, src, dst);
             if constexpr (kShare >= 2048) load_to_lds<1024>(v, src, dst);
             constexpr int kRest = kShare % 1024;
@@ -259,8 +270,8 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const auto widen = [&](int u) {
         if constexpr (!R::k16) {
             const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit), tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
-            const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 1024);
-            const int r = tid >> 4, c = tid & 15;
+            const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 512);
+            const int at_tid = here(tid), r = at_tid >> 4, c = at_tid & 15;
             const int row_pos = begin + u * kChunkUnit + r;
             const bool seen = row_pos >= key_first && row_pos <= key_last;
 #pragma unroll
@@ -272,20 +283,27 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                     const uint32_t at = src + (c >= 8 ? 68u : 0u) + 8u * (c & 7);
                     const uint32_t shift = c >= 8 ? 0u : 16u, d0 = lds_u1(at), d1 = lds_u1(at + 4), d2 = lds_u1(at + 8);
                     uint32_t codes[2] = {__builtin_amdgcn_alignbit(d1, d0, shift), __builtin_amdgcn_alignbit(d2, d1, shift)};
-                    const uint32_t lut_lane = (uint32_t)lane << 2;
+                    const uint32_t lut_lane = ((uint32_t)at_tid & 63u) << 2;
+                    const uint32_t d16 = side == 1 && seen ? lds_u16(src + (c >= 8 ? 66u : 0u)) : 0u;
+                    const h2 d = __builtin_bit_cast(h2, d16 | d16 << 16);
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) w[h][k] = lut_read(codes[h], lut_lane, 0x0c0c0400u + ((uint32_t)k << 8));
+                        for (int k = 0; k < 4; ++k) {
+                            // (a scalar in between: a bit cast of a vector's element reads its first one)
+                            uint32_t pair = lut_read(codes[h], lut_lane, 0x0c0c0400u + ((uint32_t)k << 8));
+                            if (side == 1) pair = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) * d);
+                            w[h][k] = pair;
+                        }
                 } else {
                     const uint32_t at = R::kFp8 ? src + 16u * c : src + 68u * (c >> 2) + 4u + 16u * (c & 3);
-                    const float d = side == 1 && !VF ? __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * (c >> 3) : src + 68u * (c >> 2))) : 1.f;
+                    const float d = side == 1 ? __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * (c >> 3) : src + 68u * (c >> 2))) : 1.f;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         uint32_t code = lds_u1(at + 4 * k);
                         if (side == 1) code = seen ? code : 0u;
                         uint32_t x, y;
-                        if (side == 1 && !VF) {
+                        if (side == 1) {
                             float f[4];
                             if constexpr (R::kFp8) {
                                 const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), s = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
@@ -298,19 +316,13 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                             x = pack_h2(f[0] * dd, f[1] * dd);
                             y = pack_h2(f[2] * dd, f[3] * dd);
                         } else if constexpr (R::kFp8) {
-                            if (side == 0) {
-                                x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, false));
-                                y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, true));
-                            } else {
-                                x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 0.00390625f, false));
-                                y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 0.00390625f, true));
-                            }
-                        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16, 0x4800 | (q + 128) is 9 + q / 128
-                            const uint32_t u8 = code ^ 0x80808080u, one = side == 0 ? 0x64646464u : 0x48484848u;
-                            const _Float16 zero = side == 0 ? (_Float16)1152.0f : (_Float16)9.0f;
-                            const h2 bias = {zero, zero};
-                            x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, u8, 0x04010400u)) - bias);
-                            y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(one, u8, 0x04030402u)) - bias);
+                            x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, false));
+                            y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, true));
+                        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
+                            const uint32_t u8 = code ^ 0x80808080u;
+                            const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+                            x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04010400u)) - bias);
+                            y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04030402u)) - bias);
                         }
                         w[k >> 1][2 * (k & 1)] = x;
                         w[k >> 1][2 * (k & 1) + 1] = y;
@@ -322,22 +334,12 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                     lds_put(tiles + (uint32_t)(side * M::kTile + r * M::kRow + 16 * (p ^ (side ? 4 * (r & 3) : (r & 15)))), w[h]);
                 }
             }
-            // scales: [block][row] of the keys, then of the values
-            constexpr int kKinds = VF ? 2 : 1;
-            if (tid < kKinds * R::kScales * 32) {
-                const int side = tid / (R::kScales * 32), blk = tid / 32 % R::kScales, row = tid & 31;
-                const uint32_t src = raw + (uint32_t)(side * 2 * M::kRun + row * R::kRowBytes);
-                float d;
-                if constexpr (R::kTq4) {
-                    d = F16::to_f32(*reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)(src + 66u * blk)));
-                } else {
-                    d = __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * blk : src + 68u * blk));
-                }
-                if (side == 1) {
-                    const int p = begin + u * kChunkUnit + row;
-                    d = p >= key_first && p <= key_last ? d * R::kValueGain : 0.f;
-                }
-                *reinterpret_cast<__attribute__((address_space(3))) float*>((uintptr_t)(scale + (uint32_t)(side * 512 + blk * 128 + 4 * row))) = d;
+            // key scales: [block][row]
+            if (at_tid < R::kScales * 32) {
+                const int blk = at_tid / 32, row = at_tid & 31;
+                const uint32_t src = raw + (uint32_t)(row * R::kRowBytes);
+                const float d = R::kTq4 ? F16::to_f32((uint16_t)lds_u16(src + 66u * blk)) : __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * blk : src + 68u * blk));
+                *reinterpret_cast<__attribute__((address_space(3))) float*>((uintptr_t)(scale + (uint32_t)(blk * 128 + 4 * row))) = d;
             }
         }
     };
@@ -350,10 +352,11 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     float m_run = kNegBig, l_run = 0.f;
 
     const auto multiply = [&](int u) {
+        const int at_lane = here(lane), n = at_lane & 31, b = at_lane >> 5;
         const int u0 = begin + u * kChunkUnit;
         if (u0 > any_to || u0 + kChunkUnit - 1 < any_from) return;  // uniform
         const uint32_t tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
-        const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 1024);
+        const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 512);
         // ---- scores ----
         f16v s;
         {
@@ -384,11 +387,13 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         __builtin_amdgcn_sched_barrier(0);
         // ---- terms, masks, softmax ----
         const bool masked = !(u0 >= all_from && u0 + kChunkUnit - 1 <= all_to);  // uniform
-        score_terms<CAP, 16>(s, cs, cc, P);
+        ScoreMap map = map_scores<CAP, 16>(s, cs, cc, P);
         if (sloped) {
             const float at = (float)(my_pos - u0 - 4 * b);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[i] = __builtin_fmaf(-slope2, fabsf(at - (float)((i & 3) + 8 * (i >> 2))), s[i]);
+            for (int i = 0; i < 16; ++i)
+                s[i] = __builtin_fmaf(-slope2, fabsf(at - (float)((i & 3) + 8 * (i >> 2))), __builtin_fmaf(s[i], map.ca, map.cb));
+            map = ScoreMap{1.0f, 0.f};
         }
         if (masked) {
             const int from = lo - u0 - 4 * b, to = hi - u0 - 4 * b;
@@ -405,26 +410,28 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
             top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
         }
-        if (__ballot(top > m_run) != 0ull) {
-            const float m_new = fmaxf(m_run, top);
+        top = __builtin_fmaf(top, map.ca, map.cb);
+        if (__ballot(top > m_run + kChunkSlack) != 0ull) {
+            const float m_new = top > m_run + kChunkSlack ? top : m_run;
             const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
             m_run = m_new;
             l_run *= alpha;
 #pragma unroll
             for (int k = 0; k < kDims; ++k) o[k] *= alpha;
         }
+        const float less = map.cb - m_run;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            s[i] = __builtin_amdgcn_exp2f(s[i] - m_run);
+            s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], map.ca, less));
             sum += s[i];
         }
         l_run += sum;
         __builtin_amdgcn_sched_barrier(0);
         // ---- values ----
         // lane l reads row (l & 15) >> 2 of four, 8 bytes at 8 (l & 3) of the 32 of its 16 channels
-        const int j = lane & 15;
-        const uint32_t v_at = tiles + (uint32_t)(M::kTile + (4 * b + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
+        const int j = at_lane & 15;
+        const uint32_t v_at = tiles + (uint32_t)(M::kTile + (4 * b + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(at_lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
         const auto v_operand = [&](int dt, int step) -> u4 {
             const uint32_t at = (v_at ^ (64u * (uint32_t)(dt & 3))) + 256u * (uint32_t)(dt >> 2) + (uint32_t)(step * 16 * M::kRow);
             const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
@@ -432,33 +439,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             const u2v x = __builtin_bit_cast(u2v, a), y = __builtin_bit_cast(u2v, c);
             return u4{x[0], x[1], y[0], y[1]};
         };
-        if constexpr (VF) {
-            constexpr int kPerGroup = kDims / R::kGroups;
-#pragma unroll
-            for (int g = 0; g < R::kGroups; ++g) {
-                u4 high[2], low[2];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const f4 d = lds_f4(scale + (uint32_t)(512 + 128 * g + 32 * k + 16 * b));
-                    float w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = mul_legacy(s[4 * k + i], d[i]);
-                    uint32_t h0, h1, l0, l1;
-                    split_weights(w[0], w[1], h0, l0);
-                    split_weights(w[2], w[3], h1, l1);
-                    high[k >> 1][2 * (k & 1)] = h0, high[k >> 1][2 * (k & 1) + 1] = h1;
-                    low[k >> 1][2 * (k & 1)] = l0, low[k >> 1][2 * (k & 1) + 1] = l1;
-                }
-#pragma unroll
-                for (int dt = g * kPerGroup; dt < (g + 1) * kPerGroup; ++dt)
-#pragma unroll
-                    for (int step = 0; step < 2; ++step) {
-                        const u4 a = v_operand(dt, step);
-                        o[dt] = mfma_tile<false>(a, high[step], o[dt]);
-                        o[dt] = mfma_tile<false>(a, low[step], o[dt]);
-                    }
-            }
-        } else {
+        {
             u4 w[2];
 #pragma unroll
             for (int k = 0; k < 8; ++k) w[k >> 2][k & 3] = IS_BF16 ? pack_bf2(s[2 * k], s[2 * k + 1]) : pack_h2(s[2 * k], s[2 * k + 1]);
@@ -537,7 +518,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             } else {
                 float v[4] = {acc[0], acc[1], acc[2], acc[3]};
                 const int ct = column_token(32 * wave + c, P);
-                finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, VF ? R::kOutScale : 1.0f);
+                finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, R::kOutScale);
             }
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);

@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         const uint16_t* src = P.q + ((size_t)my_tok * P.num_q_heads + (size_t)min(my_head, P.num_q_heads - 1)) * HD;
 #pragma unroll
         for (int m = 0; m < R::kOps; ++m) {
-            q_high[m] = *reinterpret_cast<const u4*>(src + R::element(m, b));
+            q_high[m] = *reinterpret_cast<const u4*>(src + R::element(m, b)) ^ P.q_flip;
             if (!col_ok) q_high[m] = u4{0u, 0u, 0u, 0u};
         }
     } else {
@@ -199,7 +199,8 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
             float v[4] = {0.f, 0.f, 0.f, 0.f};
             if ((live >> c) & 1u) {
                 const uint16_t* src = P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + c - ct * P.q_group)) * HD + 4 * lane;
-                const uint2 raw = *reinterpret_cast<const uint2*>(src);
+                uint2 raw = *reinterpret_cast<const uint2*>(src);
+                raw.x ^= P.q_flip, raw.y ^= P.q_flip;
                 v[0] = TQ::to_f32((uint16_t)raw.x), v[1] = TQ::to_f32((uint16_t)(raw.x >> 16));
                 v[2] = TQ::to_f32((uint16_t)raw.y), v[3] = TQ::to_f32((uint16_t)(raw.y >> 16));
             }
@@ -211,7 +212,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
             float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-            const int e = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+            const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
             uint32_t h0, h1, l0, l1;
@@ -389,24 +390,25 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 
         // ---- terms, masks, softmax ----
         const bool masked = !(half * 16 >= all_from && half * 16 + 15 <= all_to);  // uniform
-        score_terms<CAP, 4>(s, cs, cc, P);
+        ScoreMap map = map_scores<CAP, 4>(s, cs, cc, P);
         float x[4] = {s[0], s[1], s[2], s[3]}, p[4];
         if (sloped) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-slope2, fabsf((float)(my_pos - (pos + i))), x[i]);
+            for (int i = 0; i < 4; ++i) x[i] = __builtin_fmaf(-slope2, fabsf((float)(my_pos - (pos + i))), __builtin_fmaf(x[i], map.ca, map.cb));
+            map = ScoreMap{1.0f, 0.f};
         }
         if (masked) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) x[i] = pos + i >= lo && pos + i <= hi ? x[i] : -INFINITY;
         }
         const float top = max_over_rows(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-        const float m_new = fmaxf(m_run, top);
+        const float m_new = fmaxf(m_run, __builtin_fmaf(top, map.ca, map.cb));
         const float alpha = __builtin_amdgcn_exp2f(m_run - m_new);
         m_run = m_new;
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            p[i] = __builtin_amdgcn_exp2f(x[i] - m_new);
+            p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i], map.ca, map.cb - m_new));
             sum += p[i];
         }
         l_run = l_run * alpha + sum;
