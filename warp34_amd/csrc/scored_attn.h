@@ -31,10 +31,12 @@ struct ScoredParams {
     int tiles;        // tiles of a request (a bound)
     int entries;      // requests x tiles: tiles of the batch, some of them empty
     int target;       // slots for chunks, for each kv head; 0: no split, a workgroup for each entry
+    int rounds;       // chunks of 1 / (128 rounds) of all keys; 0: no more chunks than target
+    int records;      // partial records the scratch holds, for each kv head
     int min_halves;   // shortest chunk
-    float* part_acc;  // [slot][kv_sub][column][head_dim]
-    float* part_ml;   // [slot][kv_sub][column]{m, l}
-    int32_t* table;   // [entry]{first slot, chunks}
+    float* part_acc;  // [record][kv_sub][column][head_dim]
+    float* part_ml;   // [record][kv_sub][column]{m, l}
+    int32_t* table;   // [entry]{first record, chunks}
     uint32_t block_magic, q_group_magic;
     int rot_q, rot_out;
 };
@@ -100,82 +102,129 @@ __device__ __forceinline__ ScoredTile scored_tile(const ScoredParams& P, int ent
     const int tokens = min(min(hi - lo - first, P.tok_tile), B.total_tokens - lo - first);
     return ScoredTile{req, lo + first, valid && lo >= 0 ? max(tokens, 0) : 0, ctx + first, seq};
 }
-// First and last key that any token of a tile sees; first > last where none does.
-__device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int& first, int& last) {
+// Sums and largest numbers of a wave by lane shifts inside the vector unit (an exchange through LDS takes a hundred cycles a step).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int shifted_in(int old, int v) { return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xF, false); }
+template <typename F>
+__device__ __forceinline__ int wave_scan(int v, int none, F&& f) {  // inclusive; none: what changes nothing
+    v = f(v, shifted_in<0x111, 0xF>(none, v));  // row_shr:1, 2, 4, 8
+    v = f(v, shifted_in<0x112, 0xF>(none, v));
+    v = f(v, shifted_in<0x114, 0xF>(none, v));
+    v = f(v, shifted_in<0x118, 0xF>(none, v));
+    v = f(v, shifted_in<0x142, 0xA>(none, v));  // row_bcast:15 into rows 1 and 3, row_bcast:31 into rows 2 and 3
+    return f(v, shifted_in<0x143, 0xC>(none, v));
+}
+__device__ __forceinline__ int wave_prefix(int v) {
+    return wave_scan(v, 0, [](int a, int b) { return a + b; });
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_prefix(v), 63); }
+__device__ __forceinline__ int wave_largest(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, (int)0x80000000, [](int a, int b) { return max(a, b); }), 63);
+}
+__device__ __forceinline__ int wave_least(int v) {
+    return __builtin_amdgcn_readlane(wave_scan(v, 0x7fffffff, [](int a, int b) { return min(a, b); }), 63);
+}
+// The largest of a wave's numbers >= 0, in all lanes.
+__device__ __forceinline__ float wave_top(float v) {
+    return __int_as_float(wave_largest(__float_as_int(v)));
+}
+
+// First and last key that any token of a tile sees; first > last where none does.  A lane a token.
+__device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int lane, int& first, int& last) {
+    int lo, hi;
     if (P.document_starts == nullptr && P.prefix_ends == nullptr) {  // the first token's window, the last one's reach
-        int lo, hi;
         token_keys(P, t.tok0, t.pos0, t.seq_after, first, hi);
         token_keys(P, t.tok0, t.pos0 + t.tokens - 1, t.seq_after, lo, last);
-        return;
-    }
-    first = 0x7fffffff;
-    last = -1;
-    for (int k = 0; k < t.tokens; ++k) {
-        int lo, hi;
-        token_keys(P, t.tok0 + k, t.pos0 + k, t.seq_after, lo, hi);
-        if (lo <= hi) {
-            first = min(first, lo);
-            last = max(last, hi);
+    } else {
+        first = 0x7fffffff;
+        last = -1;
+        for (int k = lane; k < t.tokens; k += 64) {
+            token_keys(P, t.tok0 + k, t.pos0 + k, t.seq_after, lo, hi);
+            if (lo <= hi) {
+                first = min(first, lo);
+                last = max(last, hi);
+            }
         }
+        first = wave_least(first);
+        last = wave_largest(last);
     }
+    first = __builtin_amdgcn_readfirstlane(first);
+    last = __builtin_amdgcn_readfirstlane(last);
+}
+// The half units of a tile as the cut of a batch counts them: by its first and last token.  (Tokens between them may see others; then the
+// tile's chunks are longer or shorter, and no less right.)
+__device__ __forceinline__ int tile_halves_guess(const ScoredParams& P, const ScoredTile& t) {
+    if (t.tokens <= 0) return -1;
+    int lo0, hi0, lo1, hi1;
+    token_keys(P, t.tok0, t.pos0, t.seq_after, lo0, hi0);
+    token_keys(P, t.tok0 + t.tokens - 1, t.pos0 + t.tokens - 1, t.seq_after, lo1, hi1);
+    const int first = min(lo0, lo1), last = max(hi0, hi1);
+    return first <= last ? (last >> 4) - (first >> 4) + 1 : 0;
 }
 // Half units: 16 keys from a multiple of 16 on, which lie in one page.
 __device__ __forceinline__ int tile_halves(int first, int last) { return first <= last ? (last >> 4) - (first >> 4) + 1 : 0; }
 
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
-__device__ __forceinline__ int wave_prefix(int v, int lane) {  // inclusive
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d, 64);
-        v += lane >= d ? u : 0;
-    }
-    return v;
-}
-
-// The cut of a batch: chunks of `per` half units, the shortest length with which all tiles together need no more than P.target chunks;
-// a live tile has at least one.  halves: [entries] in LDS, -1 for tiles without tokens.
-constexpr int kMaxSplitEntries = 512;   // entries of a batch that is split
+// The cut of a batch.  All tiles have chunks of up to `per` half units, a tile's chunks are of one length, and a live tile has one at
+// least.  P.rounds == 0: the shortest `per` that needs no more than P.target chunks.  Otherwise a fixed share of all keys, so that the
+// workgroups, which start as others end, end together.  Tiles with several chunks have a record for each: no more than the scratch holds.
+// count(e): the half units of entry e, -1 for tiles without tokens.
+constexpr int kMaxSplitEntries = 512;  // entries of a batch that is split
+constexpr int kSlotRound = 128;        // slots for each kv head that fill the chip where there are two
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
-__device__ __forceinline__ int chunk_length(const ScoredParams& P, const int* halves, int lane) {
-    int total = 0, live = 0, longest = 0;
+template <typename Count>
+__device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Count&& count) {
+    int total = 0, live = 0;
     for (int e = lane; e < P.entries; e += 64) {
-        total += max(halves[e], 0);
-        live += halves[e] >= 0 ? 1 : 0;
-        longest = max(longest, halves[e]);
+        const int h = count(e);
+        total += max(h, 0);
+        live += h >= 0 ? 1 : 0;
     }
-    total = __builtin_amdgcn_readfirstlane(wave_sum(total));
-    live = __builtin_amdgcn_readfirstlane(wave_sum(live));
-    // too short / long enough: sum of ceil(h / per) <= total / per + live
-    int low = max(P.min_halves, (total + P.target - 1) / P.target) - 1;
-    int high = max(low + 1, (total + P.target - live - 1) / max(P.target - live, 1));
-    while (high - low > 1 && P.entries <= 64) {
+    total = wave_sum(total);
+    live = wave_sum(live);
+    const auto fits = [&](int per) {
+        int n = 0, several = 0;
+        for (int e = lane; e < P.entries; e += 64) {
+            const int c = chunks_of(count(e), per);
+            n += c;
+            several += c > 1 ? c : 0;
+        }
+        return wave_sum(n) <= P.target && wave_sum(several) <= P.records;
+    };
+    // (with a round of tiles or more there is something for every CU without a cut: only what is longer than a CU's share is cut)
+    const int share = P.rounds > 0 ? (live < kSlotRound ? P.rounds : 1) * kSlotRound : P.target;
+    int per = max(P.min_halves, (total + share - 1) / share);
+    if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per)) return per;
+    // sum of ceil(h / per) <= total / per + live, so this many halves a chunk are enough for any number of slots above live
+    int low = per, high = max(per + 1, (total + max(P.target - live, 1) - 1) / max(P.target - live, 1));
+    while (!fits(high)) {
+        low = high;
+        high *= 2;
+    }
+    while (high - low > max(1, low >> 5)) {
         const int mid = (low + high) >> 1;
-        const int n = wave_sum(lane < P.entries ? chunks_of(halves[lane], mid) : 0);
-        if (__builtin_amdgcn_readfirstlane(n) <= P.target) high = mid;
+        if (fits(mid)) high = mid;
         else low = mid;
     }
     return high;
 }
-// The tile and chunk of a slot; entry -1: the slot stays empty.
+// The tile and chunk of a slot, and the record of the tile's first chunk; entry -1: the slot stays empty.
 struct ScoredWork {
-    int entry, chunk, chunks, first_slot;
+    int entry, chunk, chunks, first_record;
 };
-__device__ __forceinline__ ScoredWork find_work(const ScoredParams& P, const int* halves, int per, int slot, int lane) {
-    int before = 0;
+template <typename Count>
+__device__ __forceinline__ ScoredWork find_work(const ScoredParams& P, int per, int slot, int lane, Count&& count) {
+    int before = 0, records = 0;
     for (int base = 0; base < P.entries; base += 64) {
-        const int mine = base + lane < P.entries ? chunks_of(halves[base + lane], per) : 0;
-        const int upto = before + wave_prefix(mine, lane);
+        const int mine = base + lane < P.entries ? chunks_of(count(base + lane), per) : 0, split = mine > 1 ? mine : 0;
+        const int upto = before + wave_prefix(mine), records_upto = records + wave_prefix(split);
         const unsigned long long hit = __ballot(slot < upto);
         if (hit != 0ull) {
             const int l = (int)__builtin_ctzll(hit);
             const int n = __builtin_amdgcn_readlane(mine, l), end = __builtin_amdgcn_readlane(upto, l);
-            return ScoredWork{base + l, slot - (end - n), n, end - n};
+            return ScoredWork{base + l, slot - (end - n), n, __builtin_amdgcn_readlane(records_upto, l) - n};
         }
         before = __builtin_amdgcn_readlane(upto, 63);
+        records = __builtin_amdgcn_readlane(records_upto, 63);
     }
     return ScoredWork{-1, 0, 0, 0};
 }
@@ -200,20 +249,23 @@ __device__ __forceinline__ void finish_row(const ScoredParams& P, int tok, int h
     if (P.lse != nullptr && lane == 0) P.lse[row] = l > 0.f || l != l ? (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f : -INFINITY;
 }
 
-// Joins the chunks of a row: a workgroup of eight waves for each column of each tile that has several; wave w adds up chunks w, w + 8, ...
-template <typename TQ, int HD>
+// Joins the chunks of rows.  SPREAD: a workgroup of eight waves for each column of each tile, wave w adds up chunks w, w + 8, ... (one
+// request has up to 128 chunks).  Otherwise a wave a column, eight columns a workgroup: many tiles of few chunks (a workgroup for each of
+// the 131 072 columns of 256 tiles and two kv heads, nearly all of which have nothing to do, took 190 us).
+template <typename TQ, int HD, bool SPREAD>
 __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, int columns, float value_scale) {
-    __shared__ __align__(16) float sums[8][HD];
-    const int entry = (int)blockIdx.x, kv_sub = (int)blockIdx.y, col = (int)blockIdx.z;
+    __shared__ __align__(16) float sums[SPREAD ? 8 : 1][SPREAD ? HD : 4];
+    const int entry = (int)blockIdx.x, kv_sub = (int)blockIdx.y;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int col = SPREAD ? (int)blockIdx.z : 8 * (int)blockIdx.z + wave;
     const ScoredTile t = scored_tile(P, entry);
     const int mine = column_token(col, P);
     if (mine >= t.tokens) return;
-    const int tok = t.tok0 + mine;
-    if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) return;
     const int first = P.table[2 * entry], chunks = P.table[2 * entry + 1];
     if (chunks <= 1) return;
+    const int tok = t.tok0 + mine;
+    if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) return;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
     const auto record = [&](int c) { return ((size_t)(first + c) * kv_subs + kv_sub) * columns + col; };
     float m = kNegBig;
@@ -223,33 +275,40 @@ __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, 
     f4 acc = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
     const int at = (4 * lane) & (HD - 1);
+    constexpr int kStep = SPREAD ? 8 : 1;
+    const int own = SPREAD ? wave : 0;
     for (int base = 0; base < chunks; base += 64) {
         const int c = base + lane;
         f2 ml = {kNegBig, 0.f};
         if (c < chunks) ml = *reinterpret_cast<const f2*>(P.part_ml + 2 * record(c));
         const float w = __builtin_amdgcn_exp2f(ml[0] - m);
         l += ml[1] * w;
-        // a wave's eight records at most, their loads together
         const int end = min(64, chunks - base);
-        f4 part[8];
+        for (int from = own; from < end; from += 8 * kStep) {  // eight records at a time, their loads together
+            f4 part[8];
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (wave + 8 * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + wave + 8 * k) * HD + at);
+            for (int k = 0; k < 8; ++k)
+                if (from + kStep * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + from + kStep * k) * HD + at);
 #pragma unroll
-        for (int k = 0; k < 8; ++k)
-            if (wave + 8 * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), wave + 8 * k));
+            for (int k = 0; k < 8; ++k)
+                if (from + kStep * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from + kStep * k));
+        }
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    if (4 * lane < HD) *reinterpret_cast<f4*>(&sums[wave][at]) = acc;
-    __syncthreads();
-    if (wave != 0) return;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+    if constexpr (SPREAD) {
+        if (4 * lane < HD) *reinterpret_cast<f4*>(&sums[wave][at]) = acc;
+        __syncthreads();
+        if (wave != 0) return;
 #pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        const f4 s = *reinterpret_cast<const f4*>(&sums[w][at]);
+        for (int k = 0; k < 4; ++k) v[k] = 0.f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] += s[k];
+        for (int w = 0; w < 8; ++w) {
+            const f4 s = *reinterpret_cast<const f4*>(&sums[w][at]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] += s[k];
+        }
     }
     const int head = (kv_sub / P.q_subgroups) * P.gqa + (kv_sub % P.q_subgroups) * P.q_group + (col - mine * P.q_group);
     finish_row<TQ, HD>(P, tok, head, lane, v, m, l, value_scale);

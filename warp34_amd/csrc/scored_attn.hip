@@ -8,21 +8,20 @@
 
 namespace w34 {
 
-constexpr int kScoredSlots = 128;       // chunks for each kv head of a batch of up to 64 tiles: with two kv heads one for every CU
-constexpr int kScoredSplitTiles = 512;  // from here on a kv head's tiles fill the chip by themselves
 constexpr int kDecodeCols = 16;         // query columns of a workgroup of the decode kernel
 constexpr int kDecodeMinHalves = 8;     // shortest chunk: a half unit for each wave
-constexpr int kChunkMinHalves = 16;     // eight units
+constexpr int kChunkMinHalves = 64;     // 32 units
+constexpr int kDecodeRounds = 4, kChunkRounds = 2;
 
 // Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
 constexpr int kChunkFrom = 128;
 
-// The tiles of a batch: the kernel, a tile's tokens, tiles of a request, chunk slots for each kv head (0: no split).
+// The tiles of a batch: the kernel, a tile's tokens, tiles of a request, slots for each kv head (0: no split).
 struct ScoredShape {
     bool chunk;
     int cols, tok_tile;
     long long tiles, entries;
-    int slots;
+    int slots, rounds;
 };
 static ScoredShape scored_shape(int num_reqs, int total_tokens, int max_q_len, int q_group) {
     ScoredShape s;
@@ -32,15 +31,12 @@ static ScoredShape scored_shape(int num_reqs, int total_tokens, int max_q_len, i
     s.tok_tile = s.cols / q_group;
     s.tiles = ((long long)q_len + s.tok_tile - 1) / s.tok_tile;
     s.entries = s.tiles * num_reqs;
-    s.slots = 0;
-    if (s.chunk) {
-        if (s.entries < kScoredSlots) s.slots = kScoredSlots;
-    } else if (s.entries < kScoredSplitTiles) {
-        s.slots = kScoredSlots * (int)((std::max<long long>(2 * s.entries, kScoredSlots) + kScoredSlots - 1) / kScoredSlots);
-    }
+    // Decode batches of up to 64 tiles: at most 128 chunks for each kv head, which two kv heads run in one round.  Others: chunks of a
+    // fixed share of the keys, and as many slots as that may need.
+    s.rounds = s.chunk ? kChunkRounds : s.entries <= 64 ? 0 : kDecodeRounds;
+    s.slots = s.entries > kMaxSplitEntries ? 0 : s.rounds == 0 ? kSlotRound : (int)(s.rounds * kSlotRound + s.entries);
     return s;
 }
-static_assert(kScoredSplitTiles <= kMaxSplitEntries, "tile counts in LDS");
 // Bytes of the partial records of a slot, and of the tiles' table.
 static size_t scored_slot_bytes(const ScoredShape& s, int kv_subs, int head_dim) { return (size_t)kv_subs * s.cols * (size_t)(head_dim + 2) * 4; }
 static size_t scored_table_bytes(long long entries) { return ((size_t)entries * 8 + 15) / 16 * 16; }
@@ -87,22 +83,24 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     P.tiles = (int)s.tiles;
     P.entries = (int)s.entries;
     P.min_halves = s.chunk ? kChunkMinHalves : kDecodeMinHalves;
-    // chunks: as many as the scratch holds, none where a tile has too few keys for two
-    long long slots = s.slots;
+    // records: as many as the scratch holds; no split where a tile has too few keys for two chunks
+    long long slots = s.slots, records = 0;
     const size_t table = scored_table_bytes(s.entries);
-    if (ex->scratch_ptr == 0 || (ex->scratch_ptr & 15u) != 0 || ex->scratch_size <= table) slots = 0;
-    else slots = std::min<long long>(slots, (long long)((ex->scratch_size - table) / scored_slot_bytes(s, kv_subs, HD)));
-    if (B.max_seq_len > 0) {
+    if (ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0 && ex->scratch_size > table)
+        records = std::min<long long>(slots, (long long)((ex->scratch_size - table) / scored_slot_bytes(s, kv_subs, HD)));
+    if (records < 2 || (B.max_seq_len > 0 && B.max_seq_len <= 16 * P.min_halves)) slots = 0;
+    if (slots > 0 && B.max_seq_len > 0) {
         const long long most = (((long long)B.max_seq_len + 30) / 16 + P.min_halves - 1) / P.min_halves;  // chunks of a tile
-        slots = B.max_seq_len <= 16 * P.min_halves ? 0 : std::min(slots, s.entries * (most + 1));
+        slots = std::min(slots, std::max<long long>(s.entries * most, 2));
     }
-    if (slots < s.entries + std::max<long long>(2, s.entries / 2)) slots = 0;
     P.target = (int)slots;
+    P.rounds = s.rounds;
+    P.records = (int)records;
     if (slots > 0) {
         uint8_t* at = reinterpret_cast<uint8_t*>((uintptr_t)ex->scratch_ptr);
         P.table = reinterpret_cast<int32_t*>(at);
         P.part_acc = reinterpret_cast<float*>(at + table);
-        P.part_ml = P.part_acc + (size_t)slots * kv_subs * s.cols * HD;
+        P.part_ml = P.part_acc + (size_t)records * kv_subs * s.cols * HD;
     }
     hipStream_t stream = (hipStream_t)ex->stream;
     const dim3 grid((unsigned)(slots > 0 ? slots : s.entries), (unsigned)kv_subs);
@@ -123,8 +121,13 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
                  : launch(scored_chunk_kernel<TQ, KVF, HD, false>, kChunkWaves * 64, lds);
     }
     if (rc || slots == 0) return rc;
-    hipLaunchKernelGGL((scored_join_kernel<TQ, HD>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P, s.cols,
-                       ScoredRows<KVF, HD>::kOutScale);
+    if (s.chunk || s.entries > 64) {
+        hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)(s.cols / 8)), dim3(512), 0, stream, P,
+                           s.cols, ScoredRows<KVF, HD>::kOutScale);
+    } else {
+        hipLaunchKernelGGL((scored_join_kernel<TQ, HD, true>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P,
+                           s.cols, ScoredRows<KVF, HD>::kOutScale);
+    }
     return (int)hipGetLastError();
 }
 

@@ -101,21 +101,16 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
 
     // ---- what this workgroup works on ----
     ScoredWork work = {(int)blockIdx.x, 0, 1, 0};
-    int per = 0x7ffffffe;
     if (P.target > 0) {
         int* halves = reinterpret_cast<int*>(smem + M::kCounts);
-        for (int e = tid; e < P.entries; e += kChunkWaves * 64) {
-            const ScoredTile t = scored_tile(P, e);
-            int first = 0, last = -1;
-            if (t.tokens > 0) tile_keys(P, t, first, last);
-            halves[e] = t.tokens > 0 ? tile_halves(first, last) : -1;
-        }
+        for (int e = tid; e < P.entries; e += kChunkWaves * 64) halves[e] = tile_halves_guess(P, scored_tile(P, e));
         __syncthreads();
-        per = (chunk_length(P, halves, lane) + 1) & ~1;
-        work = find_work(P, halves, per, (int)blockIdx.x, lane);
+        const auto count = [&](int e) { return halves[e]; };
+        const int per = chunk_length(P, lane, count);
+        work = find_work(P, per, P.target - 1 - (int)blockIdx.x, lane, count);  // a request's last tiles, which have most keys, first
         if (work.entry < 0) return;
         if (work.chunk == 0 && kv_sub == 0 && tid == 0) {
-            P.table[2 * work.entry] = work.first_slot;
+            P.table[2 * work.entry] = work.first_record;
             P.table[2 * work.entry + 1] = work.chunks;
         }
     } else {
@@ -124,12 +119,11 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const ScoredTile t = scored_tile(P, work.entry);
     if (t.tokens <= 0) return;
     int key_first, key_last;
-    tile_keys(P, t, key_first, key_last);
-    key_first = __builtin_amdgcn_readfirstlane(key_first);
-    key_last = __builtin_amdgcn_readfirstlane(key_last);
+    tile_keys(P, t, lane, key_first, key_last);
     const int all_halves = tile_halves(key_first, key_last);
-    const int begin = ((key_first >> 4) + work.chunk * min(per, all_halves)) * 16;  // keys
-    const int end = key_first > key_last ? begin : min(begin + min(per, all_halves) * 16, key_last + 1);
+    const int per = (fast_div(all_halves + work.chunks - 1, work.chunks) + 1) & ~1;  // whole units
+    const int begin = ((key_first >> 4) + work.chunk * per) * 16;  // keys
+    const int end = key_first > key_last ? begin : max(begin, min(begin + per * 16, key_last + 1));
     const int units = (end - begin + kChunkUnit - 1) / kChunkUnit;
 
     // ---- this lane's column ----
@@ -170,36 +164,68 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             q[m] = *reinterpret_cast<const u4*>(src + 16 * m) ^ P.q_flip;
             if (!col_ok) q[m] = u4{0u, 0u, 0u, 0u};
         }
+    } else if (!P.rot_q) {
+        // as given, relative to a power of two above the column's largest element: fp16 holds its 11 bits whatever its size
+        const uint16_t* src = P.q + ((size_t)my_tok * P.num_q_heads + (size_t)my_head) * HD + 8 * b;
+        float top = 0.f;
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m) {
+            q[m] = *reinterpret_cast<const u4*>(src + 16 * m) ^ P.q_flip;
+            if (!col_ok) q[m] = u4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = q[m][k];
+                top = fmaxf(top, fmaxf(fabsf(TQ::to_f32((uint16_t)w)), fabsf(TQ::to_f32((uint16_t)(w >> 16)))));
+            }
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
+        top = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
+#pragma unroll
+        for (int m = 0; m < kSteps; ++m)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t w = q[m][k];
+                q[m][k] = pack_h2(__builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)w), -e), __builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)(w >> 16)), -e));
+            }
+        const float mine = __builtin_amdgcn_ldexpf(R::kOutScale, e);
+        cs *= mine;
+        cc *= mine;
     } else {
-        // eight columns of the wave at a time: rotated where the keys are, relative to a power of two above their largest element
+        // Rotated, eight columns of the wave at a time through LDS, their loads together and those of the next eight ahead.
         uint16_t* area = reinterpret_cast<uint16_t*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
         float* scales = reinterpret_cast<float*>(smem + M::kQScale) + 32 * wave;
-#pragma unroll 1
-        for (int g = 0; g < 4; ++g) {
-#pragma unroll 1
+        uint2 raw[8];
+        const auto load_columns = [&](int g) {
+#pragma unroll
             for (int c8 = 0; c8 < 8; ++c8) {
                 const int c = 8 * g + c8, ct = column_token(32 * wave + c, P);
-                float v[4] = {0.f, 0.f, 0.f, 0.f};
-                if ((live >> c) & 1u) {
-                    const uint16_t* src = P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + 4 * lane;
-                    uint2 raw = *reinterpret_cast<const uint2*>(src);
-                    raw.x ^= P.q_flip, raw.y ^= P.q_flip;
-                    v[0] = TQ::to_f32((uint16_t)raw.x), v[1] = TQ::to_f32((uint16_t)(raw.x >> 16));
-                    v[2] = TQ::to_f32((uint16_t)raw.y), v[3] = TQ::to_f32((uint16_t)(raw.y >> 16));
-                }
-                if (P.rot_q) {
+                raw[c8] = uint2{0u, 0u};
+                if ((live >> c) & 1u)
+                    raw[c8] = *reinterpret_cast<const uint2*>(P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + 4 * lane);
+            }
+        };
+        load_columns(0);
+#pragma unroll 1
+        for (int g = 0; g < 4; ++g) {
+            uint2 now[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = apply_sign(v[k], 4 * lane + k);
-                    wht256_wave(v, lane);
-                }
-                float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+            for (int c8 = 0; c8 < 8; ++c8) now[c8] = uint2{raw[c8].x ^ P.q_flip, raw[c8].y ^ P.q_flip};
+            if (g < 3) load_columns(g + 1);
 #pragma unroll
-                for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            for (int c8 = 0; c8 < 8; ++c8) {
+                float v[4] = {TQ::to_f32((uint16_t)now[c8].x), TQ::to_f32((uint16_t)(now[c8].x >> 16)), TQ::to_f32((uint16_t)now[c8].y), TQ::to_f32((uint16_t)(now[c8].y >> 16))};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = apply_sign(v[k], 4 * lane + k);
+                wht256_wave(v, lane);
+                const float top = wave_top(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
                 const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
                 *reinterpret_cast<uint2*>(area + c8 * M::kColStride + 4 * lane) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
-                if (lane == 0) scales[c] = __builtin_amdgcn_ldexpf(1.0f, e);
+                if (lane == 0) scales[8 * g + c8] = __builtin_amdgcn_ldexpf(R::kOutScale, e);
             }
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
             __builtin_amdgcn_wave_barrier();
@@ -212,9 +238,8 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             __builtin_amdgcn_wave_barrier();
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
         }
-        const float mine = scales[n] * R::kOutScale;
-        cs *= mine;
-        cc *= mine;
+        cs *= scales[n];
+        cc *= scales[n];
     }
     __syncthreads();  // the areas become tiles
 
@@ -504,7 +529,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_wave_barrier();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
-#pragma unroll 1
+#pragma unroll 2
         for (int c8 = 0; c8 < 8; ++c8) {
             const int c = 8 * g + c8;
             if (!((live >> c) & 1u)) continue;
@@ -512,7 +537,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             const float m_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), c));
             const float l_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_run), c));
             if (work.chunks > 1) {
-                const size_t record = ((size_t)blockIdx.x * kv_subs + kv_sub) * kChunkCols + 32 * wave + c;
+                const size_t record = ((size_t)(work.first_record + work.chunk) * kv_subs + kv_sub) * kChunkCols + 32 * wave + c;
                 if (4 * lane < HD) *reinterpret_cast<f4*>(P.part_acc + record * HD + 4 * lane) = acc;
                 if (lane == 0) *reinterpret_cast<f2*>(P.part_ml + 2 * record) = f2{m_c, l_c};
             } else {

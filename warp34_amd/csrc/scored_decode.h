@@ -124,33 +124,40 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 
     // ---- what this workgroup works on ----
     ScoredWork work = {(int)blockIdx.x, 0, 1, 0};
-    int per = 0x7fffffff;
-    if (P.target > 0) {
-        int* halves = reinterpret_cast<int*>(smem + M::kCounts);
-        for (int e = tid; e < P.entries; e += kScoredWaves * 64) {
-            const ScoredTile t = scored_tile(P, e);
-            int first = 0, last = -1;
-            if (t.tokens > 0) tile_keys(P, t, first, last);
-            halves[e] = t.tokens > 0 ? tile_halves(first, last) : -1;
-        }
-        __syncthreads();
-        per = chunk_length(P, halves, lane);
-        work = find_work(P, halves, per, (int)blockIdx.x, lane);
+    ScoredTile t;
+    if (P.target > 0 && P.entries <= 64) {  // lane e: entry e, all a wave has to know
+        ScoredTile mine = {0, 0, 0, 0, 0};
+        if (lane < P.entries) mine = scored_tile(P, lane);
+        const int halves = lane < P.entries ? tile_halves_guess(P, mine) : -1;
+        const auto count = [&](int) { return halves; };
+        const int per = chunk_length(P, lane, count);
+        work = find_work(P, per, (int)blockIdx.x, lane, count);
         if (work.entry < 0) return;
-        if (work.chunk == 0 && kv_sub == 0 && tid == 0) {
-            P.table[2 * work.entry] = work.first_slot;
-            P.table[2 * work.entry + 1] = work.chunks;
+        const auto of = [&](int v) { return __builtin_amdgcn_readlane(v, work.entry); };
+        t = ScoredTile{of(mine.req), of(mine.tok0), of(mine.tokens), of(mine.pos0), of(mine.seq_after)};
+    } else {
+        if (P.target > 0) {
+            int* halves = reinterpret_cast<int*>(smem + M::kCounts);
+            for (int e = tid; e < P.entries; e += kScoredWaves * 64) halves[e] = tile_halves_guess(P, scored_tile(P, e));
+            __syncthreads();
+            const auto count = [&](int e) { return halves[e]; };
+            const int per = chunk_length(P, lane, count);
+            work = find_work(P, per, (int)blockIdx.x, lane, count);
+            if (work.entry < 0) return;
         }
+        t = scored_tile(P, work.entry);
+        if (t.tokens <= 0) return;
     }
-    const ScoredTile t = scored_tile(P, work.entry);
-    if (t.tokens <= 0) return;
     int key_first, key_last;
-    tile_keys(P, t, key_first, key_last);
-    key_first = __builtin_amdgcn_readfirstlane(key_first);
-    key_last = __builtin_amdgcn_readfirstlane(key_last);
+    tile_keys(P, t, lane, key_first, key_last);
+    if (work.chunk == 0 && kv_sub == 0 && tid == 0 && P.target > 0) {
+        P.table[2 * work.entry] = work.first_record;
+        P.table[2 * work.entry + 1] = work.chunks;
+    }
     const int all_halves = tile_halves(key_first, key_last);
-    const int begin = (key_first >> 4) + work.chunk * min(per, all_halves);
-    const int end = key_first > key_last ? begin : min(begin + min(per, all_halves), (key_last >> 4) + 1);
+    const int per = fast_div(all_halves + work.chunks - 1, work.chunks);
+    const int begin = (key_first >> 4) + work.chunk * per;
+    const int end = key_first > key_last ? begin : max(begin, min(begin + per, (key_last >> 4) + 1));
 
     // ---- this lane's column ----
     const int my_t = column_token(n, P);
@@ -210,8 +217,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
                 wht256_wave(v, lane);
             }
             float top = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+            top = wave_top(top);
             const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 #pragma unroll
             for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
@@ -566,7 +572,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         const f4 acc = *reinterpret_cast<const f4*>(joined + c * M::kColStride + ((4 * lane) & (HD - 1)));
         const float m_c = ml[2 * c], l_c = ml[2 * c + 1];
         if (work.chunks > 1) {
-            const size_t record = ((size_t)blockIdx.x * kv_subs + kv_sub) * 16 + c;
+            const size_t record = ((size_t)(work.first_record + work.chunk) * kv_subs + kv_sub) * 16 + c;
             if (4 * lane < HD) *reinterpret_cast<f4*>(P.part_acc + record * HD + 4 * lane) = acc;
             if (lane == 0) *reinterpret_cast<f2*>(P.part_ml + 2 * record) = f2{m_c, l_c};
         } else {
