@@ -510,3 +510,21 @@ def test_requests_of_any_number_of_tokens(fmt, dt, tokens):
     seqs, qs = [tokens + 200, tokens], [tokens, tokens]
     pool, bt, k, v, q, aq, ctx = case(fmt, 16, seqs, qs, 1100 + tokens, dt, kv_heads=1)
     check_scored(pool, bt, seqs, q, dt, aq, ctx, 8, cap=30.0)
+
+
+@gpu
+def test_one_long_request_among_many_short_ones():
+    """More tiles than a wave has lanes, most of them short: the long one is cut, in both kernels."""
+    seqs = [9000] + [40] * 150
+    for tokens in (1, 33):
+        qs = [tokens] * len(seqs)
+        pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1200, DT_F16, kv_heads=1, q_heads=4, head_dim=128)
+        check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 4, scratch=64 << 20, cap=30.0)
+
+
+@gpu
+@pytest.mark.parametrize("n", [520, 2100])
+def test_more_tiles_than_are_cut(n):
+    seqs = [int(x) for x in np.random.default_rng(n).integers(1, 60, n)]
+    pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, [1] * n, 1210, DT_F16, kv_heads=1, q_heads=2, head_dim=128)
+    check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 2, scratch=64 << 20, cap=30.0)

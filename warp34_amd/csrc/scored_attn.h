@@ -168,8 +168,8 @@ __device__ __forceinline__ int tile_halves(int first, int last) { return first <
 // least.  P.rounds == 0: the shortest `per` that needs no more than P.target chunks.  Otherwise a fixed share of all keys, so that the
 // workgroups, which start as others end, end together.  Tiles with several chunks have a record for each: no more than the scratch holds.
 // count(e): the half units of entry e, -1 for tiles without tokens.
-constexpr int kMaxSplitEntries = 512;  // entries of a batch that is split
-constexpr int kSlotRound = 128;        // slots for each kv head that fill the chip where there are two
+constexpr int kMaxSplitEntries = 2048;  // entries of a batch that is split
+constexpr int kSlotRound = 128;         // slots for each kv head that fill the chip where there are two
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
 template <typename Count>
 __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Count&& count) {
@@ -191,7 +191,7 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
         return wave_sum(n) <= P.target && wave_sum(several) <= P.records;
     };
     // (with a round of tiles or more there is something for every CU without a cut: only what is longer than a CU's share is cut)
-    const int share = P.rounds > 0 ? (live < kSlotRound ? P.rounds : 1) * kSlotRound : P.target;
+    const int share = P.rounds > 0 ? (live < kSlotRound ? P.rounds * kSlotRound : kSlotRound * 2 / 3) : P.target;
     int per = max(P.min_halves, (total + share - 1) / share);
     if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per)) return per;
     // sum of ceil(h / per) <= total / per + live, so this many halves a chunk are enough for any number of slots above live
@@ -250,68 +250,72 @@ __device__ __forceinline__ void finish_row(const ScoredParams& P, int tok, int h
 }
 
 // Joins the chunks of rows.  SPREAD: a workgroup of eight waves for each column of each tile, wave w adds up chunks w, w + 8, ... (one
-// request has up to 128 chunks).  Otherwise a wave a column, eight columns a workgroup: many tiles of few chunks (a workgroup for each of
-// the 131 072 columns of 256 tiles and two kv heads, nearly all of which have nothing to do, took 190 us).
+// request has up to 128 chunks).  Otherwise a wave a column, kJoinCols columns a workgroup: many tiles, of which few have several chunks (a
+// workgroup for each of the 131 072 columns of 256 tiles and two kv heads took 190 us to find that, one for eight columns 24 us).
+constexpr int kJoinCols = 64;
 template <typename TQ, int HD, bool SPREAD>
 __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, int columns, float value_scale) {
     __shared__ __align__(16) float sums[SPREAD ? 8 : 1][SPREAD ? HD : 4];
     const int entry = (int)blockIdx.x, kv_sub = (int)blockIdx.y;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int col = SPREAD ? (int)blockIdx.z : 8 * (int)blockIdx.z + wave;
     const ScoredTile t = scored_tile(P, entry);
-    const int mine = column_token(col, P);
-    if (mine >= t.tokens) return;
+    if (t.tokens <= 0) return;
     const int first = P.table[2 * entry], chunks = P.table[2 * entry + 1];
     if (chunks <= 1) return;
-    const int tok = t.tok0 + mine;
-    if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) return;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
-    const auto record = [&](int c) { return ((size_t)(first + c) * kv_subs + kv_sub) * columns + col; };
-    float m = kNegBig;
-    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, P.part_ml[2 * record(c)]);
+    const int end_col = SPREAD ? (int)blockIdx.z + 1 : kJoinCols * ((int)blockIdx.z + 1);
+    for (int col = SPREAD ? (int)blockIdx.z : kJoinCols * (int)blockIdx.z + wave; col < end_col; col += 8) {
+        const int mine = column_token(col, P);
+        if (mine >= t.tokens) return;
+        const int tok = t.tok0 + mine;
+        if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) continue;
+        const auto record = [&](int c) { return ((size_t)(first + c) * kv_subs + kv_sub) * columns + col; };
+        float m = kNegBig;
+        for (int c = lane; c < chunks; c += 64) m = fmaxf(m, P.part_ml[2 * record(c)]);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
-    f4 acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    const int at = (4 * lane) & (HD - 1);
-    constexpr int kStep = SPREAD ? 8 : 1;
-    const int own = SPREAD ? wave : 0;
-    for (int base = 0; base < chunks; base += 64) {
-        const int c = base + lane;
-        f2 ml = {kNegBig, 0.f};
-        if (c < chunks) ml = *reinterpret_cast<const f2*>(P.part_ml + 2 * record(c));
-        const float w = __builtin_amdgcn_exp2f(ml[0] - m);
-        l += ml[1] * w;
-        const int end = min(64, chunks - base);
-        for (int from = own; from < end; from += 8 * kStep) {  // eight records at a time, their loads together
-            f4 part[8];
+        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+        f4 acc = {0.f, 0.f, 0.f, 0.f};
+        float l = 0.f;
+        const int at = (4 * lane) & (HD - 1);
+        constexpr int kStep = SPREAD ? 8 : 1;
+        const int own = SPREAD ? wave : 0;
+        for (int base = 0; base < chunks; base += 64) {
+            const int c = base + lane;
+            f2 ml = {kNegBig, 0.f};
+            if (c < chunks) ml = *reinterpret_cast<const f2*>(P.part_ml + 2 * record(c));
+            const float w = __builtin_amdgcn_exp2f(ml[0] - m);
+            l += ml[1] * w;
+            const int end = min(64, chunks - base);
+            for (int from = own; from < end; from += 8 * kStep) {  // eight records at a time, their loads together
+                f4 part[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (from + kStep * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + from + kStep * k) * HD + at);
+                for (int k = 0; k < 8; ++k)
+                    if (from + kStep * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + from + kStep * k) * HD + at);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (from + kStep * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from + kStep * k));
+                for (int k = 0; k < 8; ++k)
+                    if (from + kStep * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from + kStep * k));
+            }
         }
-    }
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
-    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-    if constexpr (SPREAD) {
-        if (4 * lane < HD) *reinterpret_cast<f4*>(&sums[wave][at]) = acc;
-        __syncthreads();
-        if (wave != 0) return;
+        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+        if constexpr (SPREAD) {
+            if (4 * lane < HD) *reinterpret_cast<f4*>(&sums[wave][at]) = acc;
+            __syncthreads();
+            if (wave != 0) return;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = 0.f;
+            for (int k = 0; k < 4; ++k) v[k] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 8; ++w) {
-            const f4 s = *reinterpret_cast<const f4*>(&sums[w][at]);
+            for (int w = 0; w < 8; ++w) {
+                const f4 s = *reinterpret_cast<const f4*>(&sums[w][at]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] += s[k];
+                for (int k = 0; k < 4; ++k) v[k] += s[k];
+            }
         }
+        const int head = (kv_sub / P.q_subgroups) * P.gqa + (kv_sub % P.q_subgroups) * P.q_group + (col - mine * P.q_group);
+        finish_row<TQ, HD>(P, tok, head, lane, v, m, l, value_scale);
     }
-    const int head = (kv_sub / P.q_subgroups) * P.gqa + (kv_sub % P.q_subgroups) * P.q_group + (col - mine * P.q_group);
-    finish_row<TQ, HD>(P, tok, head, lane, v, m, l, value_scale);
 }
 
 }  // namespace w34

@@ -122,7 +122,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     }
     if (rc || slots == 0) return rc;
     if (s.chunk || s.entries > 64) {
-        hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)(s.cols / 8)), dim3(512), 0, stream, P,
+        hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)((s.cols + kJoinCols - 1) / kJoinCols)), dim3(512), 0, stream, P,
                            s.cols, ScoredRows<KVF, HD>::kOutScale);
     } else {
         hipLaunchKernelGGL((scored_join_kernel<TQ, HD, true>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P,

@@ -88,8 +88,8 @@ struct ScoredRows {
     }
 };
 
-// LDS: [TQ4 tables][query columns][tile counts], over which the waves' regions and the joined columns lie at the end; [(m, l) of the
-// waves][scales of the waves]
+// LDS: [TQ4 tables][query columns], over which the counts of the tiles lie at the start and the waves' regions and the joined columns at
+// the end; [(m, l) of the waves][scales of the waves]
 template <int KVF, int HD>
 struct ScoredLds {
     using R = ScoredRows<KVF, HD>;
@@ -98,13 +98,12 @@ struct ScoredLds {
     static constexpr int kTable = R::kTq4 ? 2 * kKeyTable : 0;
     static constexpr int kQStride = HD + 8;                       // 16-bit elements
     static constexpr int kQ = kTable, kQLow = kQ + 16 * kQStride * 2, kQScale = kQLow + 16 * kQStride * 2;
-    static constexpr int kCounts = kQScale + 64;                  // entries x 4 bytes
     static constexpr int kJoined = kScoredWaves * kRegion;
-    static constexpr int kLoopEnd = kCounts + kMaxSplitEntries * 4;
+    static constexpr int kLoopEnd = kQScale + 64;
     static constexpr int kMl = kJoined + kRegion > kLoopEnd ? kJoined + kRegion : kLoopEnd;
     static constexpr int kScale = kMl + kScoredWaves * 16 * 8;
     static constexpr int kBytes = kScale + kScoredWaves * 2 * 4 * 16 * 4;
-    static_assert(kBytes <= 160 * 1024, "decode LDS budget");
+    static_assert(kBytes <= 160 * 1024 && kMaxSplitEntries * 4 <= kJoined, "decode LDS budget");
 };
 
 template <typename TQ, int KVF, int HD, bool CAP>
@@ -137,13 +136,14 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         t = ScoredTile{of(mine.req), of(mine.tok0), of(mine.tokens), of(mine.pos0), of(mine.seq_after)};
     } else {
         if (P.target > 0) {
-            int* halves = reinterpret_cast<int*>(smem + M::kCounts);
+            int* halves = reinterpret_cast<int*>(smem);
             for (int e = tid; e < P.entries; e += kScoredWaves * 64) halves[e] = tile_halves_guess(P, scored_tile(P, e));
             __syncthreads();
             const auto count = [&](int e) { return halves[e]; };
             const int per = chunk_length(P, lane, count);
             work = find_work(P, per, (int)blockIdx.x, lane, count);
             if (work.entry < 0) return;
+            __syncthreads();  // the counts lie where the tables come
         }
         t = scored_tile(P, work.entry);
         if (t.tokens <= 0) return;
