@@ -13,6 +13,13 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
 
+// Bytes of a slab.  An address that comes out of an integer has to say that it is global memory: a flat load is counted with the LDS
+// accesses too, and every wait for a look-up would wait for the rows in flight.
+typedef __attribute__((address_space(1))) const uint8_t slab_byte;
+__device__ __forceinline__ const slab_byte* slab_at(uint64_t address) { return reinterpret_cast<const slab_byte*>((uintptr_t)address); }
+template <typename T>
+__device__ __forceinline__ T load_as(const slab_byte* p) { return *reinterpret_cast<const __attribute__((address_space(1))) T*>(p); }
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kNegBig = -1.0e30f;  // "minus infinity" that stays finite under subtraction
 // The table holds fp16(kLutGain * centroid); the gain is divided out of the query (K side)

@@ -27,9 +27,9 @@ __device__ __forceinline__ int slot_page(int slot, const ReadParams& P) {
     int page = (int)__umulhi((uint32_t)slot, P.block_magic);  // the quotient or one less
     return page + ((slot - page * P.block_size >= P.block_size) ? 1 : 0);
 }
-__device__ __forceinline__ const uint8_t* row_address(const ReadSide& S, const ReadParams& P, int slot, int head) {
+__device__ __forceinline__ const slab_byte* row_address(const ReadSide& S, const ReadParams& P, int slot, int head) {
     const int page = slot_page(slot, P);
-    return reinterpret_cast<const uint8_t*>((uintptr_t)S.base) + (uint64_t)(uint32_t)page * S.page_stride + (uint64_t)(uint32_t)head * S.head_stride +
+    return slab_at(S.base) + (uint64_t)(uint32_t)page * S.page_stride + (uint64_t)(uint32_t)head * S.head_stride +
            (uint64_t)(uint32_t)(slot - page * P.block_size) * S.token_stride;
 }
 // Lane l of a wave holds centroid l % 16; a code's low four bits pick one from the wave, all of whose lanes take part.
@@ -59,10 +59,10 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
     const int64_t row = (int64_t)blockIdx.x * rows_per_block + r;
     const int slot = r < rows_per_block && row < P.rows ? P.slots[row] : -1;
     const bool live = slot >= 0;  // else: row untouched
-    const uint8_t* src = row_address(S, P, live ? slot : 0, head);
+    const slab_byte* src = row_address(S, P, live ? slot : 0, head);
     uint4 w = {0u, 0u, 0u, 0u};
     if (S.format == WARP34_KV_FORMAT_FP16 || S.format == WARP34_KV_FORMAT_BF16) {
-        if (live) w = *reinterpret_cast<const uint4*>(src + 2 * e);
+        if (live) w = __builtin_bit_cast(uint4, load_as<u4>(src + 2 * e));
         if (S.format != TOut::kStorageFormat) {
             uint32_t* x = &w.x;
 #pragma unroll
@@ -77,10 +77,10 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
         if (S.format == WARP34_KV_FORMAT_TQ4) {  // blocks of 66 bytes: fp16 scale, 128 codes of four bits
             uint32_t word = 0u;
             if (live) {
-                const uint8_t* block = src + 66 * (e >> 7);
-                const uint16_t* codes = reinterpret_cast<const uint16_t*>(block + 2 + ((e & 127) >> 1));
-                word = (uint32_t)codes[0] | (uint32_t)codes[1] << 16;
-                d = F16::to_f32(*reinterpret_cast<const uint16_t*>(block));
+                const slab_byte* block = src + 66 * (e >> 7);
+                const slab_byte* codes = block + 2 + ((e & 127) >> 1);
+                word = (uint32_t)load_as<uint16_t>(codes) | (uint32_t)load_as<uint16_t>(codes + 2) << 16;
+                d = F16::to_f32(load_as<uint16_t>(block));
             }
             const float mine = lane_centroid();
 #pragma unroll
@@ -89,10 +89,10 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
             uint32_t codes[2] = {0u, 0u};
             const bool fp8 = S.format == WARP34_KV_FORMAT_FP8_E4M3;
             if (live) {  // Q8_0: blocks of 68 bytes
-                const uint8_t* block = fp8 ? src : src + 68 * (e >> 6);
-                const uint32_t* at = reinterpret_cast<const uint32_t*>(fp8 ? src + e : block + 4 + (e & 63));
-                codes[0] = at[0], codes[1] = at[1];
-                d = *reinterpret_cast<const float*>(fp8 ? src + 256 + 4 * (e >> 7) : block);
+                const slab_byte* block = fp8 ? src : src + 68 * (e >> 6);
+                const slab_byte* at = fp8 ? src + e : block + 4 + (e & 63);
+                codes[0] = load_as<uint32_t>(at), codes[1] = load_as<uint32_t>(at + 4);
+                d = load_as<float>(fp8 ? src + 256 + 4 * (e >> 7) : block);
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
@@ -150,18 +150,18 @@ __global__ __launch_bounds__(256) void kv_read_rotated_kernel(const ReadParams P
         live[k] = slot >= 0;
         code[k] = scale[k] = 0u;
         if (live[k]) {
-            const uint8_t* src = row_address(S, P, slot, head);
+            const slab_byte* src = row_address(S, P, slot, head);
             if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
-                const uint8_t* block = src + 66 * (e >> 7);
-                scale[k] = *reinterpret_cast<const uint16_t*>(block);
-                code[k] = *reinterpret_cast<const uint16_t*>(block + 2 + ((e & 127) >> 1));
+                const slab_byte* block = src + 66 * (e >> 7);
+                scale[k] = load_as<uint16_t>(block);
+                code[k] = load_as<uint16_t>(block + 2 + ((e & 127) >> 1));
             } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
-                code[k] = *reinterpret_cast<const uint32_t*>(src + e);
-                scale[k] = *reinterpret_cast<const uint32_t*>(src + 256 + 4 * (e >> 7));
+                code[k] = load_as<uint32_t>(src + e);
+                scale[k] = load_as<uint32_t>(src + 256 + 4 * (e >> 7));
             } else {
-                const uint8_t* block = src + 68 * (e >> 6);
-                code[k] = *reinterpret_cast<const uint32_t*>(block + 4 + (e & 63));
-                scale[k] = *reinterpret_cast<const uint32_t*>(block);
+                const slab_byte* block = src + 68 * (e >> 6);
+                code[k] = load_as<uint32_t>(block + 4 + (e & 63));
+                scale[k] = load_as<uint32_t>(block);
             }
         }
     }

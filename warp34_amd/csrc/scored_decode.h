@@ -52,9 +52,6 @@ __device__ __forceinline__ u2v key_read(uint32_t code_word, uint32_t lane_bits, 
     return *reinterpret_cast<lds_cu2*>((uintptr_t)__builtin_amdgcn_perm(code_word, lane_bits, 0x0c010400u + ((uint32_t)byte << 8)));
 }
 
-template <typename T>
-__device__ __forceinline__ T load_as(const uint8_t* p) { return *reinterpret_cast<const T*>(p); }
-
 template <bool IS_BF16>
 __device__ __forceinline__ f4 mfma_rows(u4 a, u4 b, f4 c) {
     if constexpr (IS_BF16) {
@@ -241,13 +238,13 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     const bool two_parts = !R::k16 && P.rot_q != 0;
 
     // ---- rows ----
-    const uint8_t* k_slab = reinterpret_cast<const uint8_t*>((uintptr_t)L.k_base) + (uint64_t)(uint32_t)kv_head * L.k_head_stride_bytes;
-    const uint8_t* v_slab = reinterpret_cast<const uint8_t*>((uintptr_t)L.v_base) + (uint64_t)(uint32_t)kv_head * L.v_head_stride_bytes;
+    const slab_byte* k_slab = slab_at(L.k_base) + (uint64_t)(uint32_t)kv_head * L.k_head_stride_bytes;
+    const slab_byte* v_slab = slab_at(L.v_base) + (uint64_t)(uint32_t)kv_head * L.v_head_stride_bytes;
     const int32_t* blocks = B.block_tables + (size_t)t.req * B.max_blocks_per_req;
     int slot_base = page_slot(begin * 16, P);
     int pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;  // 64 entries of the block table
-    const uint8_t* k_rows;
-    const uint8_t* v_rows;
+    const slab_byte* k_rows;
+    const slab_byte* v_rows;
     const auto locate = [&](int half) {
         const int pos = half * 16, slot = page_slot(pos, P);
         if (slot - slot_base >= 64) {  // uniform
@@ -266,7 +263,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     u2v vr8[R::kFp8 ? 2 : 1][4];
     uint32_t vr4[R::kQ8 ? 4 : R::kTq4 ? 2 : 1][4];
     const auto load_keys = [&]() {
-        const uint8_t* row = k_rows + (uint32_t)(n * R::kRowBytes);
+        const slab_byte* row = k_rows + (uint32_t)(n * R::kRowBytes);
         if constexpr (R::k16) {
 #pragma unroll
             for (int m = 0; m < R::kOps; ++m) kr[m] = load_as<u4>(row + 64 * m + 16 * b);
@@ -287,7 +284,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     const auto load_values = [&]() {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint8_t* row = v_rows + (uint32_t)((4 * b + i) * R::kRowBytes);
+            const slab_byte* row = v_rows + (uint32_t)((4 * b + i) * R::kRowBytes);
             if constexpr (R::k16) {
 #pragma unroll
                 for (int g = 0; g < R::kGroups; ++g) vr16[g][i] = load_as<u4>(row + 256 * g + 16 * n);
@@ -302,7 +299,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
                 for (int g = 0; g < 4; ++g) vr4[g][i] = load_as<uint32_t>(row + 68 * g + 4 + 4 * n);
             }
         }
-        const uint8_t* row = v_rows + (uint32_t)(n * R::kRowBytes);
+        const slab_byte* row = v_rows + (uint32_t)(n * R::kRowBytes);
         if constexpr (R::kTq4) v_scale = load_as<uint16_t>(row + 66 * (b & 1));
         if constexpr (R::kFp8) v_scales = load_as<u2_at4>(row + 256);
         if constexpr (R::kQ8) v_scale = load_as<uint32_t>(row + 68 * b);
