@@ -4,7 +4,7 @@
 
 #include "attn_launch.h"
 #include "scored_chunk.h"
-#include "scored_decode.h"
+#include "scored_decode_tq4.h"
 
 namespace w34 {
 
@@ -16,6 +16,8 @@ constexpr int kDecodeRounds = 4, kChunkRounds = 2;
 // Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
 constexpr int kChunkFrom = 128;
 
+static int decode_cols(int format) { return format == WARP34_KV_FORMAT_TQ4 ? kTq4Cols : kDecodeCols; }
+
 // The tiles of a batch: the kernel, a tile's tokens, tiles of a request, slots for each kv head (0: no split).
 struct ScoredShape {
     bool chunk;
@@ -23,11 +25,11 @@ struct ScoredShape {
     long long tiles, entries;
     int slots, rounds;
 };
-static ScoredShape scored_shape(int num_reqs, int total_tokens, int max_q_len, int q_group) {
+static ScoredShape scored_shape(int format, int num_reqs, int total_tokens, int max_q_len, int q_group) {
     ScoredShape s;
     const int q_len = max_q_len > 0 ? std::min(max_q_len, total_tokens) : total_tokens;
     s.chunk = (long long)q_len * q_group >= kChunkFrom;
-    s.cols = s.chunk ? kChunkCols : kDecodeCols;
+    s.cols = s.chunk ? kChunkCols : decode_cols(format);
     s.tok_tile = s.cols / q_group;
     s.tiles = ((long long)q_len + s.tok_tile - 1) / s.tok_tile;
     s.entries = s.tiles * num_reqs;
@@ -42,8 +44,8 @@ static size_t scored_slot_bytes(const ScoredShape& s, int kv_subs, int head_dim)
 static size_t scored_table_bytes(long long entries) { return ((size_t)entries * 8 + 15) / 16 * 16; }
 
 // Largest divisor of the q heads of a kv head that fits a column tile
-static int scored_q_group(int gqa) {
-    int d = std::min(gqa, 16);
+static int scored_q_group(int format, int gqa) {
+    int d = std::min(gqa, decode_cols(format));
     while (gqa % d != 0) --d;
     return d;
 }
@@ -77,7 +79,7 @@ template <typename TQ, int KVF, int HD>
 static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const warp34_attention_batch& B = P.B;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
-    const ScoredShape s = scored_shape(B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
+    const ScoredShape s = scored_shape(KVF, B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
     if (kv_subs > 65535 || s.entries > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
     P.tok_tile = s.tok_tile;
     P.tiles = (int)s.tiles;
@@ -113,8 +115,12 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const bool cap = P.cap2 > 0.f;
     int rc;
     if (!s.chunk) {
-        rc = cap ? launch(scored_decode_kernel<TQ, KVF, HD, true>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes)
-                 : launch(scored_decode_kernel<TQ, KVF, HD, false>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes);
+        if constexpr (KVF == WARP34_KV_FORMAT_TQ4)
+            rc = cap ? launch(scored_decode_tq4_kernel<TQ, true>, kScoredWaves * 64, Tq4Lds::kBytes)
+                     : launch(scored_decode_tq4_kernel<TQ, false>, kScoredWaves * 64, Tq4Lds::kBytes);
+        else
+            rc = cap ? launch(scored_decode_kernel<TQ, KVF, HD, true>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes)
+                     : launch(scored_decode_kernel<TQ, KVF, HD, false>, kScoredWaves * 64, ScoredLds<KVF, HD>::kBytes);
     } else {
         constexpr int lds = ChunkLds<KVF, HD>::kBytes;
         rc = cap ? launch(scored_chunk_kernel<TQ, KVF, HD, true>, kChunkWaves * 64, lds)
@@ -160,7 +166,7 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.wide_cap = scores->softcap > kWideCap ? 1 : 0;
     P.num_q_heads = num_q_heads;
     P.gqa = num_q_heads / layout->local_kv_heads;
-    P.q_group = scored_q_group(P.gqa);
+    P.q_group = scored_q_group(layout->k_format, P.gqa);
     P.q_subgroups = P.gqa / P.q_group;
     P.block_magic = block_magic_for(layout->block_size);
     P.q_group_magic = q_group_magic_for(P.q_group);
@@ -190,7 +196,7 @@ extern "C" size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_la
                                                               int num_q_heads) {
     if (!layout || layout->local_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % layout->local_kv_heads != 0 || num_reqs <= 0 || total_tokens <= 0)
         return 0;
-    const int gqa = num_q_heads / layout->local_kv_heads, group = scored_q_group(gqa);
-    const ScoredShape s = scored_shape(num_reqs, total_tokens, max_q_len, group);
+    const int gqa = num_q_heads / layout->local_kv_heads, group = scored_q_group(layout->k_format, gqa);
+    const ScoredShape s = scored_shape(layout->k_format, num_reqs, total_tokens, max_q_len, group);
     return s.slots == 0 ? 0 : scored_table_bytes(s.entries) + (size_t)s.slots * scored_slot_bytes(s, layout->local_kv_heads * (gqa / group), layout->head_dim);
 }
