@@ -129,6 +129,16 @@ __device__ __forceinline__ float wave_top(float v) {
     return __int_as_float(wave_largest(__float_as_int(v)));
 }
 
+// The largest of a wave's numbers, none of them NaN, and their sum.
+__device__ __forceinline__ float wave_most(float v) {
+    const auto f = [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); };
+    return __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(v), __float_as_int(-INFINITY), f), 63));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    const auto f = [](int a, int b) { return __float_as_int(__int_as_float(a) + __int_as_float(b)); };
+    return __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(v), 0, f), 63));
+}
+
 // First and last key that any token of a tile sees; first > last where none does.  A lane a token.
 __device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int lane, int& first, int& last) {
     int lo, hi;
@@ -271,34 +281,38 @@ __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, 
         const int tok = t.tok0 + mine;
         if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) continue;
         const auto record = [&](int c) { return ((size_t)(first + c) * kv_subs + kv_sub) * columns + col; };
-        float m = kNegBig;
-        for (int c = lane; c < chunks; c += 64) m = fmaxf(m, P.part_ml[2 * record(c)]);
+        const int at = (4 * lane) & (HD - 1);
+        constexpr int kStep = SPREAD ? 8 : 1, kBatch = SPREAD ? 16 : 8;  // chunks from one to the next of a wave; loads that travel together
+        const int own = SPREAD ? wave : 0;
+        f4 part[kBatch];
+        const auto load = [&](int from) {
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d, 64));
+            for (int k = 0; k < kBatch; ++k)
+                if (from + kStep * k < chunks) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(from + kStep * k) * HD + at);
+        };
+        const auto states = [&](int base) {
+            return base + lane < chunks ? *reinterpret_cast<const f2*>(P.part_ml + 2 * record(base + lane)) : f2{kNegBig, 0.f};
+        };
+        f2 ml = states(0);
+        load(own);  // (before their weights are known)
+        float m = ml[0];
+        for (int base = 64; base < chunks; base += 64) m = fmaxf(m, states(base)[0]);
+        m = wave_most(m);
         f4 acc = {0.f, 0.f, 0.f, 0.f};
         float l = 0.f;
-        const int at = (4 * lane) & (HD - 1);
-        constexpr int kStep = SPREAD ? 8 : 1;
-        const int own = SPREAD ? wave : 0;
         for (int base = 0; base < chunks; base += 64) {
-            const int c = base + lane;
-            f2 ml = {kNegBig, 0.f};
-            if (c < chunks) ml = *reinterpret_cast<const f2*>(P.part_ml + 2 * record(c));
+            if (base > 0) ml = states(base);
             const float w = __builtin_amdgcn_exp2f(ml[0] - m);
             l += ml[1] * w;
             const int end = min(64, chunks - base);
-            for (int from = own; from < end; from += 8 * kStep) {  // eight records at a time, their loads together
-                f4 part[8];
+            for (int from = own; from < end; from += kBatch * kStep) {
+                if (base + from > own) load(base + from);
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                    if (from + kStep * k < end) part[k] = *reinterpret_cast<const f4*>(P.part_acc + record(base + from + kStep * k) * HD + at);
-#pragma unroll
-                for (int k = 0; k < 8; ++k)
+                for (int k = 0; k < kBatch; ++k)
                     if (from + kStep * k < end) acc += part[k] * __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), from + kStep * k));
             }
         }
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d, 64);
+        l = wave_total(l);
         float v[4] = {acc[0], acc[1], acc[2], acc[3]};
         if constexpr (SPREAD) {
             if (4 * lane < HD) *reinterpret_cast<f4*>(&sums[wave][at]) = acc;

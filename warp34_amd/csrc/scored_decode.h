@@ -120,18 +120,29 @@ __device__ __forceinline__ DecodeColumn decode_column(const ScoredParams& P, con
 // two above their largest element so that fp16 holds them whatever their size, in two parts (the second is zero where nothing is
 // rotated: 11 bits are all there are).
 template <typename TQ, int COLS, int STRIDE>
-__device__ __forceinline__ void bring_queries(const ScoredParams& P, const ScoredTile& t, int head0, uint32_t live, int wave, int lane, uint16_t* high,
-                                              uint16_t* low, float* scales) {
+struct QueryColumns {
+    uint2 raw[COLS / kScoredWaves];
+    __device__ __forceinline__ void load(const ScoredParams& P, const ScoredTile& t, int head0, int wave, int lane) {
 #pragma unroll
-    for (int c = wave; c < COLS; c += kScoredWaves) {
-        const int ct = column_token(c, P);
+        for (int k = 0; k < COLS / kScoredWaves; ++k) {
+            const int c = wave + kScoredWaves * k, ct = column_token(c, P);
+            const int tok = min(t.tok0 + ct, P.B.total_tokens - 1), head = min(head0 + c - ct * P.q_group, P.num_q_heads - 1);
+            raw[k] = *reinterpret_cast<const uint2*>(P.q + ((size_t)tok * P.num_q_heads + (size_t)head) * 256 + 4 * lane);
+        }
+    }
+    __device__ __forceinline__ void bring(const ScoredParams& P, uint32_t live, int wave, int lane, uint16_t* high, uint16_t* low, float* scales) const;
+};
+template <typename TQ, int COLS, int STRIDE>
+__device__ __forceinline__ void QueryColumns<TQ, COLS, STRIDE>::bring(const ScoredParams& P, uint32_t live, int wave, int lane, uint16_t* high,
+                                                                      uint16_t* low, float* scales) const {
+#pragma unroll
+    for (int k8 = 0; k8 < COLS / kScoredWaves; ++k8) {
+        const int c = wave + kScoredWaves * k8;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if ((live >> c) & 1u) {
-            const uint16_t* src = P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + c - ct * P.q_group)) * 256 + 4 * lane;
-            uint2 raw = *reinterpret_cast<const uint2*>(src);
-            raw.x ^= P.q_flip, raw.y ^= P.q_flip;
-            v[0] = TQ::to_f32((uint16_t)raw.x), v[1] = TQ::to_f32((uint16_t)(raw.x >> 16));
-            v[2] = TQ::to_f32((uint16_t)raw.y), v[3] = TQ::to_f32((uint16_t)(raw.y >> 16));
+            const uint32_t x = raw[k8].x ^ P.q_flip, y = raw[k8].y ^ P.q_flip;
+            v[0] = TQ::to_f32((uint16_t)x), v[1] = TQ::to_f32((uint16_t)(x >> 16));
+            v[2] = TQ::to_f32((uint16_t)y), v[3] = TQ::to_f32((uint16_t)(y >> 16));
         }
         if (P.rot_q) {
 #pragma unroll
@@ -170,7 +181,10 @@ struct PageWalk {
     // rows of a half unit; half units in order
     __device__ __forceinline__ void locate(const ScoredParams& P, int half, int row_bytes, int lane, const slab_byte*& k_rows, const slab_byte*& v_rows) {
         const int pos = half * 16, slot = page_slot(pos, P);
-        if (slot - slot_base >= 64) fetch(P, slot, lane);  // uniform
+        if (slot - slot_base >= 64) {  // uniform
+            fetch(P, slot, lane);
+            asm volatile("" : "+v"(pages));  // (the wait stands here and not behind the branch, for whatever is on its way)
+        }
         const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, slot - slot_base), 0);
         const uint32_t in_page = (uint32_t)(pos - slot * P.L.block_size) * (uint32_t)row_bytes;
         k_rows = k_slab + (uint64_t)page * P.L.k_page_stride_bytes + in_page;
@@ -286,33 +300,16 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     if (col.live == 0u) return;
     const bool sloped = P.slopes != nullptr;
 
-    // ---- query operands ----
+    // ---- what comes from memory first: the queries, then the rows of this wave's first half unit ----
     u4 q_high[R::kOps], q_low[R::kOps];
-    float cs = P.scale2, cc = P.cap_arg;
-    uint16_t* qh = reinterpret_cast<uint16_t*>(smem + M::kQ);
-    uint16_t* ql = reinterpret_cast<uint16_t*>(smem + M::kQLow);
+    QueryColumns<TQ, 16, M::kQStride> columns;
     if constexpr (R::k16) {
         const uint16_t* src = P.q + ((size_t)col.tok * P.num_q_heads + (size_t)col.head) * HD;
 #pragma unroll
-        for (int m = 0; m < R::kOps; ++m) {
-            q_high[m] = *reinterpret_cast<const u4*>(src + R::element(m, b)) ^ P.q_flip;
-            if (!col.ok) q_high[m] = u4{0u, 0u, 0u, 0u};
-        }
+        for (int m = 0; m < R::kOps; ++m) q_high[m] = *reinterpret_cast<const u4*>(src + R::element(m, b));
     } else {
-        float* qs = reinterpret_cast<float*>(smem + M::kQScale);
-        bring_queries<TQ, 16, M::kQStride>(P, s0.t, head0, col.live, wave, lane, qh, ql, qs);
-        __syncthreads();
-#pragma unroll
-        for (int m = 0; m < R::kOps; ++m) {
-            q_high[m] = *reinterpret_cast<const u4*>(qh + n * M::kQStride + R::element(m, b));
-            q_low[m] = *reinterpret_cast<const u4*>(ql + n * M::kQStride + R::element(m, b));
-        }
-        cs *= qs[n];
-        cc *= qs[n];
+        columns.load(P, s0.t, head0, wave, lane);
     }
-    const bool two_parts = !R::k16 && P.rot_q != 0;
-
-    // ---- rows ----
     const slab_byte* k_rows;
     const slab_byte* v_rows;
     const auto locate = [&](int half) { walk.locate(P, half, R::kRowBytes, lane, k_rows, v_rows); };
@@ -356,6 +353,37 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         if constexpr (R::kFp8) v_scales = load_as<u2_at4>(row + 256);
         if constexpr (R::kQ8) v_scale = load_as<uint32_t>(row + 68 * b);
     };
+    int half = s0.begin + wave;
+    if (half < end) {
+        locate(half);
+        load_keys();
+        load_values();
+    }
+
+    // ---- query operands ----
+    float cs = P.scale2, cc = P.cap_arg;
+    uint16_t* qh = reinterpret_cast<uint16_t*>(smem + M::kQ);
+    uint16_t* ql = reinterpret_cast<uint16_t*>(smem + M::kQLow);
+    if constexpr (R::k16) {
+#pragma unroll
+        for (int m = 0; m < R::kOps; ++m) {
+            q_high[m] ^= P.q_flip;
+            if (!col.ok) q_high[m] = u4{0u, 0u, 0u, 0u};
+        }
+    } else {
+        float* qs = reinterpret_cast<float*>(smem + M::kQScale);
+        columns.bring(P, col.live, wave, lane, qh, ql, qs);
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < R::kOps; ++m) {
+            q_high[m] = *reinterpret_cast<const u4*>(qh + n * M::kQStride + R::element(m, b));
+            q_low[m] = *reinterpret_cast<const u4*>(ql + n * M::kQStride + R::element(m, b));
+        }
+        cs *= qs[n];
+        cc *= qs[n];
+    }
+    const bool two_parts = !R::k16 && P.rot_q != 0;
+
     // Block scales are loaded a row a lane and used four rows a lane: an exchange through 256 bytes of LDS for each kind.
     float* scale_area = reinterpret_cast<float*>(smem + M::kScale + wave * (2 * 4 * 16 * 4));
     const auto exchange = [&](float* area, uint32_t one, u2v two) {
@@ -374,12 +402,6 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     for (int k = 0; k < R::kGroups * R::kJ; ++k) o[k] = f4{0.f, 0.f, 0.f, 0.f};
     float m_run = kNegBig, l_run = 0.f;
 
-    int half = s0.begin + wave;
-    if (half < end) {
-        locate(half);
-        load_keys();
-        load_values();
-    }
     while (half < end) {
         const int next = half + kScoredWaves;
         const bool more = next < end;

@@ -17,10 +17,9 @@ typedef uint32_t u1_at2 __attribute__((aligned(2)));
 
 constexpr int kTq4Cols = 8;
 
-// TQ4 keys: the look-ups' fp16 numbers are up to 9.4e-5 from the centroids, which would be 1e-4 of a score and 2e-5 of a row's lse where a
-// few keys carry it.  So the keys have a table of their own behind the other, entries of eight bytes: the pair of the first table and the
-// pair of what is missing, 32 copies (a read of eight bytes goes by 32 lanes at a time).
-constexpr int kKeyTable = 65536;
+// The table: entries of eight bytes, the pair of fp16 numbers of a byte's two codes and the pair of what they are short of the centroids;
+// 32 copies (a read goes by 32 lanes at a time).  The fp16 numbers are up to 9.4e-5 from the centroids, which would be 1e-4 of a score and
+// 2e-5 of a row's lse where a few keys carry it: keys take both, values the first alone.
 __host__ __device__ constexpr uint32_t centroid_rest_of(int code) {
     return __builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[code] - (float)(_Float16)(kLutGain * kCentroids[code])));
 }
@@ -30,20 +29,20 @@ __device__ __forceinline__ uint32_t centroid_rest(uint32_t code) {
     for (int c = 1; c < 16; ++c) r = code == (uint32_t)c ? centroid_rest_of(c) : r;
     return r;
 }
-__device__ __forceinline__ void build_key_table(uint8_t* smem, int tid, int wave) {  // by 512 threads, as build_pair_table
+__device__ __forceinline__ void build_two_part_table(uint8_t* smem, int tid, int wave) {  // by 512 threads, as build_pair_table
     const uint32_t code = (uint32_t)tid >> 4 & 15u, lo = centroid_bits(code), lo_rest = centroid_rest(code);
     const bool odd = (wave >> 2) != 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t v = lo | (odd ? centroid_bits_of(2 * i + 1) << 16 : centroid_bits_of(2 * i) << 16);
         const uint32_t w = lo_rest | (odd ? centroid_rest_of(2 * i + 1) << 16 : centroid_rest_of(2 * i) << 16);
-        *reinterpret_cast<u4*>(smem + kKeyTable + (tid + 512 * i) * 16) = u4{v, w, v, w};
+        *reinterpret_cast<u4*>(smem + (tid + 512 * i) * 16) = u4{v, w, v, w};
     }
 }
 typedef __attribute__((address_space(3))) const u2v lds_cu2;
-// lane_bits: (lane % 32) * 8 | 0x100, whose second byte is the table's place
-__device__ __forceinline__ u2v key_read(uint32_t code_word, uint32_t lane_bits, int byte) {
-    return *reinterpret_cast<lds_cu2*>((uintptr_t)__builtin_amdgcn_perm(code_word, lane_bits, 0x0c010400u + ((uint32_t)byte << 8)));
+// table_lane: the place of the lane's copy, (lane % 32) * 8; the table lies at 0
+__device__ __forceinline__ u2v key_read(uint32_t code_word, uint32_t table_lane, int byte) {
+    return *reinterpret_cast<lds_cu2*>((uintptr_t)__builtin_amdgcn_perm(code_word, table_lane, 0x0c0c0400u + ((uint32_t)byte << 8)));
 }
 
 // fp16(w), or what that leaves of w where low is 1, of two weights
@@ -55,17 +54,17 @@ __device__ __forceinline__ uint32_t weight_part(float a, float b, float low) {
     return pack_h2(r0, r1);
 }
 
-// LDS: [value table][key table][query columns], over which the counts of the tiles lie at the start and the waves' regions at the end; [a
+// LDS: [table][query columns], over which the counts of the tiles lie at the start and the waves' regions at the end; [a
 // finished column of each wave][(m, l) of the waves][scales of the waves]
 struct Tq4Lds {
     static constexpr int kColStride = 256 + 8, kRegion = kTq4Cols * kColStride * 4;
     static constexpr int kQStride = 256 + 8;
-    static constexpr int kQ = 2 * kKeyTable, kQLow = kQ + kTq4Cols * kQStride * 2, kQScale = kQLow + kTq4Cols * kQStride * 2;
-    static constexpr int kReorder = kQScale + 64;
+    static constexpr int kQ = 65536, kQLow = kQ + kTq4Cols * kQStride * 2, kQScale = kQLow + kTq4Cols * kQStride * 2;
+    static constexpr int kLoopEnd = kQScale + 64, kReorder = kLoopEnd > kScoredWaves * kRegion ? kLoopEnd : kScoredWaves * kRegion;
     static constexpr int kMl = kReorder + kScoredWaves * 256 * 4;
     static constexpr int kScale = kMl + kScoredWaves * 16 * 8;
     static constexpr int kBytes = kScale + kScoredWaves * 2 * 64 * 4;
-    static_assert(kBytes <= 160 * 1024 && kScoredWaves * kRegion <= kReorder && kMaxSplitEntries * 4 <= kQ, "decode LDS budget");
+    static_assert(kBytes <= 160 * 1024 && kMaxSplitEntries * 4 <= kQ, "decode LDS budget");
 };
 
 template <typename TQ, bool CAP>
@@ -111,25 +110,26 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
                 for (int blk = 0; blk < 2; ++blk) vr[h][blk][i] = load_as<u1_at2>(v_rows[h] + (uint32_t)(b * 528 + 4 * n + 132 * i + 66 * blk + 2));
         v_scale = load_as<uint16_t>((b < 2 ? v_rows[0] : v_rows[1]) + (uint32_t)(n * 132 + 66 * (b & 1)));
     };
-    int half = s0.begin + 2 * wave;
-    if (half < end) {
-        locate(half);
-        load_keys();
-        load_values();
-    }
+    QueryColumns<TQ, kTq4Cols, M::kQStride> columns;
+    columns.load(P, s0.t, head0, wave, lane);
 
     const DecodeColumn col = decode_column(P, s0.t, head0, n & 7);
     const uint32_t live = col.live & 0xFFu;
     if (live == 0u) return;
     const bool sloped = P.slopes != nullptr;
 
-    // ---- tables, query operands ----
-    build_pair_table(smem, tid, wave);
-    build_key_table(smem, tid, wave);
+    // ---- table, first loads, query operands ----
+    build_two_part_table(smem, tid, wave);
+    int half = s0.begin + 2 * wave;
+    if (half < end) {
+        locate(half);
+        load_keys();
+        load_values();
+    }
     uint16_t* qh = reinterpret_cast<uint16_t*>(smem + M::kQ);
     uint16_t* ql = reinterpret_cast<uint16_t*>(smem + M::kQLow);
     float* qs = reinterpret_cast<float*>(smem + M::kQScale);
-    bring_queries<TQ, kTq4Cols, M::kQStride>(P, s0.t, head0, live, wave, lane, qh, ql, qs);
+    columns.bring(P, live, wave, lane, qh, ql, qs);
     __syncthreads();
     u4 q[16];  // [block][word of the row][half of the word]
 #pragma unroll
@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
     }
     const float cs = P.scale2 * (qs[n & 7] * kLutInvGain), cc = P.cap_arg * (qs[n & 7] * kLutInvGain);
     const float low_part = n < 8 ? 0.f : 1.f;
-    const uint32_t lut_lane = (uint32_t)lane << 2, key_lane = ((uint32_t)lane & 31u) << 3 | 0x100u;
+    const uint32_t table_lane = ((uint32_t)lane & 31u) << 3;
 
     // Scales are loaded a row a lane and used four rows a lane: an exchange through LDS, [half][block][16 rows].
     float* k_area = reinterpret_cast<float*>(smem + M::kScale + wave * (2 * 64 * 4));
@@ -169,17 +169,24 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int blk = 0; blk < 2; ++blk) part[h][blk] = f4{0.f, 0.f, 0.f, 0.f};
+        // (look-ups a step ahead of the products: the compiler on its own waits for each, to save registers)
+        u4 a[2][4];
+        const auto key_operands = [&](int m, int w, u4 (&to)[4]) {
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+            for (int hb = 0; hb < 4; ++hb) {
+                const u2v x = key_read(kr[hb >> 1][hb & 1][m], table_lane, 2 * w), y = key_read(kr[hb >> 1][hb & 1][m], table_lane, 2 * w + 1);
+                to[hb] = u4{x[0], x[1], y[0], y[1]};
+            }
+        };
+        key_operands(0, 0, a[0]);
 #pragma unroll
-            for (int w = 0; w < 2; ++w)
+        for (int mw = 0; mw < 8; ++mw) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (mw < 7) key_operands((mw + 1) >> 1, (mw + 1) & 1, a[(mw + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int blk = 0; blk < 2; ++blk) {
-                        const u2v a = key_read(kr[h][blk][m], key_lane, 2 * w), c = key_read(kr[h][blk][m], key_lane, 2 * w + 1);
-                        part[h][blk] = mfma_rows<false>(u4{a[0], a[1], c[0], c[1]}, q[8 * blk + 2 * m + w], part[h][blk]);
-                    }
+            for (int hb = 0; hb < 4; ++hb) part[hb >> 1][hb & 1] = mfma_rows<false>(a[mw & 1][hb], q[8 * (hb & 1) + mw], part[hb >> 1][hb & 1]);
+        }
         f4 s[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -190,10 +197,8 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
                 s[h][i] = mine + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(mine), 0x128, 0xF, 0xF, false));  // row_ror:8
             }
         }
-        if (more) {
-            locate(next);
-            load_keys();
-        }
+        locate(more ? next : half);  // (rows of this unit again at the end: a load under a condition would be waited for at once)
+        load_keys();
 
         // ---- terms, masks, softmax ----
         const bool masked = !(half * 16 >= col.all_from && half * 16 + 31 <= col.all_to);  // uniform
@@ -227,9 +232,21 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
 
         // ---- values ----
         exchange(v_area, v_scale);
+        uint32_t codes[2][2][2][2];  // [block][of even, of odd channels][half][pair of rows]: a byte = code of the first row | code of the second << 4
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int t2 = 0; t2 < 2; ++t2) {
+                    const uint32_t wa = vr[h][blk][2 * t2], wb = vr[h][blk][2 * t2 + 1];
+                    codes[blk][0][h][t2] = (wa & 0x0F0F0F0Fu) | ((wb << 4) & 0xF0F0F0F0u);
+                    codes[blk][1][h][t2] = ((wa >> 4) & 0x0F0F0F0Fu) | (wb & 0xF0F0F0F0u);
+                }
+        load_values();
+        u4 w[2];
 #pragma unroll
         for (int blk = 0; blk < 2; ++blk) {
-            u4 w;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 f4 d = *reinterpret_cast<const f4*>(v_area + 32 * h + 16 * blk + 4 * b);
@@ -240,30 +257,28 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
                 float pd[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) pd[i] = mul_legacy(p[4 * h + i], d[i]);
-                w[2 * h] = weight_part(pd[0], pd[1], low_part);
-                w[2 * h + 1] = weight_part(pd[2], pd[3], low_part);
-            }
-            uint32_t even[2][2], odd[2][2];  // [half][pair of rows]: a byte = code of the first row | code of the second << 4
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int t2 = 0; t2 < 2; ++t2) {
-                    const uint32_t wa = vr[h][blk][2 * t2], wb = vr[h][blk][2 * t2 + 1];
-                    even[h][t2] = (wa & 0x0F0F0F0Fu) | ((wb << 4) & 0xF0F0F0F0u);
-                    odd[h][t2] = ((wa >> 4) & 0x0F0F0F0Fu) | (wb & 0xF0F0F0F0u);
-                }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t sel = 0x0c0c0400u + ((uint32_t)(j >> 1) << 8);
-                u4 v;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int t2 = 0; t2 < 2; ++t2) v[2 * h + t2] = lut_read((j & 1) ? odd[h][t2] : even[h][t2], lut_lane, sel);
-                o[8 * blk + j] = mfma_rows<false>(v, w, o[8 * blk + j]);
+                w[blk][2 * h] = weight_part(pd[0], pd[1], low_part);
+                w[blk][2 * h + 1] = weight_part(pd[2], pd[3], low_part);
             }
         }
-        if (more) load_values();
+        u4 v[2][2];
+        const auto value_operands = [&](int j2, u4 (&to)[2]) {  // of products 2 j2 and 2 j2 + 1
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t sel = 0x0c0c0400u + ((uint32_t)(j2 & 3) << 8);
+#pragma unroll
+                for (int x = 0; x < 4; ++x) to[k][x] = lut_read(codes[j2 >> 2][k][x >> 1][x & 1], table_lane, sel);
+            }
+        };
+        value_operands(0, v[0]);
+#pragma unroll
+        for (int j2 = 0; j2 < 8; ++j2) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (j2 < 7) value_operands(j2 + 1, v[(j2 + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) o[2 * j2 + k] = mfma_rows<false>(v[j2 & 1][k], w[j2 >> 2], o[2 * j2 + k]);
+        }
         half = next;
     }
     l_run = sum_over_rows(l_run);
