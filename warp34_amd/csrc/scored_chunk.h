@@ -28,6 +28,8 @@ constexpr int kChunkUnit = 32;
 // none of its bits, and the multiplication of 128 sums a lane is spared in nearly all units.
 constexpr float kChunkSlack = 8.0f;
 
+constexpr int kKeysAhead = 2, kValuesAhead = 2;  // operands are read from LDS so many products before their own
+
 template <bool IS_BF16>
 __device__ __forceinline__ f16v mfma_tile(u4 a, u4 b, f16v c) {
     if constexpr (IS_BF16) {
@@ -63,11 +65,12 @@ struct ChunkLds {
     using R = ScoredRows<KVF, HD>;
     static constexpr int kRow = 2 * HD;                       // of a tile
     static constexpr int kTile = kChunkUnit * kRow;           // keys or values
-    static constexpr int kTable = R::kTq4 ? 65536 : 0;
-    static constexpr int kTiles = kTable;                     // two units of {keys, values}
+    static constexpr int kTable = R::kTq4 ? 256 * 128 : 0;
+    static constexpr int kTiles = kTable;                     // two units of keys
+    static constexpr int kValues = kTiles + 2 * kTile;        // three units of values
     static constexpr int kRun = 16 * R::kRowBytes;            // of a page
     static constexpr int kRawUnit = R::k16 ? 0 : (4 * kRun + 16);
-    static constexpr int kRaw = kTiles + 4 * kTile;           // two units of {keys 0-15, 16-31, values 0-15, 16-31} as stored
+    static constexpr int kRaw = kTiles + 5 * kTile;           // two units of {keys 0-15, 16-31, values 0-15, 16-31} as stored
     static constexpr int kScale = kRaw + 2 * kRawUnit;        // two units of key scales [4][32]
     static constexpr int kLoop = kScale + (R::k16 ? 0 : 2 * 4 * 32 * 4);
     // before the loop: tile counts of the batch; eight query columns of each wave at a time.  After it: eight columns of sums.
@@ -78,6 +81,16 @@ struct ChunkLds {
     static constexpr int kBytes = kLoop > kEnds ? kLoop : kEnds;
     static_assert(kBytes <= 160 * 1024 && kRun % 16 == 0, "chunk LDS budget");
 };
+
+// TQ4: the pair table (a byte's two codes, as fp16) in 32 copies.
+__device__ __forceinline__ void build_narrow_table(uint8_t* smem, int tid, int wave) {  // by 512 threads: 16 bytes at tid + 512 i, entries (tid >> 3) + 64 i
+    const uint32_t lo = centroid_bits((uint32_t)tid >> 3 & 15u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t v = lo | centroid_bits((uint32_t)(wave >> 1) + 4u * i) << 16;
+        *reinterpret_cast<u4*>(smem + (tid + 512 * i) * 16) = u4{v, v, v, v};
+    }
+}
 
 // Roundings, beside those of the inputs' types: rotated queries and TQ4 keys are one fp16 part (the keys' block scales multiply the
 // scores in 32 bits); quantised values are fp16(scale * code), TQ4 ones from the fp16 table; weights are one operand of the values'
@@ -154,7 +167,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const float slope2 = sloped && col_ok ? P.slopes[my_head] * kLog2e : 0.f;
 
     // ---- table and query operands: lane (n, b) holds Q[column n][16 m + 8 b .. + 7] ----
-    if constexpr (R::kTq4) build_pair_table(smem, tid, wave);
+    if constexpr (R::kTq4) build_narrow_table(smem, tid, wave);
     u4 q[kSteps];
     float cs = P.scale2, cc = P.cap_arg;
     if constexpr (R::k16) {
@@ -253,7 +266,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     int slot_base = page_slot(begin, P);
     int pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
     constexpr int kShare = M::kRun / 2;
-    const auto issue = [&](int u) {
+    const auto issue = [&](int u, uint32_t values) {
         const int pos = begin + u * kChunkUnit + 16 * (run & 1);
         uint64_t off = 0;
         if (pos <= key_last) {  // (a run behind the keys: rows of page 0, which nobody sees)
@@ -269,7 +282,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         if constexpr (R::k16) {
             // rows 8 part + ..: the piece that belongs to a lane's place
             constexpr int kPieces = M::kRow / 16, kRows = 64 / kPieces;  // of a row, of an instruction
-            const uint32_t dst = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile + (loads_v ? M::kTile : 0) + (run & 1) * M::kRun + part * kShare);
+            const uint32_t dst = (loads_v ? values : (uint32_t)(M::kTiles + (u & 1) * M::kTile)) + (uint32_t)((run & 1) * M::kRun + part * kShare);
             const int at_lane = here(lane), r = at_lane / kPieces, p = at_lane % kPieces;
             const auto one = [&](auto imm) {
                 constexpr int i = decltype(imm)::value;
@@ -292,9 +305,9 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         }
     };
     // ---- raw rows of unit u -> its tiles and scales; a thread takes 16 elements of a key row and of a value row ----
-    const auto widen = [&](int u) {
+    const auto widen = [&](int u, uint32_t values) {
         if constexpr (!R::k16) {
-            const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit), tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
+            const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit), keys = (uint32_t)(M::kTiles + (u & 1) * M::kTile);
             const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 512);
             const int at_tid = here(tid), r = at_tid >> 4, c = at_tid & 15;
             const int row_pos = begin + u * kChunkUnit + r;
@@ -308,7 +321,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                     const uint32_t at = src + (c >= 8 ? 68u : 0u) + 8u * (c & 7);
                     const uint32_t shift = c >= 8 ? 0u : 16u, d0 = lds_u1(at), d1 = lds_u1(at + 4), d2 = lds_u1(at + 8);
                     uint32_t codes[2] = {__builtin_amdgcn_alignbit(d1, d0, shift), __builtin_amdgcn_alignbit(d2, d1, shift)};
-                    const uint32_t lut_lane = ((uint32_t)at_tid & 63u) << 2;
+                    const uint32_t copy = ((uint32_t)at_tid & 31u) << 2;
                     const uint32_t d16 = side == 1 && seen ? lds_u16(src + (c >= 8 ? 66u : 0u)) : 0u;
                     const h2 d = __builtin_bit_cast(h2, d16 | d16 << 16);
 #pragma unroll
@@ -316,7 +329,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             // (a scalar in between: a bit cast of a vector's element reads its first one)
-                            uint32_t pair = lut_read(codes[h], lut_lane, 0x0c0c0400u + ((uint32_t)k << 8));
+                            uint32_t pair = lds_u1(((k == 0 ? codes[h] << 7 : codes[h] >> (8 * k - 7)) & 0x7F80u) | copy);
                             if (side == 1) pair = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) * d);
                             w[h][k] = pair;
                         }
@@ -356,7 +369,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int p = 2 * c + h;
-                    lds_put(tiles + (uint32_t)(side * M::kTile + r * M::kRow + 16 * (p ^ (side ? 4 * (r & 3) : (r & 15)))), w[h]);
+                    lds_put((side ? values : keys) + (uint32_t)(r * M::kRow + 16 * (p ^ (side ? 4 * (r & 3) : (r & 15)))), w[h]);
                 }
             }
             // key scales: [block][row]
@@ -376,17 +389,25 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         for (int i = 0; i < 16; ++i) o[k][i] = 0.f;
     float m_run = kNegBig, l_run = 0.f;
 
-    const auto multiply = [&](int u) {
+    u4 w[2];               // the weights of the wave's last scored unit
+    bool weighted = false;  // it has some (uniform)
+    const auto score = [&](int u) {
         const int at_lane = here(lane), n = at_lane & 31, b = at_lane >> 5;
         const int u0 = begin + u * kChunkUnit;
-        if (u0 > any_to || u0 + kChunkUnit - 1 < any_from) return;  // uniform
-        const uint32_t tiles = (uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile);
+        weighted = u0 <= any_to && u0 + kChunkUnit - 1 >= any_from;  // uniform
+        if (!weighted) return;
+        const uint32_t tiles = (uint32_t)(M::kTiles + (u & 1) * M::kTile);
         const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 512);
         // ---- scores ----
         f16v s;
         {
             const uint32_t row = tiles + (uint32_t)(n * M::kRow), swap = 16u * (uint32_t)(b ^ (n & 15));
             constexpr int kBlocks = R::k16 ? 1 : R::kScales, kPer = kSteps / kBlocks;
+            // operands are read kKeysAhead products before their own (the compiler would read each right before it, to save registers)
+            const auto k_operand = [&](int m) { return lds_u4(row + (swap ^ (uint32_t)(32 * (m & 7))) + 256u * (m >> 3)); };
+            u4 a[kKeysAhead + 1];
+#pragma unroll
+            for (int m = 0; m < kKeysAhead; ++m) a[m] = k_operand(m);
 #pragma unroll
             for (int blk = 0; blk < kBlocks; ++blk) {
                 f16v part_s;
@@ -395,7 +416,10 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
 #pragma unroll
                 for (int mm = 0; mm < kPer; ++mm) {
                     const int m = blk * kPer + mm;
-                    part_s = mfma_tile<IS_BF16>(lds_u4(row + (swap ^ (uint32_t)(32 * (m & 7))) + 256u * (m >> 3)), q[m], part_s);
+                    __builtin_amdgcn_sched_barrier(0);
+                    if (m + kKeysAhead < kSteps) a[(m + kKeysAhead) % (kKeysAhead + 1)] = k_operand(m + kKeysAhead);
+                    __builtin_amdgcn_sched_barrier(0);
+                    part_s = mfma_tile<IS_BF16>(a[m % (kKeysAhead + 1)], q[m], part_s);
                 }
                 if constexpr (R::k16) {
                     s = part_s;
@@ -452,11 +476,14 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             sum += s[i];
         }
         l_run += sum;
-        __builtin_amdgcn_sched_barrier(0);
-        // ---- values ----
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k >> 2][k & 3] = IS_BF16 ? pack_bf2(s[2 * k], s[2 * k + 1]) : pack_h2(s[2 * k], s[2 * k + 1]);
+    };
+    const auto add_values = [&](uint32_t values) {
+        if (!weighted) return;
         // lane l reads row (l & 15) >> 2 of four, 8 bytes at 8 (l & 3) of the 32 of its 16 channels
-        const int j = at_lane & 15;
-        const uint32_t v_at = tiles + (uint32_t)(M::kTile + (4 * b + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(at_lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
+        const int at_lane = here(lane), j = at_lane & 15;
+        const uint32_t v_at = values + (uint32_t)((4 * (at_lane >> 5) + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(at_lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
         const auto v_operand = [&](int dt, int step) -> u4 {
             const uint32_t at = (v_at ^ (64u * (uint32_t)(dt & 3))) + 256u * (uint32_t)(dt >> 2) + (uint32_t)(step * 16 * M::kRow);
             const s4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
@@ -464,18 +491,20 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             const u2v x = __builtin_bit_cast(u2v, a), y = __builtin_bit_cast(u2v, c);
             return u4{x[0], x[1], y[0], y[1]};
         };
-        {
-            u4 w[2];
+        u4 a[kValuesAhead + 1];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) w[k >> 2][k & 3] = IS_BF16 ? pack_bf2(s[2 * k], s[2 * k + 1]) : pack_h2(s[2 * k], s[2 * k + 1]);
+        for (int i = 0; i < kValuesAhead; ++i) a[i] = v_operand(i >> 1, i & 1);
 #pragma unroll
-            for (int dt = 0; dt < kDims; ++dt)
-#pragma unroll
-                for (int step = 0; step < 2; ++step) o[dt] = mfma_tile<IS_BF16>(v_operand(dt, step), w[step], o[dt]);
+        for (int i = 0; i < 2 * kDims; ++i) {
+            const int next = i + kValuesAhead;
+            __builtin_amdgcn_sched_barrier(0);
+            if (next < 2 * kDims) a[next % (kValuesAhead + 1)] = v_operand(next >> 1, next & 1);
+            __builtin_amdgcn_sched_barrier(0);
+            o[i >> 1] = mfma_tile<IS_BF16>(a[i % (kValuesAhead + 1)], w[i & 1], o[i >> 1]);
         }
     };
     // 16-bit value rows that no token of the tile sees count as zeros: a page's rest may hold anything
-    const auto clear_unseen = [&](int u) {
+    const auto clear_unseen = [&](int u, uint32_t values) {
         if constexpr (R::k16) {
             const int u0 = begin + u * kChunkUnit;
             if (u0 >= key_first && u0 + kChunkUnit - 1 <= key_last) return;  // uniform
@@ -483,31 +512,46 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             for (int p = tid; p < kPieces; p += kChunkWaves * 64) {
                 const int pos = u0 + p / (M::kRow / 16);
                 if (pos < key_first || pos > key_last)
-                    lds_put((uint32_t)(M::kTiles + (u & 1) * 2 * M::kTile + M::kTile + 16 * p), u4{0u, 0u, 0u, 0u});
+                    lds_put(values + (uint32_t)(16 * p), u4{0u, 0u, 0u, 0u});
             }
             chunk_barrier();
         }
     };
 
-    if (units > 0) issue(0);
+    // Waves w and w + 4 share a SIMD.  The second of them multiplies the values of a unit in the next interval, before its scores, so that
+    // the products of one run beside the other's vector work: widen, scores, softmax, values | values, widen, scores, softmax.  Values stay
+    // for two intervals: three tiles of them.
+    const bool late = wave >= 4;
+    uint32_t v_last = (uint32_t)(M::kValues + 2 * M::kTile), v_now = (uint32_t)M::kValues, v_next = (uint32_t)(M::kValues + M::kTile);
+    if (units > 0) issue(0, v_now);
     if constexpr (!R::k16) {
-        if (units > 1) issue(1);
+        if (units > 1) issue(1, 0u);
         chunk_barrier();
-        if (units > 0) widen(0);
+        if (units > 0) widen(0, v_now);
     }
     for (int u = 0; u < units; ++u) {
         chunk_barrier();  // unit u's tiles are whole, the next one's rows have landed; nobody reads what is overwritten below
         if constexpr (R::k16) {
-            if (u + 1 < units) issue(u + 1);
-            clear_unseen(u);
+            if (u + 1 < units) issue(u + 1, v_next);
+            clear_unseen(u, v_now);
         } else {
-            if (u + 2 < units) issue(u + 2);
-            if (u + 1 < units) widen(u + 1);
+            if (u + 2 < units) issue(u + 2, 0u);
         }
         __builtin_amdgcn_sched_barrier(0);
-        multiply(u);
+        if (late && u > 0) add_values(v_last);
         __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!R::k16) {
+            if (u + 1 < units) widen(u + 1, v_next);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        score(u);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!late) add_values(v_now);
+        __builtin_amdgcn_sched_barrier(0);
+        const uint32_t free = v_last;
+        v_last = v_now, v_now = v_next, v_next = free;
     }
+    if (late && units > 0) add_values(v_last);
     {
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
         l_run = __uint_as_float(r[0]) + __uint_as_float(r[1]);
