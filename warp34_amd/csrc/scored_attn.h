@@ -239,6 +239,41 @@ __device__ __forceinline__ ScoredWork find_work(const ScoredParams& P, int per, 
     return ScoredWork{-1, 0, 0, 0};
 }
 
+// The same with the longest chunks first: workgroups start in the order of their slots, so what starts last is short, and the batch ends
+// at once on all CUs.  64 classes of length; hist: in LDS, zeros at first.  For all threads of a workgroup (threads: their number).
+__device__ __forceinline__ int length_class(int halves, int chunks, float classes_per_half) {
+    return 63 - min(63, (int)((float)fast_div(halves + chunks - 1, chunks) * classes_per_half));
+}
+template <typename Count>
+__device__ __forceinline__ ScoredWork find_work_by_length(const ScoredParams& P, int per, int slot, int tid, int threads, int lane, int* hist, Count&& count) {
+    const float scale = 64.0f / (float)(per + 1);
+    for (int e = tid; e < P.entries; e += threads) {
+        const int h = count(e), c = chunks_of(h, per);
+        if (c > 0) atomicAdd(&hist[length_class(h, c, scale)], c);
+    }
+    __syncthreads();
+    const int chunks = hist[lane], chunks_upto = wave_prefix(chunks);
+    const unsigned long long classes = __ballot(slot < chunks_upto);
+    if (classes == 0ull) return ScoredWork{-1, 0, 0, 0};
+    const int cls = (int)__builtin_ctzll(classes);
+    const int rest = slot - (__builtin_amdgcn_readlane(chunks_upto, cls) - __builtin_amdgcn_readlane(chunks, cls));
+    int before = 0, records = 0;
+    for (int base = 0; base < P.entries; base += 64) {
+        const int h = base + lane < P.entries ? count(base + lane) : -1, c = chunks_of(h, per);
+        const int mine = c > 0 && length_class(h, c, scale) == cls ? c : 0, split = c > 1 ? c : 0;
+        const int upto = before + wave_prefix(mine), records_upto = records + wave_prefix(split);
+        const unsigned long long hit = __ballot(rest < upto);
+        if (hit != 0ull) {
+            const int l = (int)__builtin_ctzll(hit);
+            const int n = __builtin_amdgcn_readlane(mine, l), end = __builtin_amdgcn_readlane(upto, l);
+            return ScoredWork{base + l, rest - (end - n), n, __builtin_amdgcn_readlane(records_upto, l) - n};
+        }
+        before = __builtin_amdgcn_readlane(upto, 63);
+        records = __builtin_amdgcn_readlane(records_upto, 63);
+    }
+    return ScoredWork{-1, 0, 0, 0};
+}
+
 // The end of a row: lane l holds channels 4 l .. 4 l + 3 of the sum, un-normalised; value_scale: what the sums have to be multiplied by.
 template <typename TQ, int HD>
 __device__ __forceinline__ void finish_row(const ScoredParams& P, int tok, int head, int lane, float (&v)[4], float m, float l, float value_scale) {

@@ -21,6 +21,8 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s4v lds_s4;
 typedef __attribute__((address_space(3))) const f4 lds_f4c;
 
+typedef u4 u4_at8 __attribute__((aligned(8)));
+
 constexpr int kChunkWaves = 8;
 constexpr int kChunkCols = 32 * kChunkWaves;
 constexpr int kChunkUnit = 32;
@@ -77,7 +79,8 @@ struct ChunkLds {
     static constexpr int kColStride = HD + 8;
     static constexpr int kCounts = kTiles + kChunkWaves * 8 * kColStride * 4;
     static constexpr int kQScale = kCounts + kMaxSplitEntries * 4;
-    static constexpr int kEnds = kQScale + kChunkCols * 4;
+    static constexpr int kHist = kQScale + kChunkCols * 4;
+    static constexpr int kEnds = kHist + 64 * 4;
     static constexpr int kBytes = kLoop > kEnds ? kLoop : kEnds;
     static_assert(kBytes <= 160 * 1024 && kRun % 16 == 0, "chunk LDS budget");
 };
@@ -108,26 +111,30 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const int n = lane & 31, b = lane >> 5;
     const warp34_kv_layer_layout& L = P.L;
     const warp34_attention_batch& B = P.B;
-    const int kv_sub = (int)blockIdx.y;
+    // the kv heads of a slot start together
+    const int started = (int)(blockIdx.x + gridDim.x * blockIdx.y), kv_subs = (int)gridDim.y;
+    const int slot = kv_subs == 1 ? started : fast_div(started, kv_subs), kv_sub = started - slot * kv_subs;
     const int kv_head = P.q_subgroups == 1 ? kv_sub : fast_div(kv_sub, P.q_subgroups);
     const int head0 = kv_head * P.gqa + (kv_sub - kv_head * P.q_subgroups) * P.q_group;
 
     // ---- what this workgroup works on ----
-    ScoredWork work = {(int)blockIdx.x, 0, 1, 0};
+    ScoredWork work = {slot, 0, 1, 0};
     if (P.target > 0) {
         int* halves = reinterpret_cast<int*>(smem + M::kCounts);
+        int* hist = reinterpret_cast<int*>(smem + M::kHist);
+        if (tid < 64) hist[tid] = 0;
         for (int e = tid; e < P.entries; e += kChunkWaves * 64) halves[e] = tile_halves_guess(P, scored_tile(P, e));
         __syncthreads();
         const auto count = [&](int e) { return halves[e]; };
         const int per = chunk_length(P, lane, count);
-        work = find_work(P, per, P.target - 1 - (int)blockIdx.x, lane, count);  // a request's last tiles, which have most keys, first
+        work = find_work_by_length(P, per, slot, tid, kChunkWaves * 64, lane, hist, count);
         if (work.entry < 0) return;
         if (work.chunk == 0 && kv_sub == 0 && tid == 0) {
             P.table[2 * work.entry] = work.first_record;
             P.table[2 * work.entry + 1] = work.chunks;
         }
     } else {
-        work.entry = (int)(gridDim.x - 1 - blockIdx.x);  // the tiles with most keys first
+        work.entry = (int)gridDim.x - 1 - slot;  // the tiles with most keys first
     }
     const ScoredTile t = scored_tile(P, work.entry);
     if (t.tokens <= 0) return;
@@ -165,6 +172,59 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const uint32_t live = (uint32_t)__ballot(col_ok);
     const bool sloped = P.slopes != nullptr;
     const float slope2 = sloped && col_ok ? P.slopes[my_head] * kLog2e : 0.f;
+
+    // ---- loader: waves 2 i and 2 i + 1 bring half each of run i (keys 0-15, 16-31, values 0-15, 16-31) ----
+    const int run = wave >> 1, part = wave & 1;
+    const bool loads_v = run >= 2;
+    const uint8_t* slab = reinterpret_cast<const uint8_t*>((uintptr_t)(loads_v ? L.v_base : L.k_base)) +
+                          (uint64_t)(uint32_t)kv_head * (loads_v ? L.v_head_stride_bytes : L.k_head_stride_bytes);
+    const uint64_t page_stride = loads_v ? L.v_page_stride_bytes : L.k_page_stride_bytes;
+    const int32_t* blocks = B.block_tables + (size_t)t.req * B.max_blocks_per_req;
+    int slot_base = page_slot(begin, P);
+    int pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
+    constexpr int kShare = M::kRun / 2;
+    const auto issue = [&](int u, uint32_t values) {
+        const int pos = begin + u * kChunkUnit + 16 * (run & 1);
+        uint64_t off = 0;
+        if (pos <= key_last) {  // (a run behind the keys: rows of page 0, which nobody sees)
+            const int slot = page_slot(pos, P);
+            if (slot - slot_base >= 64) {
+                slot_base = slot;
+                pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
+            }
+            const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, slot - slot_base), 0);
+            off = (uint64_t)page * page_stride + (uint32_t)(pos - slot * L.block_size) * (uint32_t)R::kRowBytes;
+        }
+        const uint8_t* src = uniform_pointer(slab + off + part * kShare);
+        if constexpr (R::k16) {
+            // rows 8 part + ..: the piece that belongs to a lane's place
+            constexpr int kPieces = M::kRow / 16, kRows = 64 / kPieces;  // of a row, of an instruction
+            const uint32_t dst = (loads_v ? values : (uint32_t)(M::kTiles + (u & 1) * M::kTile)) + (uint32_t)((run & 1) * M::kRun + part * kShare);
+            const int at_lane = here(lane), r = at_lane / kPieces, p = at_lane % kPieces;
+            const auto one = [&](auto imm) {
+                constexpr int i = decltype(imm)::value;
+                const int row = 8 * part + i * kRows + r;
+                const uint32_t v = (uint32_t)(r * M::kRow + 16 * (p ^ (loads_v ? 4 * (row & 3) : (row & 15))));
+                load_to_lds<1024 * i>(v, src, dst);
+            };
+            one(std::integral_constant<int, 0>{});
+            one(std::integral_constant<int, 1>{});
+            if constexpr (kShare > 2048) {
+                one(std::integral_constant<int, 2>{});
+                one(std::integral_constant<int, 3>{});
+            }
+        } else {
+            const uint32_t dst = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit + run * M::kRun + part * kShare), v = 16u * (uint32_t)here(lane);
+            load_to_lds<0>(v, src, dst);
+            if constexpr (kShare >= 2048) load_to_lds<1024>(v, src, dst);
+            constexpr int kRest = kShare % 1024;
+            if (v < (uint32_t)kRest) load_to_lds<kShare - kRest>(v, src, dst);
+        }
+    };
+    // (a run's place is none of what the queries' columns go through)
+    uint32_t v_last = (uint32_t)(M::kValues + 2 * M::kTile), v_now = (uint32_t)M::kValues, v_next = (uint32_t)(M::kValues + M::kTile);
+    if (units > 0) issue(0, v_now);
+    if (!R::k16 && units > 1) issue(1, 0u);
 
     // ---- table and query operands: lane (n, b) holds Q[column n][16 m + 8 b .. + 7] ----
     if constexpr (R::kTq4) build_narrow_table(smem, tid, wave);
@@ -256,54 +316,6 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     }
     __syncthreads();  // the areas become tiles
 
-    // ---- loader: waves 2 i and 2 i + 1 bring half each of run i (keys 0-15, 16-31, values 0-15, 16-31) ----
-    const int run = wave >> 1, part = wave & 1;
-    const bool loads_v = run >= 2;
-    const uint8_t* slab = reinterpret_cast<const uint8_t*>((uintptr_t)(loads_v ? L.v_base : L.k_base)) +
-                          (uint64_t)(uint32_t)kv_head * (loads_v ? L.v_head_stride_bytes : L.k_head_stride_bytes);
-    const uint64_t page_stride = loads_v ? L.v_page_stride_bytes : L.k_page_stride_bytes;
-    const int32_t* blocks = B.block_tables + (size_t)t.req * B.max_blocks_per_req;
-    int slot_base = page_slot(begin, P);
-    int pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
-    constexpr int kShare = M::kRun / 2;
-    const auto issue = [&](int u, uint32_t values) {
-        const int pos = begin + u * kChunkUnit + 16 * (run & 1);
-        uint64_t off = 0;
-        if (pos <= key_last) {  // (a run behind the keys: rows of page 0, which nobody sees)
-            const int slot = page_slot(pos, P);
-            if (slot - slot_base >= 64) {
-                slot_base = slot;
-                pages = slot_base + lane < B.max_blocks_per_req ? blocks[slot_base + lane] : 0;
-            }
-            const uint32_t page = (uint32_t)max(__builtin_amdgcn_readlane(pages, slot - slot_base), 0);
-            off = (uint64_t)page * page_stride + (uint32_t)(pos - slot * L.block_size) * (uint32_t)R::kRowBytes;
-        }
-        const uint8_t* src = uniform_pointer(slab + off + part * kShare);
-        if constexpr (R::k16) {
-            // rows 8 part + ..: the piece that belongs to a lane's place
-            constexpr int kPieces = M::kRow / 16, kRows = 64 / kPieces;  // of a row, of an instruction
-            const uint32_t dst = (loads_v ? values : (uint32_t)(M::kTiles + (u & 1) * M::kTile)) + (uint32_t)((run & 1) * M::kRun + part * kShare);
-            const int at_lane = here(lane), r = at_lane / kPieces, p = at_lane % kPieces;
-            const auto one = [&](auto imm) {
-                constexpr int i = decltype(imm)::value;
-                const int row = 8 * part + i * kRows + r;
-                const uint32_t v = (uint32_t)(r * M::kRow + 16 * (p ^ (loads_v ? 4 * (row & 3) : (row & 15))));
-                load_to_lds<1024 * i>(v, src, dst);
-            };
-            one(std::integral_constant<int, 0>{});
-            one(std::integral_constant<int, 1>{});
-            if constexpr (kShare > 2048) {
-                one(std::integral_constant<int, 2>{});
-                one(std::integral_constant<int, 3>{});
-            }
-        } else {
-            const uint32_t dst = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit + run * M::kRun + part * kShare), v = 16u * (uint32_t)here(lane);
-            load_to_lds<0>(v, src, dst);
-            if constexpr (kShare >= 2048) load_to_lds<1024>(v, src, dst);
-            constexpr int kRest = kShare % 1024;
-            if (v < (uint32_t)kRest) load_to_lds<kShare - kRest>(v, src, dst);
-        }
-    };
     // ---- raw rows of unit u -> its tiles and scales; a thread takes 16 elements of a key row and of a value row ----
     const auto widen = [&](int u, uint32_t values) {
         if constexpr (!R::k16) {
@@ -522,10 +534,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     // the products of one run beside the other's vector work: widen, scores, softmax, values | values, widen, scores, softmax.  Values stay
     // for two intervals: three tiles of them.
     const bool late = wave >= 4;
-    uint32_t v_last = (uint32_t)(M::kValues + 2 * M::kTile), v_now = (uint32_t)M::kValues, v_next = (uint32_t)(M::kValues + M::kTile);
-    if (units > 0) issue(0, v_now);
     if constexpr (!R::k16) {
-        if (units > 1) issue(1, 0u);
         chunk_barrier();
         if (units > 0) widen(0, v_now);
     }
@@ -558,9 +567,38 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     }
     chunk_barrier();
 
-    // ---- rows out, eight columns of a wave at a time through LDS ----
+    // ---- rows out ----
+    if (work.chunks > 1 || HD != 256 || !P.rot_out) {  // as they stand: a lane has pairs of four channels of its column
+        if (!col_ok) return;
+        if (work.chunks > 1) {
+            const size_t record = ((size_t)(work.first_record + work.chunk) * kv_subs + kv_sub) * kChunkCols + col;
+            float* to = P.part_acc + record * HD + 4 * b;
+#pragma unroll
+            for (int dt = 0; dt < kDims; ++dt)
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<f4*>(to + 32 * dt + 8 * k) = f4{o[dt][4 * k], o[dt][4 * k + 1], o[dt][4 * k + 2], o[dt][4 * k + 3]};
+            if (b == 0) *reinterpret_cast<f2*>(P.part_ml + 2 * record) = f2{m_run, l_run};
+        } else {
+            const size_t row = (size_t)my_tok * P.num_q_heads + (size_t)my_head;
+            const bool some = l_run > 0.f || l_run != l_run;
+            const float inv = some ? R::kOutScale / l_run : 0.f;  // (a row without keys: zeros)
+            uint16_t* to = P.out + row * HD + 8 * b;
+            const auto pack = [&](float x, float y) { return TQ::kStorageFormat == WARP34_KV_FORMAT_BF16 ? pack_bf2(x * inv, y * inv) : pack_h2(x * inv, y * inv); };
+#pragma unroll
+            for (int dt = 0; dt < kDims; ++dt)
+#pragma unroll
+                for (int k = 0; k < 4; k += 2) {  // the half wave with b = 0 takes channels 0 .. 7 of 16, the other one 8 .. 15
+                    const auto x = __builtin_amdgcn_permlane32_swap(pack(o[dt][4 * k], o[dt][4 * k + 1]), pack(o[dt][4 * k + 4], o[dt][4 * k + 5]), false, false);
+                    const auto y = __builtin_amdgcn_permlane32_swap(pack(o[dt][4 * k + 2], o[dt][4 * k + 3]), pack(o[dt][4 * k + 6], o[dt][4 * k + 7]), false, false);
+                    *reinterpret_cast<u4_at8*>(to + 32 * dt + 8 * k) = u4{x[0], y[0], x[1], y[1]};
+                }
+            if (P.lse != nullptr && b == 0) P.lse[row] = some ? (m_run + __builtin_amdgcn_logf(l_run)) * 0.6931471805599453f : -INFINITY;
+        }
+        return;
+    }
+    // rotated back, eight columns of a wave at a time through LDS
     float* area = reinterpret_cast<float*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
-    const int kv_subs = (int)gridDim.y;
 #pragma unroll 1
     for (int g = 0; g < 4; ++g) {
         if ((n >> 3) == g) {
@@ -573,22 +611,16 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_wave_barrier();
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
-#pragma unroll 2
+#pragma unroll 4
         for (int c8 = 0; c8 < 8; ++c8) {
             const int c = 8 * g + c8;
             if (!((live >> c) & 1u)) continue;
-            const f4 acc = *reinterpret_cast<const f4*>(area + c8 * M::kColStride + ((4 * lane) & (HD - 1)));
+            const f4 acc = *reinterpret_cast<const f4*>(area + c8 * M::kColStride + 4 * lane);
             const float m_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), c));
             const float l_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_run), c));
-            if (work.chunks > 1) {
-                const size_t record = ((size_t)(work.first_record + work.chunk) * kv_subs + kv_sub) * kChunkCols + 32 * wave + c;
-                if (4 * lane < HD) *reinterpret_cast<f4*>(P.part_acc + record * HD + 4 * lane) = acc;
-                if (lane == 0) *reinterpret_cast<f2*>(P.part_ml + 2 * record) = f2{m_c, l_c};
-            } else {
-                float v[4] = {acc[0], acc[1], acc[2], acc[3]};
-                const int ct = column_token(32 * wave + c, P);
-                finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, R::kOutScale);
-            }
+            float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+            const int ct = column_token(32 * wave + c, P);
+            finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, R::kOutScale);
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_wave_barrier();
