@@ -58,6 +58,7 @@ __device__ __forceinline__ const uint8_t* uniform_pointer(const uint8_t* p) {
 __device__ __forceinline__ void chunk_barrier() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 __device__ __forceinline__ u4 lds_u4(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const u4*>((uintptr_t)at); }
 __device__ __forceinline__ uint32_t lds_u1(uint32_t at) { return *reinterpret_cast<lds_cu32*>((uintptr_t)at); }
+__device__ __forceinline__ u2v lds_u2(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const u2v*>((uintptr_t)at); }
 __device__ __forceinline__ uint32_t lds_u16(uint32_t at) { return *reinterpret_cast<__attribute__((address_space(3))) const uint16_t*>((uintptr_t)at); }
 __device__ __forceinline__ f4 lds_f4(uint32_t at) { return *reinterpret_cast<lds_f4c*>((uintptr_t)at); }
 __device__ __forceinline__ void lds_put(uint32_t at, u4 v) { *reinterpret_cast<__attribute__((address_space(3))) u4*>((uintptr_t)at) = v; }
@@ -316,81 +317,116 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     }
     __syncthreads();  // the areas become tiles
 
-    // ---- raw rows of unit u -> its tiles and scales; a thread takes 16 elements of a key row and of a value row ----
-    const auto widen = [&](int u, uint32_t values) {
-        if constexpr (!R::k16) {
-            const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit), keys = (uint32_t)(M::kTiles + (u & 1) * M::kTile);
-            const uint32_t scale = (uint32_t)(M::kScale + (u & 1) * 512);
-            const int at_tid = here(tid), r = at_tid >> 4, c = at_tid & 15;
-            const int row_pos = begin + u * kChunkUnit + r;
-            const bool seen = row_pos >= key_first && row_pos <= key_last;
+    // ---- raw rows of unit u -> its tiles and scales ----
+    // A thread takes pieces c and c + 16 (8 elements each) of a key row and of a value row.  Each piece in steps, which stand between
+    // the products of values: what a step reads from LDS the next one uses.
+    struct Widening {
+        uint32_t row, codes, keys, values, scale;  // places in LDS
+        uint32_t raw[2], d, scale_raw;
+        u4 w;
+        bool seen;
+    };
+    const auto widen_start = [&](int u, uint32_t values, Widening& x) {
+        const int at_tid = here(tid), r = at_tid >> 4, c = at_tid & 15;
+        const uint32_t raw = (uint32_t)(M::kRaw + (u & 1) * M::kRawUnit);
+        const int row_pos = begin + u * kChunkUnit + r;
+        x.seen = row_pos >= key_first && row_pos <= key_last;
+        x.row = raw + (uint32_t)(r * R::kRowBytes) + (R::kQ8 ? 68u * (uint32_t)(c >> 3) : 0u);
+        x.codes = R::kTq4 ? x.row + 4u * (uint32_t)c : R::kFp8 ? x.row + 8u * (uint32_t)c : x.row + 4u + 8u * (uint32_t)(c & 7);
+        x.keys = (uint32_t)(M::kTiles + (u & 1) * M::kTile + r * M::kRow + 16 * (c ^ (r & 15)));
+        x.values = values + (uint32_t)(r * M::kRow + 16 * (c ^ 4 * (r & 3)));
+        // key scales: [block][row], by the first threads
+        x.scale = (uint32_t)(M::kScale + (u & 1) * 512 + 4 * at_tid);
+        if (at_tid < R::kScales * 32) {
+            const uint32_t from = raw + (uint32_t)((at_tid & 31) * R::kRowBytes), blk = (uint32_t)at_tid / 32u;
+            x.scale_raw = R::kTq4 ? lds_u16(from + 66u * blk) : lds_u1(R::kFp8 ? from + 256u + 4u * blk : from + 68u * blk);
+        }
+    };
+    const auto widen_scales = [&](Widening& x) {
+        if (here(tid) < R::kScales * 32)
+            *reinterpret_cast<__attribute__((address_space(3))) float*>((uintptr_t)x.scale) = R::kTq4 ? F16::to_f32((uint16_t)x.scale_raw) : __uint_as_float(x.scale_raw);
+    };
+    const auto widen_load = [&](int piece, Widening& x) {  // piece: 2 (values) + the half of the row
+        const int side = piece >> 1, h = piece & 1;
+        const uint32_t from = x.codes + (uint32_t)(side * 2 * M::kRun), row = x.row + (uint32_t)(side * 2 * M::kRun);
+        if constexpr (R::kTq4) {
+            // (reads of four bytes must be aligned, the codes of the first half start at byte 2)
+            x.raw[0] = lds_u1(from + (h ? 68u : 0u));
+            if (h == 0) x.raw[1] = lds_u1(from + 4u);
+            if (side == 1) x.d = lds_u16(row + (h ? 66u : 0u));
+        } else if constexpr (R::kFp8) {
+            const u2v two = lds_u2(from + 128u * (uint32_t)h);
+            x.raw[0] = two[0], x.raw[1] = two[1];
+            if (side == 1) x.d = lds_u1(row + 256u + 4u * (uint32_t)h);
+        } else {
+            x.raw[0] = lds_u1(from + 136u * (uint32_t)h), x.raw[1] = lds_u1(from + 136u * (uint32_t)h + 4u);
+            if (side == 1) x.d = lds_u1(row + 136u * (uint32_t)h);
+        }
+    };
+    const auto widen_look_up = [&](int piece, Widening& x) {
+        if constexpr (R::kTq4) {
+            const uint32_t codes = (piece & 1) ? x.raw[0] : __builtin_amdgcn_alignbit(x.raw[1], x.raw[0], 16);
+            const uint32_t copy = ((uint32_t)here(tid) & 31u) << 2;
 #pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const uint32_t src = raw + (uint32_t)(side * 2 * M::kRun + r * R::kRowBytes);
-                u4 w[2];
-                if constexpr (R::kTq4) {
-                    // (reads of four bytes must be aligned, the codes of the first half start at byte 2)
-                    const uint32_t at = src + (c >= 8 ? 68u : 0u) + 8u * (c & 7);
-                    const uint32_t shift = c >= 8 ? 0u : 16u, d0 = lds_u1(at), d1 = lds_u1(at + 4), d2 = lds_u1(at + 8);
-                    uint32_t codes[2] = {__builtin_amdgcn_alignbit(d1, d0, shift), __builtin_amdgcn_alignbit(d2, d1, shift)};
-                    const uint32_t copy = ((uint32_t)at_tid & 31u) << 2;
-                    const uint32_t d16 = side == 1 && seen ? lds_u16(src + (c >= 8 ? 66u : 0u)) : 0u;
-                    const h2 d = __builtin_bit_cast(h2, d16 | d16 << 16);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t pair = lds_u1(((k == 0 ? codes << 7 : codes >> (8 * k - 7)) & 0x7F80u) | copy);
+                x.w[k] = pair;
+            }
+        }
+    };
+    const auto widen_store = [&](int piece, Widening& x) {
+        const int side = piece >> 1, h = piece & 1;
+        if constexpr (R::kTq4) {
+            if (side == 1) {
+                const uint32_t d16 = x.seen ? x.d : 0u;
+                const h2 d = __builtin_bit_cast(h2, d16 | d16 << 16);
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t pair = x.w[k];  // (a scalar in between: a bit cast of a vector's element reads its first one)
+                    x.w[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) * d);
+                }
+            }
+        } else {
+            const float d = x.seen ? __uint_as_float(x.d) : 0.f;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            // (a scalar in between: a bit cast of a vector's element reads its first one)
-                            uint32_t pair = lds_u1(((k == 0 ? codes[h] << 7 : codes[h] >> (8 * k - 7)) & 0x7F80u) | copy);
-                            if (side == 1) pair = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, pair) * d);
-                            w[h][k] = pair;
-                        }
-                } else {
-                    const uint32_t at = R::kFp8 ? src + 16u * c : src + 68u * (c >> 2) + 4u + 16u * (c & 3);
-                    const float d = side == 1 ? __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * (c >> 3) : src + 68u * (c >> 2))) : 1.f;
+            for (int k = 0; k < 2; ++k) {
+                uint32_t code = x.raw[k], lo2, hi2;
+                if (side == 1) {
+                    code = x.seen ? code : 0u;
+                    float f[4];
+                    if constexpr (R::kFp8) {
+                        const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), s = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
+                        f[0] = p[0], f[1] = p[1], f[2] = s[0], f[3] = s[1];
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        uint32_t code = lds_u1(at + 4 * k);
-                        if (side == 1) code = seen ? code : 0u;
-                        uint32_t x, y;
-                        if (side == 1) {
-                            float f[4];
-                            if constexpr (R::kFp8) {
-                                const f2 p = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, false), s = __builtin_amdgcn_cvt_pk_f32_fp8((int)code, true);
-                                f[0] = p[0], f[1] = p[1], f[2] = s[0], f[3] = s[1];
-                            } else {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(code >> (8 * i));
-                            }
-                            const float dd = seen ? d : 0.f;
-                            x = pack_h2(f[0] * dd, f[1] * dd);
-                            y = pack_h2(f[2] * dd, f[3] * dd);
-                        } else if constexpr (R::kFp8) {
-                            x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, false));
-                            y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, true));
-                        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
-                            const uint32_t u8 = code ^ 0x80808080u;
-                            const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-                            x = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04010400u)) - bias);
-                            y = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04030402u)) - bias);
-                        }
-                        w[k >> 1][2 * (k & 1)] = x;
-                        w[k >> 1][2 * (k & 1) + 1] = y;
+                        for (int i = 0; i < 4; ++i) f[i] = (float)(int8_t)(code >> (8 * i));
                     }
+                    lo2 = pack_h2(f[0] * d, f[1] * d);
+                    hi2 = pack_h2(f[2] * d, f[3] * d);
+                } else if constexpr (R::kFp8) {
+                    lo2 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, false));
+                    hi2 = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code, 1.0f, true));
+                } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
+                    const uint32_t u8 = code ^ 0x80808080u;
+                    const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+                    lo2 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04010400u)) - bias);
+                    hi2 = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u8, 0x04030402u)) - bias);
                 }
+                x.w[2 * k] = lo2;
+                x.w[2 * k + 1] = hi2;
+            }
+        }
+        lds_put((side ? x.values : x.keys) + 256u * (uint32_t)h, x.w);
+    };
+    const auto widen = [&](int u, uint32_t values) {
+        Widening x;
+        widen_start(u, values, x);
+        widen_scales(x);
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int p = 2 * c + h;
-                    lds_put((side ? values : keys) + (uint32_t)(r * M::kRow + 16 * (p ^ (side ? 4 * (r & 3) : (r & 15)))), w[h]);
-                }
-            }
-            // key scales: [block][row]
-            if (at_tid < R::kScales * 32) {
-                const int blk = at_tid / 32, row = at_tid & 31;
-                const uint32_t src = raw + (uint32_t)(row * R::kRowBytes);
-                const float d = R::kTq4 ? F16::to_f32((uint16_t)lds_u16(src + 66u * blk)) : __uint_as_float(lds_u1(R::kFp8 ? src + 256u + 4u * blk : src + 68u * blk));
-                *reinterpret_cast<__attribute__((address_space(3))) float*>((uintptr_t)(scale + (uint32_t)(blk * 128 + 4 * row))) = d;
-            }
+        for (int piece = 0; piece < 4; ++piece) {
+            widen_load(piece, x);
+            widen_look_up(piece, x);
+            widen_store(piece, x);
         }
     };
 
@@ -491,8 +527,13 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[k >> 2][k & 3] = IS_BF16 ? pack_bf2(s[2 * k], s[2 * k + 1]) : pack_h2(s[2 * k], s[2 * k + 1]);
     };
-    const auto add_values = [&](uint32_t values) {
-        if (!weighted) return;
+    // The values of a unit, and between their products the widening of another one.
+    const auto add_values = [&](uint32_t values, auto widening, int widen_unit, uint32_t widen_to) {
+        constexpr bool kWidens = decltype(widening)::value;
+        if (!weighted) {
+            if constexpr (kWidens) widen(widen_unit, widen_to);
+            return;
+        }
         // lane l reads row (l & 15) >> 2 of four, 8 bytes at 8 (l & 3) of the 32 of its 16 channels
         const int at_lane = here(lane), j = at_lane & 15;
         const uint32_t v_at = values + (uint32_t)((4 * (at_lane >> 5) + (j >> 2)) * M::kRow) + 64u * (uint32_t)(j >> 2) + 32u * (uint32_t)(at_lane >> 4 & 1) + 8u * (uint32_t)(j & 3);
@@ -503,14 +544,22 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             const u2v x = __builtin_bit_cast(u2v, a), y = __builtin_bit_cast(u2v, c);
             return u4{x[0], x[1], y[0], y[1]};
         };
+        Widening x;
+        if constexpr (kWidens) widen_start(widen_unit, widen_to, x);
         u4 a[kValuesAhead + 1];
 #pragma unroll
         for (int i = 0; i < kValuesAhead; ++i) a[i] = v_operand(i >> 1, i & 1);
 #pragma unroll
         for (int i = 0; i < 2 * kDims; ++i) {
-            const int next = i + kValuesAhead;
+            const int next = i + kValuesAhead, piece = i >> 2;
             __builtin_amdgcn_sched_barrier(0);
             if (next < 2 * kDims) a[next % (kValuesAhead + 1)] = v_operand(next >> 1, next & 1);
+            if constexpr (kWidens) {
+                if ((i & 3) == 0) widen_load(piece, x);
+                if ((i & 3) == 1) widen_look_up(piece, x);
+                if ((i & 3) == 3) widen_store(piece, x);
+                if (i == 2) widen_scales(x);
+            }
             __builtin_amdgcn_sched_barrier(0);
             o[i >> 1] = mfma_tile<IS_BF16>(a[i % (kValuesAhead + 1)], w[i & 1], o[i >> 1]);
         }
@@ -547,20 +596,17 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             if (u + 2 < units) issue(u + 2, 0u);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (late && u > 0) add_values(v_last);
-        __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!R::k16) {
-            if (u + 1 < units) widen(u + 1, v_next);
-        }
+        // (behind the last unit: old rows, to tiles that nobody reads)
+        if (late) add_values(v_last, std::integral_constant<bool, !R::k16>{}, u + 1, v_next);
         __builtin_amdgcn_sched_barrier(0);
         score(u);
         __builtin_amdgcn_sched_barrier(0);
-        if (!late) add_values(v_now);
+        if (!late) add_values(v_now, std::integral_constant<bool, !R::k16>{}, u + 1, v_next);
         __builtin_amdgcn_sched_barrier(0);
         const uint32_t free = v_last;
         v_last = v_now, v_now = v_next, v_next = free;
     }
-    if (late && units > 0) add_values(v_last);
+    if (late && units > 0) add_values(v_last, std::false_type{}, 0, 0u);
     {
         const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
         l_run = __uint_as_float(r[0]) + __uint_as_float(r[1]);
