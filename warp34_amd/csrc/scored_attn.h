@@ -191,6 +191,8 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
     }
     total = wave_sum(total);
     live = wave_sum(live);
+    // (few tiles: whole rounds of chunks, one more than fills them would take a round of its own)
+    const int limit = P.rounds > 0 && live < kSlotRound ? min(P.target, P.rounds * kSlotRound) : P.target;
     const auto fits = [&](int per) {
         int n = 0, several = 0;
         for (int e = lane; e < P.entries; e += 64) {
@@ -198,14 +200,14 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
             n += c;
             several += c > 1 ? c : 0;
         }
-        return wave_sum(n) <= P.target && wave_sum(several) <= P.records;
+        return wave_sum(n) <= limit && wave_sum(several) <= P.records;
     };
     // (with a round of tiles or more there is something for every CU without a cut: only what is longer than a CU's share is cut)
     const int share = P.rounds > 0 ? (live < kSlotRound ? P.rounds * kSlotRound : kSlotRound * 2 / 3) : P.target;
     int per = max(P.min_halves, (total + share - 1) / share);
     if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per)) return per;
     // sum of ceil(h / per) <= total / per + live, so this many halves a chunk are enough for any number of slots above live
-    int low = per, high = max(per + 1, (total + max(P.target - live, 1) - 1) / max(P.target - live, 1));
+    int low = per, high = max(per + 1, (total + max(limit - live, 1) - 1) / max(limit - live, 1));
     while (!fits(high)) {
         low = high;
         high *= 2;

@@ -157,19 +157,14 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     int lo = 0, hi = -1;
     if (col_ok) token_keys(P, my_tok, my_pos, t.seq_after, lo, hi);
     // keys that every live column of the wave sees, and that any sees
-    int all_from = col_ok ? lo : 0, all_to = col_ok ? hi : 0x7fffffff;
-    int any_from = lo <= hi ? lo : 0x7fffffff, any_to = lo <= hi ? hi : -1;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        all_from = max(all_from, __shfl_xor(all_from, d, 64));
-        all_to = min(all_to, __shfl_xor(all_to, d, 64));
-        any_from = min(any_from, __shfl_xor(any_from, d, 64));
-        any_to = max(any_to, __shfl_xor(any_to, d, 64));
-    }
-    all_from = __builtin_amdgcn_readfirstlane(all_from);
-    all_to = __builtin_amdgcn_readfirstlane(all_to);
-    any_from = __builtin_amdgcn_readfirstlane(any_from);
-    any_to = __builtin_amdgcn_readfirstlane(any_to);
+    const auto least = [](int x, int y) { return min(x, y); };
+    const auto most = [](int x, int y) { return max(x, y); };
+    const auto over_columns = [&](int v, auto&& f) {  // (rows of 16 lanes, then rows 0 and 1)
+        v = row_reduce(v, f);
+        return f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16));
+    };
+    const int all_from = over_columns(col_ok ? lo : 0, most), all_to = over_columns(col_ok ? hi : 0x7fffffff, least);
+    const int any_from = over_columns(lo <= hi ? lo : 0x7fffffff, least), any_to = over_columns(lo <= hi ? hi : -1, most);
     const uint32_t live = (uint32_t)__ballot(col_ok);
     const bool sloped = P.slopes != nullptr;
     const float slope2 = sloped && col_ok ? P.slopes[my_head] * kLog2e : 0.f;
