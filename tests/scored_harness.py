@@ -8,7 +8,7 @@ from oracle import DT_BF16
 from plain_kv import scored_attention
 
 SENTINEL = 0x5500
-CHUNK_FROM = 128  # query columns of a request from which the call takes its chunk kernel
+CHUNK_FROM = 256  # query columns of a request from which the call takes its chunk kernel
 
 
 def scores_struct(G, cap=0.0, slopes=None, documents=None, prefixes=None, lse=None):
@@ -58,7 +58,8 @@ def check_scored(pool, bt, seqs, q, dt, aq, ctx, heads, *, hb=None, scratch=8 <<
     hb.sliding_window, hb.mask_mode = kinds["window"], 1 if kinds["noncausal"] else 0
     bits, lse = run_scored(pool, hb, q, dt, heads, scratch=scratch, with_lse=with_lse, max_q_len=max_q_len, max_seq_len=max_seq_len, **terms)
     longest = int(np.diff(hb.qsl).max()) if max_q_len is None else max_q_len
-    group = next(d for d in range(min(16, heads // pool.kv_heads), 0, -1) if heads // pool.kv_heads % d == 0)
+    columns = 8 if pool.fmt == oracle.FMT_TQ4 else 16  # of a decode tile, of which a kv head's query heads fill a divisor
+    group = next(d for d in range(min(columns, heads // pool.kv_heads), 0, -1) if heads // pool.kv_heads % d == 0)
     chunk = (longest if longest > 0 else hb.total_tokens) * group >= CHUNK_FROM
     want, want_lse, bound, lse_bound = scored_attention(pool, bt, seqs, oracle.bits_to_f32(q, dt).astype(np.float64), aq, ctx,
                                                         scale=hb.sm_scale, dt=dt, chunk=chunk, **kinds, **terms)

@@ -228,7 +228,7 @@ def test_same_bits_whatever_the_pages_and_bounds():
 
 
 @gpu
-@pytest.mark.parametrize("qs", [[1, 1, 1], [1, 30, 6]])
+@pytest.mark.parametrize("qs", [[1, 1, 1], [1, 30, 6], [1, 70, 6]])
 def test_captured_call_follows_lengths_tables_and_terms(qs):
     """A graph of the call, replayed after lengths, tables, document starts and queries have changed, with eager work between; two
     graphs share the workspace."""
@@ -268,7 +268,7 @@ def test_captured_call_follows_lengths_tables_and_terms(qs):
         with torch.cuda.graph(graph):
             run(which, torch.cuda.current_stream())
         graphs.append(graph)
-    for turn, lens in enumerate(([1500, 300, 40], [700, 299, 33], [1, 1, 1] if max(qs) == 1 else [800, 31, 7])):
+    for turn, lens in enumerate(([1500, 300, 40], [700, 299, 33], [1, 1, 1] if max(qs) == 1 else [800, qs[1] + 1, 7])):
         now_ctx = [s - a for s, a in zip(lens, qs)]
         db.t["seq"].copy_(G.to_dev(np.asarray(lens, dtype=np.int32)))
         db.t["ctx"].copy_(G.to_dev(np.asarray(now_ctx, dtype=np.int32)))
@@ -419,7 +419,7 @@ def test_chunks(fmt, xf, v_xf, dt, hd, seqs, qs, terms):
 @gpu
 @pytest.mark.parametrize("kv_heads,heads", [(1, 1), (2, 16), (1, 24), (1, 17), (3, 9), (1, 64)])
 def test_chunk_head_layouts(kv_heads, heads):
-    seqs, qs = [300], [150]
+    seqs, qs = [300], [260]
     pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1020 + heads, DT_F16, kv_heads=kv_heads, q_heads=heads, head_dim=128)
     check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, heads, cap=20.0, slopes=slopes_of(heads))
 
@@ -518,8 +518,8 @@ def test_one_long_request_among_many_short_ones():
     seqs = [9000] + [40] * 150
     for tokens in (1, 33):
         qs = [tokens] * len(seqs)
-        pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1200, DT_F16, kv_heads=1, q_heads=4, head_dim=128)
-        check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 4, scratch=64 << 20, cap=30.0)
+        pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1200, DT_F16, kv_heads=1, q_heads=8, head_dim=128)
+        check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 8, scratch=64 << 20, cap=30.0)
 
 
 @gpu

@@ -10,11 +10,12 @@ namespace w34 {
 
 constexpr int kDecodeCols = 16;         // query columns of a workgroup of the decode kernel
 constexpr int kDecodeMinHalves = 8;     // shortest chunk: a half unit for each wave
-constexpr int kChunkMinHalves = 64;     // 32 units
+constexpr int kChunkMinHalves = 16;     // 8 units
+constexpr int kSpreadTiles = 8;          // chunk kernel: batches of up to so many tiles have a workgroup a column to join their chunks
 constexpr int kDecodeRounds = 4, kChunkRounds = 2;
 
 // Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
-constexpr int kChunkFrom = 128;
+constexpr int kChunkFrom = 256;
 
 static int decode_cols(int format) { return format == WARP34_KV_FORMAT_TQ4 ? kTq4Cols : kDecodeCols; }
 
@@ -127,7 +128,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
                  : launch(scored_chunk_kernel<TQ, KVF, HD, false>, kChunkWaves * 64, lds);
     }
     if (rc || slots == 0) return rc;
-    if (s.chunk || s.entries > 64) {
+    if (s.entries > (s.chunk ? kSpreadTiles : 64)) {
         hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)((s.cols + kJoinCols - 1) / kJoinCols)), dim3(512), 0, stream, P,
                            s.cols, ScoredRows<KVF, HD>::kOutScale);
     } else {
