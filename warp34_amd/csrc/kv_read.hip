@@ -118,9 +118,10 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
 //   Z = X H      A = X (lane (n, b) holds X[n][4 b .. 4 b + 3], the elements it loads), B = H; lane (n, b) gets Z[4 b + i][n]
 //   Y^T = Z^T H  those registers are the A operand Z^T as they stand; lane (n, b) gets Y[n][4 b + i], the elements it stores
 // Operands have two fp16 parts in the halves of a 16x16x32 product (22 bits), so the result is as good as the 60 additions a row in
-// 32 bits that the MFMAs stand for.  X goes in relative to the row's largest block scale: whatever the scales, the parts stay
-// inside fp16's range.
-constexpr int kReadRows = 4;
+// 32 bits that the MFMAs stand for.  X is the bare codes, of which eight bits are one part and centroids have two in a table; the scales
+// multiply Z, whose rows 4 b .. 4 b + 3 lie in one block: relative to a power of two above the row's largest scale, so that the parts
+// stay inside fp16's range whatever the scales.
+constexpr int kReadRows = 8;
 
 __device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
     u4 r;
@@ -131,9 +132,31 @@ __device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
     r[1] = hi, r[3] = lo;
     return __builtin_bit_cast(h8, r);
 }
+// Both parts of a centroid times kLutGain, in one register.
+__host__ __device__ constexpr uint32_t centroid_parts_of(int code) {
+    const _Float16 hi = (_Float16)(kLutGain * kCentroids[code]);
+    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[code] - (float)hi)) << 16;
+}
+__device__ __forceinline__ uint32_t lane_centroid_parts() {
+    const int n = lane_id() & 15;
+    uint32_t c = centroid_parts_of(0);
+#pragma unroll
+    for (int i = 1; i < 16; ++i) c = n == i ? centroid_parts_of(i) : c;
+    return c;
+}
+template <typename TOut>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    if constexpr (TOut::kStorageFormat == WARP34_KV_FORMAT_BF16) {
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{a, b}, bf2));
+    } else {
+        return pack_h2(a, b);
+    }
+}
 
+// (two waves a SIMD at least: with the whole register file the products' results would go through the accumulation registers)
 template <typename TOut, int FORMAT>
-__global__ __launch_bounds__(256) void kv_read_rotated_kernel(const ReadParams P, int first_side) {
+__global__ __launch_bounds__(256, 2) void kv_read_rotated_kernel(const ReadParams P, int first_side) {
     const ReadSide& S = P.side[first_side + (int)blockIdx.z];
     const int head = (int)blockIdx.y;
     const int lane = lane_id();
@@ -142,7 +165,7 @@ __global__ __launch_bounds__(256) void kv_read_rotated_kernel(const ReadParams P
     const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * kReadRows;
 
     uint32_t code[kReadRows];
-    uint32_t scale[kReadRows];
+    uint32_t scale[kReadRows];  // of the block that Z's rows 4 b .. 4 b + 3 lie in
     bool live[kReadRows];
 #pragma unroll
     for (int k = 0; k < kReadRows; ++k) {
@@ -152,62 +175,68 @@ __global__ __launch_bounds__(256) void kv_read_rotated_kernel(const ReadParams P
         if (live[k]) {
             const slab_byte* src = row_address(S, P, slot, head);
             if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
-                const slab_byte* block = src + 66 * (e >> 7);
-                scale[k] = load_as<uint16_t>(block);
-                code[k] = load_as<uint16_t>(block + 2 + ((e & 127) >> 1));
+                scale[k] = load_as<uint16_t>(src + 66 * (b >> 1));
+                code[k] = load_as<uint16_t>(src + 66 * (e >> 7) + 2 + ((e & 127) >> 1));
             } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
                 code[k] = load_as<uint32_t>(src + e);
-                scale[k] = load_as<uint32_t>(src + 256 + 4 * (e >> 7));
+                scale[k] = load_as<uint32_t>(src + 256 + 4 * (b >> 1));
             } else {
-                const slab_byte* block = src + 68 * (e >> 6);
-                code[k] = load_as<uint32_t>(block + 4 + (e & 63));
-                scale[k] = load_as<uint32_t>(block);
+                code[k] = load_as<uint32_t>(src + 68 * (e >> 6) + 4 + (e & 63));
+                scale[k] = load_as<uint32_t>(src + 68 * b);
             }
         }
     }
     h8 had;
-    float sign[4];
+    uint32_t flip[2] = {0u, 0u};  // the signs, as bits of the row's 16-bit numbers
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         had[i] = had[4 + i] = (__builtin_popcount((unsigned)((4 * b + i) & n)) & 1) ? (_Float16)-1.0f : (_Float16)1.0f;
-        sign[i] = apply_sign(0.0625f, e + i);
+        flip[i >> 1] |= (__float_as_uint(apply_sign(1.0f, e + i)) & 0x80000000u) >> (i & 1 ? 0 : 16);
     }
-    const float mine = FORMAT == WARP34_KV_FORMAT_TQ4 ? lane_centroid() : 0.f;
+    const uint32_t mine = FORMAT == WARP34_KV_FORMAT_TQ4 ? lane_centroid_parts() : 0u;
+    uint16_t* to = S.out + row0 * S.row_stride + (int64_t)head * 256 + e;
 #pragma unroll
-    for (int k = 0; k < kReadRows; ++k) {
-        if (!live[k]) continue;  // the whole wave
-        float x[4], d;
+    for (int k = 0; k < kReadRows; ++k) {  // (rows that are not wanted too, as zeros: no branch keeps one row waiting for another)
+        u4 x = {0u, 0u, 0u, 0u};
+        float d;
         if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
-            d = F16::to_f32((uint16_t)scale[k]);
+            d = F16::to_f32((uint16_t)scale[k]) * kLutInvGain;
+            uint32_t c[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = centroid_of(mine, code[k] >> (4 * i));
+            for (int i = 0; i < 4; ++i) c[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((i == 0 ? code[k] << 2 : code[k] >> (4 * i - 2)) & 60u), (int)mine);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                x[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x05040100u);
+                x[2 + i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x07060302u);
+            }
         } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
             d = __uint_as_float(scale[k]);
-            const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[k], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)code[k], true);
-            x[0] = lo[0], x[1] = lo[1], x[2] = hi[0], x[3] = hi[1];
-        } else {
+            x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code[k], 1.0f, false));
+            x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code[k], 1.0f, true));
+        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
             d = __uint_as_float(scale[k]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(code[k] >> (8 * i));
+            const uint32_t u = code[k] ^ 0x80808080u;
+            const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+            x[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+            x[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
         }
-        // the largest scale of the row: the blocks' lanes differ in bit 3 of n, for Q8_0 in bit 2 as well
-        float top = fabsf(d);
-        top = fmaxf(top, lane_xor<8>(top, lane));
-        if constexpr (FORMAT == WARP34_KV_FORMAT_Q8_0) top = fmaxf(top, lane_xor<4>(top, lane));
-        const float share = top > 0.f ? d * (1.0f / top) : 0.f;
+        const float top = max_over_rows(fabsf(d));
+        const int up = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+        const float share = __builtin_amdgcn_ldexpf(d, -up);
+        const f4 none = {0.f, 0.f, 0.f, 0.f};
+        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), had, none, 0, 0, 0);
+        float zs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            x[i] *= share;
-            asm("" : "+v"(x[i]));  // both parts are taken from the product rounded to 32 bits
+            zs[i] = z[i] * share;
+            asm("" : "+v"(zs[i]));  // both parts are taken from the product rounded to 32 bits
         }
-        const f4 none = {0.f, 0.f, 0.f, 0.f};
-        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(x), had, none, 0, 0, 0);
-        const float zs[4] = {z[0], z[1], z[2], z[3]};
         const f4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(zs), had, none, 0, 0, 0);
-        uint2 w;
-        w.x = pack_out<TOut>(y[0] * top * sign[0], y[1] * top * sign[1]);
-        w.y = pack_out<TOut>(y[2] * top * sign[2], y[3] * top * sign[3]);
-        *reinterpret_cast<uint2*>(S.out + (row0 + k) * S.row_stride + (int64_t)head * 256 + e) = w;
+        float v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(y[i], up - 4);
+        const uint2 w = {pack_pair<TOut>(v[0], v[1]) ^ flip[0], pack_pair<TOut>(v[2], v[3]) ^ flip[1]};
+        if (live[k]) *reinterpret_cast<uint2*>(to + k * S.row_stride) = w;
     }
 }
 
