@@ -113,15 +113,20 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
     if (live) *reinterpret_cast<uint4*>(S.out + row * S.row_stride + (int64_t)head * P.head_dim + e) = w;
 }
 
-// Rotated rows of 256 elements, a wave a row, kReadRows rows at a time so that their loads travel together.  The transform is a
+// Rotated rows of 256 elements, kReadRows rows a wave.  The transform is a
 // product of two 16 x 16 ones: with X[r][c] = x[16 r + c] and H[r][c] = (-1)^popcount(r & c), Y = H X H.  Two MFMAs do it:
-//   Z = X H      A = X (lane (n, b) holds X[n][4 b .. 4 b + 3], the elements it loads), B = H; lane (n, b) gets Z[4 b + i][n]
-//   Y^T = Z^T H  those registers are the A operand Z^T as they stand; lane (n, b) gets Y[n][4 b + i], the elements it stores
+//   Z = X H      A = X (lane (n, b) holds X[n][4 b .. 4 b + 3]), B = H; lane (n, b) gets Z[4 b + i][n]
+//   Y^T = Z^T H  those registers are the A operand Z^T as they stand; lane (n, b) gets Y[n][4 b + i]
+// Memory wants wider pieces than four elements a lane: of four rows at a time lane (n, b) loads X[n] of row b, and the pieces change
+// places by swaps of 16 and of 32 lanes; two rows' results change places so that a lane stores eight elements in a run.  (For that the
+// columns of Z are out of order, in groups of four: 0, 8, 4, 12.)
 // Operands have two fp16 parts in the halves of a 16x16x32 product (22 bits), so the result is as good as the 60 additions a row in
 // 32 bits that the MFMAs stand for.  X is the bare codes, of which eight bits are one part and centroids have two in a table; the scales
 // multiply Z, whose rows 4 b .. 4 b + 3 lie in one block: relative to a power of two above the row's largest scale, so that the parts
 // stay inside fp16's range whatever the scales.
 constexpr int kReadRows = 8;
+typedef u2v u2_at2 __attribute__((aligned(2)));
+typedef u4 u4_at4 __attribute__((aligned(4)));
 
 __device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
     u4 r;
@@ -132,17 +137,25 @@ __device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
     r[1] = hi, r[3] = lo;
     return __builtin_bit_cast(h8, r);
 }
-// Both parts of a centroid times kLutGain, in one register.
-__host__ __device__ constexpr uint32_t centroid_parts_of(int code) {
-    const _Float16 hi = (_Float16)(kLutGain * kCentroids[code]);
-    return (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[code] - (float)hi)) << 16;
+// Both parts of each centroid times kLutGain.
+struct CentroidParts {
+    uint32_t of[16];
+};
+constexpr CentroidParts make_centroid_parts() {
+    CentroidParts t{};
+    for (int c = 0; c < 16; ++c) {
+        const _Float16 hi = (_Float16)(kLutGain * kCentroids[c]);
+        t.of[c] = (uint32_t)__builtin_bit_cast(uint16_t, hi) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[c] - (float)hi)) << 16;
+    }
+    return t;
 }
-__device__ __forceinline__ uint32_t lane_centroid_parts() {
-    const int n = lane_id() & 15;
-    uint32_t c = centroid_parts_of(0);
-#pragma unroll
-    for (int i = 1; i < 16; ++i) c = n == i ? centroid_parts_of(i) : c;
-    return c;
+__device__ __constant__ constexpr CentroidParts kCentroidParts = make_centroid_parts();
+// (-1)^popcount((4 b + i) & n) for i = 0 .. 3 as fp16, twice
+__device__ __forceinline__ h8 hadamard_column(int n, int b) {
+    const uint32_t of_b = (uint32_t)(b & (n >> 2)), odd = (of_b ^ of_b >> 1) & 1u;
+    const uint32_t lo = 0x3C003C00u ^ odd * 0x80008000u ^ ((uint32_t)n & 1u) << 31;  // i = 0, 1
+    const uint32_t hi = lo ^ ((uint32_t)n >> 1 & 1u) * 0x80008000u;                  // i = 2, 3
+    return __builtin_bit_cast(h8, u4{lo, hi, lo, hi});
 }
 template <typename TOut>
 __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
@@ -161,82 +174,117 @@ __global__ __launch_bounds__(256, 2) void kv_read_rotated_kernel(const ReadParam
     const int head = (int)blockIdx.y;
     const int lane = lane_id();
     const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int n = lane & 15, b = lane >> 4, e = 16 * n + 4 * b;
+    const int n = lane & 15, b = lane >> 4;
     const int64_t row0 = ((int64_t)blockIdx.x * 4 + wave) * kReadRows;
 
-    uint32_t code[kReadRows];
-    uint32_t scale[kReadRows];  // of the block that Z's rows 4 b .. 4 b + 3 lie in
-    bool live[kReadRows];
+    constexpr int kGroups = kReadRows / 4;
+    constexpr bool kTq4 = FORMAT == WARP34_KV_FORMAT_TQ4;
+    uint32_t code[kGroups][4], scale[kGroups];  // X[n] of row b, the scale of block n % 2 or n % 4 of it
+    unsigned long long live[kGroups];
+    const uint32_t mine = kTq4 ? kCentroidParts.of[n] : 0u;
+    const int to_e = 16 * n + 8 * (b & 1);  // the elements this lane stores, of row b >> 1 of two
+    const uint32_t signs = kSignMask[to_e >> 5] >> (to_e & 31);
 #pragma unroll
-    for (int k = 0; k < kReadRows; ++k) {
-        const int slot = row0 + k < P.rows ? P.slots[row0 + k] : -1;
-        live[k] = slot >= 0;
-        code[k] = scale[k] = 0u;
-        if (live[k]) {
+    for (int g = 0; g < kGroups; ++g) {
+        const int64_t row = row0 + 4 * g + b;
+        const int slot = row < P.rows ? P.slots[row] : -1;
+        live[g] = __ballot(slot >= 0);
+        scale[g] = 0u;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) code[g][k] = 0u;
+        if (slot >= 0) {
             const slab_byte* src = row_address(S, P, slot, head);
-            if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
-                scale[k] = load_as<uint16_t>(src + 66 * (b >> 1));
-                code[k] = load_as<uint16_t>(src + 66 * (e >> 7) + 2 + ((e & 127) >> 1));
-            } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
-                code[k] = load_as<uint32_t>(src + e);
-                scale[k] = load_as<uint32_t>(src + 256 + 4 * (b >> 1));
+            if constexpr (kTq4) {
+                const u2v w = load_as<u2_at2>(src + 66 * (n >> 3) + 2 + 8 * (n & 7));
+                code[g][0] = w[0], code[g][1] = w[1];
+                scale[g] = load_as<uint16_t>(src + 66 * (n & 1));
             } else {
-                code[k] = load_as<uint32_t>(src + 68 * (e >> 6) + 4 + (e & 63));
-                scale[k] = load_as<uint32_t>(src + 68 * b);
+                const bool fp8 = FORMAT == WARP34_KV_FORMAT_FP8_E4M3;
+                const u4 w = load_as<u4_at4>(src + (fp8 ? 16 * n : 68 * (n >> 2) + 4 + 16 * (n & 3)));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) code[g][k] = w[k];
+                scale[g] = load_as<uint32_t>(src + (fp8 ? 256 + 4 * (n & 1) : 68 * (n & 3)));
             }
         }
     }
-    h8 had;
-    uint32_t flip[2] = {0u, 0u};  // the signs, as bits of the row's 16-bit numbers
+    const h8 had = hadamard_column(n, b);
+    const h8 had_cols = hadamard_column((n & 3) + ((n & 4) << 1) + ((n & 8) >> 1), b);  // of the column of Z where lane n is
+    u4 flip;  // the signs, as bits of the row's 16-bit numbers
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        had[i] = had[4 + i] = (__builtin_popcount((unsigned)((4 * b + i) & n)) & 1) ? (_Float16)-1.0f : (_Float16)1.0f;
-        flip[i >> 1] |= (__float_as_uint(apply_sign(1.0f, e + i)) & 0x80000000u) >> (i & 1 ? 0 : 16);
-    }
-    const uint32_t mine = FORMAT == WARP34_KV_FORMAT_TQ4 ? lane_centroid_parts() : 0u;
-    uint16_t* to = S.out + row0 * S.row_stride + (int64_t)head * 256 + e;
+    for (int k = 0; k < 4; ++k) flip[k] = (signs << (15 - 2 * k) & 0x8000u) | (signs << (30 - 2 * k) & 0x80000000u);
+    const int scale_from = 4 * (FORMAT == WARP34_KV_FORMAT_Q8_0 ? b : b >> 1);  // the lane (times four) that has the scale of Z's rows 4 b .. 4 b + 3
+    uint16_t* to = S.out + (row0 + (b >> 1)) * S.row_stride + (int64_t)head * 256 + to_e;
 #pragma unroll
-    for (int k = 0; k < kReadRows; ++k) {  // (rows that are not wanted too, as zeros: no branch keeps one row waiting for another)
-        u4 x = {0u, 0u, 0u, 0u};
-        float d;
-        if constexpr (FORMAT == WARP34_KV_FORMAT_TQ4) {
-            d = F16::to_f32((uint16_t)scale[k]) * kLutInvGain;
-            uint32_t c[4];
+    for (int g = 0; g < kGroups; ++g) {
+        // four rows: row k's piece b in this lane
+        uint32_t piece[4];
+        if constexpr (kTq4) {
+            const auto p = __builtin_amdgcn_permlane32_swap(code[g][0], code[g][1], false, false);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((i == 0 ? code[k] << 2 : code[k] >> (4 * i - 2)) & 60u), (int)mine);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                x[i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x05040100u);
-                x[2 + i] = __builtin_amdgcn_perm(c[2 * i + 1], c[2 * i], 0x07060302u);
+            for (int k = 0; k < 2; ++k) {
+                const auto q = __builtin_amdgcn_permlane16_swap(p[k], p[k], false, false);
+                piece[2 * k] = q[0] >> (16 * (b & 1)), piece[2 * k + 1] = q[1] >> (16 * (b & 1));
             }
-        } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
-            d = __uint_as_float(scale[k]);
-            x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code[k], 1.0f, false));
-            x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(code[k], 1.0f, true));
-        } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
-            d = __uint_as_float(scale[k]);
-            const uint32_t u = code[k] ^ 0x80808080u;
-            const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-            x[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
-            x[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
-        }
-        const float top = max_over_rows(fabsf(d));
-        const int up = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-        const float share = __builtin_amdgcn_ldexpf(d, -up);
-        const f4 none = {0.f, 0.f, 0.f, 0.f};
-        const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), had, none, 0, 0, 0);
-        float zs[4];
+        } else {
+            const auto p = __builtin_amdgcn_permlane32_swap(code[g][0], code[g][2], false, false);
+            const auto q = __builtin_amdgcn_permlane32_swap(code[g][1], code[g][3], false, false);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            zs[i] = z[i] * share;
-            asm("" : "+v"(zs[i]));  // both parts are taken from the product rounded to 32 bits
+            for (int k = 0; k < 2; ++k) {
+                const auto r = __builtin_amdgcn_permlane16_swap(p[k], q[k], false, false);
+                piece[2 * k] = r[0], piece[2 * k + 1] = r[1];
+            }
         }
-        const f4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(zs), had, none, 0, 0, 0);
-        float v[4];
+        // the scales of row b relative to a power of two above the largest
+        const float d = kTq4 ? F16::to_f32((uint16_t)scale[g]) * kLutInvGain : __uint_as_float(scale[g]);
+        float top = fmaxf(fabsf(d), fabsf(lane_xor<1>(d, lane)));
+        if constexpr (FORMAT == WARP34_KV_FORMAT_Q8_0) top = fmaxf(top, lane_xor<2>(top, lane));
+        const int above = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+        const float relative = __builtin_amdgcn_ldexpf(d, -above);
+        uint2 w[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(y[i], up - 4);
-        const uint2 w = {pack_pair<TOut>(v[0], v[1]) ^ flip[0], pack_pair<TOut>(v[2], v[3]) ^ flip[1]};
-        if (live[k]) *reinterpret_cast<uint2*>(to + k * S.row_stride) = w;
+        for (int k = 0; k < 4; ++k) {  // (rows that are not wanted too, as zeros: no branch keeps one row waiting for another)
+            const uint32_t c = piece[k];
+            const float share = __int_as_float(__builtin_amdgcn_ds_bpermute(64 * k + scale_from, __float_as_int(relative)));
+            const int up = __builtin_amdgcn_readlane(above, 16 * k);
+            u4 x = {0u, 0u, 0u, 0u};
+            if constexpr (kTq4) {
+                uint32_t v[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = (uint32_t)__builtin_amdgcn_ds_bpermute((int)((i == 0 ? c << 2 : c >> (4 * i - 2)) & 60u), (int)mine);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    x[i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x05040100u);
+                    x[2 + i] = __builtin_amdgcn_perm(v[2 * i + 1], v[2 * i], 0x07060302u);
+                }
+            } else if constexpr (FORMAT == WARP34_KV_FORMAT_FP8_E4M3) {
+                x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, false));
+                x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, true));
+            } else {  // 0x6400 | (q + 128) is 1152 + q in fp16
+                const uint32_t u = c ^ 0x80808080u;
+                const h2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+                x[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - bias);
+                x[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - bias);
+            }
+            const f4 none = {0.f, 0.f, 0.f, 0.f};
+            const f4 z = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), had_cols, none, 0, 0, 0);
+            float zs[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                zs[i] = z[i] * share;
+                asm("" : "+v"(zs[i]));  // both parts are taken from the product rounded to 32 bits
+            }
+            const f4 y = __builtin_amdgcn_mfma_f32_16x16x32_f16(two_parts(zs), had, none, 0, 0, 0);
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_ldexpf(y[i], up - 4);
+            w[k] = uint2{pack_pair<TOut>(v[0], v[1]), pack_pair<TOut>(v[2], v[3])};
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {  // rows k (lanes 0 .. 31) and k + 1
+            const auto x = __builtin_amdgcn_permlane32_swap(w[k].x, w[k + 1].x, false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(w[k].y, w[k + 1].y, false, false);
+            if ((live[g] >> (16 * (k + (b >> 1)))) & 1ull) *reinterpret_cast<u4*>(to + (4 * g + k) * S.row_stride) = u4{x[0], y[0], x[1], y[1]} ^ flip;
+        }
     }
 }
 
