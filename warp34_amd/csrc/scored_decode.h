@@ -130,6 +130,11 @@ struct QueryColumns {
             raw[k] = *reinterpret_cast<const uint2*>(P.q + ((size_t)tok * P.num_q_heads + (size_t)head) * 256 + 4 * lane);
         }
     }
+    // Waits for them: in front of the loads of rows, which may be none, so that nobody would know how many to leave on their way.
+    __device__ __forceinline__ void arrived() {
+#pragma unroll
+        for (int k = 0; k < COLS / kScoredWaves; ++k) asm volatile("" : "+v"(raw[k].x), "+v"(raw[k].y));
+    }
     __device__ __forceinline__ void bring(const ScoredParams& P, uint32_t live, int wave, int lane, uint16_t* high, uint16_t* low, float* scales) const;
 };
 template <typename TQ, int COLS, int STRIDE>
@@ -354,6 +359,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         if constexpr (R::kQ8) v_scale = load_as<uint32_t>(row + 68 * b);
     };
     int half = s0.begin + wave;
+    if constexpr (!R::k16) columns.arrived();
     if (half < end) {
         locate(half);
         load_keys();

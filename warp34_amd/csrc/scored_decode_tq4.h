@@ -20,25 +20,36 @@ constexpr int kTq4Cols = 8;
 // The table: entries of eight bytes, the pair of fp16 numbers of a byte's two codes and the pair of what they are short of the centroids;
 // 32 copies (a read goes by 32 lanes at a time).  The fp16 numbers are up to 9.4e-5 from the centroids, which would be 1e-4 of a score and
 // 2e-5 of a row's lse where a few keys carry it: keys take both, values the first alone.
-__host__ __device__ constexpr uint32_t centroid_rest_of(int code) {
-    return __builtin_bit_cast(uint16_t, (_Float16)(kLutGain * kCentroids[code] - (float)(_Float16)(kLutGain * kCentroids[code])));
-}
-__device__ __forceinline__ uint32_t centroid_rest(uint32_t code) {
-    uint32_t r = centroid_rest_of(0);
-#pragma unroll
-    for (int c = 1; c < 16; ++c) r = code == (uint32_t)c ? centroid_rest_of(c) : r;
-    return r;
-}
-__device__ __forceinline__ void build_two_part_table(uint8_t* smem, int tid, int wave) {  // by 512 threads, as build_pair_table
-    const uint32_t code = (uint32_t)tid >> 4 & 15u, lo = centroid_bits(code), lo_rest = centroid_rest(code);
-    const bool odd = (wave >> 2) != 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t v = lo | (odd ? centroid_bits_of(2 * i + 1) << 16 : centroid_bits_of(2 * i) << 16);
-        const uint32_t w = lo_rest | (odd ? centroid_rest_of(2 * i + 1) << 16 : centroid_rest_of(2 * i) << 16);
-        *reinterpret_cast<u4*>(smem + (tid + 512 * i) * 16) = u4{v, w, v, w};
+struct TwoPartPairs {
+    u2v of[256];
+};
+constexpr TwoPartPairs make_two_part_pairs() {
+    TwoPartPairs t{};
+    for (int e = 0; e < 256; ++e) {
+        uint32_t v = 0, w = 0;
+        for (int k = 0; k < 2; ++k) {
+            const float c = kLutGain * kCentroids[e >> (4 * k) & 15];
+            const _Float16 hi = (_Float16)c;
+            v |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * k);
+            w |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(c - (float)hi)) << (16 * k);
+        }
+        t.of[e] = u2v{v, w};
     }
+    return t;
 }
+__device__ __constant__ constexpr TwoPartPairs kTwoPartPairs = make_two_part_pairs();
+// By 512 threads, 16 bytes at tid + 512 i of the table: entries (tid >> 4) + 32 i, which travel while the batch is planned.
+struct TableEntries {
+    u2v of[8];
+    __device__ __forceinline__ void load(int tid) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) of[i] = kTwoPartPairs.of[(tid >> 4) + 32 * i];
+    }
+    __device__ __forceinline__ void store(uint8_t* smem, int tid) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) *reinterpret_cast<u4*>(smem + (tid + 512 * i) * 16) = u4{of[i][0], of[i][1], of[i][0], of[i][1]};
+    }
+};
 typedef __attribute__((address_space(3))) const u2v lds_cu2;
 // table_lane: the place of the lane's copy, (lane % 32) * 8; the table lies at 0
 __device__ __forceinline__ u2v key_read(uint32_t code_word, uint32_t table_lane, int byte) {
@@ -78,6 +89,8 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
     const int kv_head = P.q_subgroups == 1 ? kv_sub : fast_div(kv_sub, P.q_subgroups);
     const int head0 = kv_head * P.gqa + (kv_sub - kv_head * P.q_subgroups) * P.q_group;
 
+    TableEntries entries;
+    entries.load(tid);
     DecodeStart s0;
     if (!decode_start<true>(P, smem, tid, lane, kv_sub, s0)) return;
     const int key_first = s0.key_first, key_last = s0.key_last, end = s0.end;
@@ -119,8 +132,9 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
     const bool sloped = P.slopes != nullptr;
 
     // ---- table, first loads, query operands ----
-    build_two_part_table(smem, tid, wave);
+    entries.store(smem, tid);
     int half = s0.begin + 2 * wave;
+    columns.arrived();
     if (half < end) {
         locate(half);
         load_keys();
