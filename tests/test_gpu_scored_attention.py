@@ -162,7 +162,7 @@ def test_what_unseen_rows_hold_does_not_matter(fmt, dt, qs):
 
 
 @gpu
-@pytest.mark.parametrize("cap", [0.5, 512.0, 513.0, 1e4, 1e30])
+@pytest.mark.parametrize("cap", [1e-44, 1e-38, 0.5, 512.0, 513.0, 1e4, 1e30])
 def test_caps_of_any_size(cap):
     """Far above the scores a cap changes nothing.  (The bound's term for the cap stands for the 2^-23 that tanh is off by up to the
     size from which small arguments go through a series.)"""
@@ -175,6 +175,86 @@ def test_caps_of_any_size(cap):
         _, _, bound, lse_bound = scored_attention(pool, bt, [200], q64, aq, ctx, cap=0.0, scale=hb.sm_scale, dt=DT_F16)
     got = oracle.bits_to_f32(bits, DT_F16).astype(np.float64)
     assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dt", [(FMT_TQ4, DT_BF16), (FMT_FP16, DT_F16)])
+@pytest.mark.parametrize("tokens", [2, 70])
+@pytest.mark.parametrize("scale", [-0.0625, 0.0, 0.5])
+def test_scales_of_any_sign(fmt, dt, tokens, scale):
+    pool, bt, k, v, q, aq, ctx = case(fmt, 16, [150], [tokens], 984, dt)
+    hb = oracle.HostBatch(aq, [150], bt, context_lens_before=ctx)
+    hb.sm_scale = scale
+    check_scored(pool, bt, [150], q, dt, aq, ctx, 8, hb=hb, cap=20.0)
+
+
+@gpu
+@pytest.mark.parametrize("tokens", [2, 70])
+def test_lengths_before_may_be_left_out(tokens):
+    """Without context_lens_before a request's tokens are its last ones."""
+    seqs, qs = [150, 90], [tokens, 3]
+    pool, bt, k, v, q, aq, ctx = case(FMT_TQ4, 16, seqs, qs, 983, DT_F16)
+    hb = oracle.HostBatch(aq, seqs, bt, context_lens_before=ctx)
+    want = run_scored(pool, hb, q, DT_F16, 8, cap=20.0)
+    hb.ctx = None
+    got = run_scored(pool, hb, q, DT_F16, 8, cap=20.0)
+    assert want[0].tobytes() == got[0].tobytes() and want[1].tobytes() == got[1].tobytes()
+
+
+@gpu
+@pytest.mark.parametrize("fmt,dt", [(FMT_TQ4, DT_BF16), (FMT_BF16, DT_BF16), (FMT_Q8_0, DT_F16)])
+@pytest.mark.parametrize("tokens", [1, 70])
+def test_positions_of_any_size(fmt, dt, tokens):
+    """A window over the end of 2^30 keys gives the bits of the same keys in a short sequence."""
+    block, seq, window = 128, 1000, 300
+    pool, bt, k, v, q, aq, ctx = case(fmt, block, [seq], [tokens], 982, dt)
+    moved = (1 << 23) - 16
+    far = np.zeros((1, bt.shape[1] + moved), dtype=np.int32)
+    far[0, moved:] = bt[0]
+    results = []
+    for table, before in ((bt, 0), (far, moved * block)):
+        hb = oracle.HostBatch(aq, [seq + before], table, context_lens_before=[ctx[0] + before])
+        hb.sliding_window = window
+        documents = np.full(aq[-1], before + 640, dtype=np.int32)
+        results.append(run_scored(pool, hb, q, dt, 8, cap=20.0, slopes=slopes_of(8), documents=documents))
+    assert results[0][0].tobytes() == results[1][0].tobytes() and results[0][1].tobytes() == results[1][1].tobytes()
+
+
+@gpu
+def test_calls_on_two_streams_at_once():
+    """Own workspaces, the same pages: a decode call and a chunk call in turn on each of two streams give what they give alone."""
+    import torch
+
+    import gpu_harness as G
+    from warp34_amd import ffi
+
+    made = []
+    for seqs, qs, seed in (([3000, 100], [1, 2], 980), ([700], [130], 981)):
+        pool, bt, k, v, q, aq, ctx = case(FMT_TQ4, 16, seqs, qs, seed, DT_BF16)
+        dpool = G.DevPool(pool)
+        dpool.upload()
+        hb = oracle.HostBatch(aq, seqs, bt, context_lens_before=ctx)
+        alone = run_scored(pool, hb, q, DT_BF16, 8, cap=30.0, dpool=dpool, scratch=16 << 20)
+        made.append((dpool, G.DevBatch(hb), G.to_dev(q), aq[-1], alone))
+    fn = G.lib().warp34_paged_attention_scored_bf16
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    spaces = [torch.zeros(16 << 20, dtype=torch.uint8, device=G.DEV) for _ in range(2)]
+    calls = []
+    torch.cuda.synchronize()
+    for turn in range(6):
+        for stream, space in zip(streams, spaces):
+            dpool, db, qd, n, alone = made[(turn + (stream is streams[1])) % 2]
+            with torch.cuda.stream(stream):
+                out = torch.zeros((n, 8, 256), dtype=torch.int16, device=G.DEV)
+                lse = torch.zeros((n, 8), dtype=torch.float32, device=G.DEV)
+            layout, batch = dpool.layout(), db.struct()
+            scores, keep = scores_struct(G, cap=30.0, lse=lse)
+            ex = ffi.Warp34Exec(stream.cuda_stream, space.data_ptr(), space.numel(), 0)
+            assert fn(C.byref(ex), C.byref(layout), C.byref(batch), C.byref(scores), G.ptr(qd), G.ptr(out), 8) == 0
+            calls.append((out, lse, alone))
+    torch.cuda.synchronize()
+    for out, lse, alone in calls:
+        assert out.cpu().numpy().view(np.uint16).tobytes() == alone[0].tobytes() and lse.cpu().numpy().tobytes() == alone[1].tobytes()
 
 
 @gpu

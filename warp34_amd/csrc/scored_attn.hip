@@ -81,7 +81,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const warp34_attention_batch& B = P.B;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
     const ScoredShape s = scored_shape(KVF, B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
-    if (kv_subs > 65535 || s.entries > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
+    if (kv_subs > 65535 || s.entries * kv_subs > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
     P.tok_tile = s.tok_tile;
     P.tiles = (int)s.tiles;
     P.entries = (int)s.entries;
@@ -163,7 +163,8 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.scale2 = std::max(std::fabs(batch->sm_scale), 1.0e-30f) * kLog2e;
     P.q_flip = batch->sm_scale < 0.f ? 0x80008000u : 0u;
     P.cap2 = scores->softcap * kLog2e;
-    P.cap_arg = scores->softcap > 0.f ? 2.0f * std::fabs(batch->sm_scale) * kLog2e / scores->softcap : 0.f;
+    // (finite, so that a score of 0 stays 0 under the smallest of caps)
+    P.cap_arg = scores->softcap > 0.f ? std::min(2.0f * std::fabs(batch->sm_scale) * kLog2e / scores->softcap, 1.0e30f) : 0.f;
     P.wide_cap = scores->softcap > kWideCap ? 1 : 0;
     P.num_q_heads = num_q_heads;
     P.gqa = num_q_heads / layout->local_kv_heads;
