@@ -11,7 +11,10 @@ namespace w34 {
 constexpr int kDecodeCols = 16;         // query columns of a workgroup of the decode kernel
 constexpr int kDecodeMinHalves = 8;     // shortest chunk: a half unit for each wave
 constexpr int kChunkMinHalves = 16;     // 8 units
-constexpr int kSpreadTiles = 8;          // chunk kernel: batches of up to so many tiles have a workgroup a column to join their chunks
+// Batches of up to so many tiles have a workgroup a column to join their chunks, others a wave a column: a few tiles have many chunks each.
+// us a call, workgroups / waves: decode, 1 tile of 131 072 TQ4 keys 28.4 / 41.6, 10 tiles 34.3 / 37.8, 16 tiles 26.6 / 25.7, 32 tiles 55.7 /
+// 51.1; chunks, 1 tile of 16 000 keys 47 / 102, 8 tiles 51 / 45 and 60 / 62, 16 tiles 94 / 77.
+constexpr int kSpreadTiles = 12, kSpreadChunkTiles = 8;
 constexpr int kDecodeRounds = 4, kChunkRounds = 2;
 
 // Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
@@ -128,7 +131,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
                  : launch(scored_chunk_kernel<TQ, KVF, HD, false>, kChunkWaves * 64, lds);
     }
     if (rc || slots == 0) return rc;
-    if (s.entries > (s.chunk ? kSpreadTiles : 64)) {
+    if (s.entries > (s.chunk ? kSpreadChunkTiles : kSpreadTiles)) {
         hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)((s.cols + kJoinCols - 1) / kJoinCols)), dim3(512), 0, stream, P,
                            s.cols, ScoredRows<KVF, HD>::kOutScale);
     } else {
