@@ -41,21 +41,23 @@ struct ScoredParams {
     int rot_q, rot_out;
 };
 
-// tanh(u) = 1 - 2 / (exp(2 u) + 1) is off by some 2^-23 whatever u, which the cap multiplies: 6e-5 at this cap, beyond it small
-// arguments go through the series.
+// tanh(u) = 1 - 2 / (exp(2 u) + 1) is off by some 2^-23 whatever u, which the cap multiplies: 6e-6 of a score at a cap of 50, 6e-5 at
+// this one.  Where few keys make a row that shows in its lse: the decode kernels take small arguments through the series, and so does
+// the chunk kernel, whose queries are rounded to more than that, beyond this cap.
 constexpr float kWideCap = 512.0f;
 
 // Scores s (q . k times what the column's scale is in) become y with x = y ca + cb in the log2 domain, ca >= 0, so that the largest y is
-// the largest x and exp2's argument x - m is one fma.  No cap: y = s, x = y cs.  Cap: y = -1 / (exp(2 x / cap) + 1), x = cap2 + 2 cap2 y.
-// cs >= 0 and cc: the column's scale times scale2 / cap_arg.  (The choice stands outside the loop: one uniform branch.)
+// the largest x and exp2's argument x - m is one fma.  No cap: y = s, x = y cs.  Cap without the series: y = -1 / (exp(2 x / cap) + 1),
+// x = cap2 + 2 cap2 y.  cs >= 0 and cc: the column's scale times scale2 / cap_arg.
+// The series stands for |u| < 1/4, where what follows its last term is below 2^-26 of it.
 struct ScoreMap {
     float ca, cb;
 };
-template <bool CAP, int N, typename V>
+template <bool CAP, bool SERIES, int N, typename V>
 __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const ScoredParams& P) {
     if constexpr (!CAP) {
         return ScoreMap{cs, 0.f};
-    } else if (!P.wide_cap) {
+    } else if (!SERIES && !P.wide_cap) {  // (uniform, and outside the loop)
 #pragma unroll
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * cc));
         return ScoreMap{2.0f * P.cap2, P.cap2};
@@ -64,8 +66,11 @@ __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const S
         for (int i = 0; i < N; ++i) {
             const float a = s[i] * cc, u = a * (0.5f / kLog2e), uu = u * u;
             const float x = __builtin_fmaf(2.0f * P.cap2, __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(a)), P.cap2);
-            const float series = __builtin_fmaf(uu, __builtin_fmaf(uu, __builtin_fmaf(uu, -17.0f / 315.0f, 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
-            s[i] = fabsf(u) < 0.1f ? s[i] * cs * series : x;
+            float series = __builtin_fmaf(uu, 62.0f / 2835.0f, -17.0f / 315.0f);
+            series = __builtin_fmaf(uu, series, 2.0f / 15.0f);
+            series = __builtin_fmaf(uu, series, -1.0f / 3.0f);
+            series = s[i] * cs * __builtin_fmaf(uu, series, 1.0f);
+            s[i] = fabsf(u) < 0.25f ? series : x;
         }
         return ScoreMap{1.0f, 0.f};
     }

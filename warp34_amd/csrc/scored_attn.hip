@@ -131,12 +131,13 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
                  : launch(scored_chunk_kernel<TQ, KVF, HD, false>, kChunkWaves * 64, lds);
     }
     if (rc || slots == 0) return rc;
+    const float value_scale = KVF == WARP34_KV_FORMAT_TQ4 && !s.chunk ? kTableInvGain : ScoredRows<KVF, HD>::kOutScale;
     if (s.entries > (s.chunk ? kSpreadChunkTiles : kSpreadTiles)) {
         hipLaunchKernelGGL((scored_join_kernel<TQ, HD, false>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)((s.cols + kJoinCols - 1) / kJoinCols)), dim3(512), 0, stream, P,
-                           s.cols, ScoredRows<KVF, HD>::kOutScale);
+                           s.cols, value_scale);
     } else {
         hipLaunchKernelGGL((scored_join_kernel<TQ, HD, true>), dim3((unsigned)s.entries, (unsigned)kv_subs, (unsigned)s.cols), dim3(512), 0, stream, P,
-                           s.cols, ScoredRows<KVF, HD>::kOutScale);
+                           s.cols, value_scale);
     }
     return (int)hipGetLastError();
 }

@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         __builtin_amdgcn_sched_barrier(0);
         // ---- terms, masks, softmax ----
         const bool masked = !(u0 >= all_from && u0 + kChunkUnit - 1 <= all_to);  // uniform
-        ScoreMap map = map_scores<CAP, 16>(s, cs, cc, P);
+        ScoreMap map = map_scores<CAP, false, 16>(s, cs, cc, P);
         if (sloped) {
             const float at = (float)(my_pos - u0 - 4 * b);
 #pragma unroll

@@ -116,9 +116,10 @@ __device__ __forceinline__ DecodeColumn decode_column(const ScoredParams& P, con
     return c;
 }
 
-// Query columns of quantised rows: a wave brings every eighth of COLS columns to LDS: rotated where the keys are, relative to a power of
-// two above their largest element so that fp16 holds them whatever their size, in two parts (the second is zero where nothing is
-// rotated: 11 bits are all there are).
+// Query columns of quantised rows: a wave brings every eighth of COLS columns to LDS, rotated where the keys are, in two fp16 parts (the
+// second is zero where nothing is rotated: 11 bits are all there are).  They are relative to a power of two, so that the largest element
+// is 2^12 to 2^13: fp16 holds a query whatever its size, and the second parts of its smaller elements are still normal numbers.
+constexpr int kQueryTop = 13;
 template <typename TQ, int COLS, int STRIDE>
 struct QueryColumns {
     uint2 raw[COLS / kScoredWaves];
@@ -157,13 +158,13 @@ __device__ __forceinline__ void QueryColumns<TQ, COLS, STRIDE>::bring(const Scor
         const float top = wave_top(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
         const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
+        for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], kQueryTop - e);
         uint32_t h0, h1, l0, l1;
         split_weights(v[0], v[1], h0, l0);
         split_weights(v[2], v[3], h1, l1);
         *reinterpret_cast<uint2*>(high + c * STRIDE + 4 * lane) = uint2{h0, h1};
         *reinterpret_cast<uint2*>(low + c * STRIDE + 4 * lane) = uint2{l0, l1};
-        if (lane == 0) scales[c] = __builtin_amdgcn_ldexpf(1.0f, e);
+        if (lane == 0) scales[c] = __builtin_amdgcn_ldexpf(1.0f, e - kQueryTop);
     }
 }
 
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 
         // ---- terms, masks, softmax ----
         const bool masked = !(half * 16 >= col.all_from && half * 16 + 15 <= col.all_to);  // uniform
-        ScoreMap map = map_scores<CAP, 4>(s, cs, cc, P);
+        ScoreMap map = map_scores<CAP, true, 4>(s, cs, cc, P);
         float x[4] = {s[0], s[1], s[2], s[3]}, p[4];
         if (sloped) {
 #pragma unroll

@@ -20,6 +20,8 @@ constexpr int kTq4Cols = 8;
 // The table: entries of eight bytes, the pair of fp16 numbers of a byte's two codes and the pair of what they are short of the centroids;
 // 32 copies (a read goes by 32 lanes at a time).  The fp16 numbers are up to 9.4e-5 from the centroids, which would be 1e-4 of a score and
 // 2e-5 of a row's lse where a few keys carry it: keys take both, values the first alone.
+// What centroids are multiplied by: with kLutGain alone the second parts of small ones would be below fp16's smallest normal number.
+constexpr float kTableGain = 4096.0f * kLutGain, kTableInvGain = kLutInvGain / 4096.0f;
 struct TwoPartPairs {
     u2v of[256];
 };
@@ -28,7 +30,7 @@ constexpr TwoPartPairs make_two_part_pairs() {
     for (int e = 0; e < 256; ++e) {
         uint32_t v = 0, w = 0;
         for (int k = 0; k < 2; ++k) {
-            const float c = kLutGain * kCentroids[e >> (4 * k) & 15];
+            const float c = kTableGain * kCentroids[e >> (4 * k) & 15];
             const _Float16 hi = (_Float16)c;
             v |= (uint32_t)__builtin_bit_cast(uint16_t, hi) << (16 * k);
             w |= (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)(c - (float)hi)) << (16 * k);
@@ -152,7 +154,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
         q[2 * m] = u4{w[0], w[0], w[1], w[1]};
         q[2 * m + 1] = u4{w[2], w[2], w[3], w[3]};
     }
-    const float cs = P.scale2 * (qs[n & 7] * kLutInvGain), cc = P.cap_arg * (qs[n & 7] * kLutInvGain);
+    const float cs = P.scale2 * (qs[n & 7] * kTableInvGain), cc = P.cap_arg * (qs[n & 7] * kTableInvGain);
     const float low_part = n < 8 ? 0.f : 1.f;
     const uint32_t table_lane = ((uint32_t)lane & 31u) << 3;
 
@@ -217,7 +219,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
         // ---- terms, masks, softmax ----
         const bool masked = !(half * 16 >= col.all_from && half * 16 + 31 <= col.all_to);  // uniform
         float x[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]}, p[8];
-        ScoreMap map = map_scores<CAP, 8>(x, cs, cc, P);
+        ScoreMap map = map_scores<CAP, true, 8>(x, cs, cc, P);
         const auto at = [&](int i) { return pos + (i & 3) + 16 * (i >> 2); };
         if (sloped) {
 #pragma unroll
@@ -311,7 +313,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
     if (n < 8 && b == 0) *reinterpret_cast<f2*>(ml + (wave * 16 + n) * 2) = f2{m_run, l_run};
     __syncthreads();
     join_waves<TQ, 256, 8, kTq4Cols>(P, s0, kv_sub, head0, live, wave, lane, smem, M::kRegion, ml, reinterpret_cast<float*>(smem + M::kReorder + wave * 1024),
-                                     kLutInvGain);
+                                     kTableInvGain);
 }
 
 }  // namespace w34
