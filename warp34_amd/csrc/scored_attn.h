@@ -31,7 +31,7 @@ struct ScoredParams {
     int tiles;        // tiles of a request (a bound)
     int entries;      // requests x tiles: tiles of the batch, some of them empty
     int target;       // slots for chunks, for each kv head; 0: no split, a workgroup for each entry
-    int rounds;       // chunks of 1 / (128 rounds) of all keys; 0: no more chunks than target
+    int full_rounds;  // the cut looks for full rounds of chunks; 0: no more chunks than target
     int records;      // partial records the scratch holds, for each kv head
     int min_halves;   // shortest chunk
     float* part_acc;  // [record][kv_sub][column][head_dim]
@@ -180,11 +180,16 @@ __device__ __forceinline__ int tile_halves_guess(const ScoredParams& P, const Sc
 __device__ __forceinline__ int tile_halves(int first, int last) { return first <= last ? (last >> 4) - (first >> 4) + 1 : 0; }
 
 // The cut of a batch.  All tiles have chunks of up to `per` half units, a tile's chunks are of one length, and a live tile has one at
-// least.  P.rounds == 0: the shortest `per` that needs no more than P.target chunks.  Otherwise a fixed share of all keys, so that the
-// workgroups, which start as others end, end together.  Tiles with several chunks have a record for each: no more than the scratch holds.
+// least.  Tiles with several chunks have a record for each: no more than the scratch holds.  P.full_rounds == 0: the shortest `per` that
+// needs no more than P.target chunks.  Otherwise, where the tiles make a round of workgroups by themselves, only what is longer than an even
+// share by more than a chunk costs is cut; where they do not, the chunks make one full round, or two where one would be a chunk's
+// cost longer than an even share (a chunk more than a round takes a round of its own).  us a call, cutting all to even shares / so: 9 requests
+// of 300 to 900 BF16 tokens on 1 000 to 9 000 keys 391 / 412, packed documents (tiles of 1 to 43 units) 123 / 109; chunks of 1 / 256 of the keys
+// always / so: 600 tokens on 5 000 FP8 keys 148 / 106, 6 requests of 100 to 500 TQ4 tokens 172 / 136, prefix over FP8 331 / 334.
 // count(e): the half units of entry e, -1 for tiles without tokens.
 constexpr int kMaxSplitEntries = 2048;  // entries of a batch that is split
 constexpr int kSlotRound = 128;         // slots for each kv head that fill the chip where there are two
+constexpr int kChunkCost = 32;          // what a workgroup takes beside its keys, in half units
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
 template <typename Count>
 __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Count&& count) {
@@ -196,9 +201,7 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
     }
     total = wave_sum(total);
     live = wave_sum(live);
-    // (few tiles: whole rounds of chunks, one more than fills them would take a round of its own)
-    const int limit = P.rounds > 0 && live < kSlotRound ? min(P.target, P.rounds * kSlotRound) : P.target;
-    const auto fits = [&](int per) {
+    const auto fits = [&](int per, int limit) {
         int n = 0, several = 0;
         for (int e = lane; e < P.entries; e += 64) {
             const int c = chunks_of(count(e), per);
@@ -207,19 +210,32 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
         }
         return wave_sum(n) <= limit && wave_sum(several) <= P.records;
     };
-    // (with a round of tiles or more there is something for every CU without a cut: only what is longer than a CU's share is cut)
-    const int share = P.rounds > 0 ? (live < kSlotRound ? P.rounds * kSlotRound : kSlotRound * 2 / 3) : P.target;
-    int per = max(P.min_halves, (total + share - 1) / share);
-    if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per)) return per;
+    int limit = P.target, per;
+    if (P.full_rounds == 0) {
+        per = (total + limit - 1) / limit;
+    } else {
+        const int even = (total + kSlotRound - 1) / kSlotRound;  // what a CU has of it
+        if (live >= kSlotRound) {
+            per = even + kChunkCost;
+        } else if (fits(even + kChunkCost, min(P.target, kSlotRound))) {
+            limit = min(P.target, kSlotRound);
+            per = even;
+        } else {
+            limit = min(P.target, 2 * kSlotRound);
+            per = (even + 1) / 2;
+        }
+    }
+    per = max(per, P.min_halves);
+    if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per, limit)) return per;
     // sum of ceil(h / per) <= total / per + live, so this many halves a chunk are enough for any number of slots above live
     int low = per, high = max(per + 1, (total + max(limit - live, 1) - 1) / max(limit - live, 1));
-    while (!fits(high)) {
+    while (!fits(high, limit)) {
         low = high;
         high *= 2;
     }
     while (high - low > max(1, low >> 5)) {
         const int mid = (low + high) >> 1;
-        if (fits(mid)) high = mid;
+        if (fits(mid, limit)) high = mid;
         else low = mid;
     }
     return high;

@@ -8,16 +8,25 @@
 
 namespace w34 {
 
-constexpr int kDecodeCols = 16;         // query columns of a workgroup of the decode kernel
-constexpr int kDecodeMinHalves = 8;     // shortest chunk: a half unit for each wave
-constexpr int kChunkMinHalves = 16;     // 8 units
+constexpr int kDecodeCols = 16;  // query columns of a workgroup of the decode kernel (TQ4: kTq4Cols)
+
+// Shortest chunks, in half units of 16 keys.  Decode, us a call at 8 / 4 / 3 / 2: 700 FP16 keys 12.5 / 10.7 / 10.3 / 9.9, 3 000 TQ4 keys
+// 13.7 / 13.2 / 13.6 / 14.8, 4 requests of 300 to 900 BF16 keys 10.0 / 9.2 / 9.8 / 9.7.  Chunk kernel at 64 / 32 / 16 / 8, 32 tokens of
+// BF16: on 16 000 keys 99 / 56 / 46 / 53, 8 requests on 4 000 92 / 69 / 61 / 66, 2 on 1 000 72 / 53 / 39 / 32.
+constexpr int kDecodeMinHalves = 4, kChunkMinHalves = 16;
+// Up to so many half units, two for each wave, the keys of a decode call are not cut: the join's launch takes longer.  us a call, whole /
+// cut: 100 FP16 keys 7.6 / 10.3, 250 10.2 / 10.4, 330 12.5 / 10.7; TQ4 8.7 / 12.4, 11.6 / 12.5, 13.2 / 12.7.
+constexpr int kDecodeWhole = 16;
+
 // Batches of up to so many tiles have a workgroup a column to join their chunks, others a wave a column: a few tiles have many chunks each.
 // us a call, workgroups / waves: decode, 1 tile of 131 072 TQ4 keys 28.4 / 41.6, 10 tiles 34.3 / 37.8, 16 tiles 26.6 / 25.7, 32 tiles 55.7 /
 // 51.1; chunks, 1 tile of 16 000 keys 47 / 102, 8 tiles 51 / 45 and 60 / 62, 16 tiles 94 / 77.
 constexpr int kSpreadTiles = 12, kSpreadChunkTiles = 8;
-constexpr int kDecodeRounds = 4, kChunkRounds = 2;
 
-// Requests with at least this many query columns (tokens x q heads of a kv head) go through the chunk kernel
+// Requests with at least this many query columns (tokens x q heads of a kv head), a full tile, go through the chunk kernel.  us a call,
+// decode / chunk kernel, for 1 request on 16 000 keys, 8 on 4 000, 2 on 1 000, 1 on 64 000.  256 columns: BF16 49 / 46, 95 / 61, 19 / 39,
+// 168 / 87; TQ4 62 / 64, 129 / 75, 23 / 56, 193 / 103; Q8_0 46 / 58, 85 / 72, 19 / 48, 140 / 103.  128 columns: BF16 31 / 34, 57 / 47,
+// 16 / 29, 93 / 61; TQ4 39 / 51, 69 / 64, 17 / 45, 106 / 85; Q8_0 29 / 46, 53 / 62, 16 / 40, 77 / 84.
 constexpr int kChunkFrom = 256;
 
 static int decode_cols(int format) { return format == WARP34_KV_FORMAT_TQ4 ? kTq4Cols : kDecodeCols; }
@@ -27,7 +36,8 @@ struct ScoredShape {
     bool chunk;
     int cols, tok_tile;
     long long tiles, entries;
-    int slots, rounds;
+    int slots;
+    bool full_rounds;
 };
 static ScoredShape scored_shape(int format, int num_reqs, int total_tokens, int max_q_len, int q_group) {
     ScoredShape s;
@@ -37,10 +47,10 @@ static ScoredShape scored_shape(int format, int num_reqs, int total_tokens, int 
     s.tok_tile = s.cols / q_group;
     s.tiles = ((long long)q_len + s.tok_tile - 1) / s.tok_tile;
     s.entries = s.tiles * num_reqs;
-    // Decode batches of up to 64 tiles: at most 128 chunks for each kv head, which two kv heads run in one round.  Others: chunks of a
-    // fixed share of the keys, and as many slots as that may need.
-    s.rounds = s.chunk ? kChunkRounds : s.entries <= 64 ? 0 : kDecodeRounds;
-    s.slots = s.entries > kMaxSplitEntries ? 0 : s.rounds == 0 ? kSlotRound : (int)(s.rounds * kSlotRound + s.entries);
+    // Decode batches of up to 64 tiles: at most 128 chunks for each kv head, which two kv heads run in one round.  Others: up to two rounds,
+    // or a chunk for each tile and some more.
+    s.full_rounds = s.chunk || s.entries > 64;
+    s.slots = s.entries > kMaxSplitEntries ? 0 : (int)(s.full_rounds ? 2 * kSlotRound + s.entries : kSlotRound);
     return s;
 }
 // Bytes of the partial records of a slot, and of the tiles' table.
@@ -94,13 +104,13 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const size_t table = scored_table_bytes(s.entries);
     if (ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0 && ex->scratch_size > table)
         records = std::min<long long>(slots, (long long)((ex->scratch_size - table) / scored_slot_bytes(s, kv_subs, HD)));
-    if (records < 2 || (B.max_seq_len > 0 && B.max_seq_len <= 16 * P.min_halves)) slots = 0;
+    if (records < 2 || (B.max_seq_len > 0 && B.max_seq_len <= 16 * (s.chunk ? kChunkMinHalves : kDecodeWhole))) slots = 0;
     if (slots > 0 && B.max_seq_len > 0) {
         const long long most = (((long long)B.max_seq_len + 30) / 16 + P.min_halves - 1) / P.min_halves;  // chunks of a tile
         slots = std::min(slots, std::max<long long>(s.entries * most, 2));
     }
     P.target = (int)slots;
-    P.rounds = s.rounds;
+    P.full_rounds = s.full_rounds ? 1 : 0;
     P.records = (int)records;
     if (slots > 0) {
         uint8_t* at = reinterpret_cast<uint8_t*>((uintptr_t)ex->scratch_ptr);
