@@ -303,7 +303,9 @@ def test_same_bits_whatever_the_pages_and_bounds():
     wide = np.zeros((2, bt.shape[1] + 30), dtype=np.int32)
     wide[:, :bt.shape[1]] = bt
     c = check_scored(pool, wide, seqs, q, DT_F16, aq, ctx, 8, cap=30.0)
-    for other in (b, c):
+    d = check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 8, cap=30.0, max_seq_len=100000)
+    e = check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, 8, cap=30.0, max_seq_len=0)
+    for other in (b, c, d, e):
         assert a[0].tobytes() == other[0].tobytes() and a[1].tobytes() == other[1].tobytes()
 
 

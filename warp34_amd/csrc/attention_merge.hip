@@ -3,13 +3,14 @@
 //   lse = ln sum_p exp(lse_p)        out = sum_p exp(lse_p - lse) out_p
 //
 // in 32 bits, rounded once.  A part whose lse is minus infinity saw no key: what its row holds does not matter.  One pass: the sums
-// are kept relative to a running maximum.  Bound: HBM, every part read once.
+// are kept relative to a running maximum.  Bound: HBM, every part read once: two parts of 131 072 fp16 rows of 256 in 36.7 us (5.5 TB/s, as a large copy),
+// eight of 32 768 in 30.6; eight of 512 in 3.8, a launch.
 #include "attn_lanes.h"
 
 namespace w34 {
 
 // A thread takes eight elements of a row, head_dim / 8 threads a row.  Parts go by in groups of kMergeGroup, whose loads travel
-// together.
+// together (2 / 4 / 8: two parts of 131 072 rows 37.0 / 36.7 / 40.0 us, eight of 32 768 30.5 / 30.6 / 32.3).
 constexpr int kMergeGroup = 4;
 
 template <typename T>

@@ -62,6 +62,7 @@ __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const S
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * cc));
         return ScoreMap{2.0f * P.cap2, P.cap2};
     } else {
+        if (!SERIES) asm volatile("");  // (both ways would be worked out for every score)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float a = s[i] * cc, u = a * (0.5f / kLog2e), uu = u * u;
@@ -187,7 +188,9 @@ __device__ __forceinline__ int tile_halves(int first, int last) { return first <
 // of 300 to 900 BF16 tokens on 1 000 to 9 000 keys 391 / 412, packed documents (tiles of 1 to 43 units) 123 / 109; chunks of 1 / 256 of the keys
 // always / so: 600 tokens on 5 000 FP8 keys 148 / 106, 6 requests of 100 to 500 TQ4 tokens 172 / 136, prefix over FP8 331 / 334.
 // count(e): the half units of entry e, -1 for tiles without tokens.
-constexpr int kMaxSplitEntries = 2048;  // entries of a batch that is split
+// Entries of a batch that is cut.  us a call, up to 2 048 / up to 512: one request of 60 000 keys among 600 of 100 94 / 620, among 1 800 306 / 765;
+// 600 requests of 16 to 4 000 keys, which need no cut, 467 / 456.
+constexpr int kMaxSplitEntries = 2048;
 constexpr int kSlotRound = 128;         // slots for each kv head that fill the chip where there are two
 constexpr int kChunkCost = 32;          // what a workgroup takes beside its keys, in half units
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }

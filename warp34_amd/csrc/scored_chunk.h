@@ -3,13 +3,22 @@
 // Workgroup = 256 query columns (tokens x the q heads of a kv head) x a range of keys, eight waves of 32 columns each.  The workgroup
 // walks the keys in units of 32, one barrier a unit; between two barriers
 //   the rows of a later unit travel from the pages to LDS (LDS-direct loads: no register holds them),
-//   quantised rows of the next unit are widened into the 16-bit tiles that the products read, and
-//   every wave multiplies the present unit:  S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs.
+//   every wave multiplies:  S^T = K Q^T and O^T += V^T P^T in 32x32x16 MFMAs, and
+//   quantised rows of the next unit are widened into the 16-bit tiles that the products read, between the products of values.
 // A lane (n, b) has the scores of column n for the keys (i & 3) + 8 (i >> 2) + 4 b, i = 0 .. 15: eight of them are, where they stand, a
 // B operand of the value product over 16 keys, whose A operand comes out of row-major LDS by the transposing reads
 // (ds_read_b64_tr_b16: lane l of 16 gets column l of four rows of 16 values).  So both tiles are row-major and nothing is shuffled.
 //   key tile    row r, 16-byte piece p at p ^ (r & 15): the operand reads of 16 rows touch all banks
 //   value tile  row r, piece p at p ^ 4 (r & 3): the four rows of a transposing read touch all banks
+//
+// Why this shape: 128 sums and 64 query registers a lane are what two waves a SIMD have room for, and each operand read from LDS serves 32
+// columns.  4 requests of 2 048 tokens on 16 384 keys, 16 + 2 heads, capped: BF16 2.36 ms (990 TFLOP/s; a large matrix product of the
+// library 1 390), FP8 2.85, TQ4 3.03 (770), Q8_0 3.27.  What bounds it is a wave's own chain: of 6 700 cycles a TQ4 unit the products of a SIMD's
+// two waves take 2 050, vector work 55 % of the cycles (a cap's exponential and reciprocal, the weights' exponentials and the widening most of
+// it), LDS 32 %, and a wave waits 38 %.  Left out for timing: cap and exponentials -7 %, widening -14 %, operand reads -15 %, all three -36 %;
+// the rows' pages made no difference.  Two sums side by side for the scores need 16 registers more than there are (packed documents 107 ->
+// 119 us); operands three products ahead the same (TQ4 3.31 ms).  Values a unit later in half of the waves: -5 %; widening between
+// products: FP8 -7 %, Q8_0 -9 %, TQ4 -1.5 %.
 #pragma once
 
 #include "scored_decode.h"
@@ -27,7 +36,8 @@ constexpr int kChunkWaves = 8;
 constexpr int kChunkCols = 32 * kChunkWaves;
 constexpr int kChunkUnit = 32;
 // A column's maximum is raised only by scores that exceed it by more than this (log2 domain): a weight may be up to 2^8, which costs
-// none of its bits, and the multiplication of 128 sums a lane is spared in nearly all units.
+// none of its bits, and the multiplication of 128 sums a lane is spared in nearly all units.  us with slack / without: packed documents
+// 108 / 114, 9 requests of 300 to 900 BF16 tokens 471 / 488, 4 x 2 048 on 16 384 TQ4 keys 3 078 / 3 136.
 constexpr float kChunkSlack = 8.0f;
 
 constexpr int kKeysAhead = 2, kValuesAhead = 2;  // operands are read from LDS so many products before their own
@@ -99,7 +109,9 @@ __device__ __forceinline__ void build_narrow_table(uint8_t* smem, int tid, int w
 // Roundings, beside those of the inputs' types: rotated queries and TQ4 keys are one fp16 part (the keys' block scales multiply the
 // scores in 32 bits); quantised values are fp16(scale * code), TQ4 ones from the fp16 table; weights are one operand of the values'
 // type.  (Weights that carry the block scales would spare the values' rounding and need two parts, half as many products again: a
-// block-wide error of a weight is gathered in one channel by the rotation back.)
+// block-wide error of a weight is gathered in one channel by the rotation back.)  2-norm of the error: TQ4 4.5e-4, un-rotated 8-bit rows
+// 2.7e-4 into fp16 outputs, whose own rounding is 2.1e-4; 1.8e-3 and 1.7e-3 of 1.7e-3 into bf16 ones.  Of TQ4's the queries are 2.8e-4, values 2.1e-4,
+// weights 1.2e-4, and second parts of queries would be 64 registers more.
 template <typename TQ, int KVF, int HD, bool CAP>
 __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const ScoredParams P) {
     extern __shared__ __align__(16) uint8_t smem[];

@@ -8,6 +8,13 @@
 // Rows go from the pages to registers as they are stored; key loads of the next half unit travel during the softmax and the value
 // product, value loads during the next scores.  Only the scales of quantised rows go through LDS.
 // At the end the waves' states are joined through LDS, and the chunks' by scored_join_kernel.
+//
+// Bound: HBM over many keys (32 requests of 1k to 64k keys: FP16 411 us = 5.3 TB/s, FP8 223 = 4.8, Q8_0 235 = 4.7; a large copy of the
+// card 5.1, reads alone 6.0), round trips over few: one request on 700 FP16 keys 10.7 us, of which kernel 7.4 (arguments and lengths 1.5,
+// first rows 1.5, a half unit 1.7, join of the waves 2) and the join's launch 3.  16 windows of 4 096 BF16 keys, head_dim 128: 25.9 us, kernel 20, of
+// which 9 to 12 stream.  Q8_0 verify steps of 5 x 4 tokens on 3k to 21k keys 34.5 us: 17 for eight half units a wave, 400 vector
+// instructions each, tiles of 16 columns twice over the rows.  (Tiles of 32 columns: 34.0 there, 29.6 for 32.4 over FP8, but 24.9 for 17.6 where
+// 4 requests look at 4 000 keys: not kept.  Waves in step by a barrier every step: no gain.)
 #pragma once
 
 #include "scored_attn.h"
