@@ -329,8 +329,8 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  * (hipErrorInvalidValue).  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
  * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass.  Two calls that may run
  * at once need a workspace each.
- * The order of summation depends on the lengths, on num_reqs, max_q_len, whether max_seq_len is at most 256, and the
- * scratch, and on nothing else: the same call gives the same bits.  Requests of 256 and more query columns (max_q_len
+ * The order of summation depends on the lengths, the heads, num_reqs, max_q_len, whether max_seq_len is at most 256, and
+ * the scratch, and on nothing else: the same call gives the same bits.  Requests of 256 and more query columns (max_q_len
  * tokens x query heads of a kv head) take operands of one 16-bit part: rotated queries and quantised values are rounded
  * to fp16, weights to the values' type (2-norm of the error over TQ4 rows 4.5e-4, over un-rotated 8-bit rows 2.7e-4 into
  * fp16 outputs, whose own rounding is 2.1e-4).  Shorter ones lose nothing but the rounding of the output. */

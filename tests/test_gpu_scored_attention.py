@@ -595,6 +595,15 @@ def test_requests_of_any_number_of_tokens(fmt, dt, tokens):
 
 
 @gpu
+@pytest.mark.parametrize("kv_heads,heads", [(1, 8), (4, 8), (16, 16), (40, 40)])
+@pytest.mark.parametrize("seqs,qs", [([6000], [1]), ([500] * 20, [1] * 20), ([700, 90], [300, 40])])
+def test_kv_heads_share_the_chip(kv_heads, heads, seqs, qs):
+    """The cut of a batch goes by the number of kv heads: from 512 chunks for one of them to 16 for each of 40."""
+    pool, bt, k, v, q, aq, ctx = case(FMT_FP16, 16, seqs, qs, 1220, DT_F16, kv_heads=kv_heads, q_heads=heads, head_dim=128)
+    check_scored(pool, bt, seqs, q, DT_F16, aq, ctx, heads, scratch=64 << 20, cap=30.0)
+
+
+@gpu
 def test_one_long_request_among_many_short_ones():
     """More tiles than a wave has lanes, most of them short: the long one is cut, in both kernels."""
     seqs = [9000] + [40] * 150

@@ -31,6 +31,7 @@ struct ScoredParams {
     int tiles;        // tiles of a request (a bound)
     int entries;      // requests x tiles: tiles of the batch, some of them empty
     int target;       // slots for chunks, for each kv head; 0: no split, a workgroup for each entry
+    int round;        // slots for each kv head that fill the chip
     int full_rounds;  // the cut looks for full rounds of chunks; 0: no more chunks than target
     int records;      // partial records the scratch holds, for each kv head
     int min_halves;   // shortest chunk
@@ -62,7 +63,6 @@ __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const S
         for (int i = 0; i < N; ++i) s[i] = __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(s[i] * cc));
         return ScoreMap{2.0f * P.cap2, P.cap2};
     } else {
-        if (!SERIES) asm volatile("");  // (both ways would be worked out for every score)
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float a = s[i] * cc, u = a * (0.5f / kLog2e), uu = u * u;
@@ -70,7 +70,7 @@ __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const S
             float series = __builtin_fmaf(uu, 62.0f / 2835.0f, -17.0f / 315.0f);
             series = __builtin_fmaf(uu, series, 2.0f / 15.0f);
             series = __builtin_fmaf(uu, series, -1.0f / 3.0f);
-            series = s[i] * cs * __builtin_fmaf(uu, series, 1.0f);
+            series = P.cap2 * u * __builtin_fmaf(uu, series, 1.0f);
             s[i] = fabsf(u) < 0.25f ? series : x;
         }
         return ScoreMap{1.0f, 0.f};
@@ -191,7 +191,6 @@ __device__ __forceinline__ int tile_halves(int first, int last) { return first <
 // Entries of a batch that is cut.  us a call, up to 2 048 / up to 512: one request of 60 000 keys among 600 of 100 94 / 620, among 1 800 306 / 765;
 // 600 requests of 16 to 4 000 keys, which need no cut, 467 / 456.
 constexpr int kMaxSplitEntries = 2048;
-constexpr int kSlotRound = 128;         // slots for each kv head that fill the chip where there are two
 constexpr int kChunkCost = 32;          // what a workgroup takes beside its keys, in half units
 __device__ __forceinline__ int chunks_of(int halves, int per) { return halves < 0 ? 0 : max(1, fast_div(halves + per - 1, per)); }
 template <typename Count>
@@ -217,14 +216,14 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
     if (P.full_rounds == 0) {
         per = (total + limit - 1) / limit;
     } else {
-        const int even = (total + kSlotRound - 1) / kSlotRound;  // what a CU has of it
-        if (live >= kSlotRound) {
+        const int even = (total + P.round - 1) / P.round;  // what a CU has of it
+        if (live >= P.round) {
             per = even + kChunkCost;
-        } else if (fits(even + kChunkCost, min(P.target, kSlotRound))) {
-            limit = min(P.target, kSlotRound);
+        } else if (fits(even + kChunkCost, min(P.target, P.round))) {
+            limit = min(P.target, P.round);
             per = even;
         } else {
-            limit = min(P.target, 2 * kSlotRound);
+            limit = min(P.target, 2 * P.round);
             per = (even + 1) / 2;
         }
     }

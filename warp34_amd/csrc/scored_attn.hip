@@ -29,6 +29,8 @@ constexpr int kSpreadTiles = 12, kSpreadChunkTiles = 8;
 // 16 / 29, 93 / 61; TQ4 39 / 51, 69 / 64, 17 / 45, 106 / 85; Q8_0 29 / 46, 53 / 62, 16 / 40, 77 / 84.
 constexpr int kChunkFrom = 256;
 
+constexpr int kLeastRound = 16;  // slots for each kv head, whatever their number
+
 static int decode_cols(int format) { return format == WARP34_KV_FORMAT_TQ4 ? kTq4Cols : kDecodeCols; }
 
 // The tiles of a batch: the kernel, a tile's tokens, tiles of a request, slots for each kv head (0: no split).
@@ -36,10 +38,10 @@ struct ScoredShape {
     bool chunk;
     int cols, tok_tile;
     long long tiles, entries;
-    int slots;
+    int slots, round;
     bool full_rounds;
 };
-static ScoredShape scored_shape(int format, int num_reqs, int total_tokens, int max_q_len, int q_group) {
+static ScoredShape scored_shape(int format, int head_dim, int kv_subs, int num_reqs, int total_tokens, int max_q_len, int q_group) {
     ScoredShape s;
     const int q_len = max_q_len > 0 ? std::min(max_q_len, total_tokens) : total_tokens;
     s.chunk = (long long)q_len * q_group >= kChunkFrom;
@@ -47,10 +49,13 @@ static ScoredShape scored_shape(int format, int num_reqs, int total_tokens, int 
     s.tok_tile = s.cols / q_group;
     s.tiles = ((long long)q_len + s.tok_tile - 1) / s.tok_tile;
     s.entries = s.tiles * num_reqs;
-    // Decode batches of up to 64 tiles: at most 128 chunks for each kv head, which two kv heads run in one round.  Others: up to two rounds,
-    // or a chunk for each tile and some more.
-    s.full_rounds = s.chunk || s.entries > 64;
-    s.slots = s.entries > kMaxSplitEntries ? 0 : (int)(s.full_rounds ? 2 * kSlotRound + s.entries : kSlotRound);
+    // A round of workgroups: 256, or twice as many of the decode kernel at head_dim 128 (two to a CU).  us a call, 128 slots whatever the kv
+    // heads / so.  One kv head: Q8_0 verify 31.0 / 23.7, 12 requests over TQ4 49.6 / 33.1; four: 8 000 TQ4 keys 22.9 / 14.6, 50 000 36.2 / 24.8,
+    // verify 64 / 59; eight: 8 000 TQ4 keys 38 / 17, prefixes over FP8 1 083 / 982.
+    s.round = std::max(kLeastRound, (!s.chunk && head_dim == 128 ? 512 : 256) / kv_subs);
+    // Decode batches of few tiles: chunks for one round at most.  Others: up to two rounds, or a chunk for each tile and some more.
+    s.full_rounds = s.chunk || s.entries > std::min(64, s.round / 2);
+    s.slots = s.entries > kMaxSplitEntries ? 0 : (int)(s.full_rounds ? 2 * s.round + s.entries : s.round);
     return s;
 }
 // Bytes of the partial records of a slot, and of the tiles' table.
@@ -93,7 +98,7 @@ template <typename TQ, int KVF, int HD>
 static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const warp34_attention_batch& B = P.B;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
-    const ScoredShape s = scored_shape(KVF, B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
+    const ScoredShape s = scored_shape(KVF, HD, kv_subs, B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
     if (kv_subs > 65535 || s.entries * kv_subs > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
     P.tok_tile = s.tok_tile;
     P.tiles = (int)s.tiles;
@@ -111,6 +116,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     }
     P.target = (int)slots;
     P.full_rounds = s.full_rounds ? 1 : 0;
+    P.round = s.round;
     P.records = (int)records;
     if (slots > 0) {
         uint8_t* at = reinterpret_cast<uint8_t*>((uintptr_t)ex->scratch_ptr);
@@ -213,6 +219,7 @@ extern "C" size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_la
     if (!layout || layout->local_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % layout->local_kv_heads != 0 || num_reqs <= 0 || total_tokens <= 0)
         return 0;
     const int gqa = num_q_heads / layout->local_kv_heads, group = scored_q_group(layout->k_format, gqa);
-    const ScoredShape s = scored_shape(layout->k_format, num_reqs, total_tokens, max_q_len, group);
-    return s.slots == 0 ? 0 : scored_table_bytes(s.entries) + (size_t)s.slots * scored_slot_bytes(s, layout->local_kv_heads * (gqa / group), layout->head_dim);
+    const int kv_subs = layout->local_kv_heads * (gqa / group);
+    const ScoredShape s = scored_shape(layout->k_format, layout->head_dim, kv_subs, num_reqs, total_tokens, max_q_len, group);
+    return s.slots == 0 ? 0 : scored_table_bytes(s.entries) + (size_t)s.slots * scored_slot_bytes(s, kv_subs, layout->head_dim);
 }
