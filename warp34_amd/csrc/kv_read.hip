@@ -8,6 +8,7 @@
 // at 91 of them 22 us, with rows apart and a branch each 24); 333 Q8_0 rows 3.7 us, a launch.
 #include "attn_lanes.h"
 #include "kv_encode.h"
+#include "wht_products.h"
 
 namespace w34 {
 
@@ -131,15 +132,6 @@ constexpr int kReadRows = 4;
 typedef u2v u2_at2 __attribute__((aligned(2)));
 typedef u4 u4_at4 __attribute__((aligned(4)));
 
-__device__ __forceinline__ h8 two_parts(const float (&x)[4]) {
-    u4 r;
-    uint32_t hi, lo;
-    split_weights(x[0], x[1], hi, lo);
-    r[0] = hi, r[2] = lo;
-    split_weights(x[2], x[3], hi, lo);
-    r[1] = hi, r[3] = lo;
-    return __builtin_bit_cast(h8, r);
-}
 // Both parts of each centroid times kLutGain.
 struct CentroidParts {
     uint32_t of[16];
@@ -153,13 +145,6 @@ constexpr CentroidParts make_centroid_parts() {
     return t;
 }
 __device__ __constant__ constexpr CentroidParts kCentroidParts = make_centroid_parts();
-// (-1)^popcount((4 b + i) & n) for i = 0 .. 3 as fp16, twice
-__device__ __forceinline__ h8 hadamard_column(int n, int b) {
-    const uint32_t of_b = (uint32_t)(b & (n >> 2)), odd = (of_b ^ of_b >> 1) & 1u;
-    const uint32_t lo = 0x3C003C00u ^ odd * 0x80008000u ^ ((uint32_t)n & 1u) << 31;  // i = 0, 1
-    const uint32_t hi = lo ^ ((uint32_t)n >> 1 & 1u) * 0x80008000u;                  // i = 2, 3
-    return __builtin_bit_cast(h8, u4{lo, hi, lo, hi});
-}
 template <typename TOut>
 __device__ __forceinline__ uint32_t pack_pair(float a, float b) {
     if constexpr (TOut::kStorageFormat == WARP34_KV_FORMAT_BF16) {

@@ -13,7 +13,7 @@
 //
 // Why this shape: 128 sums and 64 query registers a lane are what two waves a SIMD have room for, and each operand read from LDS serves 32
 // columns.  4 requests of 2 048 tokens on 16 384 keys, 16 + 2 heads, capped: BF16 2.36 ms (990 TFLOP/s; a large matrix product of the
-// library 1 390), FP8 2.85, TQ4 3.03 (770), Q8_0 3.27.  What bounds it is a wave's own chain: of 6 700 cycles a TQ4 unit the products of a SIMD's
+// library 1 390), FP8 2.85, TQ4 3.01 (780), Q8_0 3.27.  What bounds it is a wave's own chain: of 6 700 cycles a TQ4 unit the products of a SIMD's
 // two waves take 2 050, vector work 55 % of the cycles (a cap's exponential and reciprocal, the weights' exponentials and the widening most of
 // it), LDS 32 %, and a wave waits 38 %.  Left out for timing: cap and exponentials -7 %, widening -14 %, operand reads -15 %, all three -36 %;
 // the rows' pages made no difference.  Two sums side by side for the scores need 16 registers more than there are (packed documents 107 ->
@@ -22,6 +22,7 @@
 #pragma once
 
 #include "scored_decode.h"
+#include "wht_products.h"
 
 namespace w34 {
 
@@ -234,6 +235,15 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     if (units > 0) issue(0, v_now);
     if (!R::k16 && units > 1) issue(1, 0u);
 
+    // where the rotations of queries and of results have a lane's four elements, their signs as bits of 16-bit numbers, and the matrix
+    const auto rotation = [&](int& piece, uint2& piece_flip, u4& had) {
+        const int at_lane = here(lane), r = at_lane & 15, c = at_lane >> 4;
+        piece = 16 * r + 4 * c;
+        const uint32_t signs = kSignMask[piece >> 5] >> (piece & 31);
+        piece_flip = uint2{(signs << 15 & 0x8000u) | (signs << 30 & 0x80000000u), (signs << 13 & 0x8000u) | (signs << 28 & 0x80000000u)};
+        had = __builtin_bit_cast(u4, hadamard_column(r, c));
+    };
+
     // ---- table and query operands: lane (n, b) holds Q[column n][16 m + 8 b .. + 7] ----
     if constexpr (R::kTq4) build_narrow_table(smem, tid, wave);
     u4 q[kSteps];
@@ -275,7 +285,13 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         cs *= mine;
         cc *= mine;
     } else {
-        // Rotated, eight columns of the wave at a time through LDS, their loads together and those of the next eight ahead.
+        // Rotated by two products a column (wht_products.h; in vector instructions, as the results' rotation back, 8 requests of 400 to 600 TQ4
+        // tokens in windows of 64 took 98.9 instead of 81.5 us), eight columns of the wave at a time through LDS, their loads together and those of
+        // the next eight ahead.  Elements go in relative to a power of two above the column's largest, as fp16 holds them.
+        int piece;
+        uint2 piece_flip;
+        u4 had;
+        rotation(piece, piece_flip, had);
         uint16_t* area = reinterpret_cast<uint16_t*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
         float* scales = reinterpret_cast<float*>(smem + M::kQScale) + 32 * wave;
         uint2 raw[8];
@@ -285,7 +301,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                 const int c = 8 * g + c8, ct = column_token(32 * wave + c, P);
                 raw[c8] = uint2{0u, 0u};
                 if ((live >> c) & 1u)
-                    raw[c8] = *reinterpret_cast<const uint2*>(P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + 4 * lane);
+                    raw[c8] = *reinterpret_cast<const uint2*>(P.q + ((size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group)) * HD + piece);
             }
         };
         load_columns(0);
@@ -293,20 +309,22 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         for (int g = 0; g < 4; ++g) {
             uint2 now[8];
 #pragma unroll
-            for (int c8 = 0; c8 < 8; ++c8) now[c8] = uint2{raw[c8].x ^ P.q_flip, raw[c8].y ^ P.q_flip};
+            for (int c8 = 0; c8 < 8; ++c8) now[c8] = uint2{raw[c8].x ^ P.q_flip ^ piece_flip.x, raw[c8].y ^ P.q_flip ^ piece_flip.y};
             if (g < 3) load_columns(g + 1);
 #pragma unroll
             for (int c8 = 0; c8 < 8; ++c8) {
-                float v[4] = {TQ::to_f32((uint16_t)now[c8].x), TQ::to_f32((uint16_t)(now[c8].x >> 16)), TQ::to_f32((uint16_t)now[c8].y), TQ::to_f32((uint16_t)(now[c8].y >> 16))};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = apply_sign(v[k], 4 * lane + k);
-                wht256_wave(v, lane);
-                const float top = wave_top(fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3]))));
+                const uint32_t two = max_u16x2(now[c8].x & 0x7FFF7FFFu, now[c8].y & 0x7FFF7FFFu);
+                const float top = TQ::to_f32((uint16_t)wave_largest((int)max(two & 0xFFFFu, two >> 16)));
                 const int e = top > 0.f && top < INFINITY ? max(__builtin_amdgcn_frexp_expf(top), -100) : 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = __builtin_amdgcn_ldexpf(v[k], -e);
-                *reinterpret_cast<uint2*>(area + c8 * M::kColStride + 4 * lane) = uint2{pack_h2(v[0], v[1]), pack_h2(v[2], v[3])};
-                if (lane == 0) scales[8 * g + c8] = __builtin_amdgcn_ldexpf(R::kOutScale, e);
+                const auto in = [&](uint32_t w) {
+                    return pack_h2(__builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)w), -e), __builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)(w >> 16)), -e));
+                };
+                const f4 none = {0.f, 0.f, 0.f, 0.f};
+                const f4 z = mfma_rows<false>(u4{in(now[c8].x), in(now[c8].y), 0u, 0u}, had, none);
+                const float zs[4] = {z[0], z[1], z[2], z[3]};
+                const f4 y = mfma_rows<false>(__builtin_bit_cast(u4, two_parts(zs)), had, none);
+                *reinterpret_cast<uint2*>(area + c8 * M::kColStride + piece) = uint2{pack_h2(y[0], y[1]), pack_h2(y[2], y[3])};
+                if (lane == 0) scales[8 * g + c8] = __builtin_amdgcn_ldexpf(R::kOutScale, e - 4);
             }
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
             __builtin_amdgcn_wave_barrier();
@@ -650,7 +668,11 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         }
         return;
     }
-    // rotated back, eight columns of a wave at a time through LDS
+    // rotated back by two products a column, eight columns of a wave at a time through LDS
+    int piece;
+    uint2 piece_flip;
+    u4 had;
+    rotation(piece, piece_flip, had);
     float* area = reinterpret_cast<float*>(smem + M::kTiles + wave * 8 * M::kColStride * 4);
 #pragma unroll 1
     for (int g = 0; g < 4; ++g) {
@@ -668,12 +690,25 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         for (int c8 = 0; c8 < 8; ++c8) {
             const int c = 8 * g + c8;
             if (!((live >> c) & 1u)) continue;
-            const f4 acc = *reinterpret_cast<const f4*>(area + c8 * M::kColStride + 4 * lane);
+            const f4 acc = *reinterpret_cast<const f4*>(area + c8 * M::kColStride + piece);
             const float m_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(m_run), c));
             const float l_c = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_run), c));
-            float v[4] = {acc[0], acc[1], acc[2], acc[3]};
             const int ct = column_token(32 * wave + c, P);
-            finish_row<TQ, HD>(P, t.tok0 + ct, head0 + 32 * wave + c - ct * P.q_group, lane, v, m_c, l_c, R::kOutScale);
+            const size_t row = (size_t)(t.tok0 + ct) * P.num_q_heads + (size_t)(head0 + 32 * wave + c - ct * P.q_group);
+            const bool some = l_c > 0.f || l_c != l_c;
+            const float inv = some ? R::kOutScale / l_c : 0.f;  // (a row without keys: zeros)
+            float v[4] = {acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm("" : "+v"(v[k]));  // both parts are taken from the product rounded to 32 bits
+            const f4 none = {0.f, 0.f, 0.f, 0.f};
+            const f4 z = mfma_rows<false>(__builtin_bit_cast(u4, two_parts(v)), had, none);
+            float zs[4] = {z[0] * 0.0625f, z[1] * 0.0625f, z[2] * 0.0625f, z[3] * 0.0625f};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) asm("" : "+v"(zs[k]));
+            const f4 y = mfma_rows<false>(__builtin_bit_cast(u4, two_parts(zs)), had, none);
+            const auto pack = [](float x0, float x1) { return TQ::kStorageFormat == WARP34_KV_FORMAT_BF16 ? pack_bf2(x0, x1) : pack_h2(x0, x1); };
+            *reinterpret_cast<uint2*>(P.out + row * HD + piece) = uint2{pack(y[0], y[1]) ^ piece_flip.x, pack(y[2], y[3]) ^ piece_flip.y};
+            if (P.lse != nullptr && lane == 0) P.lse[row] = some ? (m_c + __builtin_amdgcn_logf(l_c)) * 0.6931471805599453f : -INFINITY;
         }
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         __builtin_amdgcn_wave_barrier();
