@@ -231,7 +231,7 @@ __device__ __forceinline__ int chunk_length(const ScoredParams& P, int lane, Cou
     if (P.entries == 1 ? chunks_of(total, per) <= P.records : fits(per, limit)) return per;
     // sum of ceil(h / per) <= total / per + live, so this many halves a chunk are enough for any number of slots above live
     int low = per, high = max(per + 1, (total + max(limit - live, 1) - 1) / max(limit - live, 1));
-    while (!fits(high, limit)) {
+    while (high < 1 << 27 && !fits(high, limit)) {  // (a tile has no more half units than that)
         low = high;
         high *= 2;
     }

@@ -10,7 +10,7 @@
 // (As the 16-column kernel with the parts in products of their own, 16 keys at a time: 300 vector instructions and 40 products for what
 // takes 170 and 24 here, 209 us for 32 requests of 1k to 64k keys.)  Now 147 to 156 us, 3.9 to 4.1 TB/s: vector work 53 % of the SIMD cycles, products
 // 18 %, look-ups 40 % of the LDS cycles and a wave waits a third; waves a barrier apart at most 165 to 203 us, so what overlaps is waves out of
-// step.  One request of 131 072 keys 28.5 us: 12.5 stream 69 MB at 5.5 TB/s, 5.6 pass before (lengths 1.6, pages and first rows 3.6), the waves' join
+// step.  One request of 131 072 keys, capped, 29.2 us: 12.5 stream 69 MB at 5.5 TB/s, 5.6 pass before (lengths 1.6, pages and first rows 3.6), the waves' join
 // takes 3, the join's launch 5 to 6.
 #pragma once
 
