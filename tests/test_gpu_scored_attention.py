@@ -470,6 +470,24 @@ def test_f16_entry_takes_fp16_pages_and_bf16_entry_bf16_pages():
     assert _call("warp34_paged_attention_scored_bf16", layout_over=dict(sixteen, k_format=FMT_FP16, v_format=FMT_FP16)) == 801
 
 
+def test_descriptor_has_the_size_that_the_header_states():
+    from warp34_amd import ffi
+
+    assert C.sizeof(ffi.Warp34AttentionScores) == 40
+
+
+@pytest.mark.parametrize("kv_heads,heads", [(1, 8), (2, 16), (4, 32), (40, 40)])
+@pytest.mark.parametrize("fmt", [FMT_TQ4, FMT_FP8])
+def test_scratch_grows_with_the_batch_and_ends_where_nothing_is_cut(fmt, kv_heads, heads):
+    from warp34_amd import ffi
+
+    layout = ffi.Warp34KvLayerLayout(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, kv_heads, 256, 16, fmt, fmt, 1, 1, 0)
+    size = ffi.load().warp34_paged_attention_scored_scratch_bytes
+    sizes = [size(C.byref(layout), n, n, 1, heads) for n in (100, 300, 1000, 2000)]
+    assert sizes == sorted(sizes) and sizes[0] > 0
+    assert size(C.byref(layout), 2100, 2100, 1, heads) == 0
+
+
 def test_scratch_query():
     from warp34_amd import ffi
 
