@@ -191,7 +191,7 @@ struct PageWalk {
         blocks = P.B.block_tables + (size_t)t.req * P.B.max_blocks_per_req;
         fetch(P, page_slot(half * 16, P), lane);
     }
-    // rows of a half unit; half units in order
+    // rows of a half unit; half units in order: none from a page in front of the last one's, whose entries may be gone
     __device__ __forceinline__ void locate(const ScoredParams& P, int half, int row_bytes, int lane, const slab_byte*& k_rows, const slab_byte*& v_rows) {
         const int pos = half * 16, slot = page_slot(pos, P);
         if (slot - slot_base >= 64) {  // uniform

@@ -219,7 +219,9 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
                 s[h][i] = mine + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(mine), 0x128, 0xF, 0xF, false));  // row_ror:8
             }
         }
-        locate(more ? next : half);  // (rows of this unit again at the end: a load under a condition would be waited for at once)
+        // (behind the last unit the rows stay where they are and are loaded again: a load under a condition would be waited for at once.  The walk
+        // cannot be asked for them a second time: the page of the first half unit may lie in front of the entries that it holds by then)
+        if (more) locate(next);
         load_keys();
 
         // ---- terms, masks, softmax ----
