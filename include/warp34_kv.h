@@ -325,7 +325,8 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  * warp34_attention_merge_* joins such results by.  Layouts, batches, q_in / attn_out, masked tokens and requests
  * (their lse_out stays untouched as well) and alignments are those of warp34_paged_attention_*.  Key and value
  * rows that a token sees must be finite, and what their decoded values are must fit fp16 for the quantised formats;
- * rows that no token of the request sees may hold anything.  softcap must be finite and not negative
+ * rows that no token of the request sees may hold anything (a masked token sees none, and its own row, which the
+ * append leaves out, counts for those that do).  softcap must be finite and not negative
  * (hipErrorInvalidValue).  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
  * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass.  Two calls that may run
  * at once need a workspace each.

@@ -145,10 +145,12 @@ __device__ __forceinline__ float wave_total(float v) {
     return __int_as_float(__builtin_amdgcn_readlane(wave_scan(__float_as_int(v), 0, f), 63));
 }
 
-// First and last key that any token of a tile sees; first > last where none does.  A lane a token.
+// First and last key that any live token of a tile sees; first > last where none does.  (The append writes no rows of masked tokens: what
+// lies there is not to count as a row of the tile.)  A lane a token.
 __device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int lane, int& first, int& last) {
+    const uint8_t* token_mask = P.B.valid_token_mask;
     int lo, hi;
-    if (P.document_starts == nullptr && P.prefix_ends == nullptr) {  // the first token's window, the last one's reach
+    if (P.document_starts == nullptr && P.prefix_ends == nullptr && token_mask == nullptr) {  // the first token's window, the last one's reach
         token_keys(P, t.tok0, t.pos0, t.seq_after, first, hi);
         token_keys(P, t.tok0, t.pos0 + t.tokens - 1, t.seq_after, lo, last);
     } else {
@@ -156,7 +158,7 @@ __device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTil
         last = -1;
         for (int k = lane; k < t.tokens; k += 64) {
             token_keys(P, t.tok0 + k, t.pos0 + k, t.seq_after, lo, hi);
-            if (lo <= hi) {
+            if (lo <= hi && (token_mask == nullptr || token_mask[t.tok0 + k] != 0)) {
                 first = min(first, lo);
                 last = max(last, hi);
             }
