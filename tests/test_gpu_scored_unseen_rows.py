@@ -63,3 +63,33 @@ def test_masked_tokens_at_the_end_and_at_the_start(fmt, xf, dt, hd, tokens, seq)
     n = tokens // 2
     check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, n, tokens))
     check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, 0, n), window=4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scratch", [0, 8 << 20])
+@pytest.mark.parametrize("fmt,xf,dt,hd", FORMS)
+@pytest.mark.parametrize("tokens,seq", [(20, 309), (100, 409)])
+def test_rows_between_the_keys_of_two_tokens(fmt, xf, dt, hd, tokens, seq, scratch):
+    a, b = tokens // 4, 3 * tokens // 4
+    # masked tokens in the middle of a window's slide
+    check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, a, b), window=3, scratch=scratch)
+    # tokens whose document starts nowhere, in the same place
+    documents = np.zeros(tokens, dtype=np.int32)
+    documents[a:b] = NOWHERE
+    check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, 0, 0), window=2, documents=documents, scratch=scratch)
+    # a packed document that is masked as a whole
+    documents = seq - tokens + np.where(np.arange(tokens) < a, 0, np.where(np.arange(tokens) < b, a, b)).astype(np.int32)
+    check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, a, b), documents=documents, scratch=scratch)
+    # tokens that see a part of a prefix far behind them only
+    documents, prefixes = np.zeros(tokens, dtype=np.int32), np.zeros(tokens, dtype=np.int32)
+    documents[::3], prefixes[::3] = seq - 50, seq - 20
+    check(fmt, xf, dt, hd, seq, tokens, all_but(tokens, 0, 0), ctx=100, documents=documents, prefixes=prefixes, scratch=scratch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,xf,dt,hd", [FORMS[0], FORMS[2], FORMS[5], FORMS[6]])
+def test_gaps_in_tiles_of_many_tokens(fmt, xf, dt, hd):
+    """One query head for each kv head: 256 tokens in a tile, gaps of many sizes."""
+    live = np.random.default_rng(8).random(300) < 0.05
+    check(fmt, xf, dt, hd, 700, 300, live, window=7, heads=2)
+    check(fmt, xf, dt, hd, 700, 300, live, window=2, heads=2, block=48)

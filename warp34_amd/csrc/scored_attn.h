@@ -146,25 +146,38 @@ __device__ __forceinline__ float wave_total(float v) {
 }
 
 // First and last key that any live token of a tile sees; first > last where none does.  (The append writes no rows of masked tokens: what
-// lies there is not to count as a row of the tile.)  A lane a token.
-__device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int lane, int& first, int& last) {
+// lies there is not to count as a row of the tile.)  A lane a token.  GAPS: *gaps is false where every key in between is seen too, as far as
+// the tokens in their order tell: each one's keys touch the span of those before it.
+template <bool GAPS = false>
+__device__ __forceinline__ void tile_keys(const ScoredParams& P, const ScoredTile& t, int lane, int& first, int& last, bool* gaps = nullptr) {
     const uint8_t* token_mask = P.B.valid_token_mask;
     int lo, hi;
+    if constexpr (GAPS) *gaps = false;
     if (P.document_starts == nullptr && P.prefix_ends == nullptr && token_mask == nullptr) {  // the first token's window, the last one's reach
         token_keys(P, t.tok0, t.pos0, t.seq_after, first, hi);
         token_keys(P, t.tok0, t.pos0 + t.tokens - 1, t.seq_after, lo, last);
     } else {
+        const auto least = [](int a, int b) { return min(a, b); };
+        const auto most = [](int a, int b) { return max(a, b); };
         first = 0x7fffffff;
         last = -1;
-        for (int k = lane; k < t.tokens; k += 64) {
-            token_keys(P, t.tok0 + k, t.pos0 + k, t.seq_after, lo, hi);
-            if (lo <= hi && (token_mask == nullptr || token_mask[t.tok0 + k] != 0)) {
-                first = min(first, lo);
-                last = max(last, hi);
+        for (int base = 0; base < t.tokens; base += 64) {
+            const int k = base + lane;
+            int from = 0x7fffffff, to = -1;
+            if (k < t.tokens && (token_mask == nullptr || token_mask[t.tok0 + k] != 0)) {
+                token_keys(P, t.tok0 + k, t.pos0 + k, t.seq_after, lo, hi);
+                if (lo <= hi) from = lo, to = hi;
             }
+            const int from_upto = wave_scan(from, 0x7fffffff, least), to_upto = wave_scan(to, -1, most);
+            if constexpr (GAPS) {
+                int from_before = __shfl_up(from_upto, 1, 64), to_before = __shfl_up(to_upto, 1, 64);
+                from_before = min(lane > 0 ? from_before : 0x7fffffff, first);
+                to_before = max(lane > 0 ? to_before : -1, last);
+                if (__ballot(from <= to && to_before >= 0 && (from > to_before + 1 || to < from_before - 1)) != 0ull) *gaps = true;
+            }
+            first = min(first, __builtin_amdgcn_readlane(from_upto, 63));
+            last = max(last, __builtin_amdgcn_readlane(to_upto, 63));
         }
-        first = wave_least(first);
-        last = wave_largest(last);
     }
     first = __builtin_amdgcn_readfirstlane(first);
     last = __builtin_amdgcn_readfirstlane(last);

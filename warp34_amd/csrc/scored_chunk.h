@@ -93,7 +93,8 @@ struct ChunkLds {
     static constexpr int kQScale = kCounts + kMaxSplitEntries * 4;
     static constexpr int kHist = kQScale + kChunkCols * 4;
     static constexpr int kEnds = kHist + 64 * 4;
-    static constexpr int kBytes = kLoop > kEnds ? kLoop : kEnds;
+    static constexpr int kRanges = kLoop > kEnds ? kLoop : kEnds;  // first and last key of each token, where a tile has gaps
+    static constexpr int kBytes = kRanges + kChunkCols * 8;
     static_assert(kBytes <= 160 * 1024 && kRun % 16 == 0, "chunk LDS budget");
 };
 
@@ -153,7 +154,8 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     const ScoredTile t = scored_tile(P, work.entry);
     if (t.tokens <= 0) return;
     int key_first, key_last;
-    tile_keys(P, t, lane, key_first, key_last);
+    bool gaps;  // rows in between may be seen by no token
+    tile_keys<true>(P, t, lane, key_first, key_last, &gaps);
     const int all_halves = tile_halves(key_first, key_last);
     const int per = (fast_div(all_halves + work.chunks - 1, work.chunks) + 1) & ~1;  // whole units
     const int begin = ((key_first >> 4) + work.chunk * per) * 16;  // keys
@@ -339,6 +341,11 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         }
         cs *= scales[n];
         cc *= scales[n];
+    }
+    if (gaps && tid < t.tokens) {
+        int from = 0, to = -1;
+        if (B.valid_token_mask == nullptr || B.valid_token_mask[t.tok0 + tid] != 0) token_keys(P, t.tok0 + tid, t.pos0 + tid, t.seq_after, from, to);
+        *reinterpret_cast<u2v*>(smem + M::kRanges + 8 * tid) = u2v{(uint32_t)from, (uint32_t)to};
     }
     __syncthreads();  // the areas become tiles
 
@@ -589,19 +596,27 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             o[i >> 1] = mfma_tile<IS_BF16>(a[i % (kValuesAhead + 1)], w[i & 1], o[i >> 1]);
         }
     };
-    // 16-bit value rows that no token of the tile sees count as zeros: a page's rest may hold anything
+    // Value rows that no token of the tile sees count as zeros: they may hold anything.  Quantised ones in front of the first key and behind
+    // the last come as zeros out of the widening.  Where there are gaps 16 lanes share a row, and look at the tokens' ranges in turn.
     const auto clear_unseen = [&](int u, uint32_t values) {
-        if constexpr (R::k16) {
-            const int u0 = begin + u * kChunkUnit;
-            if (u0 >= key_first && u0 + kChunkUnit - 1 <= key_last) return;  // uniform
-            constexpr int kPieces = M::kTile / 16;
-            for (int p = tid; p < kPieces; p += kChunkWaves * 64) {
-                const int pos = u0 + p / (M::kRow / 16);
-                if (pos < key_first || pos > key_last)
-                    lds_put(values + (uint32_t)(16 * p), u4{0u, 0u, 0u, 0u});
+        const int u0 = begin + u * kChunkUnit;
+        if (!gaps && (!R::k16 || (u0 >= key_first && u0 + kChunkUnit - 1 <= key_last))) return;  // uniform
+        constexpr int kPieces = M::kTile / 16;
+        static_assert(kPieces % (kChunkWaves * 64) == 0 && (M::kRow / 16) % 16 == 0, "all lanes take part, 16 to a row");
+        for (int p = here(tid); p < kPieces; p += kChunkWaves * 64) {
+            const int pos = u0 + p / (M::kRow / 16);
+            bool seen = pos >= key_first && pos <= key_last;
+            if (gaps) {
+                int some = 0;
+                for (int k = p & 15; k < t.tokens; k += 16) {
+                    const u2v range = lds_u2((uint32_t)(M::kRanges + 8 * k));
+                    some |= pos >= (int)range[0] && pos <= (int)range[1] ? 1 : 0;
+                }
+                seen = row_reduce(some, [](int x, int y) { return x | y; }) != 0;
             }
-            chunk_barrier();
+            if (!seen) lds_put(values + (uint32_t)(16 * p), u4{0u, 0u, 0u, 0u});
         }
+        chunk_barrier();
     };
 
     // Waves w and w + 4 share a SIMD.  The second of them multiplies the values of a unit in the next interval, before its scores, so that
@@ -616,10 +631,10 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
         chunk_barrier();  // unit u's tiles are whole, the next one's rows have landed; nobody reads what is overwritten below
         if constexpr (R::k16) {
             if (u + 1 < units) issue(u + 1, v_next);
-            clear_unseen(u, v_now);
         } else {
             if (u + 2 < units) issue(u + 2, 0u);
         }
+        clear_unseen(u, v_now);
         __builtin_amdgcn_sched_barrier(0);
         // (behind the last unit: old rows, to tiles that nobody reads)
         if (late) add_values(v_last, std::integral_constant<bool, !R::k16>{}, u + 1, v_next);

@@ -48,7 +48,7 @@ __device__ __forceinline__ uint32_t pack_bf2(float x, float y) {
 struct DecodeStart {
     ScoredWork work;
     ScoredTile t;
-    int key_first, key_last, begin, end;
+    int begin, end;
 };
 template <bool PAIRS>
 __device__ __forceinline__ bool decode_start(const ScoredParams& P, uint8_t* counts, int tid, int lane, int kv_sub, DecodeStart& s) {
@@ -77,16 +77,17 @@ __device__ __forceinline__ bool decode_start(const ScoredParams& P, uint8_t* cou
         s.t = scored_tile(P, s.work.entry);
         if (s.t.tokens <= 0) return false;
     }
-    tile_keys(P, s.t, lane, s.key_first, s.key_last);
+    int key_first, key_last;
+    tile_keys(P, s.t, lane, key_first, key_last);
     if (s.work.chunk == 0 && kv_sub == 0 && tid == 0 && P.target > 0) {
         P.table[2 * s.work.entry] = s.work.first_record;
         P.table[2 * s.work.entry + 1] = s.work.chunks;
     }
-    const int halves = tile_halves(s.key_first, s.key_last);
+    const int halves = tile_halves(key_first, key_last);
     int per = fast_div(halves + s.work.chunks - 1, s.work.chunks);
     if (PAIRS) per = (per + 1) & ~1;
-    s.begin = (s.key_first >> 4) + s.work.chunk * per;
-    s.end = s.key_first > s.key_last ? s.begin : max(s.begin, min(s.begin + per, (s.key_last >> 4) + 1));
+    s.begin = (key_first >> 4) + s.work.chunk * per;
+    s.end = key_first > key_last ? s.begin : max(s.begin, min(s.begin + per, (key_last >> 4) + 1));
     return true;
 }
 
@@ -98,6 +99,9 @@ __device__ __forceinline__ int row_reduce(int v, F&& f) {
     v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, false));  // row_half_mirror
     return f(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, false));  // row_mirror
 }
+// Whether any of the 16 lanes of the lane's row has it.
+__device__ __forceinline__ bool any_of_row(bool mine, int b) { return ((uint32_t)(__ballot(mine) >> (16 * b)) & 0xFFFFu) != 0u; }
+
 // A lane's column: its token's keys [lo, hi], position and slope; of the tile: the keys that every live column sees, the live columns.
 struct DecodeColumn {
     int tok, head, pos, lo, hi;
@@ -306,7 +310,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
 
     DecodeStart s0;
     if (!decode_start<false>(P, smem, tid, lane, kv_sub, s0)) return;
-    const int key_first = s0.key_first, key_last = s0.key_last, end = s0.end;
+    const int end = s0.end;
     PageWalk walk;
     walk.start(P, s0.t, kv_head, s0.begin, lane);
     const DecodeColumn col = decode_column(P, s0.t, head0, n);
@@ -495,11 +499,11 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
         }
 
         // ---- values ----
-        // rows that no token of the tile sees count as zeros: a page's rest may hold anything
+        // rows that no live column sees count as zeros: they may hold anything
         bool row_ok[4] = {true, true, true, true};
         if (masked) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) row_ok[i] = pos + i >= key_first && pos + i <= key_last;
+            for (int i = 0; i < 4; ++i) row_ok[i] = any_of_row(pos + i >= col.lo && pos + i <= col.hi, b);
         }
         u4 w;
         if constexpr (R::k16) {

@@ -101,7 +101,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
     entries.load(tid);
     DecodeStart s0;
     if (!decode_start<true>(P, smem, tid, lane, kv_sub, s0)) return;
-    const int key_first = s0.key_first, key_last = s0.key_last, end = s0.end;
+    const int end = s0.end;
     PageWalk walk;
     walk.start(P, s0.t, kv_head, s0.begin, lane);
 
@@ -274,9 +274,9 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 f4 d = *reinterpret_cast<const f4*>(v_area + 32 * h + 16 * blk + 4 * b);
-                if (masked) {  // rows that no token of the tile sees count as zeros: a page's rest may hold anything
+                if (masked) {  // rows that no live column sees count as zeros: they may hold anything
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) d[i] = at(4 * h + i) >= key_first && at(4 * h + i) <= key_last ? d[i] : 0.f;
+                    for (int i = 0; i < 4; ++i) d[i] = any_of_row(at(4 * h + i) >= col.lo && at(4 * h + i) <= col.hi, b) ? d[i] : 0.f;
                 }
                 float pd[4];
 #pragma unroll
