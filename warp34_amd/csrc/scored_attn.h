@@ -21,7 +21,7 @@ struct ScoredParams {
     const int32_t* document_starts;
     const int32_t* prefix_ends;
     float* lse;
-    float scale2;     // |sm_scale| log2e, not 0 (hidden keys have scores of minus infinity)
+    float scale2;     // |sm_scale| log2e
     uint32_t q_flip;  // sm_scale < 0: the sign bits of a pair of query elements
     float cap2;       // cap log2e; 0: no cap
     float cap_arg;    // 2 |sm_scale| log2e / cap: exp2 of it times q.k is exp(2 x / cap)
@@ -49,11 +49,17 @@ constexpr float kWideCap = 512.0f;
 
 // Scores s (q . k times what the column's scale is in) become y with x = y ca + cb in the log2 domain, ca >= 0, so that the largest y is
 // the largest x and exp2's argument x - m is one fma.  No cap: y = s, x = y cs.  Cap without the series: y = -1 / (exp(2 x / cap) + 1),
-// x = cap2 + 2 cap2 y.  cs >= 0 and cc: the column's scale times scale2 / cap_arg.
+// x = cap2 + 2 cap2 y.  cs > 0 and cc: the column's scale times scale2 / cap_arg.
 // The series stands for |u| < 1/4, where what follows its last term is below 2^-26 of it.
 struct ScoreMap {
     float ca, cb;
 };
+// cs.  Not 0, where the scale is or where it leaves 32 bits together with a small query's: hidden keys have scores of minus infinity, which
+// would become NaN.  (1e-37 of a score is nothing beside the others.)
+__device__ __forceinline__ float score_factor(const ScoredParams& P, float column_scale) {
+    const float f = P.scale2 * column_scale;
+    return f < 1.0e-37f ? 1.0e-37f : f;
+}
 template <bool CAP, bool SERIES, int N, typename V>
 __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const ScoredParams& P) {
     if constexpr (!CAP) {

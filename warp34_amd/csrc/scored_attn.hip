@@ -180,7 +180,7 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.document_starts = scores->document_starts;
     P.prefix_ends = scores->prefix_ends;
     P.lse = scores->lse_out;
-    P.scale2 = std::max(std::fabs(batch->sm_scale), 1.0e-30f) * kLog2e;
+    P.scale2 = std::fabs(batch->sm_scale) * kLog2e;
     P.q_flip = batch->sm_scale < 0.f ? 0x80008000u : 0u;
     P.cap2 = scores->softcap * kLog2e;
     // (finite, so that a score of 0 stays 0 under the smallest of caps)

@@ -249,7 +249,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
     // ---- table and query operands: lane (n, b) holds Q[column n][16 m + 8 b .. + 7] ----
     if constexpr (R::kTq4) build_narrow_table(smem, tid, wave);
     u4 q[kSteps];
-    float cs = P.scale2, cc = P.cap_arg;
+    float cs = score_factor(P, 1.0f), cc = P.cap_arg;
     if constexpr (R::k16) {
         const uint16_t* src = P.q + ((size_t)my_tok * P.num_q_heads + (size_t)my_head) * HD + 8 * b;
 #pragma unroll
@@ -284,7 +284,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
                 q[m][k] = pack_h2(__builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)w), -e), __builtin_amdgcn_ldexpf(TQ::to_f32((uint16_t)(w >> 16)), -e));
             }
         const float mine = __builtin_amdgcn_ldexpf(R::kOutScale, e);
-        cs *= mine;
+        cs = score_factor(P, mine);
         cc *= mine;
     } else {
         // Rotated by two products a column (wht_products.h; in vector instructions, as the results' rotation back, 8 requests of 400 to 600 TQ4
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             __builtin_amdgcn_wave_barrier();
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
         }
-        cs *= scales[n];
+        cs = score_factor(P, scales[n]);
         cc *= scales[n];
     }
     if (gaps && tid < t.tokens) {

@@ -379,7 +379,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
     }
 
     // ---- query operands ----
-    float cs = P.scale2, cc = P.cap_arg;
+    float cs = score_factor(P, 1.0f), cc = P.cap_arg;
     uint16_t* qh = reinterpret_cast<uint16_t*>(smem + M::kQ);
     uint16_t* ql = reinterpret_cast<uint16_t*>(smem + M::kQLow);
     if constexpr (R::k16) {
@@ -397,7 +397,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
             q_high[m] = *reinterpret_cast<const u4*>(qh + n * M::kQStride + R::element(m, b));
             q_low[m] = *reinterpret_cast<const u4*>(ql + n * M::kQStride + R::element(m, b));
         }
-        cs *= qs[n];
+        cs = score_factor(P, qs[n]);
         cc *= qs[n];
     }
     const bool two_parts = !R::k16 && P.rot_q != 0;
