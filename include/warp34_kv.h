@@ -327,7 +327,7 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  * rows that a token sees must be finite, and what their decoded values are must fit fp16 for the quantised formats;
  * rows that no token of the request sees may hold anything (a masked token sees none, and its own row, which the
  * append leaves out, counts for those that do).  softcap must be finite and not negative
- * (hipErrorInvalidValue).  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
+ * (hipErrorInvalidValue); above 1e30 it counts as 1e30.  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
  * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass.  Two calls that may run
  * at once need a workspace each.
  * The order of summation depends on the lengths, the heads, num_reqs, max_q_len, whether max_seq_len is at most 256, and

@@ -23,3 +23,17 @@ def test_scores_that_are_all_zero(fmt, xf, tokens, scale, size):
     hb = oracle.HostBatch(aq, [150], bt, context_lens_before=ctx)
     hb.sm_scale = scale
     check_scored(pool, bt, [150], q, DT_BF16, aq, ctx, 8, hb=hb, window=100)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,xf", FORMS)
+@pytest.mark.parametrize("tokens", [2, 70])
+@pytest.mark.parametrize("cap", [1e30, 1e34, 1e36, 1.5e38, 3.4e38])
+def test_caps_beyond_every_score_change_nothing(fmt, xf, tokens, cap):
+    pool, bt, k, v, q, aq, ctx = make_case(fmt, 16, [200], [tokens], 1501, DT_BF16, xf=xf)
+    hb = oracle.HostBatch(aq, [200], bt, context_lens_before=ctx)
+    bits, lse = run_scored(pool, hb, q, DT_BF16, 8, cap=cap)
+    want, want_lse, bound, lse_bound = scored_attention(pool, bt, [200], oracle.bits_to_f32(q, DT_BF16).astype(np.float64), aq, ctx,
+                                                        scale=hb.sm_scale, dt=DT_BF16, chunk=tokens * 4 >= CHUNK_FROM)
+    got = oracle.bits_to_f32(bits, DT_BF16).astype(np.float64)
+    assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()

@@ -46,6 +46,9 @@ struct ScoredParams {
 // this one.  Where few keys make a row that shows in its lse: the decode kernels take small arguments through the series, and so does
 // the chunk kernel, whose queries are rounded to more than that, beyond this cap.
 constexpr float kWideCap = 512.0f;
+// Larger caps count as this one: no score comes near it (kNegBig is none), and twice the cap and its reciprocal, which the scales of queries
+// multiply, stay numbers of 32 bits.
+constexpr float kLargestCap = 1.0e30f;
 
 // Scores s (q . k times what the column's scale is in) become y with x = y ca + cb in the log2 domain, ca >= 0, so that the largest y is
 // the largest x and exp2's argument x - m is one fma.  No cap: y = s, x = y cs.  Cap without the series: y = -1 / (exp(2 x / cap) + 1),

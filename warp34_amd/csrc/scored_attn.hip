@@ -182,10 +182,11 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.lse = scores->lse_out;
     P.scale2 = std::fabs(batch->sm_scale) * kLog2e;
     P.q_flip = batch->sm_scale < 0.f ? 0x80008000u : 0u;
-    P.cap2 = scores->softcap * kLog2e;
+    const float cap = std::min(scores->softcap, kLargestCap);
+    P.cap2 = cap * kLog2e;
     // (finite, so that a score of 0 stays 0 under the smallest of caps)
-    P.cap_arg = scores->softcap > 0.f ? std::min(2.0f * std::fabs(batch->sm_scale) * kLog2e / scores->softcap, 1.0e30f) : 0.f;
-    P.wide_cap = scores->softcap > kWideCap ? 1 : 0;
+    P.cap_arg = cap > 0.f ? std::min(2.0f * std::fabs(batch->sm_scale) * kLog2e / cap, 1.0e30f) : 0.f;
+    P.wide_cap = cap > kWideCap ? 1 : 0;
     P.num_q_heads = num_q_heads;
     P.gqa = num_q_heads / layout->local_kv_heads;
     P.q_group = scored_q_group(layout->k_format, P.gqa);
