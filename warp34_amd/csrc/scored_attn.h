@@ -344,7 +344,7 @@ __device__ __forceinline__ void finish_row(const ScoredParams& P, int tok, int h
 }
 
 // Joins the chunks of rows.  SPREAD: a workgroup of eight waves for each column of each tile, wave w adds up chunks w, w + 8, ... (one
-// request has up to 128 chunks).  Otherwise a wave a column, kJoinCols columns a workgroup: many tiles, of which few have several chunks (a
+// request and kv head has up to 256 chunks, 512 at head_dim 128).  Otherwise a wave a column, kJoinCols columns a workgroup: many tiles, of which few have several chunks (a
 // workgroup for each of the 131 072 columns of 256 tiles and two kv heads took 190 us to find that, one for eight columns 24 us).
 constexpr int kJoinCols = 64;
 template <typename TQ, int HD, bool SPREAD>
@@ -366,7 +366,8 @@ __global__ __launch_bounds__(512) void scored_join_kernel(const ScoredParams P, 
         if (P.B.valid_token_mask != nullptr && P.B.valid_token_mask[tok] == 0) continue;
         const auto record = [&](int c) { return ((size_t)(first + c) * kv_subs + kv_sub) * columns + col; };
         const int at = (4 * lane) & (HD - 1);
-        constexpr int kStep = SPREAD ? 8 : 1, kBatch = SPREAD ? 16 : 8;  // chunks from one to the next of a wave; loads that travel together
+        constexpr int kStep = SPREAD ? 8 : 1, kBatch = 8;  // chunks from one to the next of a wave; loads that travel together
+        static_assert(64 % (kStep * kBatch) == 0, "what is loaded is added up before the weights of the next 64 chunks");
         const int own = SPREAD ? wave : 0;
         f4 part[kBatch];
         const auto load = [&](int from) {
