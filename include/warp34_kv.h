@@ -181,7 +181,8 @@ int warp34_kv_cache_write_strided_bf16(const warp34_exec* ex, const warp34_kv_la
  * the reference.  Any layout the append writes, K and V each in its own format; FP16 rows can be read
  * as bf16 and BF16 rows as fp16.  k_out or v_out may be NULL (that slab is not touched).  slot_mapping
  * is a DEVICE pointer; slots must lie inside the slabs and may come more than once.
- * Row strides are in elements and at least local_kv_heads * head_dim (hipErrorInvalidValue); head_dim
+ * Row strides are in elements and at least local_kv_heads * head_dim, and num_rows at most
+ * (2^24 - 1) * floor(2048 / head_dim) (16 in the place of 8 for rotated rows; hipErrorInvalidValue); head_dim
  * and strides are multiples of 8, outputs 16-byte aligned, 16-bit rows 16-byte, 8-bit rows 4-byte, TQ4
  * rows 2-byte aligned (hipErrorNotSupported otherwise).
  * ------------------------------------------------------------------------------------ */
@@ -330,6 +331,8 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  * (hipErrorInvalidValue); above 1e30 it counts as 1e30.  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
  * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass.  Two calls that may run
  * at once need a workspace each.
+ * A batch whose bounds make 2^23 tiles of query tokens or more (num_reqs times those of max_q_len) is refused
+ * (hipErrorInvalidValue).
  * The order of summation depends on the lengths, the heads, num_reqs, max_q_len, whether max_seq_len is at most 256, and
  * the scratch, and on nothing else: the same call gives the same bits.  Requests of 256 and more query columns (max_q_len
  * tokens x query heads of a kv head) take operands of one 16-bit part: rotated queries and quantised values are rounded
@@ -354,7 +357,8 @@ size_t warp34_paged_attention_scored_scratch_bytes(const warp34_kv_layer_layout*
  * parts; lse_out must not overlap lse_parts.  num_rows <= 0 returns 0 without a launch.  With more than
  * one part the strides are at least num_rows * head_dim and num_rows (hipErrorInvalidValue); head_dim
  * (at most 2048) and part_stride are multiples of 8, parts and out 16-byte aligned
- * (hipErrorNotSupported otherwise). */
+ * (hipErrorNotSupported otherwise).  num_rows is at most
+ * (2^24 - 1) * floor(2048 / head_dim) (hipErrorInvalidValue). */
 int warp34_attention_merge_f16(const warp34_exec* ex, const void* parts, const float* lse_parts, int num_parts,
                                int64_t part_stride, int64_t lse_part_stride, void* out, float* lse_out,
                                int64_t num_rows, int head_dim);

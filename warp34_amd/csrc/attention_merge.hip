@@ -6,6 +6,7 @@
 // are kept relative to a running maximum.  Bound: HBM, every part read once: two parts of 131 072 fp16 rows of 256 in 36.7 us (5.5 TB/s, as a large copy),
 // eight of 32 768 in 30.6; eight of 512 in 3.8, a launch.
 #include "attn_lanes.h"
+#include "attn_launch.h"
 
 namespace w34 {
 
@@ -76,7 +77,7 @@ static int attention_merge_entry(const warp34_exec* ex, const void* parts, const
     if ((head_dim & 7) != 0 || head_dim > 2048 || ((((uintptr_t)parts) | ((uintptr_t)out)) & 15u) != 0 || (part_stride & 7) != 0)
         return (int)hipErrorNotSupported;
     const int rows_per_block = 256 / (head_dim >> 3);
-    if (num_rows > (int64_t)0x7FFFFFFF * rows_per_block) return (int)hipErrorInvalidValue;
+    if (num_rows > (int64_t)0x7FFFFFFF * rows_per_block || !grid_fits((num_rows + rows_per_block - 1) / rows_per_block, 256)) return (int)hipErrorInvalidValue;
     if (num_parts > 1 && (part_stride < num_rows * head_dim || lse_part_stride < num_rows)) return (int)hipErrorInvalidValue;
     const int64_t blocks = (num_rows + rows_per_block - 1) / rows_per_block;
     hipLaunchKernelGGL((attention_merge_kernel<T>), dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)ex->stream, (const uint16_t*)parts, lse_parts,

@@ -49,6 +49,9 @@ static int ensure_dynamic_lds(KernelT kernel, int bytes, bool lds_base_zero = fa
     return 0;
 }
 
+// Whether a launch of so many workgroups side by side is one: a grid has less than 2^32 threads along each axis.
+inline bool grid_fits(long long workgroups, int threads) { return workgroups < (1ll << 32) / threads; }
+
 // ceil(2^16 / q_group), for the division of a workgroup's column by the q heads of its tile
 inline uint32_t q_group_magic_for(int q_group) { return (65536u + (uint32_t)q_group - 1u) / (uint32_t)q_group; }
 

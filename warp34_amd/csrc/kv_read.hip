@@ -7,6 +7,7 @@
 // issue and HBM together: 32 768 TQ4 rows of two kv heads, K and V, into BF16 in 18 to 19 us (84.5 MB, 4.5 to 4.7 TB/s; 62 vector instructions a row;
 // at 91 of them 22 us, with rows apart and a branch each 24); 333 Q8_0 rows 3.7 us, a launch.
 #include "attn_lanes.h"
+#include "attn_launch.h"
 #include "kv_encode.h"
 #include "wht_products.h"
 
@@ -314,6 +315,8 @@ static int kv_read_entry(const warp34_exec* ex, const warp34_kv_layer_layout* l,
     const bool rotated[2] = {rotated_rows(l->k_format, l->k_transform, l->head_dim), rotated_rows(l->v_format, l->v_transform, l->head_dim)};
     const int rows_per_block = 256 / (l->head_dim >> 3);
     const auto blocks = [&](int per_block) { return (unsigned)(((int64_t)num_rows + per_block - 1) / per_block); };
+    for (int side = 0; side < 2; ++side)
+        if (P.side[side].out && !grid_fits(blocks(rotated[side] ? 4 * kReadRows : rows_per_block), 256)) return (int)hipErrorInvalidValue;
     const unsigned heads = (unsigned)l->local_kv_heads;
     const auto launch = [&](int first, int sides) {
         hipStream_t stream = (hipStream_t)ex->stream;

@@ -99,7 +99,7 @@ static int launch_scored(const warp34_exec* ex, ScoredParams P) {
     const warp34_attention_batch& B = P.B;
     const int kv_subs = P.L.local_kv_heads * P.q_subgroups;
     const ScoredShape s = scored_shape(KVF, HD, kv_subs, B.num_reqs, B.total_tokens, B.max_q_len, P.q_group);
-    if (kv_subs > 65535 || s.entries * kv_subs > 0x7FFFFFFF) return (int)hipErrorInvalidValue;
+    if (kv_subs > 65535 || s.entries * kv_subs > 0x7FFFFFFF || !grid_fits(s.entries, kScoredWaves * 64)) return (int)hipErrorInvalidValue;
     P.tok_tile = s.tok_tile;
     P.tiles = (int)s.tiles;
     P.entries = (int)s.entries;
