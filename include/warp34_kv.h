@@ -24,7 +24,8 @@
  *     used only for launch geometry.  They can choose between forms of the attention
  *     kernels that add the same products in another order (a bound that lets a request
  *     have several tiles of query tokens, the pass for shared prefixes), and change
- *     nothing else in the results;
+ *     nothing else in the results (warp34_paged_attention_scored_*: max_q_len also how
+ *     exact they are, see there);
  *   - masked tokens / requests (valid_token_mask[tok]==0, valid_req_mask[req]==0,
  *     write slot < 0) write nothing and leave the output row untouched.
  */
@@ -326,18 +327,24 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  * warp34_attention_merge_* joins such results by.  Layouts, batches, q_in / attn_out, masked tokens and requests
  * (their lse_out stays untouched as well) and alignments are those of warp34_paged_attention_*.  Key and value
  * rows that a token sees must be finite, and what their decoded values are must fit fp16 for the quantised formats;
- * rows that no token of the request sees may hold anything (a masked token sees none, and its own row, which the
- * append leaves out, counts for those that do).  softcap must be finite and not negative
- * (hipErrorInvalidValue); above 1e30 it counts as 1e30.  sm_scale may be negative or zero.  Scratch as for the other attention calls, of the size
- * warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single pass.  Two calls that may run
- * at once need a workspace each.
+ * rows that no token of the request sees may hold anything (a masked token sees none; its own row, which the append
+ * leaves out, must be finite where another token sees it).  softcap must be finite and not negative
+ * (hipErrorInvalidValue); above 1e30 it counts as 1e30.  sm_scale may be negative or zero.  Scratch as for the other
+ * attention calls, of the size warp34_paged_attention_scored_scratch_bytes gives; with less, fewer chunks or a single
+ * pass.  Two calls that may run at once need a workspace each.
  * A batch whose bounds make 2^23 tiles of query tokens or more (num_reqs times those of max_q_len) is refused
  * (hipErrorInvalidValue).
  * The order of summation depends on the lengths, the heads, num_reqs, max_q_len, whether max_seq_len is at most 256, and
- * the scratch, and on nothing else: the same call gives the same bits.  Requests of 256 and more query columns (max_q_len
- * tokens x query heads of a kv head) take operands of one 16-bit part: rotated queries and quantised values are rounded
- * to fp16, weights to the values' type (2-norm of the error over TQ4 rows 4.5e-4, over un-rotated 8-bit rows 2.7e-4 into
- * fp16 outputs, whose own rounding is 2.1e-4).  Shorter ones lose nothing but the rounding of the output. */
+ * the scratch, and on nothing else: the same call gives the same bits.
+ * One kernel serves all requests of a call, and max_q_len chooses it (total_tokens where that is less, or max_q_len is 0),
+ * so that this bound changes how exact the results are; prompts and decode steps have calls of their own where either's
+ * time or the latter's exactness counts.  From 256 query columns on (max_q_len x query heads of a kv head, of which TQ4
+ * takes the largest divisor up to 8, the others up to 16) operands are of one 16-bit part: rotated queries, TQ4 keys and
+ * quantised values are rounded to fp16, weights to the values' type (2-norm of the error over rotated rows 4.5e-4, over
+ * un-rotated 8-bit rows 2.8e-4 into fp16 outputs, whose own rounding is 2.1e-4).  Below, queries, TQ4 keys and weights
+ * have two parts, and what shows is the rounding of the output; TQ4 values are from the table of fp16 centroids (9.4e-5).
+ * For both, values of quantised rows have fp16's absolute steps of 2^-24 as well, as fp16 outputs have: bf16 outputs
+ * (1.7e-3) show it from decoded values of 1e-5 downward (at 1e-6 an error of 3e-3 to 1e-2). */
 int warp34_paged_attention_scored_f16(const warp34_exec* ex, const warp34_kv_layer_layout* layout,
                                       const warp34_attention_batch* batch, const warp34_attention_scores* scores,
                                       const void* q_in, void* attn_out, int num_q_heads);

@@ -37,3 +37,27 @@ def test_caps_beyond_every_score_change_nothing(fmt, xf, tokens, cap):
                                                         scale=hb.sm_scale, dt=DT_BF16, chunk=tokens * 4 >= CHUNK_FROM)
     got = oracle.bits_to_f32(bits, DT_BF16).astype(np.float64)
     assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,xf", [f for f in FORMS if f[0] != FMT_BF16])
+@pytest.mark.parametrize("dt", [DT_F16, DT_BF16])
+@pytest.mark.parametrize("tokens", [2, 70])
+@pytest.mark.parametrize("size", [1e2, 1e-3, 1e-4, 1e-5, 1e-6])
+def test_values_of_any_size(fmt, xf, dt, tokens, size):
+    """Quantised values have fp16's relative and absolute steps.  The rotation back in the chunk kernel splits the row's average, and the average
+    times a Hadamard matrix of 16, into two fp16 parts each: 2^-25 of an element is left out twice, and 256 of them come together with 1 / 16."""
+    pool, bt, k, v, q, aq, ctx = make_case(fmt, 16, [300], [tokens], 1502, dt, xf=xf)
+    x = oracle.bits_to_f32(v, dt) * np.float32(size)
+    v = oracle.f32_to_bf16_bits(x) if dt == DT_BF16 else oracle.f32_to_f16_bits(x)
+    write = oracle.HostBatch([0, 300], [300], bt, context_lens_before=[0], write_slot_mapping=oracle.slot_mapping(bt[0], 0, 300, 16))
+    oracle.kv_cache_write(pool, write, k, v, dt)
+    hb = oracle.HostBatch(aq, [300], bt, context_lens_before=ctx)
+    bits, lse = run_scored(pool, hb, q, dt, 8)
+    chunk = tokens * 4 >= CHUNK_FROM
+    want, want_lse, bound, lse_bound = scored_attention(pool, bt, [300], oracle.bits_to_f32(q, dt).astype(np.float64), aq, ctx,
+                                                        scale=hb.sm_scale, dt=dt, chunk=chunk)
+    if chunk and xf == XF_WHT256:
+        bound = bound + 2 * 16 * 2.0 ** -25
+    got = oracle.bits_to_f32(bits, dt).astype(np.float64)
+    assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
