@@ -61,3 +61,20 @@ def test_values_of_any_size(fmt, xf, dt, tokens, size):
         bound = bound + 2 * 16 * 2.0 ** -25
     got = oracle.bits_to_f32(bits, dt).astype(np.float64)
     assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt,xf", FORMS)
+@pytest.mark.parametrize("tokens", [2, 70])
+@pytest.mark.parametrize("cap,size", [(1e-30, 1e20), (1e-20, 1e25), (1e-38, 1.0)])
+def test_scores_of_zero_under_small_caps_of_large_queries(fmt, xf, tokens, cap, size):
+    """Keys of zeros, whose scores are 0 whatever their factor: all keys count alike, and lse is the logarithm of their number."""
+    pool, bt, k, v, q, aq, ctx = make_case(fmt, 16, [150], [tokens], 1503, DT_BF16, xf=xf)
+    pool.k[:] = 0
+    q = oracle.f32_to_bf16_bits(oracle.bits_to_f32(q, DT_BF16) * np.float32(size))
+    hb = oracle.HostBatch(aq, [150], bt, context_lens_before=ctx)
+    bits, lse = run_scored(pool, hb, q, DT_BF16, 8, cap=cap)
+    want, want_lse, bound, lse_bound = scored_attention(pool, bt, [150], oracle.bits_to_f32(q, DT_BF16).astype(np.float64), aq, ctx,
+                                                        scale=hb.sm_scale, dt=DT_BF16, chunk=tokens * 4 >= CHUNK_FROM)
+    got = oracle.bits_to_f32(bits, DT_BF16).astype(np.float64)
+    assert (np.abs(got - want) <= bound).all() and (np.abs(lse - want_lse) <= lse_bound).all()

@@ -63,6 +63,8 @@ __device__ __forceinline__ float score_factor(const ScoredParams& P, float colum
     const float f = P.scale2 * column_scale;
     return f < 1.0e-37f ? 1.0e-37f : f;
 }
+// cc.  Finite, however small the cap and large the query: a score of 0 stays 0.
+__device__ __forceinline__ float cap_factor(const ScoredParams& P, float column_scale) { return fminf(P.cap_arg * column_scale, 3.0e38f); }
 template <bool CAP, bool SERIES, int N, typename V>
 __device__ __forceinline__ ScoreMap map_scores(V& s, float cs, float cc, const ScoredParams& P) {
     if constexpr (!CAP) {

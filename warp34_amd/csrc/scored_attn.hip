@@ -184,7 +184,7 @@ static int scored_entry(const warp34_exec* ex, const warp34_kv_layer_layout* lay
     P.q_flip = batch->sm_scale < 0.f ? 0x80008000u : 0u;
     const float cap = std::min(scores->softcap, kLargestCap);
     P.cap2 = cap * kLog2e;
-    // (finite, so that a score of 0 stays 0 under the smallest of caps)
+    // (finite under the smallest of caps; cap_factor)
     P.cap_arg = cap > 0.f ? std::min(2.0f * std::fabs(batch->sm_scale) * kLog2e / cap, 1.0e30f) : 0.f;
     P.wide_cap = cap > kWideCap ? 1 : 0;
     P.num_q_heads = num_q_heads;

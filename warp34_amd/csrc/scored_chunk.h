@@ -285,7 +285,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             }
         const float mine = __builtin_amdgcn_ldexpf(R::kOutScale, e);
         cs = score_factor(P, mine);
-        cc *= mine;
+        cc = cap_factor(P, mine);
     } else {
         // Rotated by two products a column (wht_products.h; in vector instructions, as the results' rotation back, 8 requests of 400 to 600 TQ4
         // tokens in windows of 64 took 98.9 instead of 81.5 us), eight columns of the wave at a time through LDS, their loads together and those of
@@ -340,7 +340,7 @@ __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
         }
         cs = score_factor(P, scales[n]);
-        cc *= scales[n];
+        cc = cap_factor(P, scales[n]);
     }
     if (gaps && tid < t.tokens) {
         int from = 0, to = -1;

@@ -398,7 +398,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_kernel(con
             q_low[m] = *reinterpret_cast<const u4*>(ql + n * M::kQStride + R::element(m, b));
         }
         cs = score_factor(P, qs[n]);
-        cc *= qs[n];
+        cc = cap_factor(P, qs[n]);
     }
     const bool two_parts = !R::k16 && P.rot_q != 0;
 

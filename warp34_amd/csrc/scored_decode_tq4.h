@@ -160,7 +160,7 @@ __global__ __launch_bounds__(kScoredWaves * 64, 1) void scored_decode_tq4_kernel
         q[2 * m] = u4{w[0], w[0], w[1], w[1]};
         q[2 * m + 1] = u4{w[2], w[2], w[3], w[3]};
     }
-    const float cs = score_factor(P, qs[n & 7] * kTableInvGain), cc = P.cap_arg * (qs[n & 7] * kTableInvGain);
+    const float cs = score_factor(P, qs[n & 7] * kTableInvGain), cc = cap_factor(P, qs[n & 7] * kTableInvGain);
     const float low_part = n < 8 ? 0.f : 1.f;
     const uint32_t table_lane = ((uint32_t)lane & 31u) << 3;
 
