@@ -322,6 +322,7 @@ int warp34_paged_attention_gated_f16(const warp34_exec* ex, const warp34_kv_laye
  *   keys of token t: [max(min_kv, document_starts[t]), max(max_kv, prefix_ends[t] - 1)], the latter clamped to
  *   seq_after - 1, with min_kv and max_kv of warp34_paged_attention_*
  *   out = softmax(x) V,  lse = ln sum_k exp(x); a token without keys gives zeros and minus infinity
+ * (scores below -6e29 count as those of hidden keys)
  * Packed documents are document_starts, prompts that open with a part that is seen both ways are prefix_ends,
  * score caps are softcap, heads that look near first are distance_slopes; lse_out is what
  * warp34_attention_merge_* joins such results by.  Layouts, batches, q_in / attn_out, masked tokens and requests

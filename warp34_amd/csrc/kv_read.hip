@@ -5,7 +5,8 @@
 //
 // computed in 32 bits and rounded once.  A row's bytes are read once and 2 x head_dim bytes written once.  Rotated rows are bound by vector
 // issue and HBM together: 32 768 TQ4 rows of two kv heads, K and V, into BF16 in 18 to 19 us (84.5 MB, 4.5 to 4.7 TB/s; 62 vector instructions a row;
-// at 91 of them 22 us, with rows apart and a branch each 24); 333 Q8_0 rows 3.7 us, a launch.
+// at 91 of them 22 us, with rows apart and a branch each 24); 333 Q8_0 rows 3.7 us, a launch.  Rows stored as they are: 60 000 of four kv heads, K and V, BF16
+// 92 us (5.4 TB/s, as a large copy), Q8_0 97 (3.9), FP8 88 (4.2).
 #include "attn_lanes.h"
 #include "attn_launch.h"
 #include "kv_encode.h"
@@ -117,15 +118,11 @@ __global__ __launch_bounds__(256) void kv_read_plain_kernel(const ReadParams P, 
     if (live) *reinterpret_cast<uint4*>(S.out + row * S.row_stride + (int64_t)head * P.head_dim + e) = w;
 }
 
-// Rotated rows of 256 elements, kReadRows rows a wave.  The transform is a
-// product of two 16 x 16 ones: with X[r][c] = x[16 r + c] and H[r][c] = (-1)^popcount(r & c), Y = H X H.  Two MFMAs do it:
-//   Z = X H      A = X (lane (n, b) holds X[n][4 b .. 4 b + 3]), B = H; lane (n, b) gets Z[4 b + i][n]
-//   Y^T = Z^T H  those registers are the A operand Z^T as they stand; lane (n, b) gets Y[n][4 b + i]
+// Rotated rows of 256 elements, kReadRows rows a wave, by the two products of wht_products.h.
 // Memory wants wider pieces than four elements a lane: of four rows at a time lane (n, b) loads X[n] of row b, and the pieces change
 // places by swaps of 16 and of 32 lanes; two rows' results change places so that a lane stores eight elements in a run.  (For that the
 // columns of Z are out of order, in groups of four: 0, 8, 4, 12.)
-// Operands have two fp16 parts in the halves of a 16x16x32 product (22 bits), so the result is as good as the 60 additions a row in
-// 32 bits that the MFMAs stand for.  X is the bare codes, of which eight bits are one part and centroids have two in a table; the scales
+// X is the bare codes, of which eight bits are one part and centroids have two in a table; the scales
 // multiply Z, whose rows 4 b .. 4 b + 3 lie in one block: relative to a power of two above the row's largest scale, so that the parts
 // stay inside fp16's range whatever the scales.
 // us at 4 / 8 / 16 rows a wave: 200 TQ4 rows 3.3 / 3.9 / 5.7, 2 000 3.7 / 4.4 / 6.1, 32 768 18.7 / 18.7 / 19.0.

@@ -12,10 +12,10 @@
 //   value tile  row r, piece p at p ^ 4 (r & 3): the four rows of a transposing read touch all banks
 //
 // Why this shape: 128 sums and 64 query registers a lane are what two waves a SIMD have room for, and each operand read from LDS serves 32
-// columns.  4 requests of 2 048 tokens on 16 384 keys, 16 + 2 heads, capped: BF16 2.36 ms (990 TFLOP/s; a large matrix product of the
-// library 1 390), FP8 2.85, TQ4 3.01 (780), Q8_0 3.27.  What bounds it is a wave's own chain: of 6 700 cycles a TQ4 unit the products of a SIMD's
-// two waves take 2 050, vector work 55 % of the cycles (a cap's exponential and reciprocal, the weights' exponentials and the widening most of
-// it), LDS 32 %, and a wave waits 38 %.  Left out for timing: cap and exponentials -7 %, widening -14 %, operand reads -15 %, all three -36 %;
+// columns.  4 requests of 2 048 tokens on 16 384 keys, 16 + 2 heads, capped: BF16 2.36 to 2.42 ms (980 TFLOP/s; a large matrix product of the
+// library 1 390), FP8 2.85 to 3.04, TQ4 3.03 (770), Q8_0 3.25.  What bounds it is a wave's own chain: of 6 400 cycles a TQ4 unit the products of a SIMD's
+// two waves take 2 050, vector work 54 % of the cycles (a cap's exponential and reciprocal, the weights' exponentials and the widening most of
+// it), LDS 34 %, and a wave waits 39 %.  Left out for timing: cap and exponentials -7 %, widening -14 %, operand reads -15 %, all three -36 %;
 // the rows' pages made no difference.  Two sums side by side for the scores need 16 registers more than there are (packed documents 107 ->
 // 119 us); operands three products ahead the same (TQ4 3.31 ms).  Values a unit later in half of the waves: -5 %; widening between
 // products: FP8 -7 %, Q8_0 -9 %, TQ4 -1.5 %.
@@ -111,9 +111,12 @@ __device__ __forceinline__ void build_narrow_table(uint8_t* smem, int tid, int w
 // Roundings, beside those of the inputs' types: rotated queries and TQ4 keys are one fp16 part (the keys' block scales multiply the
 // scores in 32 bits); quantised values are fp16(scale * code), TQ4 ones from the fp16 table; weights are one operand of the values'
 // type.  (Weights that carry the block scales would spare the values' rounding and need two parts, half as many products again: a
-// block-wide error of a weight is gathered in one channel by the rotation back.)  2-norm of the error: TQ4 4.5e-4, un-rotated 8-bit rows
-// 2.7e-4 into fp16 outputs, whose own rounding is 2.1e-4; 1.8e-3 and 1.7e-3 of 1.7e-3 into bf16 ones.  Of TQ4's the queries are 2.8e-4, values 2.1e-4,
-// weights 1.2e-4, and second parts of queries would be 64 registers more.
+// block-wide error of a weight is gathered in one channel by the rotation back.)  l adds up the weights before that rounding: lse keeps its
+// 32 bits, and a row's average has the roundings of its weights.  2-norm of the error: rotated rows 4.5e-4, un-rotated 8-bit rows 2.8e-4 into fp16
+// outputs, whose own rounding is 2.1e-4; 1.8e-3 and 1.7e-3 of 1.7e-3 into bf16 ones, 2.1e-3 of 1.6e-3 over BF16 rows (packed documents).  Of TQ4's
+// the queries are 2.8e-4, values 2.1e-4, weights 1.2e-4, and second parts of queries would be 64 registers more.  Values below 2^-14 have fp16's
+// absolute steps: of decoded values of 1e-5 / 1e-6 the error into bf16 outputs is 1.9e-3 / 7.3e-3.
+// Over quantised rows 13 to 24 words a lane lie in scratch memory (16-bit rows none); a version that puts sums there has ten times as many.
 template <typename TQ, int KVF, int HD, bool CAP>
 __global__ __launch_bounds__(kChunkWaves * 64, 1) void scored_chunk_kernel(const ScoredParams P) {
     extern __shared__ __align__(16) uint8_t smem[];

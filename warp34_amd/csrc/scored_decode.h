@@ -4,7 +4,8 @@
 //   S^T = K Q^T      16x16x32 MFMAs, A = 16 key rows (lane (n, b): row n), B = query columns; lane (n, b) gets the scores of keys
 //                    4 b .. 4 b + 3 for column n, so that the softmax state of a column is a scalar of four lanes
 //   O^T += V^T P^T   A = channels x keys, B = the weights where they stand: each weight has a high and a low 16-bit part in the two
-//                    halves of a product of 32 keys, over the same values, so it loses nothing
+//                    halves of a product of 32 keys, over the same values: 22 bits of it, down to 2^-24 (block scales ride on the weights
+//                    of quantised rows, so that small values come to that end first: 1e-6 has an error of 3e-3 to 1e-2 into bf16 outputs)
 // Rows go from the pages to registers as they are stored; key loads of the next half unit travel during the softmax and the value
 // product, value loads during the next scores.  Only the scales of quantised rows go through LDS.
 // At the end the waves' states are joined through LDS, and the chunks' by scored_join_kernel.
