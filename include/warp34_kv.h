@@ -195,6 +195,21 @@ int warp34_kv_cache_read_bf16(const warp34_exec* ex, const warp34_kv_layer_layou
                               int k_row_stride, int v_row_stride);
 
 /* ------------------------------------------------------------------------------------
+ * Pages of a cache copied in all layers (no counterpart in the reference, which copies no pages): for each pair i
+ * and each of the layouts, rows 0 .. rows[i] - 1 (clamped to 0 .. block_size; rows NULL: all of them) of every
+ * head of page src_pages[i] go to page dst_pages[i] of the same slabs, K and V, byte for byte, whatever
+ * their format.  A request that forks takes the partly filled page of its parent with it; a pool is packed together
+ * by moving its last pages into its gaps.  layouts is a HOST array of num_layers descriptors, src_pages,
+ * dst_pages and rows are DEVICE arrays of num_pairs.  Pairs with a negative page, or the same one twice, are passed
+ * over.  No destination may be a source or a destination of another pair, and no two layouts may share memory.
+ * hipErrorInvalidValue: missing pointers, negative num_layers, no slab, kv heads or block size; hipErrorNotSupported:
+ * formats whose rows are not those of the append, token strides below the row, strides or slabs that are not
+ * 2-byte aligned.  num_layers == 0 or num_pairs <= 0 return 0 without a launch.  One launch for 48 layers.
+ * ------------------------------------------------------------------------------------ */
+int warp34_kv_cache_copy_pages(const warp34_exec* ex, const warp34_kv_layer_layout* layouts, int num_layers,
+                               const int32_t* src_pages, const int32_t* dst_pages, const int32_t* rows, int num_pairs);
+
+/* ------------------------------------------------------------------------------------
  * Paged GQA attention (replaces op_paged_attn.cu:1266-1448 and op_kv_cache.cu:1192-1241).
  *
  * q_in / attn_out: [total_tokens, num_q_heads, head_dim] contiguous, fp16 for _f16 and

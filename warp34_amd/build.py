@@ -33,6 +33,9 @@ SOURCES = [
     (os.path.join(CSRC, "scored_attn.hip"), PRELOAD),
     (os.path.join(CSRC, "kv_read.hip"), []),
     (os.path.join(CSRC, "attention_merge.hip"), []),
+    (os.path.join(CSRC, "kv_copy.hip"), []),
+    (os.path.join(CSRC, "linear_attention.hip"), []),
+    (os.path.join(CSRC, "draft_verify.hip"), []),
     (os.path.join(CSRC, "runtime.hip"), []),
     (os.path.join(HOST, "kv_host.cpp"), []),
     (os.path.join(HOST, "prefix_cache.cpp"), []),

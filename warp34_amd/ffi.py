@@ -98,6 +98,61 @@ class Warp34AttentionScores(C.Structure):
     ]
 
 
+class Warp34LinearStateLayout(C.Structure):
+    """Where the states of linear attention are, and its heads (include/warp34_linear.h)."""
+
+    _fields_ = [
+        ("state_base", C.c_uint64),
+        ("slot_stride_bytes", C.c_uint64),
+        ("num_k_heads", C.c_int32),
+        ("num_v_heads", C.c_int32),
+        ("k_head_dim", C.c_int32),
+        ("v_head_dim", C.c_int32),
+    ]
+
+
+class Warp34LinearBatch(C.Structure):
+    """warp34_linear_attention_batch: device pointers (None: not used but for query_start_loc), bounds and strides."""
+
+    _fields_ = [
+        ("query_start_loc", C.c_void_p),
+        ("state_in_slots", C.c_void_p),
+        ("has_initial_state", C.c_void_p),
+        ("state_out_slots", C.c_void_p),
+        ("state_tokens", C.c_void_p),
+        ("valid_req_mask", C.c_void_p),
+        ("num_reqs", C.c_int32),
+        ("total_tokens", C.c_int32),
+        ("max_q_len", C.c_int32),
+        ("scale", C.c_float),
+        ("q_row_stride", C.c_int32),
+        ("k_row_stride", C.c_int32),
+        ("v_row_stride", C.c_int32),
+        ("out_row_stride", C.c_int32),
+        ("decay_row_stride", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+
+class Warp34DraftBatch(C.Structure):
+    """The fed tokens of a verify batch and the shape of its probabilities (include/warp34_drafts.h)."""
+
+    _fields_ = [
+        ("query_start_loc", C.c_void_p),
+        ("tokens", C.c_void_p),
+        ("valid_req_mask", C.c_void_p),
+        ("target_row_stride", C.c_int64),
+        ("draft_row_stride", C.c_int64),
+        ("num_reqs", C.c_int32),
+        ("total_tokens", C.c_int32),
+        ("max_q_len", C.c_int32),
+        ("vocab_size", C.c_int32),
+    ]
+
+
+assert C.sizeof(Warp34LinearStateLayout) == 32
+assert C.sizeof(Warp34LinearBatch) == 88
+assert C.sizeof(Warp34DraftBatch) == 56
 assert C.sizeof(Warp34AttentionScores) == 40
 assert C.sizeof(Warp34Exec) == 32
 assert C.sizeof(Warp34KvLayerLayout) == 104
@@ -107,6 +162,9 @@ _EX = C.POINTER(Warp34Exec)
 _LAY = C.POINTER(Warp34KvLayerLayout)
 _BAT = C.POINTER(Warp34AttentionBatch)
 _SCO = C.POINTER(Warp34AttentionScores)
+_LST = C.POINTER(Warp34LinearStateLayout)
+_LIN = C.POINTER(Warp34LinearBatch)
+_DRA = C.POINTER(Warp34DraftBatch)
 
 # name -> (restype, argtypes); every symbol the headers under include/ declare
 SIGNATURES = {
@@ -124,6 +182,15 @@ SIGNATURES = {
         (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
     "warp34_kv_cache_read_bf16":
         (C.c_int, [_EX, _LAY, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int]),
+    # (exec, layouts, num_layers, src_pages, dst_pages, rows, num_pairs)
+    "warp34_kv_cache_copy_pages": (C.c_int, [_EX, _LAY, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int]),
+    # linear attention over state slots (include/warp34_linear.h): (exec, layout, batch, q, k, v, log_decay, out)
+    "warp34_linear_attention_f16": (C.c_int, [_EX, _LST, _LIN] + [C.c_void_p] * 5),
+    "warp34_linear_attention_bf16": (C.c_int, [_EX, _LST, _LIN] + [C.c_void_p] * 5),
+    "warp34_linear_attention_scratch_bytes": (C.c_size_t, [_LST, C.c_int, C.c_int, C.c_int]),
+    # (exec, batch, target_probs, draft_probs, accept_uniforms, sample_uniforms, out_tokens, emitted_counts)
+    "warp34_verify_drafts": (C.c_int, [_EX, _DRA] + [C.c_void_p] * 6),
+    "warp34_verify_drafts_scratch_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "warp34_paged_attention_scored_f16": (C.c_int, [_EX, _LAY, _BAT, _SCO, C.c_void_p, C.c_void_p, C.c_int]),
     "warp34_paged_attention_scored_bf16": (C.c_int, [_EX, _LAY, _BAT, _SCO, C.c_void_p, C.c_void_p, C.c_int]),
     # (layout, num_reqs, total_tokens, max_q_len, num_q_heads)
