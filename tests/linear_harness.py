@@ -4,8 +4,11 @@ With fade = exp(g) and, beside the state S, its absolute twin A (A = fade A + |k
   E = fade E + 2^-22 A      a step's product, sum and factor (2^-24 each, the exponential 2^-23)
 and, where factors over several tokens are exponentials of sums of g, the rounding of their arguments
   B = fade (B + |g| A)      sum over tokens of weight * |argument|, times 2^-22 (argument and its product with log2 e).
-A state may be off by E + 2^-22 B.  Outputs: scale |q|^T (E + 2^-22 B + 2^-15 A), the last for operands of 16 bits in two parts (2^-16 each for
-states and weights) and for the sums over channels (2^-24 each of 128), and half a step of the output."""
+  A itself               weighted values as operands: two fp16 parts (2^-11 of what 2^-11 leaves: 2^-22 A), three bf16 parts (2^-24 A);
+                         a chunk's products are added up by four matrix instructions a part, each with up to two roundings of 2^-24 of the sum:
+                         8 x 2 of 2^-24 A for fp16, 12 x 2 for bf16 (E counts them token by token, too few where a token fades at once)
+A state may be off by E + 2^-22 B + OPERAND A.  Outputs: scale |q|^T (E + 2^-22 B + 2^-15 A), the last for operands of 16 bits in two parts
+(2^-16 each for states and weights) and for the sums over channels (2^-24 each of 128), and half a step of the output."""
 import ctypes as C
 
 import torch
@@ -13,6 +16,7 @@ import torch
 from plain_kv import HALF_STEP, HALF_TINY
 from oracle import DT_BF16, DT_F16
 
+OPERAND = {DT_F16: 2.0 ** -22 + 16 * 2.0 ** -24, DT_BF16: 2.0 ** -24 + 24 * 2.0 ** -24}
 TYPES = {DT_F16: torch.float16, DT_BF16: torch.bfloat16}
 
 
@@ -126,7 +130,7 @@ class Case:
             for t in range(length + 1):
                 if t == kept and self.out_list is not None and self.out_list[r] >= 0:
                     states[self.out_list[r]] = s
-                    s_bound[self.out_list[r]] = e + 2.0 ** -22 * b
+                    s_bound[self.out_list[r]] = e + 2.0 ** -22 * b + (OPERAND[self.dt] * a if t else 0)
                 if t == length:
                     break
                 row = self.starts[r] + t

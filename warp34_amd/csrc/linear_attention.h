@@ -15,7 +15,7 @@ struct LinearArgs {
     const float* g;  // nullptr: no decay
     uint16_t* out;   // nullptr: none
     uint64_t state_base, slot_stride;
-    int num_reqs, total_tokens, k_heads, v_heads, group;  // group: value heads of a key head
+    int num_reqs, total_tokens, v_heads, v_dim, group;  // group: value heads of a key head
     int q_stride, k_stride, v_stride, out_stride, g_stride;
     float scale;
 };

@@ -2,15 +2,74 @@
 #include <cmath>
 
 #include "attn_launch.h"
-#include "linear_attention.h"
+#include "linear_chunk.h"
 
 namespace w34 {
 
-template <typename T, int DK, int DV>
-static int linear_launch(const warp34_exec* ex, const warp34_linear_attention_batch* b, const LinearArgs& a) {
-    if (!grid_fits((long long)a.num_reqs * a.v_heads, 2 * DV)) return (int)hipErrorInvalidValue;
-    hipLaunchKernelGGL((linear_step_kernel<T, DK, DV>), dim3((unsigned)a.num_reqs * (unsigned)a.v_heads), dim3(2 * DV), 0, (hipStream_t)ex->stream, a);
+constexpr int kLinearGroups = 512;  // workgroups of the chunk kernel that run at once, two on each of 256 units
+constexpr int kStepTokens = 16;  // requests of up to so many tokens go by the recurrent kernel
+
+// How a batch is cut up.
+struct LinearShape {
+    int log_length;  // tokens of a part, 0: requests are walked from end to end
+    long long parts; // at most
+    size_t bytes;    // of scratch
+};
+
+static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len, bool kept, size_t scratch) {
+    const long long most = max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens;
+    const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
+    LinearShape s{0, 0, 0};
+    for (int log_length = 6; log_length < 30; ++log_length) {
+        const long long length = 1ll << log_length;
+        if (length >= most) return s;
+        // ceil(n / length) <= (n - 1) / length + 1 over the requests that have tokens, and one more for a cut behind the kept ones
+        const long long some = min((long long)num_reqs, (long long)total_tokens), parts = (total_tokens - some) / length + some * (kept ? 2 : 1);
+        const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)parts * heads * size * 4;
+        if (parts * heads > kLinearGroups) continue;
+        if (bytes > scratch || !grid_fits(parts * heads * (size / 1024), 256)) continue;
+        s.log_length = log_length, s.parts = parts, s.bytes = bytes;
+        return s;
+    }
+    return s;
+}
+
+template <typename T, int DK, int NW>
+static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const LinearShape& shape) {
+    const long long columns = (long long)a.v_heads;
+    const hipStream_t stream = (hipStream_t)ex->stream;
+    LinearParts p{nullptr, nullptr, shape.log_length, (int)shape.parts};
+    if (shape.log_length == 0) {
+        if (!grid_fits(a.num_reqs * columns, 64 * NW)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearWalk>), dim3((unsigned)(a.num_reqs * columns)), dim3(64 * NW), 0, stream, a, p);
+        return (int)hipGetLastError();
+    }
+    const long long scans = (long long)a.num_reqs * a.v_heads * (DK * a.v_dim / 1024);
+    if (!grid_fits(shape.parts * columns, 64 * NW) || !grid_fits(scans, 256)) return (int)hipErrorInvalidValue;
+    p.states = (float*)(uintptr_t)ex->scratch_ptr;
+    p.fades = p.states + shape.parts * a.v_heads * (DK * a.v_dim);
+    const dim3 grid((unsigned)(shape.parts * columns));
+    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearSums>), grid, dim3(64 * NW), 0, stream, a, p);
+    int rc = (int)hipGetLastError();
+    if (rc) return rc;
+    hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)scans), dim3(256), 0, stream, a, p, DK);
+    rc = (int)hipGetLastError();
+    if (rc || a.out == nullptr) return rc;
+    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearRows>), grid, dim3(64 * NW), 0, stream, a, p);
     return (int)hipGetLastError();
+}
+
+template <typename T, int DK, int DV>
+static int linear_launch(const warp34_exec* ex, const warp34_linear_state_layout* y, const warp34_linear_attention_batch* b, const LinearArgs& a) {
+    const int most = b->max_q_len > 0 && b->max_q_len < b->total_tokens ? b->max_q_len : b->total_tokens;
+    if (most <= kStepTokens) {
+        if (!grid_fits((long long)a.num_reqs * a.v_heads, 2 * DV)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((linear_step_kernel<T, DK, DV>), dim3((unsigned)a.num_reqs * (unsigned)a.v_heads), dim3(2 * DV), 0, (hipStream_t)ex->stream, a);
+        return (int)hipGetLastError();
+    }
+    const bool usable = ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0;
+    const LinearShape shape = linear_shape(y, b->num_reqs, b->total_tokens, b->max_q_len, b->state_tokens != nullptr, usable ? ex->scratch_size : 0);
+    return linear_chunk_launch<T, DK, DV / 32>(ex, a, shape);
 }
 
 template <typename T>
@@ -33,10 +92,10 @@ static int linear_entry(const warp34_exec* ex, const warp34_linear_state_layout*
     if (b->num_reqs <= 0 || b->total_tokens < 0 || (!out && !b->state_out_slots)) return 0;
     const LinearArgs a{b->query_start_loc, b->state_in_slots, b->has_initial_state, b->state_out_slots, b->state_tokens, b->valid_req_mask,
                        (const uint16_t*)q, (const uint16_t*)k, (const uint16_t*)v, log_decay, (uint16_t*)out, y->state_base, y->slot_stride_bytes,
-                       b->num_reqs, b->total_tokens, y->num_k_heads, y->num_v_heads, y->num_v_heads / y->num_k_heads,
+                       b->num_reqs, b->total_tokens, y->num_v_heads, y->v_head_dim, y->num_v_heads / y->num_k_heads,
                        b->q_row_stride, b->k_row_stride, b->v_row_stride, b->out_row_stride, b->decay_row_stride, b->scale};
-    if (y->k_head_dim == 128) return y->v_head_dim == 128 ? linear_launch<T, 128, 128>(ex, b, a) : linear_launch<T, 128, 64>(ex, b, a);
-    return y->v_head_dim == 128 ? linear_launch<T, 64, 128>(ex, b, a) : linear_launch<T, 64, 64>(ex, b, a);
+    if (y->k_head_dim == 128) return y->v_head_dim == 128 ? linear_launch<T, 128, 128>(ex, y, b, a) : linear_launch<T, 128, 64>(ex, y, b, a);
+    return y->v_head_dim == 128 ? linear_launch<T, 64, 128>(ex, y, b, a) : linear_launch<T, 64, 64>(ex, y, b, a);
 }
 
 }  // namespace w34
@@ -44,8 +103,11 @@ static int linear_entry(const warp34_exec* ex, const warp34_linear_state_layout*
 using namespace w34;
 
 extern "C" size_t warp34_linear_attention_scratch_bytes(const warp34_linear_state_layout* layout, int num_reqs, int total_tokens, int max_q_len) {
-    (void)layout, (void)num_reqs, (void)total_tokens, (void)max_q_len;
-    return 0;
+    if (!layout || num_reqs <= 0 || total_tokens <= 0 || layout->num_v_heads <= 0 || layout->num_v_heads > (1 << 20) ||
+        (layout->k_head_dim != 64 && layout->k_head_dim != 128) || (layout->v_head_dim != 64 && layout->v_head_dim != 128))
+        return 0;
+    if ((max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens) <= kStepTokens) return 0;
+    return linear_shape(layout, num_reqs, total_tokens, max_q_len, true, ~(size_t)0).bytes;
 }
 extern "C" int warp34_linear_attention_f16(const warp34_exec* ex, const warp34_linear_state_layout* layout, const warp34_linear_attention_batch* batch,
                                            const void* q, const void* k, const void* v, const float* log_decay, void* out) {
