@@ -7,6 +7,7 @@
 namespace w34 {
 
 constexpr int kLinearGroups = 512;  // workgroups of the chunk kernel that run at once, two on each of 256 units
+constexpr int kLinearMostStride = 1 << 23;  // elements: a chunk's rows are within 2^31 bytes
 constexpr int kStepTokens = 16;  // requests of up to so many tokens go by the recurrent kernel
 
 // How a batch is cut up.
@@ -26,7 +27,7 @@ static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_req
         // ceil(n / length) <= (n - 1) / length + 1 over the requests that have tokens, and one more for a cut behind the kept ones
         const long long some = min((long long)num_reqs, (long long)total_tokens), parts = (total_tokens - some) / length + some * (kept ? 2 : 1);
         const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)parts * heads * size * 4;
-        if (parts * heads > kLinearGroups) continue;
+        if (min(parts, num_reqs * ((most + length - 1) / length)) * heads > kLinearGroups) continue;
         if (bytes > scratch || !grid_fits(parts * heads * (size / 1024), 256)) continue;
         s.log_length = log_length, s.parts = parts, s.bytes = bytes;
         return s;
@@ -82,6 +83,9 @@ static int linear_entry(const warp34_exec* ex, const warp34_linear_state_layout*
     const int k_row = y->num_k_heads * y->k_head_dim, v_row = y->num_v_heads * y->v_head_dim;
     if (b->q_row_stride < k_row || b->k_row_stride < k_row || b->v_row_stride < v_row || (out && b->out_row_stride < v_row) ||
         (log_decay && b->decay_row_stride != 0 && b->decay_row_stride < y->num_v_heads))
+        return (int)hipErrorInvalidValue;
+    if (b->q_row_stride > kLinearMostStride || b->k_row_stride > kLinearMostStride || b->v_row_stride > kLinearMostStride ||
+        (out && b->out_row_stride > kLinearMostStride))
         return (int)hipErrorInvalidValue;
     const bool states = b->state_in_slots != nullptr || b->state_out_slots != nullptr;
     if (states && (!y->state_base || y->slot_stride_bytes < 4ull * (uint64_t)v_row * (uint64_t)y->k_head_dim)) return (int)hipErrorInvalidValue;

@@ -2,7 +2,7 @@
 //
 //   O_i = 2^G_i S^T q_i + sum_{j <= i} (q_i . k_j) 2^(G_i - G_j) v_j          S' = 2^G_end S + sum_j k_j (2^(G_end - G_j) v_j)^T
 //
-// Workgroup = 32 NW columns of a value head, a wave 32 of them with their part of the state in registers; 32x32x16 MFMAs:
+// Workgroup = the columns of a value head, a wave 32 of them with their part of the state in registers; 32x32x16 MFMAs:
 //   P^T = K Q^T        one 32x32 tile a wave (three of them: a chunk's second half of keys is not seen by its first half of queries),
 //                      weighted, and laid into LDS as the operands of the product below
 //   O^T = S^T Q^T      the state's registers are the operand as they stand: lane (n, b) has column n for rows (i & 3) + 8 (i >> 2) + 4 b,
@@ -15,8 +15,6 @@
 // show their own rounding only; v' has three for bf16 where the state itself comes out (24 bits), two for fp16.  fp16 has little range:
 // v' and S are scaled by powers of two of a wave, P by one of a row, to put the largest at 2^14; what is lost are bits 2^-39 below it.
 #pragma once
-
-#include <type_traits>
 
 #include "linear_attention.h"
 
@@ -66,7 +64,7 @@ __device__ __forceinline__ bool linear_find_part(const LinearArgs& a, int log_le
             const int o = __shfl_up(run, by, 64);
             if (lane >= by) run += o;
         }
-        const int total = __shfl(run, 63, 64);
+        const int total = __builtin_amdgcn_readlane(run, 63);
         if (index < total) {
             const int owner = __builtin_ctzll(__ballot(index < run));
             req = __builtin_amdgcn_readfirstlane(base + owner);
@@ -94,17 +92,26 @@ __device__ __forceinline__ f16v linear_mfma(u4 a, u4 b, f16v c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
     }
 }
+template <typename T>
+__device__ __forceinline__ uint32_t linear_pack(float x, float y) {
+    if constexpr (T::kStorageFormat == WARP34_KV_FORMAT_BF16) {
+        typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f2{x, y}, bf2));
+    } else {
+        return pack_h2(x, y);
+    }
+}
 // Two numbers as PARTS pairs of 16 bits whose sums they are.
 template <typename T, int PARTS>
 __device__ __forceinline__ void linear_split(float x, float y, uint32_t (&w)[PARTS]) {
 #pragma unroll
     for (int p = 0; p < PARTS; ++p) {
+        w[p] = linear_pack<T>(x, y);
+        if (p + 1 == PARTS) break;
         if constexpr (T::kStorageFormat == WARP34_KV_FORMAT_BF16) {
-            w[p] = (uint32_t)T::from_f32(x) | (uint32_t)T::from_f32(y) << 16;
             x -= __uint_as_float(w[p] << 16);
             y -= __uint_as_float(w[p] & 0xFFFF0000u);
         } else {
-            w[p] = pack_h2(x, y);
             x -= half_lo_to_f32(w[p]);
             y -= half_hi_to_f32(w[p]);
         }
@@ -122,53 +129,57 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-// Where 16 bytes of a row are: operand reads of 16 rows and the four rows of a transposing read touch all banks.
-template <int PIECES>
-__device__ __forceinline__ uint32_t linear_piece(int row, int piece) {
-    static_assert(PIECES == 8 || PIECES == 16, "rows of 128 or 256 bytes");
-    const int x = PIECES == 16 ? (row & 3) << 2 | (row >> 2 & 3) : (row >> 1 & 1) << 2 | (row >> 2 & 3);
-    return (uint32_t)(row * PIECES * 16 + (piece ^ x) * 16);
+// Bytes from a row to the next one: 32 more than the row, so that the four rows of a transposing read touch different banks, as do any eight
+// rows of an operand read, and addresses are one register and constants.
+constexpr int linear_row(int bytes) { return bytes + 32; }
+
+// `rows` rows of `width` 16-bit elements from `base` on: loads behind the last row give zeros, stores there are dropped.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t linear_rows(const uint16_t* base, int rows, int stride, int width) {
+    return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 2 * ((rows - 1) * stride + width), 0x00020000);
 }
 
 enum { kLinearWalk, kLinearSums, kLinearRows };  // a whole request; what a part adds to the state; a part's rows
 
 template <int DK, int NW>
 struct LinearLds {
-    static constexpr int kQ = 0, kK = kLinearChunk * DK * 2, kV = 2 * kK, kP = kV + kLinearChunk * NW * 64;
-    static constexpr int kG = kP + 3 * 4096;       // [64] G as two numbers
-    static constexpr int kW = kG + 64 * 8;         // [64] 2^(G_end - G_j)
-    static constexpr int kFade = kW + 64 * 4;      // 2^G_end
-    static constexpr int kRow = kFade + 16;        // [3][32] what P's rows are to be multiplied by (fp16)
-    static constexpr int kBytes = kRow + 3 * 32 * 4;
+    static constexpr int kKRow = linear_row(DK * 2), kVRow = linear_row(NW * 64);
+    static constexpr int kQ = 0, kK = kLinearChunk * kKRow, kV = 2 * kK, kP = kV + kLinearChunk * kVRow;
+    static constexpr int kRow = kP + 3 * 4096;     // [3][32] what P's rows are to be multiplied by (fp16)
+    static constexpr int kTables = kRow + 3 * 32 * 4;
+    // of a chunk and of the next one: [64] G as two numbers, [64] 2^(G_end - G_j), 2^G_end and G_end
+    static constexpr int kG = 0, kW = 64 * 8, kFade = kW + 64 * 4, kTableBytes = kFade + 16;
+    static constexpr int kBytes = kTables + 2 * kTableBytes;
 };
 
 template <typename T, int DK, int NW, int MODE>
-__global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearArgs a, const LinearParts p) {
+__global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_chunk_kernel(const LinearArgs a, const LinearParts p) {
     typedef LinearLds<DK, NW> L;
     constexpr bool kBf16 = T::kStorageFormat == WARP34_KV_FORMAT_BF16;
-    constexpr int kThreads = 64 * NW, KP = DK / 8, VP = 4 * NW, KT = DK / 32;  // pieces of 16 bytes a row, tiles of 32 channels
+    constexpr int DV = 32 * NW, kThreads = 64 * NW, KP = DK / 8, VP = 4 * NW, KT = DK / 32;  // pieces of 16 bytes a row, tiles of 32 channels
     constexpr int kLoads = kLinearChunk * KP / kThreads;
     constexpr int kParts = !kBf16 ? 2 : MODE == kLinearRows ? 2 : 3;  // of weighted values
     __shared__ __attribute__((aligned(16))) uint8_t smem[L::kBytes];
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), n32 = lane & 31, b = lane >> 5;
-    const int slices = a.v_dim / (32 * NW), columns = a.v_heads * slices;
-    int at = (int)(blockIdx.x % (uint32_t)columns), group = (int)(blockIdx.x / (uint32_t)columns);
+    const int group = (int)(blockIdx.x / (uint32_t)a.v_heads);
+    int head = (int)(blockIdx.x - (uint32_t)group * (uint32_t)a.v_heads);
     // workgroups go round the eight dies: value heads of the same keys on the same one
-    if (a.v_heads % 8 == 0) at = (at % 8) * (columns / 8) + at / 8;
-    const int head = at / slices, slice = at - head * slices, kh = head / a.group;
+    if (a.v_heads % 8 == 0) head = (head % 8) * (a.v_heads / 8) + head / 8;
+    const int kh = head / a.group;
     int req = group, part = 0;
     if (MODE == kLinearWalk) {
         if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
     } else {
         if (!linear_find_part(a, p.log_length, group, req, part)) return;
     }
-    const LinearRequest r = linear_request(a, req, head, DK * a.v_dim);
-    const int col0 = slice * 32 * NW, my_col = col0 + 32 * wave + n32;
+    LinearRequest r = linear_request(a, req, head, DK * DV);
+    r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.n = __builtin_amdgcn_readfirstlane(r.n), r.kept = __builtin_amdgcn_readfirstlane(r.kept);
+    const int state_at = 4 * b * DV + 32 * wave + n32;  // element of the state that is this lane's first
 
     int begin = 0, stop = r.n;
     if (MODE != kLinearWalk) linear_part_range(r.n, r.kept, p.log_length, part, begin, stop);
     else if (a.out == nullptr) stop = r.kept;
+    begin = __builtin_amdgcn_readfirstlane(begin), stop = __builtin_amdgcn_readfirstlane(stop);
 
     f16v s[KT];
 #pragma unroll
@@ -178,12 +189,12 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
     int unit = 0;  // s holds the state times 2^unit (fp16)
     // this wave's share of a part's state in scratch
     float* const mine = MODE == kLinearWalk ? nullptr
-                                            : p.states + ((int64_t)group * a.v_heads + head) * (DK * a.v_dim) + (int64_t)(slice * NW + wave) * (32 * DK) + lane * 4;
+                                            : p.states + ((int64_t)group * a.v_heads + head) * (DK * DV) + wave * (32 * DK) + lane * 4;
     if (MODE == kLinearWalk && r.in != nullptr) {
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[d][i] = r.in[(32 * d + (i & 3) + 8 * (i >> 2) + 4 * b) * a.v_dim + my_col];
+            for (int i = 0; i < 16; ++i) s[d][i] = r.in[state_at + (32 * d + (i & 3) + 8 * (i >> 2)) * DV];
     }
     if (MODE == kLinearRows) {
 #pragma unroll
@@ -197,74 +208,88 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
     }
     const auto put_state = [&]() {
         const float by = power_of_two(-unit);
+        int first = state_at;
+        asm volatile("" : "+v"(first));  // addresses are worked out here, not kept in registers through the chunks
+        float* const to = r.out + first;
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) r.out[(32 * d + (i & 3) + 8 * (i >> 2) + 4 * b) * a.v_dim + my_col] = kBf16 ? s[d][i] : s[d][i] * by;
+            for (int i = 0; i < 16; ++i) to[(32 * d + (i & 3) + 8 * (i >> 2)) * DV] = kBf16 ? s[d][i] : s[d][i] * by;
     };
     if (MODE == kLinearWalk && r.kept == 0 && r.out != nullptr) put_state();
 
-    // a chunk on its way: rows behind its last token are zeros, whatever is there
-    const bool with_q = MODE != kLinearSums && a.out != nullptr;
-    uint4 qx[kLoads], kx[kLoads], vx[4];
+    // a chunk on its way
+    const bool with_q = MODE == kLinearRows || (MODE == kLinearWalk && a.out != nullptr);
+    u4 qx[kLoads], kx[kLoads], vx[4];
     float gx = 0.f;
     int chunk_end = begin;
     const auto chunk_stop = [&](int t) { return min(t + kLinearChunk, MODE == kLinearWalk && t < r.kept ? r.kept : stop); };
+    const int k_row = tid / KP, k_piece = tid % KP, v_row = tid / VP, v_piece = tid % VP;  // its first 16 bytes; the others are rows further down
     const auto fetch = [&](int t, int end) {
-        const int last = end - 1;
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int x = tid + i * kThreads, row = x / KP, piece = x % KP;
-            const int64_t tok = r.lo + min(t + row, last);
-            kx[i] = *reinterpret_cast<const uint4*>(a.k + tok * a.k_stride + kh * DK + piece * 8);
-            if (with_q) qx[i] = *reinterpret_cast<const uint4*>(a.q + tok * a.q_stride + kh * DK + piece * 8);
-            if (t + row > last) kx[i] = qx[i] = uint4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int x = tid + i * kThreads, row = x / VP, piece = x % VP;
-            const int64_t tok = r.lo + min(t + row, last);
-            vx[i] = *reinterpret_cast<const uint4*>(a.v + tok * a.v_stride + head * a.v_dim + col0 + piece * 8);
-            if (t + row > last) vx[i] = uint4{0, 0, 0, 0};
-        }
-        gx = 0.f;
-        if (a.g != nullptr && wave == NW - 1 && t + lane <= last) gx = a.g[(int64_t)(r.lo + t + lane) * a.g_stride + head];
-    };
-    const auto at_lds = [&](uint32_t offset) { return smem + offset; };
-    const auto put = [&]() {
-#pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int x = tid + i * kThreads;
-            *reinterpret_cast<uint4*>(at_lds(L::kK + linear_piece<KP>(x / KP, x % KP))) = kx[i];
-            if (with_q) *reinterpret_cast<uint4*>(at_lds(L::kQ + linear_piece<KP>(x / KP, x % KP))) = qx[i];
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int x = tid + i * kThreads;
-            *reinterpret_cast<uint4*>(at_lds(L::kV + linear_piece<VP>(x / VP, x % VP))) = vx[i];
-        }
+        const int rows = end - t;
+        const int64_t tok = r.lo + t;
         if (wave == NW - 1) {
-            double run = (double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634;
-#pragma unroll
-            for (int by = 1; by < 64; by *= 2) {
-                const double o = __shfl_up(run, by, 64);
-                if (lane >= by) run += o;
-            }
-            const double all = __shfl(run, 63, 64);
-            const float hi = (float)run;
-            *reinterpret_cast<float2*>(at_lds(L::kG + lane * 8)) = make_float2(hi, (float)(run - hi));
-            *reinterpret_cast<float*>(at_lds(L::kW + lane * 4)) = __builtin_amdgcn_exp2f((float)(all - run));
-            if (lane == 0) *reinterpret_cast<float2*>(at_lds(L::kFade)) = make_float2(__builtin_amdgcn_exp2f((float)all), (float)all);
+            gx = 0.f;
+            if (a.g != nullptr && lane < rows) gx = a.g[(tok + lane) * a.g_stride + head];
         }
+        const auto k = linear_rows(a.k + tok * a.k_stride + kh * DK, rows, a.k_stride, DK), v = linear_rows(a.v + tok * a.v_stride + head * DV, rows, a.v_stride, DV);
+        const auto q = linear_rows(a.q + tok * a.q_stride + kh * DK, rows, a.q_stride, DK);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) kx[i] = __builtin_amdgcn_raw_buffer_load_b128(k, 2 * a.k_stride * (k_row + i * (kThreads / KP)) + 16 * k_piece, 0, 0);
+        if (with_q) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) qx[i] = __builtin_amdgcn_raw_buffer_load_b128(q, 2 * a.q_stride * (k_row + i * (kThreads / KP)) + 16 * k_piece, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vx[i] = __builtin_amdgcn_raw_buffer_load_b128(v, 2 * a.v_stride * (v_row + i * (kThreads / VP)) + 16 * v_piece, 0, 0);
     };
-    const auto operand = [&](uint32_t offset) { return *reinterpret_cast<const u4*>(at_lds(offset)); };
-    // rows 16 step + 4 b + 0 .. 3 and the same + 8, columns 8 first_piece + n32
-    const auto transposed = [&](uint32_t base, auto pieces, int first_piece, int step) -> u4 {
-        constexpr int PIECES = decltype(pieces)::value;
-        const int j = lane & 15, row = 16 * step + 4 * b + (j >> 2), piece = first_piece + 2 * (lane >> 4 & 1) + (j >> 1 & 1);
-        const uint32_t lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem + base + 8u * (uint32_t)(j & 1);
-        const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(lds + linear_piece<PIECES>(row, piece))));
-        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(lds + linear_piece<PIECES>(row + 8, piece))));
+    // k and v as they are, q in the order of the state's rows: of 16 channels 0 .. 3, 8 .. 11 and 4 .. 7, 12 .. 15
+    const auto put = [&]() {
+        uint8_t* const kt = smem + L::kK + k_row * L::kKRow + k_piece * 16;
+        uint8_t* const qt = smem + L::kQ + k_row * L::kKRow + (k_piece >> 1) * 32 + (k_piece & 1) * 8;
+        uint8_t* const vt = smem + L::kV + v_row * L::kVRow + v_piece * 16;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            *reinterpret_cast<u4*>(kt + i * (kThreads / KP) * L::kKRow) = kx[i];
+            if (with_q) {
+                *reinterpret_cast<u2v*>(qt + i * (kThreads / KP) * L::kKRow) = u2v{qx[i][0], qx[i][1]};
+                *reinterpret_cast<u2v*>(qt + i * (kThreads / KP) * L::kKRow + 16) = u2v{qx[i][2], qx[i][3]};
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<u4*>(vt + i * (kThreads / VP) * L::kVRow) = vx[i];
+    };
+    // the last wave's: the tables of the chunk that has been fetched
+    uint8_t* tables = smem + L::kTables;  // of the present chunk, and of the next one
+    uint8_t* next_tables = tables + L::kTableBytes;
+    const auto put_tables = [&](uint8_t* to) {
+        double run = (double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634;
+#pragma unroll
+        for (int by = 1; by < 64; by *= 2) {
+            const double o = __shfl_up(run, by, 64);
+            if (lane >= by) run += o;
+        }
+        const double all = __shfl(run, 63, 64);
+        const float hi = (float)run;
+        *reinterpret_cast<float2*>(to + L::kG + lane * 8) = make_float2(hi, (float)(run - hi));
+        *reinterpret_cast<float*>(to + L::kW + lane * 4) = __builtin_amdgcn_exp2f((float)(all - run));
+        if (lane == 0) *reinterpret_cast<float2*>(to + L::kFade) = make_float2(__builtin_amdgcn_exp2f((float)all), (float)all);
+    };
+    const uint8_t* const k_at = smem + L::kK + n32 * L::kKRow + 8 * b;   // of key n32: channels 4 b and 8 + 4 b of 16
+    const uint8_t* const q_at = smem + L::kQ + n32 * L::kKRow + 16 * b;  // of query n32
+    const auto k_operand = [&](int kt, int step) {
+        const u2v x = *reinterpret_cast<const u2v*>(k_at + 32 * kt * L::kKRow + 32 * step), y = *reinterpret_cast<const u2v*>(k_at + 32 * kt * L::kKRow + 32 * step + 16);
+        return u4{x[0], x[1], y[0], y[1]};
+    };
+    const auto q_operand = [&](int qt, int step) { return *reinterpret_cast<const u4*>(q_at + 32 * qt * L::kKRow + 32 * step); };
+    uint8_t* const p_at = smem + L::kP + lane * 16;
+    // transposed: rows 16 step + 4 b + 0 .. 3 and the same + 8, a column a lane of 32
+    const int j16 = lane & 15, tr_row = 4 * b + (j16 >> 2), tr_byte = 32 * (lane >> 4 & 1) + 8 * (j16 & 3);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
+    const uint32_t kt_at = lds0 + (uint32_t)(L::kK + tr_row * L::kKRow + tr_byte), vt_at = lds0 + (uint32_t)(L::kV + tr_row * L::kVRow + 64 * wave + tr_byte);
+    const auto transposed = [&](uint32_t at, int row_bytes) -> u4 {
+        const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
+        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(at + 8u * (uint32_t)row_bytes)));
         const u2v u = __builtin_bit_cast(u2v, x), w = __builtin_bit_cast(u2v, y);
         return u4{u[0], u[1], w[0], w[1]};
     };
@@ -272,17 +297,15 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
     // Tile 0: queries 0 .. 31 over keys 0 .. 31, 1: queries 32 .. 63 over keys 0 .. 31, 2: over keys 32 .. 63.
     const auto weights = [&](int tile) {
         const int kt = tile == 2 ? 1 : 0, qt = tile == 0 ? 0 : 1;
-        f16v x;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = 0.f;
+        f16v x = {};
 #pragma unroll
         for (int step = 0; step < DK / 16; ++step)
-            x = linear_mfma<T>(operand(L::kK + linear_piece<KP>(32 * kt + n32, 2 * step + b)), operand(L::kQ + linear_piece<KP>(32 * qt + n32, 2 * step + b)), x);
-        const float2 gi = *reinterpret_cast<const float2*>(at_lds(L::kG + (32 * qt + n32) * 8));
+            x = linear_mfma<T>(k_operand(kt, step), q_operand(qt, step), x);
+        const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + (32 * qt + n32) * 8);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int key = (i & 3) + 8 * (i >> 2) + 4 * b;
-            const float2 gj = *reinterpret_cast<const float2*>(at_lds(L::kG + (32 * kt + key) * 8));
+            const float2 gj = *reinterpret_cast<const float2*>(tables + L::kG + (32 * kt + key) * 8);
             const float w = x[i] * __builtin_amdgcn_exp2f((gi.x - gj.x) + (gi.y - gj.y));
             x[i] = tile == 1 || key <= n32 ? w : 0.f;
         }
@@ -296,7 +319,7 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
             const float by = power_of_two(e);
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] *= by;
-            if (b == 0) *reinterpret_cast<float*>(at_lds(L::kRow + (tile * 32 + n32) * 4)) = power_of_two(-e);
+            if (b == 0) *reinterpret_cast<float*>(smem + L::kRow + (tile * 32 + n32) * 4) = power_of_two(-e);
         }
 #pragma unroll
         for (int step = 0; step < 2; ++step) {
@@ -307,30 +330,28 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 linear_split<T, 2>(x[8 * step + 2 * k], x[8 * step + 2 * k + 1], w);
                 hi[k] = w[0], lo[k] = w[1];
             }
-            *reinterpret_cast<u4*>(at_lds(L::kP + tile * 4096 + step * 1024 + lane * 16)) = hi;
-            *reinterpret_cast<u4*>(at_lds(L::kP + tile * 4096 + 2048 + step * 1024 + lane * 16)) = lo;
+            *reinterpret_cast<u4*>(p_at + tile * 4096 + step * 1024) = hi;
+            *reinterpret_cast<u4*>(p_at + tile * 4096 + 2048 + step * 1024) = lo;
         }
     };
 
     float part_sum = 0.f;  // of g, for the scan over parts
-    if (begin < stop) fetch(begin, chunk_end = chunk_stop(begin));
+    if (begin < stop) {
+        fetch(begin, chunk_end = chunk_stop(begin));
+        if (wave == NW - 1) put_tables(tables);
+    }
     for (int t = begin; t < stop;) {
-        const int end = chunk_end, length = end - t;
-        __syncthreads();
+        const int end = chunk_end;
         put();
         __syncthreads();
-        if (end < stop) fetch(end, chunk_end = chunk_stop(end));
-        const bool two = length > 32;
-        f16v o[2];
+        if (end < stop) {
+            fetch(end, chunk_end = chunk_stop(end));
+            if (wave == NW - 1) put_tables(next_tables);
+        }
+        f16v o[2] = {};
         if (with_q) {
-            if (NW == 4) {
-                if (wave == 0 || (wave < 3 && two)) weights(wave);
-            } else if (wave == 0) {
-                weights(0);
-                if (two) weights(1);
-            } else if (two) {
-                weights(2);
-            }
+            if (NW == 4 ? wave < 3 : wave == 1) weights(NW == 4 ? wave : 2);
+            if (NW == 2 && wave == 0) weights(0), weights(1);
             // the state's part of the rows
             int e = 0;
             if constexpr (!kBf16) {
@@ -342,10 +363,6 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 e = scale_exponent(wave_max(top));
             }
             const float by = power_of_two(e);
-#pragma unroll
-            for (int q = 0; q < 2; ++q)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[q][i] = 0.f;
 #pragma unroll
             for (int step = 0; step < DK / 16; ++step) {
                 u4 part_of[2];
@@ -360,17 +377,14 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 }
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    if (q == 1 && !two) continue;
-                    const u2v x = *reinterpret_cast<const u2v*>(at_lds(L::kQ + linear_piece<KP>(32 * q + n32, 2 * step) + 8 * b));
-                    const u2v y = *reinterpret_cast<const u2v*>(at_lds(L::kQ + linear_piece<KP>(32 * q + n32, 2 * step + 1) + 8 * b));
-                    const u4 qo = {x[0], x[1], y[0], y[1]};
+                    const u4 qo = q_operand(q, step);
                     o[q] = linear_mfma<T>(part_of[0], qo, o[q]);
                     o[q] = linear_mfma<T>(part_of[1], qo, o[q]);
                 }
             }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const float2 gi = *reinterpret_cast<const float2*>(at_lds(L::kG + (32 * q + n32) * 8));
+                const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + (32 * q + n32) * 8);
                 const float f = __builtin_amdgcn_exp2f(gi.x + gi.y) * (kBf16 ? 1.f : power_of_two(-e - unit));
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[q][i] *= f;
@@ -378,45 +392,42 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
         }
         u4 v[4];
 #pragma unroll
-        for (int step = 0; step < 4; ++step) v[step] = transposed(L::kV, std::integral_constant<int, VP>{}, 4 * wave, step);
+        for (int step = 0; step < 4; ++step) v[step] = transposed(vt_at + 16 * step * L::kVRow, L::kVRow);
         if (with_q) {
             __syncthreads();
 #pragma unroll
             for (int tile = 0; tile < 3; ++tile) {
-                if (tile > 0 && !two) continue;
                 const int kt = tile == 2 ? 1 : 0, qt = tile == 0 ? 0 : 1;
                 if constexpr (kBf16) {
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) o[qt] = linear_mfma<T>(v[2 * kt + (x & 1)], operand(L::kP + tile * 4096 + x * 1024 + lane * 16), o[qt]);
+                    for (int x = 0; x < 4; ++x) o[qt] = linear_mfma<T>(v[2 * kt + (x & 1)], *reinterpret_cast<const u4*>(p_at + tile * 4096 + x * 1024), o[qt]);
                 } else {
-                    f16v sum;
+                    f16v sum = {};
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) sum[i] = 0.f;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) sum = linear_mfma<T>(v[2 * kt + (x & 1)], operand(L::kP + tile * 4096 + x * 1024 + lane * 16), sum);
-                    const float f = *reinterpret_cast<const float*>(at_lds(L::kRow + (tile * 32 + n32) * 4));
+                    for (int x = 0; x < 4; ++x) sum = linear_mfma<T>(v[2 * kt + (x & 1)], *reinterpret_cast<const u4*>(p_at + tile * 4096 + x * 1024), sum);
+                    const float f = *reinterpret_cast<const float*>(smem + L::kRow + (tile * 32 + n32) * 4);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[qt][i] = __builtin_fmaf(sum[i], f, o[qt][i]);
                 }
             }
             // lanes n32 and n32 + 32 have one row's columns in turns of four: exchanged, each has eight in a row
+            const auto rows = linear_rows(a.out + (int64_t)(r.lo + t) * a.out_stride + head * DV, end - t, a.out_stride, DV);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int row = t + 32 * q + n32;
-                uint16_t* to = a.out + (int64_t)(r.lo + row) * a.out_stride + head * a.v_dim + col0 + 32 * wave + 8 * b;
                 uint32_t w[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) w[k] = (uint32_t)T::from_f32(o[q][2 * k] * a.scale) | (uint32_t)T::from_f32(o[q][2 * k + 1] * a.scale) << 16;
+                for (int k = 0; k < 8; ++k) w[k] = linear_pack<T>(o[q][2 * k] * a.scale, o[q][2 * k + 1] * a.scale);
+                const int to = 2 * (a.out_stride * (32 * q + n32) + 32 * wave + 8 * b);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const auto x = __builtin_amdgcn_permlane32_swap(w[4 * k], w[4 * k + 2], false, false);
                     const auto y = __builtin_amdgcn_permlane32_swap(w[4 * k + 1], w[4 * k + 3], false, false);
-                    if (row < end) *reinterpret_cast<u4*>(to + 16 * k) = u4{x[0], y[0], x[1], y[1]};
+                    __builtin_amdgcn_raw_buffer_store_b128(u4{x[0], y[0], x[1], y[1]}, rows, to + 32 * k, 0, 0);
                 }
             }
         }
         // the state moves on
-        const float2 fade = *reinterpret_cast<const float2*>(at_lds(L::kFade));
+        const float2 fade = *reinterpret_cast<const float2*>(tables + L::kFade);
         if (MODE == kLinearSums) part_sum += fade.y;
         if (MODE != kLinearRows || end < stop) {
             int next = unit;
@@ -437,9 +448,8 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 for (int i = 0; i < 16; ++i) s[d][i] *= by;
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
-                if (16 * step >= length) continue;
                 u4 x[kParts];
-                const f4 w0 = *reinterpret_cast<const f4*>(at_lds(L::kW + (16 * step + 4 * b) * 4)), w1 = *reinterpret_cast<const f4*>(at_lds(L::kW + (16 * step + 8 + 4 * b) * 4));
+                const f4 w0 = *reinterpret_cast<const f4*>(tables + L::kW + (16 * step + 4 * b) * 4), w1 = *reinterpret_cast<const f4*>(tables + L::kW + (16 * step + 8 + 4 * b) * 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const f4 w = k < 2 ? w0 : w1;
@@ -452,13 +462,18 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 }
 #pragma unroll
                 for (int d = 0; d < KT; ++d) {
-                    const u4 k = transposed(L::kK, std::integral_constant<int, KP>{}, 4 * d, step);
+                    const u4 k = transposed(kt_at + 16 * step * L::kKRow + 64 * d, L::kKRow);
 #pragma unroll
                     for (int q = 0; q < kParts; ++q) s[d] = linear_mfma<T>(k, x[q], s[d]);
                 }
             }
         }
         t = end;
+        {
+            uint8_t* const x = tables;
+            tables = next_tables, next_tables = x;
+        }
+        __syncthreads();
         if (MODE == kLinearWalk && t == r.kept && r.out != nullptr) put_state();
     }
     if (MODE == kLinearSums) {
@@ -472,7 +487,7 @@ __global__ __launch_bounds__(64 * NW, 2) void linear_chunk_kernel(const LinearAr
                 for (int i = 0; i < 4; ++i) x[i] = kBf16 ? s[d][4 * ig + i] : s[d][4 * ig + i] * by;
                 *reinterpret_cast<f4*>(mine + (d * 4 + ig) * 256) = x;
             }
-        if (tid == 0 && slice == 0) p.fades[(int64_t)group * a.v_heads + head] = __builtin_amdgcn_exp2f(part_sum);
+        if (tid == 0) p.fades[(int64_t)group * a.v_heads + head] = __builtin_amdgcn_exp2f(part_sum);
     }
 }
 
