@@ -5,8 +5,7 @@
 // Workgroup = the columns of a value head, a wave 32 of them with their part of the state in registers; 32x32x16 MFMAs:
 //   P^T = K Q^T        one 32x32 tile a wave (three of them: a chunk's second half of keys is not seen by its first half of queries),
 //                      weighted, and laid into LDS as the operands of the product below
-//   O^T = S^T Q^T      the state's registers are the operand as they stand: lane (n, b) has column n for rows (i & 3) + 8 (i >> 2) + 4 b,
-//                      eight of them are 16 channels of which q is read in the same order
+//   O^T = S^T Q^T      the state's registers are the operand as they stand: lane (n, b) has column n for channels 16 (i >> 3) + 8 b + (i & 7)
 //   O^T += V^T P^T     v through transposing reads (ds_read_b64_tr_b16: lane l of 16 gets column l of four rows of 16 values)
 //   S += K^T V'        k and v through transposing reads, v weighted in registers
 // Weights are exponentials of differences of G, which is summed in 64 bits and held as two 32-bit numbers: where all but the last
@@ -129,9 +128,10 @@ __device__ __forceinline__ float wave_max(float x) {
     return x;
 }
 
-// Bytes from a row to the next one: 32 more than the row, so that the four rows of a transposing read touch different banks, as do any eight
-// rows of an operand read, and addresses are one register and constants.
-constexpr int linear_row(int bytes) { return bytes + 32; }
+// Rows in LDS are 16 bytes longer than they need to be, and of 16 rows the place of one is its number with the two pairs of bits exchanged: an
+// operand read of 16 rows touches all banks, and so do the four rows of a transposing read, 64 bytes apart with two columns of 32 each.
+constexpr int linear_row(int bytes) { return bytes + 16; }
+__device__ __forceinline__ int linear_place(int row) { return (row & ~15) | (row & 3) << 2 | (row >> 2 & 3); }
 
 // `rows` rows of `width` 16-bit elements from `base` on: loads behind the last row give zeros, stores there are dropped.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t linear_rows(const uint16_t* base, int rows, int stride, int width) {
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     }
     LinearRequest r = linear_request(a, req, head, DK * DV);
     r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.n = __builtin_amdgcn_readfirstlane(r.n), r.kept = __builtin_amdgcn_readfirstlane(r.kept);
-    const int state_at = 4 * b * DV + 32 * wave + n32;  // element of the state that is this lane's first
+    const int state_at = 8 * b * DV + 32 * wave + n32;  // element of the state that is this lane's first
 
     int begin = 0, stop = r.n;
     if (MODE != kLinearWalk) linear_part_range(r.n, r.kept, p.log_length, part, begin, stop);
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[d][i] = r.in[state_at + (32 * d + (i & 3) + 8 * (i >> 2)) * DV];
+            for (int i = 0; i < 16; ++i) s[d][i] = r.in[state_at + (32 * d + 16 * (i >> 3) + (i & 7)) * DV];
     }
     if (MODE == kLinearRows) {
 #pragma unroll
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[(32 * d + (i & 3) + 8 * (i >> 2)) * DV] = kBf16 ? s[d][i] : s[d][i] * by;
+            for (int i = 0; i < 16; ++i) to[(32 * d + 16 * (i >> 3) + (i & 7)) * DV] = kBf16 ? s[d][i] : s[d][i] * by;
     };
     if (MODE == kLinearWalk && r.kept == 0 && r.out != nullptr) put_state();
 
@@ -243,18 +243,16 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
 #pragma unroll
         for (int i = 0; i < 4; ++i) vx[i] = __builtin_amdgcn_raw_buffer_load_b128(v, 2 * a.v_stride * (v_row + i * (kThreads / VP)) + 16 * v_piece, 0, 0);
     };
-    // k and v as they are, q in the order of the state's rows: of 16 channels 0 .. 3, 8 .. 11 and 4 .. 7, 12 .. 15
     const auto put = [&]() {
-        uint8_t* const kt = smem + L::kK + k_row * L::kKRow + k_piece * 16;
-        uint8_t* const qt = smem + L::kQ + k_row * L::kKRow + (k_piece >> 1) * 32 + (k_piece & 1) * 8;
-        uint8_t* const vt = smem + L::kV + v_row * L::kVRow + v_piece * 16;
+        uint8_t* const kt = smem + L::kK + linear_place(k_row) * L::kKRow + k_piece * 16;
+        uint8_t* const vt = smem + L::kV + linear_place(v_row) * L::kVRow + v_piece * 16;
+        // a thread's further rows are whole sixteens away, or eights (two places)
+        constexpr auto further = [](int rows) { return (rows & ~15) + (rows & 8 ? 2 : 0); };
+        static_assert(kThreads / KP % 8 == 0 && kThreads / VP % 16 == 0, "rows of a pass");
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            *reinterpret_cast<u4*>(kt + i * (kThreads / KP) * L::kKRow) = kx[i];
-            if (with_q) {
-                *reinterpret_cast<u2v*>(qt + i * (kThreads / KP) * L::kKRow) = u2v{qx[i][0], qx[i][1]};
-                *reinterpret_cast<u2v*>(qt + i * (kThreads / KP) * L::kKRow + 16) = u2v{qx[i][2], qx[i][3]};
-            }
+            *reinterpret_cast<u4*>(kt + further(i * (kThreads / KP)) * L::kKRow) = kx[i];
+            if (with_q) *reinterpret_cast<u4*>(kt + (L::kQ - L::kK) + further(i * (kThreads / KP)) * L::kKRow) = qx[i];
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<u4*>(vt + i * (kThreads / VP) * L::kVRow) = vx[i];
@@ -275,21 +273,19 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         *reinterpret_cast<float*>(to + L::kW + lane * 4) = __builtin_amdgcn_exp2f((float)(all - run));
         if (lane == 0) *reinterpret_cast<float2*>(to + L::kFade) = make_float2(__builtin_amdgcn_exp2f((float)all), (float)all);
     };
-    const uint8_t* const k_at = smem + L::kK + n32 * L::kKRow + 8 * b;   // of key n32: channels 4 b and 8 + 4 b of 16
-    const uint8_t* const q_at = smem + L::kQ + n32 * L::kKRow + 16 * b;  // of query n32
-    const auto k_operand = [&](int kt, int step) {
-        const u2v x = *reinterpret_cast<const u2v*>(k_at + 32 * kt * L::kKRow + 32 * step), y = *reinterpret_cast<const u2v*>(k_at + 32 * kt * L::kKRow + 32 * step + 16);
-        return u4{x[0], x[1], y[0], y[1]};
-    };
-    const auto q_operand = [&](int qt, int step) { return *reinterpret_cast<const u4*>(q_at + 32 * qt * L::kKRow + 32 * step); };
+    const uint8_t* const row_at = smem + linear_place(n32) * L::kKRow + 16 * b;  // channels 8 b .. + 7 of 16 of row n32
+    const auto k_operand = [&](int kt, int step) { return *reinterpret_cast<const u4*>(row_at + L::kK + 32 * kt * L::kKRow + 32 * step); };
+    const auto q_operand = [&](int qt, int step) { return *reinterpret_cast<const u4*>(row_at + L::kQ + 32 * qt * L::kKRow + 32 * step); };
     uint8_t* const p_at = smem + L::kP + lane * 16;
-    // transposed: rows 16 step + 4 b + 0 .. 3 and the same + 8, a column a lane of 32
-    const int j16 = lane & 15, tr_row = 4 * b + (j16 >> 2), tr_byte = 32 * (lane >> 4 & 1) + 8 * (j16 & 3);
+    // transposed: rows 16 step + 4 b + 0 .. 3 and the same + 8, a column a lane of 32.  Of 16 channels of k the second four and the third change
+    // places, so that eight registers of a lane's state are eight channels in a row, 8 b .. + 7 of 16, as q and k are read above.
+    const int j16 = lane & 15, tr_place = 4 * (j16 >> 2) + b, tr_byte = 32 * (lane >> 4 & 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    const uint32_t kt_at = lds0 + (uint32_t)(L::kK + tr_row * L::kKRow + tr_byte), vt_at = lds0 + (uint32_t)(L::kV + tr_row * L::kVRow + 64 * wave + tr_byte);
+    const uint32_t kt_at = lds0 + (uint32_t)(L::kK + tr_place * L::kKRow + tr_byte + 16 * (j16 & 1) + 4 * (j16 & 2));
+    const uint32_t vt_at = lds0 + (uint32_t)(L::kV + tr_place * L::kVRow + 64 * wave + tr_byte + 8 * (j16 & 3));
     const auto transposed = [&](uint32_t at, int row_bytes) -> u4 {
         const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
-        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(at + 8u * (uint32_t)row_bytes)));
+        const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(at + 2u * (uint32_t)row_bytes)));
         const u2v u = __builtin_bit_cast(u2v, x), w = __builtin_bit_cast(u2v, y);
         return u4{u[0], u[1], w[0], w[1]};
     };
@@ -502,7 +498,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(const LinearArgs a, co
     const int first = linear_first_part(a, p.log_length, req), parts = linear_parts_of(r.n, r.kept, p.log_length);
     const int x = block * 256 + (int)threadIdx.x;  // [32 columns][32 channels][4 x 8 channels][lane]
     const int lane = x & 63, ig = x >> 6 & 3, tiles = k_dim / 32, d = (x >> 8) % tiles, w = (x >> 8) / tiles;
-    const int row = 32 * d + 8 * ig + 4 * (lane >> 5), col = 32 * w + (lane & 31);
+    const int row = 32 * d + 16 * (ig >> 1) + 8 * (lane >> 5) + 4 * (ig & 1), col = 32 * w + (lane & 31);
     f4 s = {0.f, 0.f, 0.f, 0.f};
     if (r.in != nullptr) {
 #pragma unroll
