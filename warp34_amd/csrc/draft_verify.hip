@@ -5,7 +5,7 @@
 // in 64 bits: a running sum over 10^5 entries in 32 bits is 10^-7 off at each of them, which moves one border in a thousand draws.
 //
 // One row of p (and of q) a request is all that is read, by as many workgroups as there are tiles of kDraftTile entries; a second launch, a
-// wave a request, finds the tile by the tiles' sums and the entry inside it.
+// workgroup a request, finds the tile by the tiles' sums and the entry inside it.
 // Bound: latency for a few requests, HBM for many.
 #include "../../include/warp34_drafts.h"
 #include "attn_launch.h"
@@ -163,94 +163,132 @@ __global__ __launch_bounds__(kDraftThreads) void draft_sums_kernel(const DraftAr
     if (threadIdx.x == 0) a.sums[(int64_t)req * a.tiles + tile] = s;
 }
 
-// The token drawn by one wave, the same in every lane.  mine: the sums of the lane's tiles, `each` in a row.
-__device__ int draw_token(const DraftWeights& w, double u, double2 mine, int each, int tiles) {
-    const int lane = lane_id();
-    const double run_p = wave_run(mine.x), run_rest = wave_run(mine.y);
-    const double total_p = lane_value(run_p, 63), total_rest = lane_value(run_rest, 63);
-    const bool from_rest = w.refused >= 0 && total_rest > 0.0;
-    const double total = from_rest ? total_rest : total_p, target = u * total;
-    if (!(total > 0.0)) return -1;
-    const double have = from_rest ? mine.y : mine.x, run = from_rest ? run_rest : run_p;
-    // the lowest lane whose tiles pass the target, or the last one with any weight, which stands in where rounding leaves none
-    const unsigned long long weighted = __ballot(have > 0.0), past = __ballot(have > 0.0 && run > target);
-    if (weighted == 0) return -1;
-    const int owner = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(weighted);
-    double before = lane_value(run - have, owner);
-    int last = -1;  // the last entry with any weight so far
-    constexpr int kStep = 64 * 16;
-    for (int64_t x = (int64_t)owner * each * kDraftTile; x < min((int64_t)(owner + 1) * each * kDraftTile, (int64_t)w.vocab); x += 2 * kStep) {
-        DraftEntries<4> e[2];
-        e[0].load(w, (int)x + lane * 16);
-        if (x + kStep < w.vocab) e[1].load(w, (int)x + kStep + lane * 16);
+// The entry of tile `owner`, in front of which weigh `before`, at which the running sum passes the target, by a workgroup: the wave whose entries
+// pass it, of these the lane, of its entries the one.  Where rounding lets none pass, the last one with any weight stands in (the tile has some).
+// The result is that wave's; the others get -1.
+__device__ __forceinline__ int draw_entry(DraftWeights w, bool from_rest, double target, int owner, double before, double* waves) {
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    if (!from_rest) w.q = nullptr, w.refused = -1;
+    DraftEntries<kDraftEntries / 4> e;
+    e.load(w, owner * kDraftTile + (int)threadIdx.x * kDraftEntries);
+    double sum = 0.0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            if (x + half * kStep >= w.vocab) break;
-            double v[16], sum = 0.0;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = from_rest ? e[half].rest(w, i) : e[half].whole(i), sum += v[i];
-            const double upto = wave_run(sum);
-            double at = before + (upto - sum);
-            int here = -1, some = -1;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                at += v[i];
-                if (v[i] > 0.0) {
-                    some = e[half].x0 + i;
-                    if (at > target && here < 0) here = some;
-                }
-            }
-            const unsigned long long hits = __ballot(here >= 0), any = __ballot(some >= 0);
-            if (hits) return __builtin_amdgcn_readlane(here, __builtin_ctzll(hits));
-            if (any) last = __builtin_amdgcn_readlane(some, 63 - __builtin_clzll(any));
-            before += lane_value(upto, 63);
-        }
+    for (int i = 0; i < kDraftEntries; ++i) sum += e.rest(w, i);
+    const double run = wave_run(sum);
+    __syncthreads();
+    if (lane == 63) waves[wave] = run;
+    __syncthreads();
+    int mine = -1;
+    double at = before;
+    for (int k = 0; k < kDraftThreads / 64; ++k) {
+        const double have = waves[k];
+        if (have > 0.0) mine = k, before = at;
+        at += have;
+        if (have > 0.0 && at > target) break;
     }
-    return last;
+    if (wave != mine) return -1;
+    const unsigned long long some = __ballot(sum > 0.0), past = __ballot(sum > 0.0 && before + run > target);
+    const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+    before += lane_value(run - sum, l);
+    const int first = owner * kDraftTile + (wave * 64 + l) * kDraftEntries, x = first + lane;
+    double v = 0.0;
+    if (lane < kDraftEntries && x < w.vocab) {
+        const double p = proper(w.p[x]);
+        v = w.q != nullptr ? p - proper(w.q[x]) : x == w.refused ? 0.0 : p;
+        v = v > 0.0 ? v : 0.0;
+    }
+    const double upto = wave_run(v);
+    const unsigned long long any = __ballot(v > 0.0), hit = __ballot(v > 0.0 && before + upto > target);
+    return first + (hit ? __builtin_ctzll(hit) : 63 - __builtin_clzll(any));
 }
 
-// By the first wave: the request's tokens.
-__device__ __forceinline__ void put_tokens(const DraftArgs& a, int req, const DraftRow& d, int drawn) {
-    for (int i = lane_id(); i < d.n; i += 64) a.out_tokens[d.lo + i] = i < d.accepted ? a.tokens[d.lo + i + 1] : i == d.accepted ? drawn : -1;
-    if (lane_id() == 0) a.counts[req] = d.n > 0 ? d.accepted + 1 : 0;
+// A request's tokens but for the one drawn, by a workgroup.
+__device__ __forceinline__ void put_tokens(const DraftArgs& a, int req, const DraftRow& d, bool drawn) {
+    for (int i = (int)threadIdx.x; i < d.n; i += kDraftThreads) {
+        if (i != d.accepted) a.out_tokens[d.lo + i] = i < d.accepted ? a.tokens[d.lo + i + 1] : -1;
+        else if (!drawn) a.out_tokens[d.lo + i] = -1;
+    }
+    if (threadIdx.x == 0) a.counts[req] = d.n > 0 ? d.accepted + 1 : 0;
 }
 
-// Behind the sums: a wave a request.  What it needs of memory it asks for in two steps: the request's row, u and its sums, then the tile.
-__global__ __launch_bounds__(64) void draft_draw_kernel(const DraftArgs a) {
-    const int req = (int)blockIdx.x;
+// Behind the sums: a workgroup a request.  It asks for the request's row, u and the first sums at once, then for the tile's entries; each wave
+// finds the tile for itself.  Four waves and not one: the tile's entries are a quarter of the code, and it is fetched cold.
+__global__ __launch_bounds__(kDraftThreads) void draft_draw_kernel(const DraftArgs a) {
+    __shared__ double waves[4];
+    const int req = (int)blockIdx.x, lane = lane_id();
     if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
+    const double2* stored = a.sums + (int64_t)req * a.tiles;
+    double2 mine[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) mine[k] = stored[min(64 * k + lane, a.tiles - 1)];
     const DraftRow d = a.rows[req];
     const double u = a.sample_u[req];
-    int drawn = -1;
+    const auto tile = [&](int t0) {
+        double2 s = t0 == 0 ? mine[0] : mine[1];
+        if (t0 >= 128 && t0 + lane < a.tiles) s = stored[t0 + lane];
+        return t0 + lane < a.tiles ? s : make_double2(0.0, 0.0);
+    };
+    int owner = -1;
     if (d.n > 0) {
-        const int each = (a.tiles + 63) / 64, first = lane_id() * each;
-        const double2* stored = a.sums + (int64_t)req * a.tiles;
-        double2 mine = make_double2(0.0, 0.0);
-        for (int t = first; t < min(first + each, a.tiles); ++t) mine.x += stored[t].x, mine.y += stored[t].y;
-        drawn = draw_token(draft_weights(a, d), u, mine, each, a.tiles);
+        const DraftWeights w = draft_weights(a, d);
+        double2 all = make_double2(0.0, 0.0);
+        for (int t0 = 0; t0 < a.tiles; t0 += 64) {
+            const double2 s = tile(t0);
+            all.x += s.x, all.y += s.y;
+        }
+        const double total_p = lane_value(wave_run(all.x), 63), total_rest = lane_value(wave_run(all.y), 63);
+        const bool from_rest = w.refused >= 0 && total_rest > 0.0;
+        const double target = u * (from_rest ? total_rest : total_p);
+        double before = 0.0, base = 0.0;
+        for (int t0 = 0; t0 < a.tiles; t0 += 64) {
+            const double2 s = tile(t0);
+            const double have = from_rest ? s.y : s.x, run = wave_run(have);
+            const unsigned long long some = __ballot(have > 0.0), past = __ballot(have > 0.0 && base + run > target);
+            if (some) {
+                const int l = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+                owner = t0 + l, before = base + lane_value(run - have, l);
+            }
+            if (past) break;
+            base += lane_value(run, 63);
+        }
+        if (owner >= 0) {
+            const int token = draw_entry(w, from_rest, target, owner, before, waves);
+            if (token >= 0 && lane == 0) a.out_tokens[d.lo + d.accepted] = token;
+        }
     }
-    put_tokens(a, req, d, drawn);
+    put_tokens(a, req, d, owner >= 0);
 }
 
-// Without a workspace: a workgroup a request, which makes the sums itself.
+// Without a workspace: a workgroup a request, which makes the sums itself, once for the total and once to find the tile.
 __global__ __launch_bounds__(kDraftThreads) void draft_alone_kernel(const DraftArgs a) {
     __shared__ double waves[8];
     const int req = (int)blockIdx.x;
     if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
     const DraftRow d = draft_row(a, req);
-    int drawn = -1;
+    int owner = -1;
     if (d.n > 0) {
         const DraftWeights w = draft_weights(a, d);
-        const int each = (a.tiles + 63) / 64, first = lane_id() * each;
-        double2 mine = make_double2(0.0, 0.0);
+        double2 all = make_double2(0.0, 0.0);
         for (int t = 0; t < a.tiles; ++t) {
             const double2 s = tile_sums(w, t, waves);
-            if (t >= first && t < first + each) mine.x += s.x, mine.y += s.y;
+            all.x += s.x, all.y += s.y;
         }
-        if (threadIdx.x >= 64) return;
-        drawn = draw_token(w, a.sample_u[req], mine, each, a.tiles);
+        const bool from_rest = w.refused >= 0 && all.y > 0.0;
+        const double target = (double)a.sample_u[req] * (from_rest ? all.y : all.x);
+        double before = 0.0, base = 0.0;
+        for (int t = 0; t < a.tiles; ++t) {
+            const double2 s = tile_sums(w, t, waves);
+            const double have = from_rest ? s.y : s.x;
+            if (have > 0.0) owner = t, before = base;
+            base += have;
+            if (have > 0.0 && base > target) break;
+        }
+        if (owner >= 0) {
+            const int token = draw_entry(w, from_rest, target, owner, before, waves);
+            if (token >= 0 && lane_id() == 0) a.out_tokens[d.lo + d.accepted] = token;
+        }
     }
-    if (threadIdx.x < 64) put_tokens(a, req, d, drawn);
+    put_tokens(a, req, d, owner >= 0);
 }
 
 static int draft_tiles(int vocab) { return (int)(((int64_t)vocab + kDraftTile - 1) / kDraftTile); }
@@ -281,7 +319,7 @@ extern "C" int warp34_verify_drafts(const warp34_exec* ex, const warp34_draft_ba
         hipLaunchKernelGGL(draft_sums_kernel, dim3((unsigned)((long long)batch->num_reqs * a.tiles)), dim3(kDraftThreads), 0, (hipStream_t)ex->stream, a);
         const int rc = (int)hipGetLastError();
         if (rc) return rc;
-        hipLaunchKernelGGL(draft_draw_kernel, dim3((unsigned)batch->num_reqs), dim3(64), 0, (hipStream_t)ex->stream, a);
+        hipLaunchKernelGGL(draft_draw_kernel, dim3((unsigned)batch->num_reqs), dim3(kDraftThreads), 0, (hipStream_t)ex->stream, a);
     } else {
         hipLaunchKernelGGL(draft_alone_kernel, dim3((unsigned)batch->num_reqs), dim3(kDraftThreads), 0, (hipStream_t)ex->stream, a);
     }
