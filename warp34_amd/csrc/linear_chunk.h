@@ -16,6 +16,7 @@
 #pragma once
 
 #include "linear_attention.h"
+#include "wave_sums.h"
 
 namespace w34 {
 
@@ -261,13 +262,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     uint8_t* tables = smem + L::kTables;  // of the present chunk, and of the next one
     uint8_t* next_tables = tables + L::kTableBytes;
     const auto put_tables = [&](uint8_t* to) {
-        double run = (double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634;
-#pragma unroll
-        for (int by = 1; by < 64; by *= 2) {
-            const double o = __shfl_up(run, by, 64);
-            if (lane >= by) run += o;
-        }
-        const double all = __shfl(run, 63, 64);
+        const double run = wave_run((double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634), all = lane_value(run, 63);
         const float hi = (float)run;
         *reinterpret_cast<float2*>(to + L::kG + lane * 8) = make_float2(hi, (float)(run - hi));
         *reinterpret_cast<float*>(to + L::kW + lane * 4) = __builtin_amdgcn_exp2f((float)(all - run));
@@ -340,10 +335,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         const int end = chunk_end;
         put();
         __syncthreads();
-        if (end < stop) {
-            fetch(end, chunk_end = chunk_stop(end));
-            if (wave == NW - 1) put_tables(next_tables);
-        }
+        if (end < stop) fetch(end, chunk_end = chunk_stop(end));
         f16v o[2] = {};
         if (with_q) {
             if (NW == 4 ? wave < 3 : wave == 1) weights(NW == 4 ? wave : 2);
@@ -465,6 +457,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             }
         }
         t = end;
+        if (wave == NW - 1 && t < stop) put_tables(next_tables);
         {
             uint8_t* const x = tables;
             tables = next_tables, next_tables = x;
