@@ -26,6 +26,8 @@ typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) s4v lds_s4;
 
 constexpr int kLinearChunk = 64;
+constexpr float kLeastHold = 1.f / 65536;  // a state's registers take their factor up when it falls below this
+constexpr double kNearFades = 100.0;       // log2 of what 32 tokens may fade by to be weighted by two factors
 constexpr float kLeastDecay = -200.f;  // e^-200 times any fp32 number is zero in 32 bits: smaller ones, minus infinity among them, change nothing
 
 // A prompt cut into parts of `length` tokens, which run at once, and once more behind the tokens that its state keeps.
@@ -101,7 +103,8 @@ __device__ __forceinline__ uint32_t linear_pack(float x, float y) {
         return pack_h2(x, y);
     }
 }
-// Two numbers as PARTS pairs of 16 bits whose sums they are.
+// Two numbers as PARTS pairs of 16 bits whose sums they are.  (What a pair of bf16 leaves of its numbers is also a dot product with (-1, 0) and
+// (0, -1), half as many instructions, but v_dot2_f32_bf16 issues every 16 cycles: a chunk of rows took 7 % longer.)
 template <typename T, int PARTS>
 __device__ __forceinline__ void linear_split(float x, float y, uint32_t (&w)[PARTS]) {
 #pragma unroll
@@ -111,9 +114,9 @@ __device__ __forceinline__ void linear_split(float x, float y, uint32_t (&w)[PAR
         if constexpr (T::kStorageFormat == WARP34_KV_FORMAT_BF16) {
             x -= __uint_as_float(w[p] << 16);
             y -= __uint_as_float(w[p] & 0xFFFF0000u);
-        } else {
-            x -= half_lo_to_f32(w[p]);
-            y -= half_hi_to_f32(w[p]);
+        } else {  // as in split_weights(): one mixed-precision fma each
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(x) : "v"(x), "v"(w[p]));
+            asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(y) : "v"(y), "v"(w[p]));
         }
     }
 }
@@ -147,8 +150,9 @@ struct LinearLds {
     static constexpr int kQ = 0, kK = kLinearChunk * kKRow, kV = 2 * kK, kP = kV + kLinearChunk * kVRow;
     static constexpr int kRow = kP + 3 * 4096;     // [3][32] what P's rows are to be multiplied by (fp16)
     static constexpr int kTables = kRow + 3 * 32 * 4;
-    // of a chunk and of the next one: [64] G as two numbers, [64] 2^(G_end - G_j), 2^G_end and G_end
-    static constexpr int kG = 0, kW = 64 * 8, kFade = kW + 64 * 4, kTableBytes = kFade + 16;
+    // of a chunk and of the next one, [64] each: G as two numbers, what v, the state's part of a row and P are multiplied by
+    static constexpr int kG = 0, kW = 64 * 8, kState = kW + 256, kAcross = kState + 256, kUp = kAcross + 256, kDown = kUp + 256, kChunk = kDown + 256;
+    static constexpr int kTableBytes = kChunk + 16;
     static constexpr int kBytes = kTables + 2 * kTableBytes;
 };
 
@@ -187,7 +191,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     for (int d = 0; d < KT; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[d][i] = 0.f;
-    int unit = 0;  // s holds the state times 2^unit (fp16)
+    int unit = 0;  // s holds the state times 2^unit (fp16), or over `hold` (bf16)
+    float hold = 1.f;
     // this wave's share of a part's state in scratch
     float* const mine = MODE == kLinearWalk ? nullptr
                                             : p.states + ((int64_t)group * a.v_heads + head) * (DK * DV) + wave * (32 * DK) + lane * 4;
@@ -208,14 +213,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             }
     }
     const auto put_state = [&]() {
-        const float by = power_of_two(-unit);
+        const float by = kBf16 ? hold : power_of_two(-unit);
         int first = state_at;
         asm volatile("" : "+v"(first));  // addresses are worked out here, not kept in registers through the chunks
         float* const to = r.out + first;
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) to[(32 * d + 16 * (i >> 3) + (i & 7)) * DV] = kBf16 ? s[d][i] : s[d][i] * by;
+            for (int i = 0; i < 16; ++i) to[(32 * d + 16 * (i >> 3) + (i & 7)) * DV] = s[d][i] * by;
     };
     if (MODE == kLinearWalk && r.kept == 0 && r.out != nullptr) put_state();
 
@@ -229,10 +234,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     const auto fetch = [&](int t, int end) {
         const int rows = end - t;
         const int64_t tok = r.lo + t;
-        if (wave == NW - 1) {
-            gx = 0.f;
-            if (a.g != nullptr && lane < rows) gx = a.g[(tok + lane) * a.g_stride + head];
-        }
         const auto k = linear_rows(a.k + tok * a.k_stride + kh * DK, rows, a.k_stride, DK), v = linear_rows(a.v + tok * a.v_stride + head * DV, rows, a.v_stride, DV);
         const auto q = linear_rows(a.q + tok * a.q_stride + kh * DK, rows, a.q_stride, DK);
 #pragma unroll
@@ -243,6 +244,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) vx[i] = __builtin_amdgcn_raw_buffer_load_b128(v, 2 * a.v_stride * (v_row + i * (kThreads / VP)) + 16 * v_piece, 0, 0);
+    };
+    const auto fetch_decays = [&](int t, int end) {
+        gx = 0.f;
+        if (a.g != nullptr && t + lane < end) gx = a.g[(int64_t)(r.lo + t + lane) * a.g_stride + head];
     };
     const auto put = [&]() {
         uint8_t* const kt = smem + L::kK + linear_place(k_row) * L::kKRow + k_piece * 16;
@@ -258,15 +263,26 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
 #pragma unroll
         for (int i = 0; i < 4; ++i) *reinterpret_cast<u4*>(vt + i * (kThreads / VP) * L::kVRow) = vx[i];
     };
-    // the last wave's: the tables of the chunk that has been fetched
+    // The last wave's: the tables of a chunk, before which the state is its registers times `held`.  Their g is fetched a chunk before that.
     uint8_t* tables = smem + L::kTables;  // of the present chunk, and of the next one
     uint8_t* next_tables = tables + L::kTableBytes;
-    const auto put_tables = [&](uint8_t* to) {
-        const double run = wave_run((double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634), all = lane_value(run, 63);
-        const float hi = (float)run;
+    const auto put_tables = [&](uint8_t* to, float held) {
+        const double run = wave_run((double)(gx < kLeastDecay ? kLeastDecay : gx) * 1.4426950408889634);
+        const double all = lane_value(run, 63), half = lane_value(run, 31), start = lane_value(run, 0), middle = lane_value(run, 32);
+        const float hi = (float)run, fade = __builtin_amdgcn_exp2f((float)all), next = fade * held;
+        const bool again = !kBf16 || next < kLeastHold;  // the registers take the factor up
+        const auto put = [&](int at, float x) { *reinterpret_cast<float*>(to + at + lane * 4) = x; };
         *reinterpret_cast<float2*>(to + L::kG + lane * 8) = make_float2(hi, (float)(run - hi));
-        *reinterpret_cast<float*>(to + L::kW + lane * 4) = __builtin_amdgcn_exp2f((float)(all - run));
-        if (lane == 0) *reinterpret_cast<float2*>(to + L::kFade) = make_float2(__builtin_amdgcn_exp2f((float)all), (float)all);
+        put(L::kW, __builtin_amdgcn_exp2f((float)(all - run)) * (again ? 1.f : 1.f / next));
+        if constexpr (MODE != kLinearSums) {
+            const double centre = lane < 32 ? 0.5 * (start + half) : 0.5 * (middle + all);
+            put(L::kState, __builtin_amdgcn_exp2f((float)run) * (held * a.scale));
+            put(L::kAcross, __builtin_amdgcn_exp2f((float)(lane < 32 ? half - run : run - half)));
+            put(L::kUp, __builtin_amdgcn_exp2f((float)(run - centre)));
+            put(L::kDown, __builtin_amdgcn_exp2f((float)(centre - run)));
+        }
+        const float near = start - half < kNearFades && middle - all < kNearFades ? 1.f : 0.f;
+        if (lane == 0) *reinterpret_cast<f4*>(to + L::kChunk) = f4{next, again ? 1.f : 0.f, (float)all, near};
     };
     const uint8_t* const row_at = smem + linear_place(n32) * L::kKRow + 16 * b;  // channels 8 b .. + 7 of 16 of row n32
     const auto k_operand = [&](int kt, int step) { return *reinterpret_cast<const u4*>(row_at + L::kK + 32 * kt * L::kKRow + 32 * step); };
@@ -286,19 +302,34 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     };
 
     // Tile 0: queries 0 .. 31 over keys 0 .. 31, 1: queries 32 .. 63 over keys 0 .. 31, 2: over keys 32 .. 63.
-    const auto weights = [&](int tile) {
+    const auto weights = [&](int tile, bool near) {
         const int kt = tile == 2 ? 1 : 0, qt = tile == 0 ? 0 : 1;
         f16v x = {};
 #pragma unroll
         for (int step = 0; step < DK / 16; ++step)
             x = linear_mfma<T>(k_operand(kt, step), q_operand(qt, step), x);
-        const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + (32 * qt + n32) * 8);
+        // 2^(G_i - G_j) as a product: by way of G at the border between the halves, or at the middle of the half where it fades by little there
+        if (tile == 1 || near) {
+            const float row = *reinterpret_cast<const float*>(tables + (tile == 1 ? L::kAcross : L::kUp) + (32 * qt + n32) * 4) * a.scale;
+            const uint8_t* const columns = tables + (tile == 1 ? L::kAcross : L::kDown) + (32 * kt + 4 * b) * 4;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const int key = (i & 3) + 8 * (i >> 2) + 4 * b;
-            const float2 gj = *reinterpret_cast<const float2*>(tables + L::kG + (32 * kt + key) * 8);
-            const float w = x[i] * __builtin_amdgcn_exp2f((gi.x - gj.x) + (gi.y - gj.y));
-            x[i] = tile == 1 || key <= n32 ? w : 0.f;
+            for (int ig = 0; ig < 4; ++ig) {
+                const f4 w = *reinterpret_cast<const f4*>(columns + 32 * ig);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float y = x[4 * ig + i] * row * w[i];
+                    x[4 * ig + i] = tile == 1 || i + 8 * ig + 4 * b <= n32 ? y : 0.f;
+                }
+            }
+        } else {
+            const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + (32 * qt + n32) * 8);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int key = (i & 3) + 8 * (i >> 2) + 4 * b;
+                const float2 gj = *reinterpret_cast<const float2*>(tables + L::kG + (32 * kt + key) * 8);
+                const float y = x[i] * __builtin_amdgcn_exp2f((gi.x - gj.x) + (gi.y - gj.y)) * a.scale;
+                x[i] = key <= n32 ? y : 0.f;
+            }
         }
         if constexpr (!kBf16) {
             float top = 0.f;
@@ -329,17 +360,27 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
     float part_sum = 0.f;  // of g, for the scan over parts
     if (begin < stop) {
         fetch(begin, chunk_end = chunk_stop(begin));
-        if (wave == NW - 1) put_tables(tables);
+        if (wave == NW - 1) {
+            fetch_decays(begin, chunk_end);
+            put_tables(tables, 1.f);
+            if (chunk_end < stop) fetch_decays(chunk_end, chunk_stop(chunk_end));
+        }
     }
     for (int t = begin; t < stop;) {
         const int end = chunk_end;
         put();
         __syncthreads();
+        const f4 chunk = *reinterpret_cast<const f4*>(tables + L::kChunk);
         if (end < stop) fetch(end, chunk_end = chunk_stop(end));
+        if (wave == NW - 1 && end < stop) {  // while the other waves weight P
+            const bool again = chunk[1] != 0.f;
+            put_tables(next_tables, again ? 1.f : chunk[0]);
+            if (chunk_end < stop) fetch_decays(chunk_end, chunk_stop(chunk_end));
+        }
         f16v o[2] = {};
         if (with_q) {
-            if (NW == 4 ? wave < 3 : wave == 1) weights(NW == 4 ? wave : 2);
-            if (NW == 2 && wave == 0) weights(0), weights(1);
+            if (NW == 4 ? wave < 3 : wave == 1) weights(NW == 4 ? wave : 2, chunk[3] != 0.f);
+            if (NW == 2 && wave == 0) weights(0, chunk[3] != 0.f), weights(1, true);
             // the state's part of the rows
             int e = 0;
             if constexpr (!kBf16) {
@@ -372,8 +413,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             }
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + (32 * q + n32) * 8);
-                const float f = __builtin_amdgcn_exp2f(gi.x + gi.y) * (kBf16 ? 1.f : power_of_two(-e - unit));
+                const float f = *reinterpret_cast<const float*>(tables + L::kState + (32 * q + n32) * 4) * (kBf16 ? 1.f : power_of_two(-e - unit));
 #pragma unroll
                 for (int i = 0; i < 16; ++i) o[q][i] *= f;
             }
@@ -404,7 +444,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             for (int q = 0; q < 2; ++q) {
                 uint32_t w[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) w[k] = linear_pack<T>(o[q][2 * k] * a.scale, o[q][2 * k + 1] * a.scale);
+                for (int k = 0; k < 8; ++k) w[k] = linear_pack<T>(o[q][2 * k], o[q][2 * k + 1]);
                 const int to = 2 * (a.out_stride * (32 * q + n32) + 32 * wave + 8 * b);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
@@ -415,8 +455,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             }
         }
         // the state moves on
-        const float2 fade = *reinterpret_cast<const float2*>(tables + L::kFade);
-        if (MODE == kLinearSums) part_sum += fade.y;
+        const bool again = chunk[1] != 0.f;
+        if (MODE == kLinearSums) part_sum += chunk[2];
         if (MODE != kLinearRows || end < stop) {
             int next = unit;
             if constexpr (!kBf16) {
@@ -428,12 +468,15 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
                 const float largest = wave_max(fmaxf(half_lo_to_f32(top), half_hi_to_f32(top)));
                 if (largest > 0.f && largest < INFINITY) next = scale_exponent(largest);
             }
-            const float by = kBf16 ? fade.x : fade.x * power_of_two(next - unit), values = power_of_two(next);
+            const float by = kBf16 ? chunk[0] : chunk[0] * power_of_two(next - unit), values = power_of_two(next);
             unit = next;
+            hold = again ? 1.f : chunk[0];
+            if (again) {
 #pragma unroll
-            for (int d = 0; d < KT; ++d)
+                for (int d = 0; d < KT; ++d)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) s[d][i] *= by;
+                    for (int i = 0; i < 16; ++i) s[d][i] *= by;
+            }
 #pragma unroll
             for (int step = 0; step < 4; ++step) {
                 u4 x[kParts];
@@ -457,7 +500,6 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             }
         }
         t = end;
-        if (wave == NW - 1 && t < stop) put_tables(next_tables);
         {
             uint8_t* const x = tables;
             tables = next_tables, next_tables = x;
@@ -466,14 +508,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         if (MODE == kLinearWalk && t == r.kept && r.out != nullptr) put_state();
     }
     if (MODE == kLinearSums) {
-        const float by = power_of_two(-unit);
+        const float by = kBf16 ? hold : power_of_two(-unit);
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
             for (int ig = 0; ig < 4; ++ig) {
                 f4 x;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = kBf16 ? s[d][4 * ig + i] : s[d][4 * ig + i] * by;
+                for (int i = 0; i < 4; ++i) x[i] = s[d][4 * ig + i] * by;
                 *reinterpret_cast<f4*>(mine + (d * 4 + ig) * 256) = x;
             }
         if (tid == 0) p.fades[(int64_t)group * a.v_heads + head] = __builtin_amdgcn_exp2f(part_sum);
