@@ -20,11 +20,15 @@ struct LinearArgs {
     float scale;
 };
 
+// States: an address that comes out of an integer has to say that it is global memory, or its loads and stores count with those of LDS.
+typedef __attribute__((address_space(1))) float linear_float;
+typedef __attribute__((address_space(1))) f4 linear_f4;
+
 struct LinearRequest {
     int lo, n;     // its rows
     int kept;      // the state written is the one behind that many of them
-    const float* in;  // of the head, nullptr: zeros
-    float* out;       // of the head, nullptr: not written
+    const linear_float* in;  // of the head, nullptr: zeros
+    linear_float* out;       // of the head, nullptr: not written
 };
 __device__ __forceinline__ LinearRequest linear_request(const LinearArgs& a, int req, int head, int state_size) {
     LinearRequest r;
@@ -33,7 +37,7 @@ __device__ __forceinline__ LinearRequest linear_request(const LinearArgs& a, int
     r.kept = a.state_tokens == nullptr ? r.n : min(max(a.state_tokens[req], 0), r.n);
     const int in = a.state_in_slots == nullptr || (a.has_initial_state != nullptr && a.has_initial_state[req] == 0) ? -1 : a.state_in_slots[req];
     const int out = a.state_out_slots == nullptr ? -1 : a.state_out_slots[req];
-    float* base = reinterpret_cast<float*>((uintptr_t)a.state_base);
+    linear_float* base = reinterpret_cast<linear_float*>((uintptr_t)a.state_base);
     const uint64_t stride = a.slot_stride / 4, mine = (uint64_t)head * state_size;
     r.in = in < 0 ? nullptr : base + (uint64_t)in * stride + mine;
     r.out = out < 0 ? nullptr : base + (uint64_t)out * stride + mine;
@@ -56,13 +60,13 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
     for (int i = 0; i < R; ++i) s[i] = f4{0.f, 0.f, 0.f, 0.f};
     if (r.in != nullptr) {
 #pragma unroll
-        for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const f4*>(r.in + (row0 + i) * DV + col);
+        for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const linear_f4*>(r.in + (row0 + i) * DV + col);
     }
     const int kh = head / a.group, steps = a.out == nullptr ? r.kept : r.n;
     for (int t = 0; t <= steps; ++t) {
         if (t == r.kept && r.out != nullptr) {
 #pragma unroll
-            for (int i = 0; i < R; ++i) *reinterpret_cast<f4*>(r.out + (row0 + i) * DV + col) = s[i];
+            for (int i = 0; i < R; ++i) *reinterpret_cast<linear_f4*>(r.out + (row0 + i) * DV + col) = s[i];
         }
         if (t == steps) break;
         const int64_t tok = r.lo + t;

@@ -216,7 +216,7 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         const float by = kBf16 ? hold : power_of_two(-unit);
         int first = state_at;
         asm volatile("" : "+v"(first));  // addresses are worked out here, not kept in registers through the chunks
-        float* const to = r.out + first;
+        linear_float* const to = r.out + first;
 #pragma unroll
         for (int d = 0; d < KT; ++d)
 #pragma unroll
@@ -471,15 +471,14 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             const float by = kBf16 ? chunk[0] : chunk[0] * power_of_two(next - unit), values = power_of_two(next);
             unit = next;
             hold = again ? 1.f : chunk[0];
-            if (again) {
+            if (__builtin_amdgcn_readfirstlane(again)) {
 #pragma unroll
                 for (int d = 0; d < KT; ++d)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) s[d][i] *= by;
             }
-#pragma unroll
-            for (int step = 0; step < 4; ++step) {
-                u4 x[kParts];
+            // values are weighted, and keys asked for, a step ahead of their products
+            const auto weigh = [&](int step, u4 (&x)[kParts]) {
                 const f4 w0 = *reinterpret_cast<const f4*>(tables + L::kW + (16 * step + 4 * b) * 4), w1 = *reinterpret_cast<const f4*>(tables + L::kW + (16 * step + 8 + 4 * b) * 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -491,11 +490,30 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
 #pragma unroll
                     for (int q = 0; q < kParts; ++q) x[q][k] = parts[q];
                 }
+            };
+            u4 x[2][kParts], k[2][KT];
+            weigh(0, x[0]);
 #pragma unroll
-                for (int d = 0; d < KT; ++d) {
-                    const u4 k = transposed(kt_at + 16 * step * L::kKRow + 64 * d, L::kKRow);
+            for (int d = 0; d < KT; ++d) k[0][d] = transposed(kt_at + 64 * d, L::kKRow);
 #pragma unroll
-                    for (int q = 0; q < kParts; ++q) s[d] = linear_mfma<T>(k, x[q], s[d]);
+            for (int step = 0; step < 4; ++step) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (step < 3) {
+#pragma unroll
+                    for (int d = 0; d < KT; ++d) k[(step + 1) & 1][d] = transposed(kt_at + 16 * (step + 1) * L::kKRow + 64 * d, L::kKRow);
+                    weigh(step + 1, x[(step + 1) & 1]);
+                }
+#pragma unroll
+                for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                    for (int d = 0; d < KT; ++d) s[d] = linear_mfma<T>(k[step & 1][d], x[step & 1][q], s[d]);
+                if (step < 3) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, 2 * KT + 2, 0);
+#pragma unroll
+                    for (int i = 0; i < kParts * KT; ++i) {
+                        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                        __builtin_amdgcn_sched_group_barrier(0x002, 20 / KT, 0);
+                    }
                 }
             }
         }
