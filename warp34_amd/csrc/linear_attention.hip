@@ -21,6 +21,11 @@ static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_req
     const long long most = max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens;
     const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
     LinearShape s{0, 0, 0};
+    // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make three launches and
+    // half as much work again.  us, 4.1 a chunk for a round of up to 256 workgroups against 19 and 0.0226 a chunk of a head: 2 x 300 tokens of 32
+    // heads walked 23, in parts 31; 2 x 1 024 67 / 52, 4 x 1 024 70 / 73, 8 x 1 024 75 / 111, 4 x 4 096 271 / 211, 8 x 4 096 301 / 375.
+    const long long groups = num_reqs * heads, chunks = total_tokens / kLinearChunk * heads + groups / 2;
+    if (181 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 840 + chunks) return s;
     for (int log_length = 6; log_length < 30; ++log_length) {
         const long long length = 1ll << log_length;
         if (length >= most) return s;

@@ -212,6 +212,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
                 for (int i = 0; i < 4; ++i) s[d][4 * ig + i] = x[i];
             }
     }
+#pragma unroll
+    for (int d = 0; d < KT; ++d) asm volatile("" : "+v"(s[d]));
     const auto put_state = [&]() {
         const float by = kBf16 ? hold : power_of_two(-unit);
         int first = state_at;
@@ -366,10 +368,25 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
             if (chunk_end < stop) fetch_decays(chunk_end, chunk_stop(chunk_end));
         }
     }
+    // A chunk's rows go out when the next chunk's v takes their place, each thread's 16 bytes by itself: whole rows side by side.
+    u4 ox[4];
+    const auto take_rows = [&]() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ox[i] = *reinterpret_cast<const u4*>(smem + L::kV + (linear_place(v_row) + i * (kThreads / VP)) * L::kVRow + v_piece * 16);
+    };
+    const auto store_rows = [&](int from, int to) {
+        const auto rows = linear_rows(a.out + (int64_t)(r.lo + from) * a.out_stride + head * DV, to - from, a.out_stride, DV);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) __builtin_amdgcn_raw_buffer_store_b128(ox[i], rows, 2 * a.out_stride * (v_row + i * (kThreads / VP)) + 16 * v_piece, 0, 0);
+    };
+    int before = begin;  // where the chunk before the present one begins
     for (int t = begin; t < stop;) {
         const int end = chunk_end;
+        if (with_q && t > begin) take_rows();
         put();
         __syncthreads();
+        if (with_q && t > begin) store_rows(before, t);
+        before = t;
         const f4 chunk = *reinterpret_cast<const f4*>(tables + L::kChunk);
         if (end < stop) fetch(end, chunk_end = chunk_stop(end));
         if (wave == NW - 1 && end < stop) {  // while the other waves weight P
@@ -438,21 +455,13 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
                     for (int i = 0; i < 16; ++i) o[qt][i] = __builtin_fmaf(sum[i], f, o[qt][i]);
                 }
             }
-            // lanes n32 and n32 + 32 have one row's columns in turns of four: exchanged, each has eight in a row
-            const auto rows = linear_rows(a.out + (int64_t)(r.lo + t) * a.out_stride + head * DV, end - t, a.out_stride, DV);
+            // to where v was, whose operands are in registers: lane (n32, b) has columns 8 k + 4 b .. + 3 of row n32
+            uint8_t* const to = smem + L::kV + linear_place(n32) * L::kVRow + 64 * wave + 8 * b;
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                uint32_t w[8];
+            for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) w[k] = linear_pack<T>(o[q][2 * k], o[q][2 * k + 1]);
-                const int to = 2 * (a.out_stride * (32 * q + n32) + 32 * wave + 8 * b);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const auto x = __builtin_amdgcn_permlane32_swap(w[4 * k], w[4 * k + 2], false, false);
-                    const auto y = __builtin_amdgcn_permlane32_swap(w[4 * k + 1], w[4 * k + 3], false, false);
-                    __builtin_amdgcn_raw_buffer_store_b128(u4{x[0], y[0], x[1], y[1]}, rows, to + 32 * k, 0, 0);
-                }
-            }
+                for (int k = 0; k < 4; ++k)
+                    *reinterpret_cast<u2v*>(to + 32 * q * L::kVRow + 16 * k) = u2v{linear_pack<T>(o[q][4 * k], o[q][4 * k + 1]), linear_pack<T>(o[q][4 * k + 2], o[q][4 * k + 3])};
         }
         // the state moves on
         const bool again = chunk[1] != 0.f;
@@ -525,6 +534,10 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         __syncthreads();
         if (MODE == kLinearWalk && t == r.kept && r.out != nullptr) put_state();
     }
+    if (with_q && begin < stop) {
+        take_rows();
+        store_rows(before, stop);
+    }
     if (MODE == kLinearSums) {
         const float by = kBf16 ? hold : power_of_two(-unit);
 #pragma unroll
@@ -539,6 +552,8 @@ __global__ __launch_bounds__(64 * NW, NW == 4 || DK == 64 ? 2 : 1) void linear_c
         if (tid == 0) p.fades[(int64_t)group * a.v_heads + head] = __builtin_amdgcn_exp2f(part_sum);
     }
 }
+
+constexpr int kScanAhead = 4;
 
 // The states that the parts start from, and the one that is kept: S = fade_p S + U_p over a request's parts.  A thread has four elements of a
 // head's state, in the order of the registers of the kernel above.
@@ -563,15 +578,31 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(const LinearArgs a, co
     };
     if (r.kept == 0 && r.out != nullptr) keep();
     float* slot = p.states + ((int64_t)first * a.v_heads + head) * size + (int64_t)x * 4;
-    for (int part = 0; part < parts && first + part < p.most; ++part, slot += (int64_t)a.v_heads * size) {
-        const f4 u = *reinterpret_cast<const f4*>(slot);
-        const float fade = p.fades[(int64_t)(first + part) * a.v_heads + head];
-        *reinterpret_cast<f4*>(slot) = s;
+    const int64_t step = (int64_t)a.v_heads * size;
+    const int count = min(parts, p.most - first);
+    // what four parts add travels while the four before them are gone through
+    f4 u[kScanAhead];
+    float fade[kScanAhead];
+    const auto fetch = [&](int i, int part) {
+        if (part < count) u[i] = *reinterpret_cast<const f4*>(slot + part * step), fade[i] = p.fades[(int64_t)(first + part) * a.v_heads + head];
+    };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(fade, s[i], u[i]);
-        int begin, end;
-        linear_part_range(r.n, r.kept, p.log_length, part, begin, end);
-        if (end == r.kept && r.out != nullptr) keep();
+    for (int i = 0; i < kScanAhead; ++i) fetch(i, i);
+    for (int part0 = 0; part0 < count; part0 += kScanAhead) {
+#pragma unroll
+        for (int k = 0; k < kScanAhead; ++k) {
+            const int part = part0 + k;
+            if (part >= count) break;
+            const f4 add = u[k];
+            const float by = fade[k];
+            fetch(k, part + kScanAhead);
+            *reinterpret_cast<f4*>(slot + part * step) = s;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(by, s[i], add[i]);
+            int begin, end;
+            linear_part_range(r.n, r.kept, p.log_length, part, begin, end);
+            if (end == r.kept && r.out != nullptr) keep();
+        }
     }
 }
 
