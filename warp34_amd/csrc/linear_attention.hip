@@ -6,7 +6,7 @@
 
 namespace w34 {
 
-constexpr int kLinearGroups = 512;  // workgroups of the chunk kernel that run at once, two on each of 256 units
+constexpr int kLinearGroups = 320;  // of the chunk kernel: one on each of 256 units, and some for parts that are short
 constexpr int kLinearMostStride = 1 << 23;  // elements: a chunk's rows are within 2^31 bytes
 constexpr int kStepTokens = 16;  // requests of up to so many tokens go by the recurrent kernel
 
@@ -22,10 +22,11 @@ static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_req
     const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
     LinearShape s{0, 0, 0};
     // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make three launches and
-    // half as much work again.  us, 4.1 a chunk for a round of up to 256 workgroups against 19 and 0.0226 a chunk of a head: 2 x 300 tokens of 32
-    // heads walked 23, in parts 31; 2 x 1 024 67 / 52, 4 x 1 024 70 / 73, 8 x 1 024 75 / 111, 4 x 4 096 271 / 211, 8 x 4 096 301 / 375.
-    const long long groups = num_reqs * heads, chunks = total_tokens / kLinearChunk * heads + groups / 2;
-    if (181 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 840 + chunks) return s;
+    // half as much work again.  us, 3.55 a chunk for a round of up to 256 workgroups against 19 and 0.0226 a chunk of a head: 333 tokens of 16
+    // heads walked 24.0, in parts 20.5, of 32 heads 25.0 / 28.5; 1 024 tokens of 32 heads 59.6 / 32.6, 4 x 1 024 64 / 71, 8 192 447 / 109,
+    // 4 x 4 096 244 / 206, 5 x 4 096 247 / 333.
+    const long long groups = num_reqs * heads, chunks = (long long)total_tokens / kLinearChunk * heads + groups / 2;
+    if (157 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 840 + chunks) return s;
     for (int log_length = 6; log_length < 30; ++log_length) {
         const long long length = 1ll << log_length;
         if (length >= most) return s;
@@ -40,28 +41,28 @@ static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_req
     return s;
 }
 
-template <typename T, int DK, int NW>
+template <typename T, int DK, int DV>
 static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const LinearShape& shape) {
     const long long columns = (long long)a.v_heads;
     const hipStream_t stream = (hipStream_t)ex->stream;
     LinearParts p{nullptr, nullptr, shape.log_length, (int)shape.parts};
     if (shape.log_length == 0) {
-        if (!grid_fits(a.num_reqs * columns, 64 * NW)) return (int)hipErrorInvalidValue;
-        hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearWalk>), dim3((unsigned)(a.num_reqs * columns)), dim3(64 * NW), 0, stream, a, p);
+        if (!grid_fits(a.num_reqs * columns, 4 * DV)) return (int)hipErrorInvalidValue;
+        hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearWalk>), dim3((unsigned)(a.num_reqs * columns)), dim3(4 * DV), 0, stream, a, p);
         return (int)hipGetLastError();
     }
-    const long long scans = (long long)a.num_reqs * a.v_heads * (DK * a.v_dim / 1024);
-    if (!grid_fits(shape.parts * columns, 64 * NW) || !grid_fits(scans, 256)) return (int)hipErrorInvalidValue;
+    const long long scans = (long long)a.num_reqs * a.v_heads * (DK * DV / 1024);
+    if (!grid_fits(shape.parts * columns, 4 * DV) || !grid_fits(scans, 256)) return (int)hipErrorInvalidValue;
     p.states = (float*)(uintptr_t)ex->scratch_ptr;
-    p.fades = p.states + shape.parts * a.v_heads * (DK * a.v_dim);
+    p.fades = p.states + shape.parts * a.v_heads * (DK * DV);
     const dim3 grid((unsigned)(shape.parts * columns));
-    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearSums>), grid, dim3(64 * NW), 0, stream, a, p);
+    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearSums>), grid, dim3(4 * DV), 0, stream, a, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
     hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)scans), dim3(256), 0, stream, a, p, DK);
     rc = (int)hipGetLastError();
     if (rc || a.out == nullptr) return rc;
-    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, NW, kLinearRows>), grid, dim3(64 * NW), 0, stream, a, p);
+    hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearRows>), grid, dim3(4 * DV), 0, stream, a, p);
     return (int)hipGetLastError();
 }
 
@@ -75,7 +76,7 @@ static int linear_launch(const warp34_exec* ex, const warp34_linear_state_layout
     }
     const bool usable = ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0;
     const LinearShape shape = linear_shape(y, b->num_reqs, b->total_tokens, b->max_q_len, b->state_tokens != nullptr, usable ? ex->scratch_size : 0);
-    return linear_chunk_launch<T, DK, DV / 32>(ex, a, shape);
+    return linear_chunk_launch<T, DK, DV>(ex, a, shape);
 }
 
 template <typename T>
