@@ -325,4 +325,25 @@ struct RequestPages {
 bool reserve_kv_pages_from(KvPool& pool, PrefixPageCache& cache, std::vector<int32_t>* dst, size_t target_pages);
 void free_kv_pages(KvPool& pool, const std::vector<int32_t>& pages);
 
+// ---- page copies (no counterpart in the reference) ------------------------------------------------
+// The host side of warp34_kv_cache_copy_pages: pair i copies the first rows[i] rows of page src[i] to page dst[i].  No page
+// is both source and destination of the copies that one call adds.
+struct PageCopies {
+    std::vector<int32_t> src, dst, rows;
+    void add(int32_t from, int32_t to, int32_t count) {
+        if (count > 0) src.push_back(from), dst.push_back(to), rows.push_back(count);
+    }
+};
+// A second request that goes on from the parent's committed tokens: it shares the protected prefix, whose path it locks once
+// more, and has a page of its own, and a copy, for each private page of the parent (the last one as far as it is filled).
+// Returns false, with nothing taken, where the pool (after evicting from the cache) has too few pages.  A parent with private
+// draft pages needs the draft model's pool, whose copies go to draft_copies.  The parent must not write to the pages before the
+// copies have run.  Throws std::invalid_argument where the parent has fewer pages than its committed tokens fill.
+bool fork_request_pages(KvPool& pool, PrefixPageCache& cache, const RequestPages& parent, RequestPages* child, PageCopies* copies,
+                        KvPool* draft_pool = nullptr, PageCopies* draft_copies = nullptr);
+// Moves the requests' private KV pages from page `below` on to free pages under it, the lowest first, rewrites their page
+// lists and frees the pages they left; returns how many found no place.  Pages of the prefix cache stay.  What is
+// freed may be written only by work that runs behind the copies.
+size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& requests, size_t below, PageCopies* copies);
+
 }  // namespace warp34_host
