@@ -4,7 +4,8 @@
 //
 // Workgroup = the columns of a value head, a wave 16 of them with their part of the state in registers; 16x16x32 MFMAs:
 //   P^T = K Q^T        in tiles of 16 x 16, a pair of them a wave, weighted, and laid into LDS as the operands of the product below
-//   O^T = S^T Q^T      the state's registers are the operand as they stand: lane (n, g) has column n for channels 8 g .. + 7 of 32 in two tiles
+//   O^T = S^T Q^T      the state's registers are the operand as they stand: lane (n, g) has column n for channels 16 m + 4 g + i; q is laid into
+//                      LDS in the order of two such tiles, and k is read in it
 //   O^T += V^T P^T     v through transposing reads (ds_read_b64_tr_b16: lane l of 16 gets column l of four rows of 16 values)
 //   S += K^T V'        k and v through transposing reads, v weighted in registers
 // Weights are exponentials of differences of G, which is summed in 64 bits and held as two 32-bit numbers: where all but the last
@@ -124,16 +125,29 @@ __device__ __forceinline__ int scale_exponent(float top) {
     return e == 0 || e == 255 ? 0 : min(141 - e, 100);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
-__device__ __forceinline__ float wave_max(float x) {
-#pragma unroll
-    for (int by = 32; by; by /= 2) x = fmaxf(x, __shfl_xor(x, by, 64));
-    return x;
+__device__ __forceinline__ float wave_max(float x) {  // without LDS
+    const int lane = lane_id();
+    x = fmaxf(x, lane_xor<1>(x, lane));
+    x = fmaxf(x, lane_xor<2>(x, lane));
+    x = fmaxf(x, lane_xor<4>(x, lane));
+    x = fmaxf(x, lane_xor<8>(x, lane));
+    return max_over_rows(x);
 }
 
-// Rows in LDS are 16 bytes longer than they need to be, and of 16 rows the place of one is its number with the two pairs of bits exchanged: operand
-// reads of eight rows touch different banks, and so do the four rows of a transposing read, 64 bytes apart.
-constexpr int linear_row(int bytes) { return bytes + 16; }
-__device__ __forceinline__ int linear_place(int row) { return (row & ~15) | (row & 3) << 2 | (row >> 2 & 3); }
+// Where 16 bytes of a row are in LDS, as the number they are found under in it: rows of PIECES = 8 or 16.  A wave's 16-byte reads go by lanes 0 .. 3,
+// 12 .. 15 and 20 .. 27, then 4 .. 11, 16 .. 19 and 28 .. 31 (and the same of its second half): pieces g and g + 1 of rows {0 .. 3, 12 .. 15} and {4 .. 11}
+// must differ, which they do where rows 12 .. 15 have the other halves of the pairs that rows 0 .. 3 have.  A transposing read takes 32 bytes of eight
+// rows at a time: there the pairs must differ.  Cycles a read without and with a conflict: 4 and 8, transposing 2 and 4.
+template <int PIECES>
+__device__ __forceinline__ int linear_turn(int row) {
+    constexpr int kHalf = PIECES / 2;
+    const int x = PIECES == 16 ? row & 15 : row >> 1 & 7, low = x & (kHalf - 1);
+    return x < kHalf ? 2 * low : 2 * (low ^ (kHalf / 2)) + 1;
+}
+template <int PIECES>
+__device__ __forceinline__ uint32_t linear_place(int row, int piece) {
+    return (uint32_t)(row * PIECES * 16 + (piece ^ linear_turn<PIECES>(row)) * 16);
+}
 
 // `rows` rows of `width` 16-bit elements from `base` on: loads behind the last row give zeros, stores there are dropped.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t linear_rows(const uint16_t* base, int rows, int stride, int width) {
@@ -144,7 +158,7 @@ enum { kLinearWalk, kLinearSums, kLinearRows };  // a whole request; what a part
 
 template <int DK, int DV>
 struct LinearLds {
-    static constexpr int kKRow = linear_row(DK * 2), kVRow = linear_row(DV * 2);
+    static constexpr int kKRow = DK * 2, kVRow = DV * 2;
     static constexpr int kQ = 0, kK = kLinearChunk * kKRow, kV = 2 * kK, kP = kV + kLinearChunk * kVRow;
     static constexpr int kRow = kP + 6 * 2048;     // [6][16] what P's rows are to be multiplied by (fp16)
     static constexpr int kTables = kRow + 6 * 16 * 4;
@@ -177,7 +191,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
     }
     LinearRequest r = linear_request(a, req, head, DK * DV);
     r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.n = __builtin_amdgcn_readfirstlane(r.n), r.kept = __builtin_amdgcn_readfirstlane(r.kept);
-    const int state_at = 8 * g4 * DV + 16 * wave + n16;  // element of the state that is this lane's first
+    const int state_at = 4 * g4 * DV + 16 * wave + n16;  // element of the state that is this lane's first
 
     int begin = 0, stop = r.n;
     if (MODE != kLinearWalk) linear_part_range(r.n, r.kept, p.log_length, part, begin, stop);
@@ -195,7 +209,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
         for (int m = 0; m < KM; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[m][i] = r.in[state_at + (32 * (m >> 1) + 4 * (m & 1) + i) * DV];
+            for (int i = 0; i < 4; ++i) s[m][i] = r.in[state_at + (16 * m + i) * DV];
     }
     if (MODE == kLinearRows) {
 #pragma unroll
@@ -212,7 +226,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
         for (int m = 0; m < KM; ++m)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) to[(32 * (m >> 1) + 4 * (m & 1) + i) * DV] = s[m][i] * by;
+            for (int i = 0; i < 4; ++i) to[(16 * m + i) * DV] = s[m][i] * by;
     };
     if (MODE == kLinearWalk && r.kept == 0 && r.out != nullptr) put_state();
 
@@ -242,13 +256,19 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         gx = 0.f;
         if (a.g != nullptr && t + lane < end) gx = a.g[(int64_t)(r.lo + t + lane) * a.g_stride + head];
     };
-    uint8_t* const k_to = smem + linear_place(k_row) * L::kKRow + k_piece * 16;
-    uint8_t* const v_to = smem + L::kV + linear_place(v_row) * L::kVRow + v_piece * 16;
+    // k and v as they are; of 32 channels of q, fours 0 and 4, 1 and 5, 2 and 6, 3 and 7 side by side
+    uint8_t* const k_to = smem + L::kK + linear_place<KP>(k_row, k_piece);
+    uint8_t* const v_to = smem + L::kV + linear_place<VP>(v_row, v_piece);
+    uint8_t* const q_to = smem + L::kQ + linear_place<KP>(k_row, (k_piece & ~3) | (2 * k_piece & 3)) + 8 * (k_piece >> 1 & 1);
+    uint8_t* const q_to2 = smem + L::kQ + linear_place<KP>(k_row, (k_piece & ~3) | (2 * k_piece & 3) | 1) + 8 * (k_piece >> 1 & 1);
     const auto put = [&]() {
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            *reinterpret_cast<u4*>(k_to + L::kK + i * (kThreads / KP) * L::kKRow) = kx[i];
-            if (with_q) *reinterpret_cast<u4*>(k_to + L::kQ + i * (kThreads / KP) * L::kKRow) = qx[i];
+            *reinterpret_cast<u4*>(k_to + i * (kThreads / KP) * L::kKRow) = kx[i];
+            if (with_q) {
+                *reinterpret_cast<u2v*>(q_to + i * (kThreads / KP) * L::kKRow) = u2v{qx[i][0], qx[i][1]};
+                *reinterpret_cast<u2v*>(q_to2 + i * (kThreads / KP) * L::kKRow) = u2v{qx[i][2], qx[i][3]};
+            }
         }
 #pragma unroll
         for (int i = 0; i < kVLoads; ++i) *reinterpret_cast<u4*>(v_to + i * (kThreads / VP) * L::kVRow) = vx[i];
@@ -274,14 +294,19 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         const float near = start - half < kNearFades && middle - all < kNearFades ? 1.f : 0.f;
         if (lane == 0) *reinterpret_cast<f4*>(to + L::kChunk) = f4{next, again ? 1.f : 0.f, (float)all, near};
     };
-    const uint8_t* const row_at = smem + linear_place(n16) * L::kKRow + 16 * g4;  // of row n16 of sixteen channels 8 g .. + 7 of 32
-    const auto q_operand = [&](int sixteen, int step) { return *reinterpret_cast<const u4*>(row_at + L::kQ + 16 * sixteen * L::kKRow + 64 * step); };
-    const auto k_operand = [&](int sixteen, int step) { return *reinterpret_cast<const u4*>(row_at + L::kK + 16 * sixteen * L::kKRow + 64 * step); };
-    // transposed: rows 4 g .. + 3 and 16 + 4 g .. + 3 of 32, a column a lane of 16.  Of 32 channels of k a tile takes every other four, so that the
-    // registers of two tiles of the state are eight channels in a row, as q is read above.
+    // of row n16 of sixteen channels 4 g .. + 3 and 16 + 4 g .. + 3 of 32
+    const uint32_t q_at = linear_place<KP>(n16, g4), k_at = linear_place<KP>(n16, g4 >> 1) + 8 * (g4 & 1);
+    const auto q_operand = [&](int sixteen, int step) { return *reinterpret_cast<const u4*>(smem + L::kQ + 16 * sixteen * L::kKRow + (q_at ^ (64u * step))); };
+    const auto k_operand = [&](int sixteen, int step) {
+        const uint8_t* const at = smem + L::kK + 16 * sixteen * L::kKRow;
+        const u2v x = *reinterpret_cast<const u2v*>(at + (k_at ^ (64u * step))), y = *reinterpret_cast<const u2v*>(at + (k_at ^ (64u * step + 32u)));
+        return u4{x[0], x[1], y[0], y[1]};
+    };
+    // transposed: rows 4 g .. + 3 and 16 + 4 g .. + 3 of 32, a column a lane of 16
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)smem;
-    const int tr_place = linear_place(4 * g4 + (n16 >> 2)), tr_piece = n16 & 3;
-    const uint32_t kt_at = lds0 + (uint32_t)(L::kK + tr_place * L::kKRow + 16 * tr_piece), vt_at = lds0 + (uint32_t)(L::kV + tr_place * L::kVRow + 32 * wave + 8 * tr_piece);
+    const int tr_row = 4 * g4 + (n16 >> 2);
+    const uint32_t kt_at = linear_place<KP>(tr_row, n16 >> 1 & 1) + 8 * (n16 & 1);
+    const uint32_t vt_at = lds0 + L::kV + linear_place<VP>(tr_row, 2 * wave + (n16 >> 1 & 1)) + 8 * (n16 & 1);
     const auto transposed = [&](uint32_t at, int row_bytes) -> u4 {
         const s4v x = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)at));
         const s4v y = __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lds_s4*>((uintptr_t)(at + 16u * (uint32_t)row_bytes)));
@@ -413,12 +438,14 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
                     linear_split<T, 2>(x, y, w);
                     part_of[0][k] = w[0], part_of[1][k] = w[1];
                 }
+                // a product's result is an operand of another one 32 cycles after its start at the earliest, twice the time of its own: sums take turns
+                u4 qo[4];
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const u4 qo = q_operand(q, step);
-                    o[q] = linear_mfma<T>(part_of[0], qo, o[q]);
-                    o[q] = linear_mfma<T>(part_of[1], qo, o[q]);
-                }
+                for (int q = 0; q < 4; ++q) qo[q] = q_operand(q, step);
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) o[q] = linear_mfma<T>(part_of[x], qo[q], o[q]);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -432,13 +459,14 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         for (int u = 0; u < 2; ++u) v[u] = transposed(vt_at + 32 * u * L::kVRow, L::kVRow);
         if (with_q) {
             __syncthreads();
+            f4 rest[4] = {};
 #pragma unroll
             for (int pair = 0; pair < 6; ++pair) {
                 const int q = pair < 4 ? pair : pair - 2, u = pair < 4 ? 0 : 1;
                 const u4 hi = *reinterpret_cast<const u4*>(smem + L::kP + pair * 2048 + lane * 16), lo = *reinterpret_cast<const u4*>(smem + L::kP + pair * 2048 + 1024 + lane * 16);
                 if constexpr (kBf16) {
                     o[q] = linear_mfma<T>(v[u], hi, o[q]);
-                    o[q] = linear_mfma<T>(v[u], lo, o[q]);
+                    rest[q] = linear_mfma<T>(v[u], lo, rest[q]);
                 } else {
                     f4 sum = {};
                     sum = linear_mfma<T>(v[u], hi, sum);
@@ -449,10 +477,10 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
                 }
             }
             // to where v was, whose operands are in registers: lane (n, g) has columns 4 g .. + 3 of row n
-            uint8_t* const to = smem + L::kV + linear_place(n16) * L::kVRow + 32 * wave + 8 * g4;
+            uint8_t* const to = smem + L::kV + linear_place<VP>(n16, 2 * wave + (g4 >> 1)) + 8 * (g4 & 1);
 #pragma unroll
             for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<u2v*>(to + 16 * q * L::kVRow) = u2v{linear_pack<T>(o[q][0], o[q][1]), linear_pack<T>(o[q][2], o[q][3])};
+                *reinterpret_cast<u2v*>(to + 16 * q * L::kVRow) = u2v{linear_pack<T>(o[q][0] + rest[q][0], o[q][1] + rest[q][1]), linear_pack<T>(o[q][2] + rest[q][2], o[q][3] + rest[q][3])};
         }
         // the state moves on
         if (MODE == kLinearSums) part_sum += chunk[2];
@@ -490,12 +518,13 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
                     for (int q = 0; q < kParts; ++q) x[q][k] = parts[q];
                 }
+                u4 k[KM];
 #pragma unroll
-                for (int m = 0; m < KM; ++m) {
-                    const u4 k = transposed(kt_at + 32 * u * L::kKRow + 64 * (m >> 1) + 8 * (m & 1), L::kKRow);
+                for (int m = 0; m < KM; ++m) k[m] = transposed(lds0 + L::kK + 32 * u * L::kKRow + (kt_at ^ (32u * m)), L::kKRow);
 #pragma unroll
-                    for (int q = 0; q < kParts; ++q) s[m] = linear_mfma<T>(k, x[q], s[m]);
-                }
+                for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                    for (int m = 0; m < KM; ++m) s[m] = linear_mfma<T>(k[m], x[q], s[m]);
             }
         }
         t = end;
@@ -531,7 +560,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(const LinearArgs a, co
     const int first = linear_first_part(a, p.log_length, req), parts = linear_parts_of(r.n, r.kept, p.log_length);
     const int x = block * 256 + (int)threadIdx.x;  // [16 columns][16 channels][lane]
     const int lane = x & 63, tiles = k_dim / 16, m = (x >> 6) % tiles, w = (x >> 6) / tiles;
-    const int row = 32 * (m >> 1) + 8 * (lane >> 4) + 4 * (m & 1), col = 16 * w + (lane & 15);
+    const int row = 16 * m + 4 * (lane >> 4), col = 16 * w + (lane & 15);
     f4 s = {0.f, 0.f, 0.f, 0.f};
     if (r.in != nullptr) {
 #pragma unroll
