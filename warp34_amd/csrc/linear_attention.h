@@ -63,6 +63,21 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
         for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const linear_f4*>(r.in + (row0 + i) * DV + col);
     }
     const int kh = head / a.group, steps = a.out == nullptr ? r.kept : r.n;
+    // a token's rows are asked for while the one before it is gone through
+    uint4 kx[R / 8], qx[R / 8];
+    uint2 vx = {0, 0};
+    float gx = 0.f;
+    const auto fetch = [&](int t) {
+        const int64_t tok = r.lo + t;
+#pragma unroll
+        for (int i = 0; i < R / 8; ++i) {
+            kx[i] = reinterpret_cast<const uint4*>(a.k + tok * a.k_stride + kh * DK + row0)[i];
+            qx[i] = reinterpret_cast<const uint4*>(a.q + tok * a.q_stride + kh * DK + row0)[i];
+        }
+        vx = *reinterpret_cast<const uint2*>(a.v + tok * a.v_stride + head * DV + col);
+        if (a.g != nullptr) gx = a.g[tok * a.g_stride + head];
+    };
+    if (steps > 0) fetch(0);
     for (int t = 0; t <= steps; ++t) {
         if (t == r.kept && r.out != nullptr) {
 #pragma unroll
@@ -71,17 +86,14 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
         if (t == steps) break;
         const int64_t tok = r.lo + t;
         uint32_t kw[R / 2], qw[R / 2];
-        const uint4* kp = reinterpret_cast<const uint4*>(a.k + tok * a.k_stride + kh * DK + row0);
-        const uint4* qp = reinterpret_cast<const uint4*>(a.q + tok * a.q_stride + kh * DK + row0);
 #pragma unroll
         for (int i = 0; i < R / 8; ++i) {
-            const uint4 kx = kp[i], qx = qp[i];
-            kw[4 * i] = kx.x, kw[4 * i + 1] = kx.y, kw[4 * i + 2] = kx.z, kw[4 * i + 3] = kx.w;
-            qw[4 * i] = qx.x, qw[4 * i + 1] = qx.y, qw[4 * i + 2] = qx.z, qw[4 * i + 3] = qx.w;
+            kw[4 * i] = kx[i].x, kw[4 * i + 1] = kx[i].y, kw[4 * i + 2] = kx[i].z, kw[4 * i + 3] = kx[i].w;
+            qw[4 * i] = qx[i].x, qw[4 * i + 1] = qx[i].y, qw[4 * i + 2] = qx[i].z, qw[4 * i + 3] = qx[i].w;
         }
-        const uint2 vx = *reinterpret_cast<const uint2*>(a.v + tok * a.v_stride + head * DV + col);
-        const float fade = a.g == nullptr ? 1.f : expf(a.g[tok * a.g_stride + head]);
+        const float fade = a.g == nullptr ? 1.f : expf(gx);
         const f4 v = {T::to_f32((uint16_t)vx.x), T::to_f32((uint16_t)(vx.x >> 16)), T::to_f32((uint16_t)vx.y), T::to_f32((uint16_t)(vx.y >> 16))};
+        if (t + 1 < steps) fetch(t + 1);
         f4 o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < R; ++i) {
