@@ -41,7 +41,7 @@ typedef struct {
     int32_t        total_tokens;
     int32_t        max_q_len;
     float          scale;
-    int32_t        q_row_stride;      /* elements between tokens: of q, k, v, out (multiples of 8, at least heads * dim) */
+    int32_t        q_row_stride;      /* elements between tokens: of q, k, v, out (multiples of 8, at least heads * dim, at most 2^23) */
     int32_t        k_row_stride;
     int32_t        v_row_stride;
     int32_t        out_row_stride;
@@ -63,13 +63,16 @@ _Static_assert(sizeof(warp34_linear_attention_batch) == 88, "warp34_linear_atten
  * out may be NULL: only the states move on (the accepted part of a drafted step, say: state_tokens may be what
  * warp34_verify_drafts has written).  A request without tokens copies its state from slot to slot; the same slot may be the input
  * of several requests.  A request's output slot may be its own input slot; apart from that no output slot may be another request's
- * input or output.  Rows of no request are left as they were.  States are fp32 throughout; a prompt's products take 16-bit operands
+ * input or output.  Rows of no request are left as they were.  The rows and the states that a request reads must be finite, for its
+ * outputs those behind state_tokens too; masked requests and rows behind the last one may hold anything, and for the states what is
+ * behind state_tokens.  States are fp32 throughout; a prompt's products take 16-bit operands
  * split so that the states keep 2^-22 of their terms' size and outputs show their own rounding only.
  * Scratch (16-byte aligned, of warp34_linear_attention_scratch_bytes): prompts are cut into parts that run at once; with less, into
  * fewer, without any a request's heads run side by side and its tokens one part after another.  The order of summation depends on
  * max_q_len, num_reqs, total_tokens, the layout, the request's lengths and the scratch, and on nothing else: the same call gives the
  * same bits.  Two calls that may run at once need a workspace each.
- * hipErrorInvalidValue: a missing ex, layout, batch, query_start_loc, q, k or v, counts or strides out of range, a decay stride
+ * hipErrorInvalidValue: a missing ex, layout, batch, query_start_loc, q, k or v, counts (more than 2^20 heads) or strides out of
+ * range, a missing state_base where slots are named, a decay stride
  * that is neither 0 nor at least num_v_heads, a scale that is not finite; hipErrorNotSupported: other head dimensions, alignments.
  * No requests or no tokens bound (num_reqs <= 0, total_tokens < 0) return 0 without a launch. */
 int warp34_linear_attention_f16(const warp34_exec* ex, const warp34_linear_state_layout* layout,

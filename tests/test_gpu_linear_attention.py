@@ -95,6 +95,27 @@ def test_states_behind_the_kept_tokens(lens, kept, dt):
 
 @pytest.mark.gpu
 @BOTH
+@pytest.mark.parametrize("lens,kept,mask", [([5, 4, 3], [2, 0, 3], [1, 1, 0]), ([200, 130, 64], [70, 128, 3], [1, 1, 0]),
+                                            ([700, 65, 300], [333, 1, 299], [1, 1, 0])])
+def test_what_is_not_kept_may_hold_anything(lens, kept, mask, dt):
+    """No number in the rows behind the kept tokens, of a masked request and in the slots that requests of zeros would have: the states are unmoved by them."""
+    c = make(lens, dt, seed=24, kept=kept, mask=mask, has_initial=[1, 0, 1], slots=6)
+    want = c.want()
+    for r, length in enumerate(lens):
+        left = 0 if not mask[r] else kept[r]
+        for x in (c.q, c.k, c.v, c.g):
+            x[c.starts[r] + left:c.starts[r] + length] = float("nan")
+    c.states[1] = float("nan")
+    want[2][1] = 0.0
+    for with_out in (False, True):
+        out, states = c.call(with_out=with_out)
+        assert bool(states[1].isnan().all())
+        states[1] = 0.0
+        c.check((out, states), with_out=False, want=want)
+
+
+@pytest.mark.gpu
+@BOTH
 @pytest.mark.parametrize("lens", [[6, 1], [333, 128]])
 def test_decays(lens, dt):
     import torch
@@ -202,6 +223,7 @@ OK = dict(ex=True, layout=True, batch=True, qsl=1 << 12, q=1 << 20, k=1 << 21, v
     (dict(hk=0), 1), (dict(hv=0), 1), (dict(hv=3), 1), (dict(hk=-2), 1), (dict(scale=float("nan")), 1), (dict(scale=float("inf")), 1),
     (dict(qs=248), 1), (dict(ks=0), 1), (dict(vs=504), 1), (dict(os=504), 1), (dict(gs=3), 1), (dict(gs=-4), 1), (dict(base=0), 1),
     (dict(slot=4 * 4 * 128 * 128 - 16), 1), (dict(hv=1 << 21, hk=1 << 21), 1),
+    (dict(qs=(1 << 23) + 8), 1), (dict(ks=(1 << 23) + 8), 1), (dict(vs=(1 << 23) + 8), 1), (dict(os=(1 << 23) + 8), 1),
     (dict(dk=96), 801), (dict(dv=256, vs=1024, os=1024), 801), (dict(qs=260), 801), (dict(ks=257), 801), (dict(vs=516), 801), (dict(os=513), 801),
     (dict(q=(1 << 20) + 8), 801), (dict(k=(1 << 21) + 2), 801), (dict(v=(1 << 22) + 4), 801), (dict(out=(1 << 24) + 8), 801),
     (dict(base=(1 << 25) + 4), 801), (dict(slot=4 * 4 * 128 * 128 + 8), 801), (dict(g=(1 << 23) + 2), 801),
@@ -218,3 +240,14 @@ def test_refusals(name, args, code):
                                   a["os"], a["gs"], 0)
     assert getattr(ffi.load(), name)(C.byref(ex) if a["ex"] else None, C.byref(layout) if a["layout"] else None, C.byref(batch) if a["batch"] else None,
                                      a["q"], a["k"], a["v"], a["g"], a["out"]) == code
+
+
+@pytest.mark.parametrize("args", [dict(reqs=0), dict(tokens=0), dict(tokens=16), dict(most=16), dict(hv=0), dict(hv=1 << 21), dict(dk=96), dict(dv=32)])
+def test_no_scratch(args):
+    from warp34_amd import ffi
+
+    a = dict(OK, reqs=1, tokens=5000, most=5000)
+    need = lambda a: ffi.load().warp34_linear_attention_scratch_bytes(  # noqa: E731
+        C.byref(ffi.Warp34LinearStateLayout(a["base"], a["slot"], a["hk"], a["hv"], a["dk"], a["dv"])), a["reqs"], a["tokens"], a["most"])
+    assert need(a) > 0 and ffi.load().warp34_linear_attention_scratch_bytes(None, 1, 5000, 5000) == 0
+    assert need(dict(a, **args)) == 0

@@ -117,7 +117,8 @@ extern "C" size_t warp34_linear_attention_scratch_bytes(const warp34_linear_stat
         (layout->k_head_dim != 64 && layout->k_head_dim != 128) || (layout->v_head_dim != 64 && layout->v_head_dim != 128))
         return 0;
     if ((max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens) <= kStepTokens) return 0;
-    return linear_shape(layout, num_reqs, total_tokens, max_q_len, true, ~(size_t)0).bytes;
+    const size_t all = linear_shape(layout, num_reqs, total_tokens, max_q_len, false, ~(size_t)0).bytes;
+    return max(all, linear_shape(layout, num_reqs, total_tokens, max_q_len, true, ~(size_t)0).bytes);
 }
 extern "C" int warp34_linear_attention_f16(const warp34_exec* ex, const warp34_linear_state_layout* layout, const warp34_linear_attention_batch* batch,
                                            const void* q, const void* k, const void* v, const float* log_decay, void* out) {
