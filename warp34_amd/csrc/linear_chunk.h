@@ -427,25 +427,28 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
                 e = scale_exponent(wave_max(top));
             }
             const float by = power_of_two(e);
+            u4 part_of[2][2], qo[2][4];
+            const auto operands = [&](int step) {
 #pragma unroll
-            for (int step = 0; step < DK / 32; ++step) {
-                u4 part_of[2];
+                for (int q = 0; q < 4; ++q) qo[step & 1][q] = q_operand(q, step);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     uint32_t w[2];
                     float x = s[2 * step + (k >> 1)][2 * (k & 1)], y = s[2 * step + (k >> 1)][2 * (k & 1) + 1];
                     if (!kBf16) x *= by, y *= by;
                     linear_split<T, 2>(x, y, w);
-                    part_of[0][k] = w[0], part_of[1][k] = w[1];
+                    part_of[step & 1][0][k] = w[0], part_of[step & 1][1][k] = w[1];
                 }
-                // a product's result is an operand of another one 32 cycles after its start at the earliest, twice the time of its own: sums take turns
-                u4 qo[4];
+            };
+            operands(0);
 #pragma unroll
-                for (int q = 0; q < 4; ++q) qo[q] = q_operand(q, step);
+            for (int step = 0; step < DK / 32; ++step) {
+                if (step + 1 < DK / 32) operands(step + 1);
+                // a product's result is an operand of another one 32 cycles after its start at the earliest, twice the time of its own: sums take turns
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) o[q] = linear_mfma<T>(part_of[x], qo[q], o[q]);
+                    for (int q = 0; q < 4; ++q) o[q] = linear_mfma<T>(part_of[step & 1][x], qo[step & 1][q], o[q]);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
@@ -504,27 +507,34 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[m][i] *= by;
             }
+            u4 x[2][kParts], k[2][KM];
+            const auto operands = [&](int u) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                u4 x[kParts];
+                for (int m = 0; m < KM; ++m) k[u][m] = transposed(lds0 + L::kK + 32 * u * L::kKRow + (kt_at ^ (32u * m)), L::kKRow);
                 const f4 w0 = *reinterpret_cast<const f4*>(tables + L::kW + (32 * u + 4 * g4) * 4), w1 = *reinterpret_cast<const f4*>(tables + L::kW + (32 * u + 16 + 4 * g4) * 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const f4 w = k < 2 ? w0 : w1;
-                    float y = T::to_f32((uint16_t)v[u][k]) * w[2 * (k & 1)], z = T::to_f32((uint16_t)(v[u][k] >> 16)) * w[2 * (k & 1) + 1];
+                for (int i = 0; i < 4; ++i) {
+                    const f4 w = i < 2 ? w0 : w1;
+                    float y = T::to_f32((uint16_t)v[u][i]) * w[2 * (i & 1)], z = T::to_f32((uint16_t)(v[u][i] >> 16)) * w[2 * (i & 1) + 1];
                     if (!kBf16) y *= values, z *= values;
                     uint32_t parts[kParts];
                     linear_split<T, kParts>(y, z, parts);
 #pragma unroll
-                    for (int q = 0; q < kParts; ++q) x[q][k] = parts[q];
+                    for (int q = 0; q < kParts; ++q) x[u][q][i] = parts[q];
                 }
-                u4 k[KM];
+            };
+            operands(0);
 #pragma unroll
-                for (int m = 0; m < KM; ++m) k[m] = transposed(lds0 + L::kK + 32 * u * L::kKRow + (kt_at ^ (32u * m)), L::kKRow);
+            for (int u = 0; u < 2; ++u) {
+                if (u == 0) operands(1);
 #pragma unroll
                 for (int q = 0; q < kParts; ++q)
 #pragma unroll
-                    for (int m = 0; m < KM; ++m) s[m] = linear_mfma<T>(k[m], x[q], s[m]);
+                    for (int m = 0; m < KM; ++m) s[m] = linear_mfma<T>(k[u][m], x[u][q], s[m]);
+                if constexpr (!kBf16) {  // a product, three instructions of the next weighting in its shade (6 x 100 ... 1 900 tokens 87.2 -> 84.2 us, of bf16 slower)
+                    if (u == 0)
+                        for (int i = 0; i < KM * kParts; ++i) __builtin_amdgcn_sched_group_barrier(8, 1, 0), __builtin_amdgcn_sched_group_barrier(2, 3, 0);
+                }
             }
         }
         t = end;
