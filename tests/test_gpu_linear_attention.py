@@ -61,7 +61,7 @@ def test_rows_of_packed_projections(lens, dt):
 
 @pytest.mark.gpu
 @BOTH
-@pytest.mark.parametrize("lens", [[3, 1, 5, 0, 2], [80, 1, 300, 0, 129]])
+@pytest.mark.parametrize("lens", [[3, 1, 5, 0, 2], [80, 1, 300, 0, 129], [600, 0, 1, 700, 0]])
 def test_slots(lens, dt):
     """A slot read by two requests, one moved on in place, none to start from, none to go to, a request without tokens."""
     c = make(lens, dt, seed=12, slots=7, state_in=[0, 0, 2, 5, -1], state_out=[3, -1, 2, 6, 4])

@@ -8,34 +8,39 @@ namespace w34 {
 
 constexpr int kLinearGroups = 320;  // of the chunk kernel: one on each of 256 units, and some for parts that are short
 constexpr int kLinearMostStride = 1 << 23;  // elements: a chunk's rows are within 2^31 bytes
+// Up to so many parts of a request are joined by the kernel of the rows, each part reading what those before it add; more by a launch of their own:
+// 6 parts 21.2 -> 17.8 us, 8 parts of 32 heads 116.5 -> 112.0, 16 parts of 4 heads 20.9 -> 24.0 and of 16 heads 70.1 -> 69.5.
+constexpr int kLinearJoined = 8;
 constexpr int kStepTokens = 16;  // requests of up to so many tokens go by the recurrent kernel
 
 // How a batch is cut up.
 struct LinearShape {
     int log_length;  // tokens of a part, 0: requests are walked from end to end
     long long parts; // at most
+    bool joined;     // by the rows' kernel
     size_t bytes;    // of scratch
 };
 
-static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len, bool kept, size_t scratch) {
+static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len, bool kept, bool rows, size_t scratch) {
     const long long most = max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens;
     const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
-    LinearShape s{0, 0, 0};
-    // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make three launches and
-    // half as much work again.  us, 3.55 a chunk for a round of up to 256 workgroups against 19 and 0.0226 a chunk of a head: 333 tokens of 16
-    // heads walked 24.0, in parts 20.5, of 32 heads 25.0 / 28.5; 1 024 tokens of 32 heads 59.6 / 32.6, 4 x 1 024 64 / 71, 8 192 447 / 109,
-    // 4 x 4 096 244 / 206, 5 x 4 096 247 / 333.
+    LinearShape s{0, 0, false, 0};
+    // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make two or three launches
+    // and half as much work again.  us, 3.55 a chunk for a round of up to 256 workgroups against 15.4 and 0.0226 a chunk of a head: 130 tokens of 16
+    // heads walked 13.7, in parts 15.8, 333 tokens 23.9 / 17.7, of 32 heads 24.5 / 19.4, twice 25.7 / 25.4, six times 31.2 / 31.1; 3 x 500 tokens
+    // 34.6 / 38.7, 4 x 1 024 65.6 / 66.9, 4 x 4 096 247 / 211, 5 x 4 096 263 / 389.
     const long long groups = num_reqs * heads, chunks = (long long)total_tokens / kLinearChunk * heads + groups / 2;
-    if (157 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 840 + chunks) return s;
+    if (157 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 680 + chunks) return s;
     for (int log_length = 6; log_length < 30; ++log_length) {
         const long long length = 1ll << log_length;
         if (length >= most) return s;
-        // ceil(n / length) <= (n - 1) / length + 1 over the requests that have tokens, and one more for a cut behind the kept ones
-        const long long some = min((long long)num_reqs, (long long)total_tokens), parts = (total_tokens - some) / length + some * (kept ? 2 : 1);
-        const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)parts * heads * size * 4;
+        // ceil(n / length) <= n / length + 1 over the requests, and one more for a cut behind the kept tokens of those that have some
+        const long long parts = total_tokens / length + num_reqs + (kept ? min(num_reqs, total_tokens) : 0);
+        const bool joined = rows && (most + length - 1) / length + kept <= kLinearJoined;
+        const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)(parts + (joined ? num_reqs : 0)) * heads * size * 4;
         if (min(parts, num_reqs * ((most + length - 1) / length)) * heads > kLinearGroups) continue;
         if (bytes > scratch || !grid_fits(parts * heads * (size / 1024), 256)) continue;
-        s.log_length = log_length, s.parts = parts, s.bytes = bytes;
+        s.log_length = log_length, s.parts = parts, s.joined = joined, s.bytes = bytes;
         return s;
     }
     return s;
@@ -45,7 +50,7 @@ template <typename T, int DK, int DV>
 static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const LinearShape& shape) {
     const long long columns = (long long)a.v_heads;
     const hipStream_t stream = (hipStream_t)ex->stream;
-    LinearParts p{nullptr, nullptr, shape.log_length, (int)shape.parts};
+    LinearParts p{nullptr, nullptr, nullptr, shape.log_length, (int)shape.parts};
     if (shape.log_length == 0) {
         if (!grid_fits(a.num_reqs * columns, 4 * DV)) return (int)hipErrorInvalidValue;
         hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearWalk>), dim3((unsigned)(a.num_reqs * columns)), dim3(4 * DV), 0, stream, a, p);
@@ -54,14 +59,18 @@ static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const
     const long long scans = (long long)a.num_reqs * a.v_heads * (DK * DV / 1024);
     if (!grid_fits(shape.parts * columns, 4 * DV) || !grid_fits(scans, 256)) return (int)hipErrorInvalidValue;
     p.states = (float*)(uintptr_t)ex->scratch_ptr;
-    p.fades = p.states + shape.parts * a.v_heads * (DK * DV);
+    const long long slot = (long long)a.v_heads * (DK * DV);
+    if (shape.joined) p.starts = p.states + shape.parts * slot;
+    p.fades = p.states + (shape.parts + (shape.joined ? a.num_reqs : 0)) * slot;
     const dim3 grid((unsigned)(shape.parts * columns));
     hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearSums>), grid, dim3(4 * DV), 0, stream, a, p);
     int rc = (int)hipGetLastError();
     if (rc) return rc;
-    hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)scans), dim3(256), 0, stream, a, p, DK);
-    rc = (int)hipGetLastError();
-    if (rc || a.out == nullptr) return rc;
+    if (!shape.joined) {
+        hipLaunchKernelGGL(linear_scan_kernel, dim3((unsigned)scans), dim3(256), 0, stream, a, p, DK);
+        rc = (int)hipGetLastError();
+        if (rc || a.out == nullptr) return rc;
+    }
     hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearRows>), grid, dim3(4 * DV), 0, stream, a, p);
     return (int)hipGetLastError();
 }
@@ -75,7 +84,7 @@ static int linear_launch(const warp34_exec* ex, const warp34_linear_state_layout
         return (int)hipGetLastError();
     }
     const bool usable = ex->scratch_ptr != 0 && (ex->scratch_ptr & 15u) == 0;
-    const LinearShape shape = linear_shape(y, b->num_reqs, b->total_tokens, b->max_q_len, b->state_tokens != nullptr, usable ? ex->scratch_size : 0);
+    const LinearShape shape = linear_shape(y, b->num_reqs, b->total_tokens, b->max_q_len, b->state_tokens != nullptr, a.out != nullptr, usable ? ex->scratch_size : 0);
     return linear_chunk_launch<T, DK, DV>(ex, a, shape);
 }
 
@@ -117,8 +126,9 @@ extern "C" size_t warp34_linear_attention_scratch_bytes(const warp34_linear_stat
         (layout->k_head_dim != 64 && layout->k_head_dim != 128) || (layout->v_head_dim != 64 && layout->v_head_dim != 128))
         return 0;
     if ((max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens) <= kStepTokens) return 0;
-    const size_t all = linear_shape(layout, num_reqs, total_tokens, max_q_len, false, ~(size_t)0).bytes;
-    return max(all, linear_shape(layout, num_reqs, total_tokens, max_q_len, true, ~(size_t)0).bytes);
+    size_t bytes = 0;  // of the calls that such a batch may come in
+    for (int way = 0; way < 4; ++way) bytes = max(bytes, linear_shape(layout, num_reqs, total_tokens, max_q_len, way & 1, way & 2, ~(size_t)0).bytes);
+    return bytes;
 }
 extern "C" int warp34_linear_attention_f16(const warp34_exec* ex, const warp34_linear_state_layout* layout, const warp34_linear_attention_batch* batch,
                                            const void* q, const void* k, const void* v, const float* log_decay, void* out) {

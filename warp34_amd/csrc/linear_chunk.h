@@ -33,12 +33,13 @@ constexpr float kLeastDecay = -200.f;  // e^-200 times any fp32 number is zero i
 struct LinearParts {
     float* states;  // [part][value head][k_head_dim * v_head_dim] in the order of the registers: what a part adds, then what it starts from
     float* fades;   // [part][value head] 2^(sum of the part's g)
+    float* starts;  // [request][value head] as in states, where the rows' kernel joins the parts by itself: what the requests start from; else nullptr
     int log_length;
     int most;  // parts that there is room for
 };
 
 __device__ __forceinline__ int linear_parts_of(int n, int kept, int log_length) {
-    const int whole = (n + (1 << log_length) - 1) >> log_length;
+    const int whole = max(1, (n + (1 << log_length) - 1) >> log_length);  // a request without tokens has a part for its state
     return whole + (kept > 0 && kept < n && (kept & ((1 << log_length) - 1)) != 0 ? 1 : 0);
 }
 __device__ __forceinline__ void linear_part_range(int n, int kept, int log_length, int part, int& begin, int& end) {
@@ -203,17 +204,41 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
     for (int m = 0; m < KM; ++m) s[m] = f4{0.f, 0.f, 0.f, 0.f};
     int unit = 0;  // s holds the state times 2^unit (fp16), or over `hold` (bf16)
     float hold = 1.f;
-    // this wave's share of a part's state in scratch
-    float* const mine = MODE == kLinearWalk ? nullptr : p.states + ((int64_t)group * a.v_heads + head) * (DK * DV) + wave * (16 * DK) + lane * 4;
-    if (MODE == kLinearWalk && r.in != nullptr) {
+    // this wave's share of a part's state in scratch, and of the one that its request starts from
+    const auto share = [&](float* states, int i) { return states + ((int64_t)i * a.v_heads + head) * (DK * DV) + wave * (16 * DK) + lane * 4; };
+    float* const mine = MODE == kLinearWalk ? nullptr : share(p.states, group);
+    const bool joins = MODE != kLinearWalk && p.starts != nullptr;
+    if ((MODE == kLinearWalk || (MODE == kLinearSums && joins && part == 0)) && r.in != nullptr) {
 #pragma unroll
         for (int m = 0; m < KM; ++m)
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[m][i] = r.in[state_at + (16 * m + i) * DV];
     }
-    if (MODE == kLinearRows) {
+    if (MODE == kLinearSums && joins && part == 0 && r.in != nullptr) {
+        float* const to = share(p.starts, req);
+#pragma unroll
+        for (int m = 0; m < KM; ++m) *reinterpret_cast<f4*>(to + m * 256) = s[m], s[m] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (MODE == kLinearRows && !joins) {
 #pragma unroll
         for (int m = 0; m < KM; ++m) s[m] = *reinterpret_cast<const f4*>(mine + m * 256);
+    }
+    if (MODE == kLinearRows && joins) {  // as linear_scan_kernel() does
+        if (r.in != nullptr) {
+            const float* const from = share(p.starts, req);
+#pragma unroll
+            for (int m = 0; m < KM; ++m) s[m] = *reinterpret_cast<const f4*>(from + m * 256);
+        }
+        for (int i = 0; i < part; ++i) {
+            const float* const from = share(p.states, group - part + i);
+            const float fade = p.fades[(int64_t)(group - part + i) * a.v_heads + head];
+#pragma unroll
+            for (int m = 0; m < KM; ++m) {
+                const f4 u = *reinterpret_cast<const f4*>(from + m * 256);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[m][c] = __builtin_fmaf(fade, s[m][c], u[c]);
+            }
+        }
     }
     // The loads end here: pending in front of the loop, they would be waited for in it, and with them the chunk that is on its way there.
 #pragma unroll
@@ -228,7 +253,17 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
             for (int i = 0; i < 4; ++i) to[(16 * m + i) * DV] = s[m][i] * by;
     };
-    if (MODE == kLinearWalk && r.kept == 0 && r.out != nullptr) put_state();
+    if ((MODE == kLinearWalk || (MODE == kLinearRows && joins && part == 0)) && r.kept == 0 && r.out != nullptr) put_state();
+
+    if (MODE == kLinearRows && joins && r.kept > 0 && stop == r.kept && r.out != nullptr) {  // the state behind the part
+        const float fade = p.fades[(int64_t)group * a.v_heads + head];
+#pragma unroll
+        for (int m = 0; m < KM; ++m) {
+            const f4 u = *reinterpret_cast<const f4*>(mine + m * 256);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r.out[state_at + (16 * m + i) * DV] = __builtin_fmaf(fade, s[m][i], u[i]);
+        }
+    }
 
     // a chunk on its way
     const bool with_q = MODE == kLinearRows || (MODE == kLinearWalk && a.out != nullptr);
