@@ -29,7 +29,7 @@ typedef struct {
     int64_t        draft_row_stride;
     int32_t        num_reqs;
     int32_t        total_tokens;
-    int32_t        max_q_len;         /* host's bound on n, 0: not known */
+    int32_t        max_q_len;         /* host's bound on n, 0: not known; nothing depends on it as yet */
     int32_t        vocab_size;
 } warp34_draft_batch;
 
@@ -47,7 +47,7 @@ _Static_assert(sizeof(warp34_draft_batch) == 56, "warp34_draft_batch ABI size");
  * Scratch (16-byte aligned, warp34_verify_drafts_scratch_bytes): the vocabulary is summed by many workgroups; without it by one for
  * each request, with the same tokens but for those within the rounding of a 64-bit sum of a border.
  * hipErrorInvalidValue: a missing pointer, vocab_size < 1, strides below vocab_size, more than 2^20 requests; num_reqs <= 0 or
- * total_tokens <= 0 return 0 without a launch. */
+ * total_tokens <= 0 return 0 without a launch, nothing is written.  Two calls that may run at once need a workspace each. */
 int warp34_verify_drafts(const warp34_exec* ex, const warp34_draft_batch* batch, const float* target_probs,
                          const float* draft_probs, const float* accept_uniforms, const float* sample_uniforms,
                          int32_t* out_tokens, int32_t* emitted_counts);

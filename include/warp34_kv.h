@@ -202,9 +202,11 @@ int warp34_kv_cache_read_bf16(const warp34_exec* ex, const warp34_kv_layer_layou
  * by moving its last pages into its gaps.  layouts is a HOST array of num_layers descriptors, src_pages,
  * dst_pages and rows are DEVICE arrays of num_pairs.  Pairs with a negative page, or the same one twice, are passed
  * over.  No destination may be a source or a destination of another pair, and no two layouts may share memory.
- * hipErrorInvalidValue: missing pointers, negative num_layers, no slab, kv heads or block size; hipErrorNotSupported:
+ * hipErrorInvalidValue: missing pointers, negative num_layers, no slab, kv heads or block size, more than 2^24 pairs
+ * or 174 000 kv heads; hipErrorNotSupported:
  * formats whose rows are not those of the append, token strides below the row, strides or slabs that are not
- * 2-byte aligned.  num_layers == 0 or num_pairs <= 0 return 0 without a launch.  One launch for 48 layers.
+ * 2-byte aligned.  num_layers == 0 or num_pairs <= 0 return 0 without a launch.  One launch for
+ * 48 layers alike in heads and page size and 174 762 heads of pages.
  * ------------------------------------------------------------------------------------ */
 int warp34_kv_cache_copy_pages(const warp34_exec* ex, const warp34_kv_layer_layout* layouts, int num_layers,
                                const int32_t* src_pages, const int32_t* dst_pages, const int32_t* rows, int num_pairs);

@@ -114,6 +114,18 @@ def test_heads_and_many_pairs(heads):
 
 
 @pytest.mark.gpu
+def test_more_pairs_than_a_launch_takes():
+    """A whole pool's pairs, nearly all of them without work: of 96 slabs and 16 heads a launch takes 10 922."""
+    n, src, dst = 25000, [3, 0, 7], [1, 5, 6]
+    p = Pool([(FMT_TQ4, FMT_TQ4)] * 48, 8, heads=16, hd=128, bs=4, seed=10)
+    at = [0, 10921, n - 1]
+    pairs = [[-1] * n for _ in range(3)]
+    for i, s, d in zip(at, src, dst):
+        pairs[0][i], pairs[1][i], pairs[2][i] = s, d, 3
+    p.check(pairs[0], pairs[1], rows=pairs[2])
+
+
+@pytest.mark.gpu
 def test_pages_far_into_a_large_slab():
     """Page offsets beyond 2^32 bytes."""
     import torch
@@ -171,6 +183,7 @@ def test_captured_and_on_another_stream():
 @pytest.mark.parametrize("args,code", [
     (dict(ex=False), 1), (dict(layouts=False), 1), (dict(n=-1), 1), (dict(src=None), 1), (dict(dst=None), 1), (dict(kb=0), 1), (dict(vb=0), 1),
     (dict(heads=0), 1), (dict(bs=0), 1), (dict(bs=-16), 1), (dict(hd=0), 1), (dict(pairs=(1 << 31) - 1, heads=8), 1),
+    (dict(pairs=(1 << 24) + 1), 1), (dict(heads=180000), 1),
     (dict(fmt=9), 801), (dict(fmt=-1), 801), (dict(hd=192), 801), (dict(fmt=FMT_FP8, hd=128), 801), (dict(fmt=FMT_Q8_0, hd=96), 801), (dict(tok=130), 801),
     (dict(kb=(1 << 20) + 1), 801), (dict(page=16 * 132 * 2 + 1), 801), (dict(tok=133), 801), (dict(tok=1 << 32), 801),
     (dict(n=0), 0), (dict(pairs=0), 0), (dict(pairs=-2), 0), (dict(pairs=0, src=None, dst=None), 0)])

@@ -13,6 +13,7 @@ struct CopySlab {
     uint32_t token_stride, row_bytes;
 };
 constexpr int kCopySlabs = 96;
+constexpr int kCopyMostPairs = 1 << 24;
 struct CopyArgs {
     const int32_t *src_pages, *dst_pages, *rows;
     int num_pairs, heads, block_size, reserved;
@@ -76,11 +77,12 @@ static uint32_t copy_row_bytes(int format, int head_dim) {
 
 static int kv_copy_entry(const warp34_exec* ex, const warp34_kv_layer_layout* layouts, int num_layers, const int32_t* src_pages, const int32_t* dst_pages,
                          const int32_t* rows, int num_pairs) {
-    if (!ex || num_layers < 0 || (num_layers > 0 && !layouts) || (num_pairs > 0 && (!src_pages || !dst_pages))) return (int)hipErrorInvalidValue;
+    if (!ex || num_layers < 0 || (num_layers > 0 && !layouts) || (num_pairs > 0 && (!src_pages || !dst_pages)) || num_pairs > kCopyMostPairs)
+        return (int)hipErrorInvalidValue;
     for (int l = 0; l < num_layers; ++l) {  // everything is looked at before anything is launched
         const warp34_kv_layer_layout& y = layouts[l];
         if (!y.k_base || !y.v_base || y.local_kv_heads <= 0 || y.block_size <= 0 || y.head_dim <= 0 || y.head_dim > 4096) return (int)hipErrorInvalidValue;
-        if (num_pairs > 0 && !grid_fits(2ll * kCopySlabs * num_pairs * (long long)y.local_kv_heads, 256)) return (int)hipErrorInvalidValue;
+        if (!grid_fits((long long)kCopySlabs * y.local_kv_heads, 256)) return (int)hipErrorInvalidValue;
         const uint32_t kr = copy_row_bytes(y.k_format, y.head_dim), vr = copy_row_bytes(y.v_format, y.head_dim);
         if (!kr || !vr || y.k_token_stride_bytes < kr || y.v_token_stride_bytes < vr || (y.k_token_stride_bytes | y.v_token_stride_bytes) >> 31)
             return (int)hipErrorNotSupported;
@@ -102,12 +104,17 @@ static int kv_copy_entry(const warp34_exec* ex, const warp34_kv_layer_layout* la
                 if (a.slabs[s].token_stride != a.slabs[s].row_bytes) bits |= a.slabs[s].token_stride;
             }
         }
-        const dim3 grid((unsigned)((long long)n * num_pairs * a.heads));
-        if ((bits & 15u) == 0) hipLaunchKernelGGL(kv_copy_kernel<16>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
-        else if ((bits & 3u) == 0) hipLaunchKernelGGL(kv_copy_kernel<4>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
-        else hipLaunchKernelGGL(kv_copy_kernel<2>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
-        const int rc = (int)hipGetLastError();
-        if (rc) return rc;
+        const int most = (int)(((1ll << 32) / 256 - 1) / ((long long)n * a.heads));  // pairs that a launch has room for
+        for (int first = 0; first < num_pairs; first += most) {
+            a.src_pages = src_pages + first, a.dst_pages = dst_pages + first, a.rows = rows ? rows + first : nullptr;
+            a.num_pairs = min(most, num_pairs - first);
+            const dim3 grid((unsigned)((long long)n * a.num_pairs * a.heads));
+            if ((bits & 15u) == 0) hipLaunchKernelGGL(kv_copy_kernel<16>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
+            else if ((bits & 3u) == 0) hipLaunchKernelGGL(kv_copy_kernel<4>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
+            else hipLaunchKernelGGL(kv_copy_kernel<2>, grid, dim3(256), 0, (hipStream_t)ex->stream, a);
+            const int rc = (int)hipGetLastError();
+            if (rc) return rc;
+        }
     }
     return 0;
 }
