@@ -11,7 +11,16 @@ constexpr int kLinearMostStride = 1 << 23;  // elements: a chunk's rows are with
 // Up to so many parts of a request are joined by the kernel of the rows, each part reading what those before it add; more by a launch of their own:
 // 6 parts 21.2 -> 17.8 us, 8 parts of 32 heads 116.5 -> 112.0, 16 parts of 4 heads 20.9 -> 24.0 and of 16 heads 70.1 -> 69.5.
 constexpr int kLinearJoined = 8;
-constexpr int kStepTokens = 16;  // requests of up to so many tokens go by the recurrent kernel
+
+static long long linear_most(int total_tokens, int max_q_len) { return max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens; }
+
+// Whether a batch goes by the recurrent kernel, whose time grows with a request's tokens, or by chunks, of which it is one up to 64 tokens and whose
+// workgroups have a unit each: up to 4 tokens where one round of those holds the batch, up to 8 where there are more.  us recurrent / by chunks, of
+// 32 heads of 128 x 128: 8 requests of 4 tokens 12.1 / 12.3, of 8 16.0 / 12.4; 16 of 8 21.8 / 22.5, of 10 24.5 / 22.6; 32 of 4 34.6 / 46.0, of 8
+// 43.6 / 46.6, of 12 53.1 / 47.8; of 64 x 64: 8 of 4 5.8 / 6.0, 16 of 5 8.7 / 8.5, 32 of 8 14.9 / 14.2.
+static bool linear_steps(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len) {
+    return linear_most(total_tokens, max_q_len) <= ((long long)num_reqs * y->num_v_heads * y->v_head_dim <= 256 * 128 ? 4 : 8);
+}
 
 // How a batch is cut up.
 struct LinearShape {
@@ -22,7 +31,7 @@ struct LinearShape {
 };
 
 static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len, bool kept, bool rows, size_t scratch) {
-    const long long most = max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens;
+    const long long most = linear_most(total_tokens, max_q_len);
     const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
     LinearShape s{0, 0, false, 0};
     // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make two or three launches
@@ -77,8 +86,7 @@ static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const
 
 template <typename T, int DK, int DV>
 static int linear_launch(const warp34_exec* ex, const warp34_linear_state_layout* y, const warp34_linear_attention_batch* b, const LinearArgs& a) {
-    const int most = b->max_q_len > 0 && b->max_q_len < b->total_tokens ? b->max_q_len : b->total_tokens;
-    if (most <= kStepTokens) {
+    if (linear_steps(y, b->num_reqs, b->total_tokens, b->max_q_len)) {
         if (!grid_fits((long long)a.num_reqs * a.v_heads, 2 * DV)) return (int)hipErrorInvalidValue;
         hipLaunchKernelGGL((linear_step_kernel<T, DK, DV>), dim3((unsigned)a.num_reqs * (unsigned)a.v_heads), dim3(2 * DV), 0, (hipStream_t)ex->stream, a);
         return (int)hipGetLastError();
@@ -125,7 +133,7 @@ extern "C" size_t warp34_linear_attention_scratch_bytes(const warp34_linear_stat
     if (!layout || num_reqs <= 0 || total_tokens <= 0 || layout->num_v_heads <= 0 || layout->num_v_heads > (1 << 20) ||
         (layout->k_head_dim != 64 && layout->k_head_dim != 128) || (layout->v_head_dim != 64 && layout->v_head_dim != 128))
         return 0;
-    if ((max_q_len > 0 && max_q_len < total_tokens ? max_q_len : total_tokens) <= kStepTokens) return 0;
+    if (linear_steps(layout, num_reqs, total_tokens, max_q_len)) return 0;
     size_t bytes = 0;  // of the calls that such a batch may come in
     for (int way = 0; way < 4; ++way) bytes = max(bytes, linear_shape(layout, num_reqs, total_tokens, max_q_len, way & 1, way & 2, ~(size_t)0).bytes);
     return bytes;
