@@ -131,6 +131,27 @@ def test_accepted_and_drawn_tokens(lens, vocab, certain):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scratch", ["queried", 0])
+def test_rows_far_apart(scratch):
+    """Rows beyond 2^31 elements."""
+    import torch
+
+    import gpu_harness as G
+
+    d = Drafts([4], 3000, 11)
+    d.u[:2] = 0
+    want, dev, stride = d.want(), d.device(), (1 << 30) + 5
+    for name in ("p", "q"):
+        far = torch.empty(3 * stride + 3000, dtype=torch.float32, device=G.DEV)
+        for i in range(4):
+            far[i * stride:i * stride + 3000] = dev[name][i]
+        dev[name] = far
+    dev["batch"].target_row_stride = dev["batch"].draft_row_stride = stride
+    got = d.call(dev, scratch=scratch)
+    assert want[1][0] >= 3 and (got[0] == want[0]).all() and (got[1] == want[1]).all()
+
+
+@pytest.mark.gpu
 def test_every_draft_accepted_and_every_draft_refused():
     d = Drafts([5, 5, 1, 3], 4000, 7)
     d.u[:] = 0

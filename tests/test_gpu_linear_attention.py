@@ -155,6 +155,21 @@ def test_scratch_of_any_size(lens, heads, dt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens,pad", [([3, 300], 1), ([2, 4], 1), ([300], 4)])
+def test_rows_and_slots_far_into_memory(lens, pad):
+    """Rows beyond 2^31 elements, slots beyond 2^32 bytes."""
+    far = (1 << 23) - 512
+    c = make(lens, DT_BF16, seed=25, pads=(0, 0, far, 0, 0) if pad == 1 else (0, far // 8 * 8, 0, far, 0), v_heads=4, slots=2 * len(lens))
+    c.check(c.call())
+    if pad != 1:
+        return
+    c = make(lens, DT_BF16, seed=26, k_heads=2, v_heads=32, slots=2300, state_in=[2290, 2291], state_out=[2298, 2299])
+    out, bound, states, s_bound = c.want()
+    got = c.call()
+    c.check((got[0], got[1][2280:]), want=(out, bound, states[2280:], s_bound[2280:]))
+
+
+@pytest.mark.gpu
 @BOTH
 @pytest.mark.parametrize("lens", [[3, 4], [700, 300]])
 def test_same_call_same_bits(lens, dt):
@@ -178,7 +193,7 @@ def test_on_another_stream(lens):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("lens", [[1, 4, 2], [300, 65, 640]])
+@pytest.mark.parametrize("lens", [[1, 4, 2], [8, 1, 5], [300, 65, 400], [300, 65, 640]])
 def test_captured(lens):
     """In place in a captured graph: every replay moves the states on, as eager calls do, with eager work between."""
     import torch
