@@ -6,7 +6,7 @@
 
 namespace w34 {
 
-constexpr int kLinearGroups = 320;  // of the chunk kernel: one on each of 256 units, and some for parts that are short
+constexpr int kLinearPlaces = 256;  // of workgroups of eight waves, a unit each; of four waves there is room for more, and half as many count as one
 constexpr int kLinearMostStride = 1 << 23;  // elements: a chunk's rows are within 2^31 bytes
 // Up to so many parts of a request are joined by the kernel of the rows, each part reading what those before it add; more by a launch of their own:
 // 6 parts 21.2 -> 17.8 us, 8 parts of 32 heads 116.5 -> 112.0, 16 parts of 4 heads 20.9 -> 24.0 and of 16 heads 70.1 -> 69.5.
@@ -24,43 +24,55 @@ static bool linear_steps(const warp34_linear_state_layout* y, int num_reqs, int 
 
 // How a batch is cut up.
 struct LinearShape {
-    int log_length;  // tokens of a part, 0: requests are walked from end to end
-    long long parts; // at most
-    bool joined;     // by the rows' kernel
-    size_t bytes;    // of scratch
+    int length;       // tokens of a part, 0: requests are walked from end to end
+    long long parts;  // at most
+    bool joined;      // by the rows' kernel
+    size_t bytes;     // of scratch
 };
 
+// A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make two or three launches and
+// half as much work again, in rounds of as many workgroups as there are places.  How long they are, and whether there are any, goes by these times, in
+// us, of
+//   a walk   3.5 + 3.4 a chunk of the longest request, up to 4.1 where all places are taken, and as much longer as there are more workgroups
+//   parts    6 a chunk of a part and a round, 12 and 12 more for each round behind the first + 0.5 a part of the longest request, or 5 + 0.25 where a
+//            launch joins them.
+// Measured, 32 heads of 128 x 128 walked and in parts: 333 tokens 24.5 / 19.4, twice 25.7 / 25.4; 500 31.7 / 22.1, three times 34.6 / 38.7; 1 024 59 / 30,
+// four times 65.6 / 66.9; 8 192 447 / 103; 4 x 4 096 247 / 211, 5 x 4 096 263 / 389.
 static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_reqs, int total_tokens, int max_q_len, bool kept, bool rows, size_t scratch) {
-    const long long most = linear_most(total_tokens, max_q_len);
-    const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim;
+    const long long most = (linear_most(total_tokens, max_q_len) + kLinearChunk - 1) / kLinearChunk, total = total_tokens / kLinearChunk + 1;  // in chunks
+    const long long heads = y->num_v_heads, size = (long long)y->k_head_dim * y->v_head_dim, places = kLinearPlaces * (128 / y->v_head_dim);
+    const double full = (double)num_reqs * heads / places;
     LinearShape s{0, 0, false, 0};
-    // A request walked from end to end takes a chunk's time for each of its chunks, however few the workgroups are; parts make two or three launches
-    // and half as much work again.  us, 3.55 a chunk for a round of up to 256 workgroups against 15.4 and 0.0226 a chunk of a head: 130 tokens of 16
-    // heads walked 13.7, in parts 15.8, 333 tokens 23.9 / 17.7, of 32 heads 24.5 / 19.4, twice 25.7 / 25.4, six times 31.2 / 31.1; 3 x 500 tokens
-    // 34.6 / 38.7, 4 x 1 024 65.6 / 66.9, 4 x 4 096 247 / 211, 5 x 4 096 263 / 389.
-    const long long groups = num_reqs * heads, chunks = (long long)total_tokens / kLinearChunk * heads + groups / 2;
-    if (157 * ((most + kLinearChunk - 1) / kLinearChunk) * max(groups, 256ll) / 256 <= 680 + chunks) return s;
-    for (int log_length = 6; log_length < 30; ++log_length) {
-        const long long length = 1ll << log_length;
-        if (length >= most) return s;
-        // ceil(n / length) <= n / length + 1 over the requests, and one more for a cut behind the kept tokens of those that have some
+    double best = 3.5 + most * (3.4 + 0.7 * min(full, 1.0)) * max(full, 1.0);
+    for (long long chunks = 1; chunks < most; chunks += 1 + chunks / 32) {
+        const long long cuts = (most + chunks - 1) / chunks, length = chunks * kLinearChunk;
+        if ((cuts - 1) * heads >= 2 * places) continue;
+        // those there will be, about, and those there are room for: ceil(n / length) <= n / length + 1 over the requests, and one more for a cut
+        // behind the kept tokens of those that have some
+        const long long about = min(num_reqs * cuts, total / chunks + (num_reqs + 1) / 2);
         const long long parts = total_tokens / length + num_reqs + (kept ? min(num_reqs, total_tokens) : 0);
-        const bool joined = rows && (most + length - 1) / length + kept <= kLinearJoined;
+        const bool joined = rows && cuts + kept <= kLinearJoined;
         const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)(parts + (joined ? num_reqs : 0)) * heads * size * 4;
-        if (min(parts, num_reqs * ((most + length - 1) / length)) * heads > kLinearGroups) continue;
-        if (bytes > scratch || !grid_fits(parts * heads * (size / 1024), 256)) continue;
-        s.log_length = log_length, s.parts = parts, s.joined = joined, s.bytes = bytes;
-        return s;
+        const double time = (12.0 + 6.0 * chunks) * ((about * heads + places - 1) / places) + (joined ? 0.5 * cuts : 5.0 + 0.25 * cuts);
+        if (time >= best || bytes > scratch || !grid_fits(parts * heads * (size / 1024), 256)) continue;
+        best = time;
+        s.length = (int)length, s.parts = parts, s.joined = joined, s.bytes = bytes;
     }
     return s;
+}
+
+static LinearLength linear_length(int tokens) {
+    int s = 31;
+    while (tokens > 1ll << (s - 31)) ++s;
+    return tokens > 0 ? LinearLength{tokens, (uint32_t)(((1ull << s) + (uint64_t)tokens - 1) / (uint64_t)tokens), s - 32} : LinearLength{0, 0, 0};
 }
 
 template <typename T, int DK, int DV>
 static int linear_chunk_launch(const warp34_exec* ex, const LinearArgs& a, const LinearShape& shape) {
     const long long columns = (long long)a.v_heads;
     const hipStream_t stream = (hipStream_t)ex->stream;
-    LinearParts p{nullptr, nullptr, nullptr, shape.log_length, (int)shape.parts};
-    if (shape.log_length == 0) {
+    LinearParts p{nullptr, nullptr, nullptr, linear_length(shape.length), (int)shape.parts};
+    if (shape.length == 0) {
         if (!grid_fits(a.num_reqs * columns, 4 * DV)) return (int)hipErrorInvalidValue;
         hipLaunchKernelGGL((linear_chunk_kernel<T, DK, DV, kLinearWalk>), dim3((unsigned)(a.num_reqs * columns)), dim3(4 * DV), 0, stream, a, p);
         return (int)hipGetLastError();

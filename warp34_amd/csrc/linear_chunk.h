@@ -36,37 +36,45 @@ constexpr float kLeastHold = 1.f / 65536;  // a state's registers take their fac
 constexpr double kNearFades = 100.0;       // log2 of what 32 tokens may fade by to be weighted by two factors
 constexpr float kLeastDecay = -200.f;  // e^-200 times any fp32 number is zero in 32 bits: smaller ones, minus infinity among them, change nothing
 
-// A prompt cut into parts of `length` tokens, which run at once, and once more behind the tokens that its state keeps.
+// Tokens of a part, a multiple of 64, and how many of them are in a number below 2^31: n / tokens = n * ceil(2^s / tokens) >> s for s = 31 + log2 of
+// the tokens, rounded up.
+struct LinearLength {
+    int tokens;
+    uint32_t factor;
+    int shift;  // s - 32
+    __device__ __forceinline__ int in(int n) const { return (int)(__umulhi((uint32_t)n, factor) >> shift); }
+};
+// A prompt cut into parts, which run at once, and once more behind the tokens that its state keeps.
 struct LinearParts {
     float* states;  // [part][value head][k_head_dim * v_head_dim] in the order of the registers: what a part adds, then what it starts from
     float* fades;   // [part][value head] 2^(sum of the part's g)
     float* starts;  // [request][value head] as in states, where the rows' kernel joins the parts by itself: what the requests start from; else nullptr
-    int log_length;
+    LinearLength length;
     int most;  // parts that there is room for
 };
 
-__device__ __forceinline__ int linear_parts_of(int n, int kept, int log_length) {
-    const int whole = max(1, (n + (1 << log_length) - 1) >> log_length);  // a request without tokens has a part for its state
-    return whole + (kept > 0 && kept < n && (kept & ((1 << log_length) - 1)) != 0 ? 1 : 0);
+__device__ __forceinline__ int linear_parts_of(int n, int kept, const LinearLength& length) {
+    const int whole = n <= 0 ? 1 : length.in(n - 1) + 1;  // a request without tokens has a part for its state
+    return whole + (kept > 0 && kept < n && kept != length.in(kept) * length.tokens ? 1 : 0);
 }
-__device__ __forceinline__ void linear_part_range(int n, int kept, int log_length, int part, int& begin, int& end) {
-    const int length = 1 << log_length, cut = kept >> log_length;
-    const bool extra = kept > 0 && kept < n && (kept & (length - 1)) != 0;
+__device__ __forceinline__ void linear_part_range(int n, int kept, const LinearLength& length, int part, int& begin, int& end) {
+    const int cut = length.in(kept);
+    const bool extra = kept > 0 && kept < n && kept != cut * length.tokens;
     const int p = extra && part > cut ? part - 1 : part;
-    begin = p << log_length, end = min(begin + length, n);
+    begin = p * length.tokens, end = n - begin < length.tokens ? n : begin + length.tokens;
     if (extra && part == cut) end = kept;
     if (extra && part == cut + 1) begin = kept;
 }
-__device__ __forceinline__ int linear_request_parts(const LinearArgs& a, int req, int log_length) {
+__device__ __forceinline__ int linear_request_parts(const LinearArgs& a, int req, const LinearLength& length) {
     if (req >= a.num_reqs || (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0)) return 0;
     const int lo = max(0, a.query_start_loc[req]), n = max(0, min(a.query_start_loc[req + 1], a.total_tokens) - lo);
-    return linear_parts_of(n, a.state_tokens == nullptr ? n : min(max(a.state_tokens[req], 0), n), log_length);
+    return linear_parts_of(n, a.state_tokens == nullptr ? n : min(max(a.state_tokens[req], 0), n), length);
 }
 // Request and number within it of a part; false behind the last one.  A wave looks at 64 requests at a time.
-__device__ __forceinline__ bool linear_find_part(const LinearArgs& a, int log_length, int index, int& req, int& part) {
+__device__ __forceinline__ bool linear_find_part(const LinearArgs& a, const LinearLength& length, int index, int& req, int& part) {
     const int lane = lane_id();
     for (int base = 0; base < a.num_reqs; base += 64) {
-        const int mine = linear_request_parts(a, base + lane, log_length);
+        const int mine = linear_request_parts(a, base + lane, length);
         int run = mine;
 #pragma unroll
         for (int by = 1; by < 64; by *= 2) {
@@ -85,9 +93,9 @@ __device__ __forceinline__ bool linear_find_part(const LinearArgs& a, int log_le
     return false;
 }
 // Number of the first part of a request.
-__device__ __forceinline__ int linear_first_part(const LinearArgs& a, int log_length, int req) {
+__device__ __forceinline__ int linear_first_part(const LinearArgs& a, const LinearLength& length, int req) {
     int count = 0;
-    for (int base = 0; base < req; base += 64) count += base + lane_id() < req ? linear_request_parts(a, base + lane_id(), log_length) : 0;
+    for (int base = 0; base < req; base += 64) count += base + lane_id() < req ? linear_request_parts(a, base + lane_id(), length) : 0;
 #pragma unroll
     for (int by = 32; by; by /= 2) count += __shfl_xor(count, by, 64);
     return __builtin_amdgcn_readfirstlane(count);
@@ -195,14 +203,14 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
     if (MODE == kLinearWalk) {
         if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
     } else {
-        if (!linear_find_part(a, p.log_length, group, req, part)) return;
+        if (!linear_find_part(a, p.length, group, req, part)) return;
     }
     LinearRequest r = linear_request(a, req, head, DK * DV);
     r.lo = __builtin_amdgcn_readfirstlane(r.lo), r.n = __builtin_amdgcn_readfirstlane(r.n), r.kept = __builtin_amdgcn_readfirstlane(r.kept);
     const int state_at = 4 * g4 * DV + 16 * wave + n16;  // element of the state that is this lane's first
 
     int begin = 0, stop = r.n;
-    if (MODE != kLinearWalk) linear_part_range(r.n, r.kept, p.log_length, part, begin, stop);
+    if (MODE != kLinearWalk) linear_part_range(r.n, r.kept, p.length, part, begin, stop);
     else if (a.out == nullptr) stop = r.kept;
     begin = __builtin_amdgcn_readfirstlane(begin), stop = __builtin_amdgcn_readfirstlane(stop);
 
@@ -609,7 +617,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(const LinearArgs a, co
     const int head = at % a.v_heads, req = at / a.v_heads;
     if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
     const LinearRequest r = linear_request(a, req, head, size);
-    const int first = linear_first_part(a, p.log_length, req), parts = linear_parts_of(r.n, r.kept, p.log_length);
+    const int first = linear_first_part(a, p.length, req), parts = linear_parts_of(r.n, r.kept, p.length);
     const int x = block * 256 + (int)threadIdx.x;  // [16 columns][16 channels][lane]
     const int lane = x & 63, tiles = k_dim / 16, m = (x >> 6) % tiles, w = (x >> 6) / tiles;
     const int row = 16 * m + 4 * (lane >> 4), col = 16 * w + (lane & 15);
@@ -646,7 +654,7 @@ __global__ __launch_bounds__(256) void linear_scan_kernel(const LinearArgs a, co
 #pragma unroll
             for (int i = 0; i < 4; ++i) s[i] = __builtin_fmaf(by, s[i], add[i]);
             int begin, end;
-            linear_part_range(r.n, r.kept, p.log_length, part, begin, end);
+            linear_part_range(r.n, r.kept, p.length, part, begin, end);
             if (end == r.kept && r.out != nullptr) keep();
         }
     }
