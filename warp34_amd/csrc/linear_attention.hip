@@ -47,10 +47,10 @@ static LinearShape linear_shape(const warp34_linear_state_layout* y, int num_req
     for (long long chunks = 1; chunks < most; chunks += 1 + chunks / 32) {
         const long long cuts = (most + chunks - 1) / chunks, length = chunks * kLinearChunk;
         if ((cuts - 1) * heads >= 2 * places) continue;
-        // those there will be, about, and those there are room for: ceil(n / length) <= n / length + 1 over the requests, and one more for a cut
-        // behind the kept tokens of those that have some
+        // those there will be, about, and those there are room for: ceil(n / length) <= (n - 1) / length + 1 over the requests, of which those
+        // without tokens have one too, and one more for a cut behind the kept tokens
         const long long about = min(num_reqs * cuts, total / chunks + (num_reqs + 1) / 2);
-        const long long parts = total_tokens / length + num_reqs + (kept ? min(num_reqs, total_tokens) : 0);
+        const long long parts = (total_tokens - 1) / length + num_reqs + (kept ? min(num_reqs, total_tokens) : 0);
         const bool joined = rows && cuts + kept <= kLinearJoined;
         const size_t bytes = ((size_t)parts * heads * 4 + 15) / 16 * 16 + (size_t)(parts + (joined ? num_reqs : 0)) * heads * size * 4;
         const double time = (12.0 + 6.0 * chunks) * ((about * heads + places - 1) / places) + (joined ? 0.5 * cuts : 5.0 + 0.25 * cuts);
