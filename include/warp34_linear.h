@@ -8,7 +8,8 @@
  * and has_initial_state.
  *
  * One entry serves prompts, single tokens and drafted tokens.  max_q_len, the host's bound on a request's tokens (0: not known,
- * total_tokens), chooses between two kernels that add in another order, and changes nothing else. */
+ * total_tokens), chooses between kernels that add in another order and, of prompts, how they are cut, and changes nothing else; a
+ * bound that is wrong costs time only. */
 #ifndef WARP34_LINEAR_H
 #define WARP34_LINEAR_H
 
@@ -69,11 +70,11 @@ _Static_assert(sizeof(warp34_linear_attention_batch) == 88, "warp34_linear_atten
  * split so that the states keep 2^-22 of their terms' size and outputs show their own rounding only.
  * Scratch (16-byte aligned, of warp34_linear_attention_scratch_bytes): prompts are cut into parts that run at once; with less, into
  * fewer, without any a request's heads run side by side and its tokens one part after another.  The order of summation depends on
- * max_q_len, num_reqs, total_tokens, the layout, the request's lengths and the scratch, and on nothing else: the same call gives the
- * same bits.  Two calls that may run at once need a workspace each.
+ * max_q_len, num_reqs, total_tokens, the layout, the request's lengths, the scratch, and on which of out and state_tokens are there, and
+ * on nothing else: the same call gives the same bits.  Two calls that may run at once need a workspace each.
  * hipErrorInvalidValue: a missing ex, layout, batch, query_start_loc, q, k or v, counts (more than 2^20 heads) or strides out of
- * range, a missing state_base where slots are named, a decay stride
- * that is neither 0 nor at least num_v_heads, a scale that is not finite; hipErrorNotSupported: other head dimensions, alignments.
+ * range, a missing state_base where slots are named, a decay stride that is neither 0 nor at least num_v_heads, a scale that is not
+ * finite; hipErrorNotSupported: other head dimensions, alignments.
  * No requests or no tokens bound (num_reqs <= 0, total_tokens < 0) return 0 without a launch. */
 int warp34_linear_attention_f16(const warp34_exec* ex, const warp34_linear_state_layout* layout,
                                 const warp34_linear_attention_batch* batch, const void* q, const void* k, const void* v,
