@@ -193,6 +193,37 @@ def test_on_another_stream(lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("lens", [([700, 64], [300, 200]), ([4, 2], [900]), ([8] * 5, [1] * 40)])
+def test_two_calls_at_once(lens):
+    """On two streams, each with a workspace of its own, one behind the other many times: the bits of calls alone."""
+    import torch
+
+    import gpu_harness as G
+    from warp34_amd import ffi
+
+    cases = [make(x, dt, seed=27 + i, slots=2 * len(x)) for i, (x, dt) in enumerate(zip(lens, (DT_BF16, DT_F16)))]
+    alone = [c.call() for c in cases]
+    calls, keep = [], []
+    for c in cases:
+        out, states = c.fresh()
+        layout, batch = c.structs(states)
+        need = G.lib().warp34_linear_attention_scratch_bytes(C.byref(layout), len(c.lens), c.n, max(c.lens))
+        work, stream = torch.zeros(max(16, need), dtype=torch.uint8, device=G.DEV), torch.cuda.Stream()
+        ex = ffi.Warp34Exec(stream.cuda_stream, work.data_ptr(), need, 0)
+        fn = G.lib().warp34_linear_attention_f16 if c.dt == DT_F16 else G.lib().warp34_linear_attention_bf16
+        keep.append((out, states, layout, batch, work, stream, ex))
+        calls.append((fn, (C.byref(ex), C.byref(layout), C.byref(batch), G.ptr(c.q), G.ptr(c.k), G.ptr(c.v), G.ptr(c.g), G.ptr(out))))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for fn, args in calls:
+            assert fn(*args) == 0
+    torch.cuda.synchronize()
+    for c, (want, states), mine in zip(cases, alone, keep):
+        got = mine[0][:c.n, :c.hv * c.dv].reshape(want.shape)
+        assert torch.equal(got.view(torch.int16), want.view(torch.int16)) and torch.equal(mine[1], states)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lens", [[1, 4, 2], [8, 1, 5], [300, 65, 400], [300, 65, 640]])
 def test_captured(lens):
     """In place in a captured graph: every replay moves the states on, as eager calls do, with eager work between."""
