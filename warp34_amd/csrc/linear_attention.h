@@ -80,12 +80,12 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
         if (a.g != nullptr) gx = a.g[tok * a.g_stride + head];
     };
     if (steps > 0) fetch(0);
-    for (int t = 0; t <= steps; ++t) {
-        if (t == r.kept && r.out != nullptr) {
+    if (r.kept == 0 && r.out != nullptr) {
 #pragma unroll
-            for (int i = 0; i < R; ++i) *reinterpret_cast<linear_f4*>(r.out + (row0 + i) * DV + col) = s[i];
-        }
-        if (t == steps) break;
+        for (int i = 0; i < R; ++i) *reinterpret_cast<linear_f4*>(r.out + (row0 + i) * DV + col) = s[i];
+    }
+    for (int t = 0; t < steps; ++t) {
+        const bool keeps = t + 1 == r.kept && r.out != nullptr;
         const int64_t tok = r.lo + t;
         uint32_t kw[R / 2], qw[R / 2];
 #pragma unroll
@@ -105,6 +105,7 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
                 s[i][c] = __builtin_fmaf(ki, v[c], fade * s[i][c]);
                 o[c] = __builtin_fmaf(qi, s[i][c], o[c]);
             }
+            if (keeps) *reinterpret_cast<linear_f4*>(r.out + (row0 + i) * DV + col) = s[i];
         }
         if (a.out == nullptr) continue;
 #pragma unroll
