@@ -48,8 +48,8 @@ __device__ __forceinline__ LinearRequest linear_request(const LinearArgs& a, int
 // A wave keeps 32 columns of a head's state in registers, lane l columns 4 (l & 7) .. + 3 of rows DK / 8 (l >> 3) .. + DK / 8 - 1, so that a row is
 // read in runs of 128 bytes and the state passes once through the chip however many tokens there are.  The waves of a workgroup have the head's
 // other columns and the same q and k; nothing is exchanged between them.  All in 32 bits.
-// Bound: HBM, the state read once and written once: 64 single tokens of 32 heads of 128 x 128, 270 MB, 54 us (5.0 TB/s, the rate of a large copy);
-// 16 x 5 tokens 16.5 us, where the tokens' 5 x 64 multiply-adds a lane come to the same; one token 4.2 us, a launch and two round trips.
+// Bound: HBM, the state read once and written once: 64 single tokens of 32 heads of 128 x 128, 270 MB, 53.4 us (5.05 TB/s, the rate of a large copy);
+// 16 x 5 tokens 15.8 us, where the tokens' 5 x 64 multiply-adds a lane come to the same; one token 4.2 us, a launch and two round trips.
 template <typename T, int DK, int DV>
 __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a) {
     constexpr int R = DK / 8;
@@ -57,13 +57,6 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
     if (a.valid_req_mask != nullptr && a.valid_req_mask[req] == 0) return;
     const int lane = lane_id(), row0 = (lane >> 3) * R, col = ((int)threadIdx.x >> 6) * 32 + (lane & 7) * 4;
     const LinearRequest r = linear_request(a, req, head, DK * DV);
-    f4 s[R];
-#pragma unroll
-    for (int i = 0; i < R; ++i) s[i] = f4{0.f, 0.f, 0.f, 0.f};
-    if (r.in != nullptr) {
-#pragma unroll
-        for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const linear_f4*>(r.in + (row0 + i) * DV + col);
-    }
     const int kh = head / a.group, steps = a.out == nullptr ? r.kept : r.n;
     // a token's rows are asked for while the one before it is gone through
     uint4 kx[R / 8], qx[R / 8];
@@ -80,6 +73,13 @@ __global__ __launch_bounds__(2 * DV) void linear_step_kernel(const LinearArgs a)
         if (a.g != nullptr) gx = a.g[tok * a.g_stride + head];
     };
     if (steps > 0) fetch(0);
+    f4 s[R];
+#pragma unroll
+    for (int i = 0; i < R; ++i) s[i] = f4{0.f, 0.f, 0.f, 0.f};
+    if (r.in != nullptr) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) s[i] = *reinterpret_cast<const linear_f4*>(r.in + (row0 + i) * DV + col);
+    }
     if (r.kept == 0 && r.out != nullptr) {
 #pragma unroll
         for (int i = 0; i < R; ++i) *reinterpret_cast<linear_f4*>(r.out + (row0 + i) * DV + col) = s[i];
