@@ -336,7 +336,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         put(L::kW, __builtin_amdgcn_exp2f((float)(all - run)) * (again ? 1.f : 1.f / next));
         if constexpr (MODE != kLinearSums) {
             const double centre = lane < 32 ? 0.5 * (start + half) : 0.5 * (middle + all);
-            put(L::kState, __builtin_amdgcn_exp2f((float)run) * (held * a.scale));
+            put(L::kState, __builtin_amdgcn_exp2f((float)run) * held);
             put(L::kAcross, __builtin_amdgcn_exp2f((float)(lane < 32 ? half - run : run - half)));
             put(L::kUp, __builtin_amdgcn_exp2f((float)(run - centre)));
             put(L::kDown, __builtin_amdgcn_exp2f((float)(centre - run)));
@@ -376,15 +376,16 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
             for (int k = 0; k < 2; ++k) x[k] = linear_mfma<T>(k_operand(keys + k, step), q, x[k]);
         }
-        // 2^(G_i - G_j) as a product: by way of G at the border between the halves, or at the middle of the half where it fades by little there
+        // 2^(G_i - G_j) as a product: by way of G at the border between the halves, or at the middle of the half where it fades by little there.
+        // The factors, up to 2^50, are multiplied by each other first: q . k times one of them need not be a number.
         const int i0 = 16 * query + n16, j0 = 16 * keys + 4 * g4;
         if (across || near) {
-            const float row = *reinterpret_cast<const float*>(tables + (across ? L::kAcross : L::kUp) + i0 * 4) * a.scale;
+            const float row = *reinterpret_cast<const float*>(tables + (across ? L::kAcross : L::kUp) + i0 * 4);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 const f4 w = *reinterpret_cast<const f4*>(tables + (across ? L::kAcross : L::kDown) + (j0 + 16 * k) * 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[k][i] = j0 + 16 * k + i <= i0 ? x[k][i] * row * w[i] : 0.f;
+                for (int i = 0; i < 4; ++i) x[k][i] = j0 + 16 * k + i <= i0 ? x[k][i] * (row * w[i]) : 0.f;
             }
         } else {
             const float2 gi = *reinterpret_cast<const float2*>(tables + L::kG + i0 * 8);
@@ -393,7 +394,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const float2 gj = *reinterpret_cast<const float2*>(tables + L::kG + (j0 + 16 * k + i) * 8);
-                    const float y = x[k][i] * __builtin_amdgcn_exp2f((gi.x - gj.x) + (gi.y - gj.y)) * a.scale;
+                    const float y = x[k][i] * __builtin_amdgcn_exp2f((gi.x - gj.x) + (gi.y - gj.y));
                     x[k][i] = j0 + 16 * k + i <= i0 ? y : 0.f;
                 }
         }
@@ -532,8 +533,11 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
             // to where v was, whose operands are in registers: lane (n, g) has columns 4 g .. + 3 of row n
             uint8_t* const to = smem + L::kV + linear_place<VP>(n16, 2 * wave + (g4 >> 1)) + 8 * (g4 & 1);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                *reinterpret_cast<u2v*>(to + 16 * q * L::kVRow) = u2v{linear_pack<T>(o[q][0] + rest[q][0], o[q][1] + rest[q][1]), linear_pack<T>(o[q][2] + rest[q][2], o[q][3] + rest[q][3])};
+            for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[q][i] = (o[q][i] + rest[q][i]) * a.scale;
+                *reinterpret_cast<u2v*>(to + 16 * q * L::kVRow) = u2v{linear_pack<T>(o[q][0], o[q][1]), linear_pack<T>(o[q][2], o[q][3])};
+            }
         }
         // the state moves on
         if (MODE == kLinearSums) part_sum += chunk[2];
