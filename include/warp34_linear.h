@@ -66,8 +66,12 @@ _Static_assert(sizeof(warp34_linear_attention_batch) == 88, "warp34_linear_atten
  * of several requests.  A request's output slot may be its own input slot; apart from that no output slot may be another request's
  * input or output.  Rows of no request are left as they were.  The rows and the states that a request reads must be finite, for its
  * outputs those behind state_tokens too; masked requests and rows behind the last one may hold anything, and for the states what is
- * behind state_tokens.  States are fp32 throughout; a prompt's products take 16-bit operands
- * split so that the states keep 2^-22 of their terms' size and outputs show their own rounding only.
+ * behind state_tokens.
+ * Exactness, in parts of the terms' size (of a state: faded |S| + sum of weighted |k| |v|^T; of an output: scale |q|^T times that): a prompt's products take
+ * 16-bit operands in parts, which leave states, fp32 throughout, within 2^-20 for each 64 tokens that still count, and outputs within 2^-15 (bf16) or 2^-19 (fp16)
+ * beside their state's error and their own rounding; where terms cancel, that shows.  fp16 adds, of each of its operands, 2^-50 of the largest value of
+ * a column weighted at its chunk's end, state of a column, or weight of a row; weights below 2^-126 count as zero.  What is summed up (q . k, S^T q, k v^T) has to stay
+ * below 2^100 in size.
  * Scratch (16-byte aligned, of warp34_linear_attention_scratch_bytes): prompts are cut into parts that run at once; with less, into
  * fewer, without any a request's heads run side by side and its tokens one part after another.  The order of summation depends on
  * max_q_len, num_reqs, total_tokens, the layout, the request's lengths, the scratch, and on which of out and state_tokens are there, and

@@ -12,7 +12,8 @@
 // tokens have faded away, the sums are large and the differences small.
 // Operands of 16 bits are rounded states, weights and weighted values.  P and S have two parts (16 bits of bf16, 22 of fp16), so that outputs
 // show their own rounding only; v' has three for bf16 where the state itself comes out (24 bits), two for fp16.  fp16 has little range:
-// v' and S are scaled by powers of two of a wave, P by one of a row, to put the largest at 2^14; what is lost are bits 2^-39 below it.
+// weighted values and S are scaled by a power of two of their column, P by one of its row, to put the largest at 2^14, and what the first part leaves is
+// held times 2^11 and has sums of its own.  So 22 bits stay of what is up to 2^28 below the largest, and bits 2^-50 below it are lost.
 //
 // Bound: instruction issue.  A wave's chunk is 100 products of 16 cycles and 460 vector instructions of four, the two waves of a SIMD take 6 900 of the
 // 8 200 cycles that a chunk of a full batch lasts: splits and products of a wave wait for each other, and the clock falls to 1.8 .. 2.0 GHz.  8 x 4 096 tokens of 32
@@ -118,6 +119,7 @@ __device__ __forceinline__ uint32_t linear_pack(float x, float y) {
         return pack_h2(x, y);
     }
 }
+constexpr float kRestUp = 2048.f, kRestDown = 1.f / 2048.f;  // the second part of fp16 is held times that
 // Two numbers as PARTS pairs of 16 bits whose sums they are.  (What a pair of bf16 leaves of its numbers is also a dot product with (-1, 0) and
 // (0, -1), half as many instructions, but v_dot2_f32_bf16 issues every 16 cycles: a chunk of rows took 7 % longer.)
 template <typename T, int PARTS>
@@ -132,23 +134,16 @@ __device__ __forceinline__ void linear_split(float x, float y, uint32_t (&w)[PAR
         } else {  // as in split_weights(): one mixed-precision fma each
             asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,0] op_sel_hi:[0,0,1]" : "=v"(x) : "v"(x), "v"(w[p]));
             asm("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[0,0,1] op_sel_hi:[0,0,1]" : "=v"(y) : "v"(y), "v"(w[p]));
+            x *= kRestUp, y *= kRestUp;
         }
     }
 }
-// The e for which 2^e puts `top` at 2^14, at most 100: 2^e and 2^-e are numbers.  0 for zero, and for what is not finite.
+// The e for which 2^e puts `top` at 2^14, at most 126: 2^e and 2^-e are numbers.  0 for zero, and for what is not finite.
 __device__ __forceinline__ int scale_exponent(float top) {
     const int e = (int)(__float_as_uint(top) >> 23 & 255u);
-    return e == 0 || e == 255 ? 0 : min(141 - e, 100);
+    return e == 0 || e == 255 ? 0 : min(141 - e, 126);
 }
 __device__ __forceinline__ float power_of_two(int e) { return __builtin_amdgcn_ldexpf(1.0f, e); }
-__device__ __forceinline__ float wave_max(float x) {  // without LDS
-    const int lane = lane_id();
-    x = fmaxf(x, lane_xor<1>(x, lane));
-    x = fmaxf(x, lane_xor<2>(x, lane));
-    x = fmaxf(x, lane_xor<4>(x, lane));
-    x = fmaxf(x, lane_xor<8>(x, lane));
-    return max_over_rows(x);
-}
 
 // Where 16 bytes of a row are in LDS, as the number they are found under in it: rows of PIECES = 8 or 16.  A wave's 16-byte reads go by lanes 0 .. 3,
 // 12 .. 15 and 20 .. 27, then 4 .. 11, 16 .. 19 and 28 .. 31 (and the same of its second half): pieces g and g + 1 of rows {0 .. 3, 12 .. 15} and {4 .. 11}
@@ -217,8 +212,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
     f4 s[KM];
 #pragma unroll
     for (int m = 0; m < KM; ++m) s[m] = f4{0.f, 0.f, 0.f, 0.f};
-    int unit = 0;  // s holds the state times 2^unit (fp16), or over `hold` (bf16)
-    float hold = 1.f;
+    float hold = 1.f;  // s holds the state over it (bf16; fp16: 1)
     // this wave's share of a part's state in scratch, and of the one that its request starts from
     const auto share = [&](float* states, int i) { return states + ((int64_t)i * a.v_heads + head) * (DK * DV) + wave * (16 * DK) + lane * 4; };
     float* const mine = MODE == kLinearWalk ? nullptr : share(p.states, group);
@@ -259,7 +253,7 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
     for (int m = 0; m < KM; ++m) asm volatile("" : "+v"(s[m]));
     const auto put_state = [&]() {
-        const float by = kBf16 ? hold : power_of_two(-unit);
+        const float by = hold;
         int first = state_at;
         asm volatile("" : "+v"(first));  // addresses are worked out here, not kept in registers through the chunks
         linear_float* const to = r.out + first;
@@ -468,16 +462,19 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
                 weights(2 * wave + 1, near);
             }
             // the state's part of the rows
-            int e = 0;
+            float by = 1.f;
+            f4 down = {1.f, 1.f, 1.f, 1.f}, low[4] = {};  // fp16: the rest's sums
             if constexpr (!kBf16) {
                 float top = 0.f;
 #pragma unroll
                 for (int m = 0; m < KM; ++m)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(s[m][i]));
-                e = scale_exponent(wave_max(top));
+                const int e = scale_exponent(max_over_rows(top));  // of the lane's column; the product has columns 4 g .. + 3
+                by = power_of_two(e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) down[i] = __shfl(power_of_two(-e), 4 * g4 + i, 64);
             }
-            const float by = power_of_two(e);
             u4 part_of[2][2], qo[2][4];
             const auto operands = [&](int step) {
 #pragma unroll
@@ -499,13 +496,19 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) o[q] = linear_mfma<T>(part_of[step & 1][x], qo[step & 1][q], o[q]);
+                    for (int q = 0; q < 4; ++q) {
+                        f4& to = !kBf16 && x ? low[q] : o[q];
+                        to = linear_mfma<T>(part_of[step & 1][x], qo[step & 1][q], to);
+                    }
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const float f = *reinterpret_cast<const float*>(tables + L::kState + (16 * q + n16) * 4) * (kBf16 ? 1.f : power_of_two(-e - unit));
+                const float f = *reinterpret_cast<const float*>(tables + L::kState + (16 * q + n16) * 4);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[q][i] *= f;
+                for (int i = 0; i < 4; ++i) {
+                    if (!kBf16) o[q][i] = __builtin_fmaf(low[q][i], kRestDown, o[q][i]) * down[i];
+                    o[q][i] *= f;
+                }
             }
         }
         u4 v[2];
@@ -522,12 +525,10 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
                     o[q] = linear_mfma<T>(v[u], hi, o[q]);
                     rest[q] = linear_mfma<T>(v[u], lo, rest[q]);
                 } else {
-                    f4 sum = {};
-                    sum = linear_mfma<T>(v[u], hi, sum);
-                    sum = linear_mfma<T>(v[u], lo, sum);
+                    const f4 sum = linear_mfma<T>(v[u], hi, f4{}), low = linear_mfma<T>(v[u], lo, f4{});
                     const float f = *reinterpret_cast<const float*>(smem + L::kRow + (pair * 16 + n16) * 4);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[q][i] = __builtin_fmaf(sum[i], f, o[q][i]);
+                    for (int i = 0; i < 4; ++i) o[q][i] = __builtin_fmaf(__builtin_fmaf(low[i], kRestDown, sum[i]), f, o[q][i]);
                 }
             }
             // to where v was, whose operands are in registers: lane (n, g) has columns 4 g .. + 3 of row n
@@ -542,52 +543,60 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         // the state moves on
         if (MODE == kLinearSums) part_sum += chunk[2];
         if (MODE != kLinearRows || end < stop) {
-            int next = unit;
-            if constexpr (!kBf16) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int u = 0; u < 2; ++u)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) top = max_u16x2(top, v[u][k] & 0x7FFF7FFFu);
-                const float largest = wave_max(fmaxf(half_lo_to_f32(top), half_hi_to_f32(top)));
-                if (largest > 0.f && largest < INFINITY) next = scale_exponent(largest);
-            }
-            const float by = kBf16 ? chunk[0] : chunk[0] * power_of_two(next - unit), values = power_of_two(next);
-            unit = next;
             hold = again ? 1.f : chunk[0];
-            if (again) {
-#pragma unroll
-                for (int m = 0; m < KM; ++m)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[m][i] *= by;
-            }
-            u4 x[2][kParts], k[2][KM];
-            const auto operands = [&](int u) {
-#pragma unroll
-                for (int m = 0; m < KM; ++m) k[u][m] = transposed(lds0 + L::kK + 32 * u * L::kKRow + (kt_at ^ (32u * m)), L::kKRow);
+            float y[2][8], values = 1.f;  // weighted values
+            const auto weigh = [&](int u) {
                 const f4 w0 = *reinterpret_cast<const f4*>(tables + L::kW + (32 * u + 4 * g4) * 4), w1 = *reinterpret_cast<const f4*>(tables + L::kW + (32 * u + 16 + 4 * g4) * 4);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const f4 w = i < 2 ? w0 : w1;
-                    float y = T::to_f32((uint16_t)v[u][i]) * w[2 * (i & 1)], z = T::to_f32((uint16_t)(v[u][i] >> 16)) * w[2 * (i & 1) + 1];
-                    if (!kBf16) y *= values, z *= values;
+                    y[u][2 * i] = T::to_f32((uint16_t)v[u][i]) * w[2 * (i & 1)], y[u][2 * i + 1] = T::to_f32((uint16_t)(v[u][i] >> 16)) * w[2 * (i & 1) + 1];
+                }
+            };
+            u4 x[2][kParts], k[2][KM];
+            const auto operands = [&](int u) {
+#pragma unroll
+                for (int m = 0; m < KM; ++m) k[u][m] = transposed(lds0 + L::kK + 32 * u * L::kKRow + (kt_at ^ (32u * m)), L::kKRow);
+                if (kBf16) weigh(u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
                     uint32_t parts[kParts];
-                    linear_split<T, kParts>(y, z, parts);
+                    linear_split<T, kParts>(kBf16 ? y[u][2 * i] : y[u][2 * i] * values, kBf16 ? y[u][2 * i + 1] : y[u][2 * i + 1] * values, parts);
 #pragma unroll
                     for (int q = 0; q < kParts; ++q) x[u][q][i] = parts[q];
                 }
             };
-            operands(0);
+            if constexpr (kBf16) {
+                if (again) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u == 0) operands(1);
+                    for (int m = 0; m < KM; ++m)
 #pragma unroll
-                for (int q = 0; q < kParts; ++q)
+                        for (int i = 0; i < 4; ++i) s[m][i] *= chunk[0];
+                }
+                operands(0);
 #pragma unroll
-                    for (int m = 0; m < KM; ++m) s[m] = linear_mfma<T>(k[u][m], x[u][q], s[m]);
-                if constexpr (!kBf16) {  // a product, three instructions of the next weighting in its shade (6 x 100 ... 1 900 tokens 87.2 -> 84.2 us, of bf16 slower)
-                    if (u == 0)
-                        for (int i = 0; i < KM * kParts; ++i) __builtin_amdgcn_sched_group_barrier(8, 1, 0), __builtin_amdgcn_sched_group_barrier(2, 3, 0);
+                for (int u = 0; u < 2; ++u) {
+                    if (u == 0) operands(1);
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                        for (int m = 0; m < KM; ++m) s[m] = linear_mfma<T>(k[u][m], x[u][q], s[m]);
+                }
+            } else {
+                weigh(0), weigh(1);
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(fabsf(y[0][i]), fabsf(y[1][i])));
+                const int e = scale_exponent(max_over_rows(top));  // of the lane's column, which is that of its part of the state
+                values = power_of_two(e);
+                const float down = power_of_two(-e);
+                operands(0), operands(1);
+#pragma unroll
+                for (int m = 0; m < KM; ++m) {
+                    f4 sum = linear_mfma<T>(k[0][m], x[0][0], f4{}), low = linear_mfma<T>(k[0][m], x[0][1], f4{});
+                    sum = linear_mfma<T>(k[1][m], x[1][0], sum), low = linear_mfma<T>(k[1][m], x[1][1], low);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[m][i] = __builtin_fmaf(__builtin_fmaf(low[i], kRestDown, sum[i]), down, chunk[0] * s[m][i]);
                 }
             }
         }
@@ -604,9 +613,8 @@ __global__ __launch_bounds__(4 * DV, 2) void linear_chunk_kernel(const LinearArg
         store_rows(before, stop);
     }
     if (MODE == kLinearSums) {
-        const float by = kBf16 ? hold : power_of_two(-unit);
 #pragma unroll
-        for (int m = 0; m < KM; ++m) *reinterpret_cast<f4*>(mine + m * 256) = s[m] * by;
+        for (int m = 0; m < KM; ++m) *reinterpret_cast<f4*>(mine + m * 256) = s[m] * hold;
         if (tid == 0) p.fades[(int64_t)group * a.v_heads + head] = __builtin_amdgcn_exp2f(part_sum);
     }
 }
