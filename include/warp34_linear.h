@@ -8,8 +8,9 @@
  * and has_initial_state.
  *
  * One entry serves prompts, single tokens and drafted tokens.  max_q_len, the host's bound on a request's tokens (0: not known,
- * total_tokens), chooses between kernels that add in another order and, of prompts, how they are cut, and changes nothing else; a
- * bound that is wrong costs time only. */
+ * total_tokens), chooses the kernel for the whole batch: up to 4 tokens (8 where num_reqs * num_v_heads * v_head_dim is above 32 768) one token after the
+ * other, all in fp32, each off by 2^-22 of its terms' size at most; beyond, chunks of 64 tokens, of the exactness given below, cut by it into parts.  A bound that is wrong
+ * costs time, or that exactness, and nothing else. */
 #ifndef WARP34_LINEAR_H
 #define WARP34_LINEAR_H
 
