@@ -343,7 +343,10 @@ bool fork_request_pages(KvPool& pool, PrefixPageCache& cache, const RequestPages
                         KvPool* draft_pool = nullptr, PageCopies* draft_copies = nullptr);
 // Moves the requests' private KV pages from page `below` on to free pages under it, the lowest first, rewrites their page
 // lists and frees the pages they left; returns how many found no place.  Pages of the prefix cache stay.  What is
-// freed may be written only by work that runs behind the copies.
-size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& requests, size_t below, PageCopies* copies);
+// freed may be written only by work that runs behind the copies.  Rows of committed tokens travel, and no others: between a step's
+// append and its commit, written_tokens says for each request how many of its tokens, the drafted ones among them, have rows (throws
+// std::invalid_argument where it is not as long as requests, before anything is moved).
+size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& requests, size_t below, PageCopies* copies,
+                          const std::vector<size_t>* written_tokens = nullptr);
 
 }  // namespace warp34_host

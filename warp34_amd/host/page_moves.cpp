@@ -9,13 +9,13 @@
 namespace warp34_host {
 
 namespace {
-// Rows of page `index` of a request that hold committed tokens.
-size_t committed_rows(const RequestPages& r, size_t index, size_t page_size) {
+// Rows of page `index` of a request that hold its first `tokens`.
+size_t filled_rows(size_t tokens, size_t index, size_t page_size) {
     const size_t first = index * page_size;
-    return r.token_ids.size() <= first ? 0 : std::min(page_size, r.token_ids.size() - first);
+    return tokens <= first ? 0 : std::min(page_size, tokens - first);
 }
 void add_copies(const RequestPages& parent, const std::vector<int32_t>& from, const std::vector<int32_t>& to, size_t page_size, PageCopies* out) {
-    for (size_t i = parent.protected_pages; i < to.size(); ++i) out->add(from[i], to[i], (int32_t)committed_rows(parent, i, page_size));
+    for (size_t i = parent.protected_pages; i < to.size(); ++i) out->add(from[i], to[i], (int32_t)filled_rows(parent.token_ids.size(), i, page_size));
 }
 }  // namespace
 
@@ -53,11 +53,16 @@ bool fork_request_pages(KvPool& pool, PrefixPageCache& cache, const RequestPages
     return true;
 }
 
-size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& requests, size_t below, PageCopies* copies) {
+size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& requests, size_t below, PageCopies* copies,
+                          const std::vector<size_t>* written_tokens) {
+    if (written_tokens && written_tokens->size() != requests.size())
+        throw std::invalid_argument("pack_request_pages: written tokens of other requests");
     std::vector<int32_t> left;  // freed behind the last move, so that no page is taken and given in one batch of copies
     size_t without = 0;
-    for (RequestPages* r : requests) {
+    for (size_t n = 0; n < requests.size(); ++n) {
+        RequestPages* const r = requests[n];
         const size_t page_size = r->page_size ? r->page_size : pool.block_size;
+        const size_t tokens = std::max(r->token_ids.size(), written_tokens ? (*written_tokens)[n] : 0);
         for (size_t i = r->protected_pages; i < r->kv_pages.size(); ++i) {
             int32_t& page = r->kv_pages[i];
             if (page < 0 || (size_t)page < below) continue;
@@ -67,7 +72,7 @@ size_t pack_request_pages(KvPool& pool, const std::vector<RequestPages*>& reques
                 ++without;
                 continue;
             }
-            copies->add(page, *to, (int32_t)committed_rows(*r, i, page_size));
+            copies->add(page, *to, (int32_t)filled_rows(tokens, i, page_size));
             left.push_back(page);
             page = *to;
         }
