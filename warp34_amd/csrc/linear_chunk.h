@@ -15,9 +15,9 @@
 // weighted values and S are scaled by a power of two of their column, P by one of its row, to put the largest at 2^14, and what the first part leaves is
 // held times 2^11 and has sums of its own.  So 22 bits stay of what is up to 2^28 below the largest, and bits 2^-50 below it are lost.
 //
-// Bound: instruction issue.  A wave's chunk is 100 products of 16 cycles and 460 vector instructions of four, the two waves of a SIMD take 6 900 of the
-// 8 200 cycles that a chunk of a full batch lasts: splits and products of a wave wait for each other, and the clock falls to 1.8 .. 2.0 GHz.  8 x 4 096 tokens of 32
-// heads of 128 x 128 walked in 268 .. 278 us (3.5 a chunk, 250 TFLOP/s, 3.1 TB/s), 8 192 tokens in parts in 103, 333 tokens of 16 heads in 18.
+// Bound: instruction issue.  A wave's chunk is 98 products of 16 cycles and 477 vector instructions of four, the two waves of a SIMD take 6 950 of the
+// 8 600 cycles that a chunk of a full batch lasts: splits and products of a wave wait for each other, and the clock falls to 1.8 .. 2.0 GHz.  8 x 4 096 tokens of 32
+// heads of 128 x 128 walked in 270 .. 280 us (3.5 a chunk, 250 TFLOP/s, 3.1 TB/s), 8 192 tokens in parts in 103, 333 tokens of 16 heads in 19.
 // Tile: a wave has 16 columns so that eight waves hold a state of 128 x 128 in 32 registers each and share one copy of k and q.  Four waves of 32
 // columns with 32x32x16 products took 301 us, two workgroups of four waves of 16 columns, each with a copy, 3 to 40 % longer.  A chunk laid
 // into LDS beside the one at work, for two barriers instead of three, took 9 % longer.
