@@ -12,8 +12,9 @@
 // tokens have faded away, the sums are large and the differences small.
 // Operands of 16 bits are rounded states, weights and weighted values.  P and S have two parts (16 bits of bf16, 22 of fp16), so that outputs
 // show their own rounding (8 and 11 bits) as long as their terms do not cancel by as much as lies between; v' has three for bf16 where the
-// state itself comes out (24 bits), two for fp16.  fp16 has little range: weighted values and S are scaled by a power of two of their column, P by one of its row, to put the largest at 2^14, and what the first part leaves is
-// held times 2^11 and has sums of its own.  So 22 bits stay of what is up to 2^28 below the largest, and bits 2^-50 below it are lost.
+// state itself comes out (24 bits), two for fp16.  fp16 has little range: weighted values and S are scaled by a power of two of their
+// column, P by one of its row, to put the largest at 2^14, and what the first part leaves is held times 2^11 and has sums of its own.
+// So 22 bits stay of what is up to 2^28 below the largest, and bits 2^-50 below it are lost.
 //
 // Bound: instruction issue.  A wave's chunk is 98 products of 16 cycles and 477 vector instructions of four, the two waves of a SIMD take 6 950 of the
 // 8 600 cycles that a chunk of a full batch lasts: splits and products of a wave wait for each other, and the clock falls to 1.8 .. 2.0 GHz.  8 x 4 096 tokens of 32
